@@ -198,6 +198,41 @@ int rlt_paged_attention_uses_mfma(int32_t q_dtype, int32_t kv_dtype, int32_t hea
 int rlt_paged_attention_uses_prefill(int32_t q_dtype, int32_t kv_dtype, int32_t head_dim,
                                      int32_t max_q_len);
 
+/*
+ * Attention of a draft tree's nodes over a paged KV pool: the packed window form
+ * (cu_seqlens_q, one block table per sequence) with a tree in place of the causal window.
+ * Sequence s owns q rows cu[s] .. cu[s + 1] - 1, the N nodes of its tree (at most max_q_len),
+ * whose keys and values already lie in the cache at the last N positions
+ * context_lengths[s] - N + j.  A row sees every position of the prefix
+ * [0, context_lengths[s] - N) and the nodes j of its own tree whose bit is set: bit j % 64 of
+ * word j / 64 of its tree_mask row (int64 [num_q_rows, mask_words], mask_stride words
+ * between rows; rlt_tree_masks makes the ancestors' bits from the parents).  Bits past the
+ * tree are ignored; a row that sees nothing gives zeros.  With window > 0 a row sees the
+ * last `window` of those positions.  Keys, values and scales at positions that a row does
+ * not see have no effect on it, whatever they hold.  Other arguments as
+ * rlt_paged_attention; the pool is of q's type (no scales) or fp8-e4m3 (scale_mode 1 or 2).
+ * At most 256 nodes per tree, head_dim <= 256 (RLT_ERR_UNSUPPORTED beyond).  A row's bits
+ * depend on the lengths of the whole batch (how its keys are split over the CUs), within
+ * rounding.  No counterpart in the reference, whose drafts are chains.  The grid is static:
+ * safe under graph capture.
+ */
+size_t rlt_tree_attention_workspace_size(int32_t num_seqs, int32_t head_dim);
+
+int rlt_tree_attention(const void* q, int64_t q_row_stride, int64_t q_head_stride,
+                       const void* key_cache, const void* value_cache, int64_t k_block_stride,
+                       int64_t k_token_stride, int64_t k_head_stride, int64_t v_block_stride,
+                       int64_t v_token_stride, int64_t v_head_stride, int32_t num_blocks,
+                       const int32_t* block_tables, int64_t table_stride, int32_t table_width,
+                       const int32_t* context_lengths, const int32_t* cu_seqlens_q,
+                       const int64_t* tree_mask, int64_t mask_stride, int32_t mask_words,
+                       int32_t num_seqs, int32_t max_q_len, int32_t num_q_rows,
+                       const float* key_scale, const float* value_scale, int32_t scale_mode,
+                       int64_t s_block_stride, int64_t s_token_stride, int64_t s_head_stride,
+                       int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim,
+                       int32_t block_size, int32_t q_dtype, int32_t kv_dtype, int32_t window,
+                       void* out, int64_t out_row_stride, int64_t out_head_stride,
+                       void* workspace, size_t workspace_bytes, hipStream_t stream);
+
 /* ---------------------------------------------------------------- sampler */
 
 /*

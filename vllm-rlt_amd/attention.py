@@ -64,6 +64,9 @@ class AttentionBackend:
     def prefill_store(self, *args, **kwargs):
         return self.kernel.prefill_store(*args, **kwargs)
 
+    def tree(self, *args, **kwargs):
+        return self.kernel.tree(*args, **kwargs)
+
     def windowed(self, *args, **kwargs):
         method = getattr(self.kernel, "windowed", None)
         if method is None:
@@ -171,6 +174,31 @@ class MI355XPagedAttention:
                                                 block_tables, context_lengths, cu_seqlens_q,
                                                 int(max_seqlen_q), key_scale, value_scale,
                                                 row_lengths, self.compensate)
+
+    def tree(self, q, key_cache, value_cache, block_tables, context_lengths, cu_seqlens_q,
+             max_seqlen_q, tree_mask, key_scale=None, value_scale=None, *, window=0):
+        """Attention of draft trees: ``prefill`` with a tree in place of the causal window.
+
+        Sequence s owns q rows ``cu_seqlens_q[s]`` to ``cu_seqlens_q[s + 1] - 1``, the nodes of
+        its tree (at most ``max_seqlen_q``, which is at most 256), whose keys and values are
+        already in the cache at its last positions: node j at ``context_lengths[s] - nodes +
+        j``.  A row sees the whole prefix before node 0 and the nodes of its own tree whose bit
+        is set in its ``tree_mask`` row (int64 ``[q rows, words]``, bit ``j % 64`` of word
+        ``j // 64``; ``sampling.tree_masks`` makes a node's ancestors and itself from the
+        parents), with ``window > 0`` the last ``window`` of those positions.  A row that sees
+        nothing gives zeros; what a row does not see has no effect on it, whatever it holds.
+        The pool is of q's type, or float8_e4m3fn with per-tensor or per-vector scales.
+        A row's last bits depend on the lengths of the whole batch, since its keys are split
+        over the CUs by them.  No reference counterpart (its drafts are chains).
+        """
+        if type(window) is not int or window < 0:
+            raise ValueError("window must be a nonnegative integer")
+        _lib.require_gpu(q, key_cache, value_cache, block_tables, context_lengths, cu_seqlens_q,
+                         tree_mask, key_scale, value_scale)
+        # argument checks, workspace and launch: torch.ops.rlt_mi355x.tree_attention
+        return _lib.ops().tree_attention(q, key_cache, value_cache, block_tables,
+                                         context_lengths, cu_seqlens_q, int(max_seqlen_q),
+                                         tree_mask, key_scale, value_scale, window)
 
     def uses_mfma(self, q_dtype, kv_dtype, head_dim):
         lib = _lib.library()

@@ -621,6 +621,102 @@ Tensor paged_attention_store(const Tensor& q, const Tensor& k_new_in, const Tens
                          std::nullopt, cu_seqlens_q, max_seqlen_q, 0, row_lengths, compensate);
 }
 
+// ---------------------------------------------------------------- draft trees
+
+// Attention of the nodes of draft trees (rlt_tree_attention): packed rows, an ancestor mask in
+// place of the causal window.
+Tensor tree_attention(const Tensor& q, const Tensor& key_cache, const Tensor& value_cache,
+                      const Tensor& block_tables, const Tensor& context_lengths,
+                      const Tensor& cu_seqlens_q, int64_t max_seqlen_q, const Tensor& tree_mask,
+                      const OptTensor& key_scale, const OptTensor& value_scale, int64_t window) {
+  TORCH_CHECK_VALUE(window >= 0 && window <= INT32_MAX, "window must be a nonnegative integer");
+  TORCH_CHECK_VALUE(q.dim() == 3 && key_cache.dim() == 4 && value_cache.dim() == 4,
+                    "q must be [rows, heads, dim] and caches [block, token, kv_head, dim]");
+  same_device(q, key_cache, value_cache, block_tables, context_lengths, cu_seqlens_q, tree_mask,
+              key_scale, value_scale);
+  const int64_t rows = q.size(0), heads = q.size(1), head_dim = q.size(2);
+  TORCH_CHECK_VALUE(head_dim >= 1 && head_dim <= 256,
+                    "the MI355X attention backend supports head_dim <= 256");
+  TORCH_CHECK_VALUE(key_cache.sizes() == value_cache.sizes() &&
+                        key_cache.scalar_type() == value_cache.scalar_type(),
+                    "key and value caches must share shape and dtype");
+  const int64_t num_blocks = key_cache.size(0), block_size = key_cache.size(1);
+  const int64_t kv_heads = key_cache.size(2);
+  TORCH_CHECK_VALUE(kv_heads >= 1 && heads >= 1 && heads % kv_heads == 0 &&
+                        key_cache.size(3) == head_dim,
+                    "q heads must be a positive multiple of KV heads with equal head_dim");
+  TORCH_CHECK_VALUE(num_blocks >= 1 && block_size >= 1 && num_blocks <= INT32_MAX,
+                    "the KV pool must hold at least one block");
+  TORCH_CHECK_VALUE(key_cache.stride(3) == 1 && value_cache.stride(3) == 1 && q.stride(2) == 1,
+                    "paged attention requires a contiguous head dimension");
+  const bool fp8 = key_cache.scalar_type() == at::kFloat8_e4m3fn;
+  TORCH_CHECK_VALUE(logit_dtype(q.scalar_type()), "q must be float32, bfloat16 or float16");
+  TORCH_CHECK_VALUE(fp8 || key_cache.scalar_type() == q.scalar_type(),
+                    "the KV pool must have q's dtype or be float8_e4m3fn");
+  int32_t mode = 0;
+  int64_t s_strides[3] = {0, 0, 0};
+  TORCH_CHECK_VALUE(key_scale.has_value() == value_scale.has_value(),
+                    "key_scale and value_scale must be given together");
+  TORCH_CHECK_VALUE(fp8 == key_scale.has_value(),
+                    "an FP8 KV pool needs key_scale / value_scale, any other takes none");
+  if (fp8) {
+    TORCH_CHECK_VALUE(key_scale->scalar_type() == at::kFloat &&
+                          value_scale->scalar_type() == at::kFloat,
+                      "FP8 scales must be float32");
+    if (key_scale->dim() == 0 && value_scale->dim() == 0) {
+      mode = 1;
+    } else {
+      TORCH_CHECK_VALUE(key_scale->dim() == 3 && key_scale->strides() == value_scale->strides() &&
+                            key_scale->sizes() == key_cache.sizes().slice(0, 3) &&
+                            value_scale->sizes() == key_scale->sizes(),
+                        "per-vector FP8 scales must be [block, token, kv_head] views of the pool "
+                        "sharing strides");
+      mode = 2;
+      for (int i = 0; i < 3; ++i) s_strides[i] = key_scale->stride(i);
+    }
+  }
+  TORCH_CHECK_VALUE(block_tables.dim() == 2 && block_tables.scalar_type() == at::kInt &&
+                        (block_tables.stride(1) == 1 || block_tables.size(1) <= 1),
+                    "block_tables must be int32 [sequences, width] with unit column stride");
+  const int64_t num_seqs = block_tables.size(0), width = block_tables.size(1);
+  TORCH_CHECK_VALUE(context_lengths.dim() == 1 && context_lengths.size(0) == num_seqs &&
+                        cu_seqlens_q.dim() == 1 && cu_seqlens_q.size(0) == num_seqs + 1,
+                    "cu_seqlens_q must be [sequences + 1] and lengths [sequences]");
+  need(context_lengths, at::kInt, "context_lengths");
+  need(cu_seqlens_q, at::kInt, "cu_seqlens_q");
+  TORCH_CHECK_VALUE(max_seqlen_q >= 0 && max_seqlen_q <= 256,
+                    "a draft tree holds at most 256 nodes");
+  TORCH_CHECK_VALUE(tree_mask.dim() == 2 && tree_mask.size(0) == rows &&
+                        tree_mask.scalar_type() == at::kLong &&
+                        tree_mask.size(1) * 64 >= max_seqlen_q &&
+                        (tree_mask.stride(1) == 1 || tree_mask.size(1) <= 1),
+                    "tree_mask must be int64 [q rows, words] with unit column stride and a bit "
+                    "for each of max_seqlen_q nodes");
+  TORCH_CHECK_VALUE(width * block_size <= INT32_MAX - 4096 && rows <= INT32_MAX,
+                    "a sequence's table covers at most 2^31 - 4097 positions");
+  const c10::hip::HIPGuardMasqueradingAsCUDA guard(q.device());
+  Tensor output = at::empty({rows, heads, head_dim}, q.options());
+  if (rows == 0 || num_seqs == 0 || max_seqlen_q == 0) return output;
+  const Tensor ws = workspace(rlt_tree_attention_workspace_size((int32_t)num_seqs, (int32_t)head_dim), q);
+  const int64_t mask_stride = std::max(tree_mask.stride(0), tree_mask.size(1));
+  TORCH_CHECK_VALUE(rows == 1 || tree_mask.stride(0) >= tree_mask.size(1),
+                    "tree_mask rows must not overlap");
+  const int status = rlt_tree_attention(
+      ptr(q), q.stride(0), q.stride(1), ptr(key_cache), ptr(value_cache), key_cache.stride(0),
+      key_cache.stride(1), key_cache.stride(2), value_cache.stride(0), value_cache.stride(1),
+      value_cache.stride(2), (int32_t)num_blocks, (const int32_t*)ptr(block_tables),
+      block_tables.stride(0), (int32_t)width, (const int32_t*)ptr(context_lengths),
+      (const int32_t*)ptr(cu_seqlens_q), (const int64_t*)ptr(tree_mask), mask_stride,
+      (int32_t)tree_mask.size(1), (int32_t)num_seqs, (int32_t)max_seqlen_q, (int32_t)rows,
+      (const float*)ptr(key_scale), (const float*)ptr(value_scale), mode, s_strides[0],
+      s_strides[1], s_strides[2], (int32_t)heads, (int32_t)kv_heads, (int32_t)head_dim,
+      (int32_t)block_size, dtype_code(q.scalar_type()), dtype_code(key_cache.scalar_type()),
+      (int32_t)window, ptr(output), output.stride(0), output.stride(1), ptr(ws), ws.numel(),
+      stream_of(q));
+  check_status(status, "rlt_tree_attention");
+  return output;
+}
+
 }  // namespace
 
 TORCH_LIBRARY(rlt_mi355x, m) {
@@ -645,6 +741,9 @@ TORCH_LIBRARY(rlt_mi355x, m) {
         "Tensor(b!) value_cache, Tensor block_tables, Tensor context_lengths, "
         "Tensor cu_seqlens_q, int max_seqlen_q, Tensor(c!)? key_scale=None, "
         "Tensor(d!)? value_scale=None, Tensor? row_lengths=None, bool compensate=False) -> Tensor");
+  m.def("tree_attention(Tensor q, Tensor key_cache, Tensor value_cache, Tensor block_tables, "
+        "Tensor context_lengths, Tensor cu_seqlens_q, int max_seqlen_q, Tensor tree_mask, "
+        "Tensor? key_scale=None, Tensor? value_scale=None, int window=0) -> Tensor");
 }
 
 TORCH_LIBRARY_IMPL(rlt_mi355x, CUDA, m) {
@@ -657,4 +756,5 @@ TORCH_LIBRARY_IMPL(rlt_mi355x, CUDA, m) {
   m.impl("verify_distributions", &verify_distributions);
   m.impl("verify_accept", &verify_accept);
   m.impl("paged_attention_store", &paged_attention_store);
+  m.impl("tree_attention", &tree_attention);
 }

@@ -38,6 +38,12 @@ def _(q, k_new, v_new, key_cache, value_cache, block_tables, context_lengths, cu
     return torch.empty_like(q)
 
 
+@torch.library.register_fake("rlt_mi355x::tree_attention")
+def _(q, key_cache, value_cache, block_tables, context_lengths, cu_seqlens_q, max_seqlen_q,
+      tree_mask, key_scale=None, value_scale=None, window=0):
+    return q.new_empty(q.shape)
+
+
 @torch.library.register_fake("rlt_mi355x::spec_probs")
 def _(logits, temperature, top_k, top_p, max_top_k, apply_top_p):
     return logits.new_empty(logits.shape, dtype=torch.float32)
@@ -166,7 +172,7 @@ def finalize_rows(descriptor: torch.Tensor, tables: torch.Tensor, key_pool: torc
     _kv.finalize_rows(descriptor, tables, key_pool, value_pool, block_size)
 
 
-OPS = ("paged_attention", "paged_attention_store", "spec_probs", "categorical", "spec_accept", "greedy_accept",
+OPS = ("paged_attention", "paged_attention_store", "tree_attention", "spec_probs", "categorical", "spec_accept", "greedy_accept",
        "propose_drafts", "verify_distributions", "verify_accept", "merge_random_round",
        "rejection_rows", "store_kv",
        "store_fp8", "finalize_rows")
