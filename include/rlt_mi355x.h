@@ -427,6 +427,77 @@ int rlt_greedy_accept(const int64_t* draft_tokens, const int64_t* drafts, const 
                       int64_t vocab, int64_t* targets, int64_t* accepted, int64_t* next_token,
                       hipStream_t stream);
 
+/*
+ * Greedy verify round of draft trees.  Node 0 of a request is its last committed token,
+ * node j + 1 its draft j, the child of node parents[r, j] (an earlier node: 0 .. j; a draft
+ * with any other parent is never reached).  targets = argmax of every node's logit row
+ * (first maximal column, NaN the maximum).  The walk starts at node 0 and goes to the first
+ * draft j < drafts[r] whose parent is the current node and whose token is its target, until
+ * there is none: path[r, 0 .. accepted[r]] are the nodes it visits (path[r, 0] = 0; -1 behind
+ * the path), next_token the last one's target.  The emitted tokens are targets[r, path[r, i]],
+ * i = 0 .. accepted[r].  A chain (parents[r, j] = j) gives rlt_greedy_accept's results.
+ *   draft_tokens, parents int64 [n, width], drafts int64 [n], target_logits
+ *   [n, width + 1, V] (RLT_F32 / RLT_BF16 / RLT_F16; row_stride elements between consecutive
+ *   rows) -> targets, path int64 [n, width + 1], accepted, next_token int64 [n].
+ * width <= 255, V <= 2^20.  No counterpart in the reference (its drafts are chains;
+ * vllm_rlt/worker/async_speculative.py:706-720 is the chain's round).
+ */
+size_t rlt_greedy_tree_accept_workspace_size(int64_t n, int32_t width, int64_t vocab);
+
+int rlt_greedy_tree_accept(const int64_t* draft_tokens, const int64_t* parents,
+                           const int64_t* drafts, const void* target_logits, int32_t logits_dtype,
+                           int64_t row_stride, int64_t n, int32_t width, int64_t vocab,
+                           int64_t* targets, int64_t* path, int64_t* accepted, int64_t* next_token,
+                           void* workspace, size_t workspace_bytes, hipStream_t stream);
+
+/*
+ * Sampled verify round of draft trees (nodes and parents as rlt_greedy_tree_accept): the
+ * emitted tokens are distributed as if drawn from p one by one.  At a node the weights are
+ * y = p[node] with R = 1; its drafts j < drafts[r] are tried in index order, each one drawn
+ * from q[node]: accepted when u_accept[r, j] * R * q[node, t] < y[t] (t its token), else
+ * y = max(y - R q[node], 0) and R = sum y.  The walk goes on at an accepted draft's node; where
+ * none is left, the final token is drawn from y by inverse CDF with u_final[r] as in
+ * rlt_categorical.  All in float64; rows of p and q count as distributions as they stand.
+ * error[r] is set, and the final token 0, where drafts[r] is outside [0, width], a tried draft
+ * has a token outside the vocabulary, no q mass or weights that are not finite, or where the
+ * weights left have no finite positive mass.
+ *   draft_tokens, parents int64 [n, width], drafts int64 [n], q fp32 [n, width, V] (row i:
+ *   the distribution that node i's children were drawn from; the last node has none), p fp32
+ *   [n, width + 1, V], u_accept fp32 [n, width], u_final fp32 [n] (contiguous)
+ *   -> path (as above), tokens int64 [n, width + 1] (the accepted tokens, the final one,
+ *   zeros), accepted, final_token int64 [n], error uint8 (bool) [n].
+ * width <= 255, V <= 2^20.  Workspace: rlt_tree_accept_workspace_size.  The chain's round is
+ * vllm_rlt/worker/speculative_sampling.py:104-181.
+ */
+size_t rlt_tree_accept_workspace_size(int64_t n, int32_t width, int64_t vocab);
+
+int rlt_tree_accept(const int64_t* draft_tokens, const int64_t* parents, const int64_t* drafts,
+                    const float* q, const float* p, const float* u_accept, const float* u_final,
+                    int64_t n, int32_t width, int64_t vocab, int64_t* path, int64_t* tokens,
+                    int64_t* accepted, int64_t* final_token, uint8_t* error, void* workspace,
+                    size_t workspace_bytes, hipStream_t stream);
+
+/*
+ * Log probabilities of given tokens, with rank, entropy and the top alternatives of their
+ * rows.  Row i of the call is logit row rows[i] (int64 [count]; NULL: row i) of
+ * logits [num_rows, V] (RLT_F32 / RLT_BF16 / RLT_F16, row stride in elements), t = tokens[i]:
+ *   logprob[i] = x_t - log sum e^x, rank[i] = 1 + the columns before t in descending order
+ *   (equal logits by ascending column, NaN first), entropy[i] = -sum p log p (nats),
+ *   top_tokens / top_logprob [count, top_n] = the first top_n columns in that order.
+ * Sums in float64, outputs rounded once.  Logits of -inf weigh nothing; a row with a NaN, with
+ * +inf or without a logit above -inf gives NaN log probabilities and entropy.  A row index outside
+ * [0, num_rows) gives NaN, rank 0 and tokens -1; a token outside the vocabulary NaN and rank
+ * 0 beside the row's entropy and alternatives.  top_n <= 64, V <= 2^20, count <= 65535.
+ * No counterpart in the reference.
+ */
+size_t rlt_token_logprobs_workspace_size(int64_t count, int64_t vocab, int32_t top_n);
+
+int rlt_token_logprobs(const void* logits, int32_t logits_dtype, int64_t row_stride,
+                       int64_t num_rows, int64_t vocab, const int64_t* rows, const int64_t* tokens,
+                       int64_t count, int32_t top_n, float* logprob, int64_t* rank, float* entropy,
+                       float* top_logprob, int64_t* top_tokens, void* workspace,
+                       size_t workspace_bytes, hipStream_t stream);
+
 /* ---------------------------------------------------------------- KV write side */
 
 /*
@@ -483,6 +554,25 @@ int rlt_kv_finalize(const int64_t* descriptors, int64_t count, const int32_t* ta
                     int32_t layers, int64_t num_blocks, void* key_pool, void* value_pool,
                     int64_t block_stride, int64_t layer_stride, int64_t token_stride,
                     int64_t bytes_per_token, int32_t elt_bytes, hipStream_t stream);
+
+/*
+ * The accepted path of draft trees, moved behind the prefix.  Request r's node j lies at
+ * position starts[r] + j of its tables; for j = 1 .. accepted[r] the bytes_per_token bytes at
+ * position starts[r] + path[r, j] go to position starts[r] + j, in every layer of both pools
+ * [block, layer, token, ...] (strides in elements of elt_bytes; the same call again for the
+ * fp32 scale pools of an fp8 cache).  tables int32 [n, planes, width]: every plane moves.
+ * path int64 [n, path_width] (path_stride between rows) ascends from path[r, 0] = 0, as the
+ * tree rounds return it; entries with path[r, j] <= j stay.  In place and in order: blocks of
+ * one table, and the blocks of different requests and planes that hold drafts, must be
+ * distinct.  Positions beyond the table or entries outside the pool copy nothing.
+ * path_width <= 256.  No counterpart in the reference, where a chain's path lies in place.
+ */
+int rlt_kv_commit_path(const int32_t* tables, int64_t n, int32_t planes, int32_t width,
+                       int32_t block_size, const int64_t* starts, const int64_t* path,
+                       int64_t path_stride, int32_t path_width, const int64_t* accepted,
+                       int32_t layers, int64_t num_blocks, void* key_pool, void* value_pool,
+                       int64_t block_stride, int64_t layer_stride, int64_t token_stride,
+                       int64_t bytes_per_token, int32_t elt_bytes, hipStream_t stream);
 
 /* ---------------------------------------------------------------- routing / metadata */
 
@@ -618,6 +708,15 @@ int rlt_merge_random_round(const int64_t* target, int64_t num_rows, const int64_
                            int64_t* accepted_out, int64_t* next_tokens_out,
                            int64_t* next_positions_out, int64_t* next_values_out,
                            int64_t* error_out, hipStream_t stream);
+
+/* Mask rows of draft trees for rlt_tree_attention: q row cu_seqlens_q[s] + i is node i of
+ * sequence s and sees itself and its ancestors; node i's parent is parents[s, i - 1] (int64
+ * [num_seqs, width], parent_stride between rows), node 0 the root.  A parent outside [0, i), or a
+ * node past width, ends the walk.  mask int64 [rows, words]; rows of no sequence are cleared.
+ * No counterpart in the reference. */
+int rlt_tree_masks(const int64_t* parents, int64_t parent_stride, int32_t width,
+                   const int32_t* cu_seqlens_q, int32_t num_seqs, int64_t* mask, int32_t words,
+                   int64_t rows, hipStream_t stream);
 
 #ifdef __cplusplus
 }

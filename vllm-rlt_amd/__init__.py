@@ -16,6 +16,9 @@ Drop-in host layer over ``librlt_mi355x.so`` (hand-written gfx950 HIP kernels):
   ``finalize_rows``, the KV writers the verify window's keys and values go through
   (vllm_rlt/kernels/routing.py:147-223, vllm_rlt/kernels/graph_kv.py:52-67,
   vllm_rlt/kernels/triton_attention.py:579-623).
+* draft trees in place of chains (no reference counterpart): ``MI355XPagedAttention.tree``
+  with ``routing.tree_masks``, ``sampling.tree_accept`` / ``greedy_tree_accept``,
+  ``kv_write.commit_tree_kv``; and ``sampling.token_logprobs`` for the emitted tokens.
 * ``ops``: the same entry points as ``torch.ops.rlt_mi355x.*`` operators (ROCm device
   implementations and fake shape functions; the reference's torch_bindings pattern).
 * ``routing``: device metadata and request routing of the asynchronous verify step
@@ -39,6 +42,7 @@ from .sampling import (  # noqa: F401
     categorical,
     greedy_accept,
     greedy_accept_batched,
+    greedy_tree_accept,
     merge_random_round,
     propose_drafts,
     RandomRoundMerge,
@@ -46,13 +50,19 @@ from .sampling import (  # noqa: F401
     rejection_rows,
     rejection_sample,
     speculative_accept,
+    token_logprobs,
+    TokenLogprobs,
+    tree_accept,
+    TreeAcceptResult,
     verify_accept,
     verify_distributions,
 )
 from .kv_write import (  # noqa: F401
+    commit_tree_kv,
     finalize_rows,
     masked_kv_store,
     store_fp8,
     store_kv,
     write_graph_kv,
 )
+from .routing import tree_masks  # noqa: F401

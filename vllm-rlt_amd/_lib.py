@@ -139,6 +139,19 @@ _SIGNATURES = {
         _p, _p, _p, _p, _sz, _p]),
     "rlt_greedy_accept": (ctypes.c_int, [
         _p, _p, _p, _i32, _i64, _i64, _i32, _i64, _p, _p, _p, _p]),
+    "rlt_greedy_tree_accept_workspace_size": (_sz, [_i64, _i32, _i64]),
+    "rlt_greedy_tree_accept": (ctypes.c_int, [
+        _p, _p, _p, _p, _i32, _i64, _i64, _i32, _i64, _p, _p, _p, _p, _p, _sz, _p]),
+    "rlt_tree_accept_workspace_size": (_sz, [_i64, _i32, _i64]),
+    "rlt_tree_accept": (ctypes.c_int, [
+        _p, _p, _p, _p, _p, _p, _p, _i64, _i32, _i64, _p, _p, _p, _p, _p, _p, _sz, _p]),
+    "rlt_token_logprobs_workspace_size": (_sz, [_i64, _i64, _i32]),
+    "rlt_token_logprobs": (ctypes.c_int, [
+        _p, _i32, _i64, _i64, _i64, _p, _p, _i64, _i32, _p, _p, _p, _p, _p, _p, _sz, _p]),
+    "rlt_kv_commit_path": (ctypes.c_int, [
+        _p, _i64, _i32, _i32, _i32, _p, _p, _i64, _i32, _p, _i32, _i64, _p, _p, _i64, _i64, _i64,
+        _i64, _i32, _p]),
+    "rlt_tree_masks": (ctypes.c_int, [_p, _i64, _i32, _p, _i32, _p, _i32, _i64, _p]),
     "rlt_kv_store": (ctypes.c_int, [
         _p, _p, _i64, _i64, _i64, _i64, _p, _p, _i64, _i64, _i64, _i64, _i32,
         _p, _p, _p, _p, _i64, _i32, _i32, _i32, _p]),

@@ -184,7 +184,7 @@ class MI355XPagedAttention:
         already in the cache at its last positions: node j at ``context_lengths[s] - nodes +
         j``.  A row sees the whole prefix before node 0 and the nodes of its own tree whose bit
         is set in its ``tree_mask`` row (int64 ``[q rows, words]``, bit ``j % 64`` of word
-        ``j // 64``; ``sampling.tree_masks`` makes a node's ancestors and itself from the
+        ``j // 64``; ``routing.tree_masks`` makes a node's ancestors and itself from the
         parents), with ``window > 0`` the last ``window`` of those positions.  A row that sees
         nothing gives zeros; what a row does not see has no effect on it, whatever it holds.
         The pool is of q's type, or float8_e4m3fn with per-tensor or per-vector scales.

@@ -19,7 +19,7 @@ BUILD = os.path.join(HERE, "_build")
 LIB = os.path.join(HERE, "librlt_mi355x.so")
 OPS_LIB = os.path.join(HERE, "_C.so")
 SOURCES = ["paged_attention.hip", "spec_sampling.hip", "probabilities.hip", "kv_write.hip", "routing.hip",
-           "tree_attention.hip"]
+           "tree_attention.hip", "tree_accept.hip", "logprobs.hip"]
 
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 FLAGS = [

@@ -157,6 +157,73 @@ inline int elt_size(int dtype) {
   return dtype == RLT_F32 ? 4 : dtype == RLT_FP8_E4M3 ? 1 : 2;
 }
 
+// The accepted path of a draft tree moves behind the prefix: for accepted node j = 1 ..
+// accepted[r], the bytes at position start + path[j] go to position start + j, in every layer
+// of both pools.  A path ascends, so path[j] >= j: a thread that takes one 16-byte column of a
+// layer through the moves in order never overwrites a source that it still needs, in place
+// and without a second buffer; eight moves are loaded before the first is stored.  Copied
+// bytes bound it (at few requests the chain of loads path -> table -> pool).
+constexpr int kMaxPath = 255;
+constexpr int kMovesAhead = 8;
+
+template <int UNIT>
+struct CopyUnit;
+template <> struct CopyUnit<16> { typedef uint4 T; };
+template <> struct CopyUnit<4> { typedef uint32_t T; };
+template <> struct CopyUnit<1> { typedef uint8_t T; };
+
+template <int UNIT>
+__global__ __launch_bounds__(256) void rlt_kv_commit_kernel(
+    const int32_t* __restrict__ tables, int32_t planes, int32_t width, int32_t block_size,
+    const int64_t* __restrict__ starts, const int64_t* __restrict__ path, int64_t path_stride,
+    int32_t path_width, const int64_t* __restrict__ accepted, int32_t layers, int64_t num_blocks,
+    uint8_t* __restrict__ key_pool, uint8_t* __restrict__ value_pool, int64_t bs, int64_t ls,
+    int64_t ts, int64_t row_bytes) {
+  typedef typename CopyUnit<UNIT>::T T;
+  __shared__ int64_t from[kMaxPath], to[kMaxPath];  // byte offsets within a layer of the pool
+  const int64_t r = blockIdx.x / planes;
+  const int plane = (int)(blockIdx.x % planes);
+  const int layer = (int)(blockIdx.y >> 1);
+  uint8_t* const pool = (blockIdx.y & 1 ? value_pool : key_pool) + layer * ls;
+  const int64_t a = accepted[r];
+  const int count = (int)(a < 0 ? 0 : a > path_width - 1 ? path_width - 1 : a);
+  if (count == 0) return;
+  const int t = threadIdx.x;
+  if (t < count) {
+    // (blocks of 256 threads hold the longest path)
+    const int64_t start = starts[r], node = path[r * path_stride + t + 1];
+    const int32_t* const table = tables + (r * planes + plane) * (int64_t)width;
+    int64_t f = -1, g = -1;
+    const int64_t src = start + node, dst = start + t + 1;
+    if (start >= 0 && node > t + 1 && node <= kMaxPath && dst / block_size < width &&
+        src / block_size < width) {
+      const int64_t sb = table[src / block_size], db = table[dst / block_size];
+      if (sb >= 0 && sb < num_blocks && db >= 0 && db < num_blocks) {
+        f = sb * bs + (src % block_size) * ts;
+        g = db * bs + (dst % block_size) * ts;
+      }
+    }
+    from[t] = f;
+    to[t] = g;
+  }
+  __syncthreads();
+  const int64_t units = row_bytes / UNIT;
+  for (int64_t c = (int64_t)blockIdx.z * 256 + t; c < units; c += (int64_t)gridDim.z * 256) {
+    uint8_t* const col = pool + c * UNIT;
+    for (int j = 0; j < count; j += kMovesAhead) {
+      T x[kMovesAhead];
+#pragma unroll
+      for (int i = 0; i < kMovesAhead; ++i) {
+        x[i] = T{};
+        if (j + i < count && from[j + i] >= 0) x[i] = *(const T*)(col + from[j + i]);
+      }
+#pragma unroll
+      for (int i = 0; i < kMovesAhead; ++i)
+        if (j + i < count && from[j + i] >= 0) *(T*)(col + to[j + i]) = x[i];
+    }
+  }
+}
+
 }  // namespace
 
 extern "C" {
@@ -254,6 +321,38 @@ int rlt_kv_finalize(const int64_t* descriptors, int64_t count, const int32_t* ta
   hipLaunchKernelGGL(rlt_kv_finalize_kernel, grid, dim3(256), 0, stream, descriptors, tables,
                      slots, width, planes, block_size, layers, num_blocks, (uint8_t*)key_pool,
                      (uint8_t*)value_pool, bs, ls, ts, bytes_per_token, unit);
+  return rlt_launch_status();
+}
+
+int rlt_kv_commit_path(const int32_t* tables, int64_t n, int32_t planes, int32_t width,
+                       int32_t block_size, const int64_t* starts, const int64_t* path,
+                       int64_t path_stride, int32_t path_width, const int64_t* accepted,
+                       int32_t layers, int64_t num_blocks, void* key_pool, void* value_pool,
+                       int64_t block_stride, int64_t layer_stride, int64_t token_stride,
+                       int64_t bytes_per_token, int32_t elt_bytes, hipStream_t stream) {
+  if (n < 0 || planes < 1 || width < 0 || block_size < 1 || path_width < 0 || layers < 1 ||
+      num_blocks < 0 || bytes_per_token < 1 || elt_bytes < 1 || (n > 1 && path_stride < path_width))
+    return RLT_ERR_ARGUMENT;
+  if (path_width > kMaxPath + 1 || layers > 32767 || n * planes > 0x7fffffff)
+    return RLT_ERR_UNSUPPORTED;
+  if (n == 0 || path_width < 2 || width == 0) return RLT_OK;
+  if (!tables || !starts || !path || !accepted || !key_pool || !value_pool) return RLT_ERR_ARGUMENT;
+  const int64_t bs = block_stride * elt_bytes, ls = layer_stride * elt_bytes,
+                ts = token_stride * elt_bytes;
+  const int64_t all = bs | ls | ts | bytes_per_token | (int64_t)(uintptr_t)key_pool |
+                      (int64_t)(uintptr_t)value_pool;
+  const int unit = all % 16 == 0 ? 16 : all % 4 == 0 ? 4 : 1;
+  const int64_t wgs = (bytes_per_token / unit + 255) / 256;
+  const dim3 grid((unsigned)(n * planes), (unsigned)(2 * layers), (unsigned)(wgs > 64 ? 64 : wgs));
+#define RLT_COMMIT(U)                                                                            \
+  hipLaunchKernelGGL(rlt_kv_commit_kernel<U>, grid, dim3(256), 0, stream, tables, planes, width, \
+                     block_size, starts, path, path_stride, path_width, accepted, layers,        \
+                     num_blocks, (uint8_t*)key_pool, (uint8_t*)value_pool, bs, ls, ts,           \
+                     bytes_per_token)
+  if (unit == 16) RLT_COMMIT(16);
+  else if (unit == 4) RLT_COMMIT(4);
+  else RLT_COMMIT(1);
+#undef RLT_COMMIT
   return rlt_launch_status();
 }
 

@@ -13,6 +13,7 @@
 //  * rlt_expand_kv_kernel         -- vllm_rlt/kernels/metadata.py:7-24 expand_kv_addresses
 //  * rlt_depth_tables_kernel      -- the per-row depth-table gather of
 //                                    vllm_rlt/worker/async_speculative.py:449-470
+//  * rlt_tree_masks_kernel        -- the ancestor masks of draft trees (no counterpart)
 //
 // Every index read from memory (slot, plane, position, segment bounds) is checked
 // against the buffer it addresses: an out-of-range gather source reads zeros, an
@@ -177,6 +178,35 @@ inline bool grid_ok(int64_t x, int64_t y, int64_t z = 1) {
   return x > 0 && x <= 0x7fffffff && y > 0 && y <= 65535 && z > 0 && z <= 65535;
 }
 
+// Mask rows of draft trees: node i of sequence s (q row cu[s] + i) sees itself and its
+// ancestors.  One thread per row walks the parents up to the root, node 0.
+__global__ __launch_bounds__(kThreads) void rlt_tree_masks_kernel(
+    const int64_t* __restrict__ parents, int64_t parent_stride, int width,
+    const int32_t* __restrict__ cu, int num_seqs, uint64_t* __restrict__ mask, int words,
+    int64_t rows) {
+  const int64_t row = (int64_t)blockIdx.x * kThreads + threadIdx.x;
+  if (row >= rows) return;
+  uint64_t* const out = mask + row * words;
+  for (int w = 0; w < words; ++w) out[w] = 0;
+  // the last sequence that begins at or before the row (empty ones begin there too)
+  int lo = 0, hi = num_seqs;  // cu[lo] <= row is kept, cu[hi] > row or hi == num_seqs
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (cu[mid] <= row) lo = mid;
+    else hi = mid;
+  }
+  if (num_seqs == 0 || row < cu[lo] || row >= cu[lo + 1]) return;  // in no sequence
+  const int64_t* const up = parents + lo * parent_stride;
+  int64_t node = row - cu[lo];
+  for (;;) {
+    if (node < 64 * (int64_t)words) out[node >> 6] |= 1ull << (node & 63);
+    if (node == 0 || node > width) break;
+    const int64_t p = up[node - 1];
+    if (p < 0 || p >= node) break;  // no earlier node: the walk ends
+    node = p;
+  }
+}
+
 }  // namespace
 
 extern "C" {
@@ -326,6 +356,20 @@ int rlt_depth_tables(const int32_t* tables, int64_t row_stride, int64_t plane_st
   hipLaunchKernelGGL(rlt_depth_tables_kernel, dim3((unsigned)n), dim3(kThreads), 0, stream,
                      tables, row_stride, plane_stride, planes, width, depth, positions, active,
                      block_size, out_table, out_stride, blocks, offsets, lengths);
+  return rlt_launch_status();
+}
+
+int rlt_tree_masks(const int64_t* parents, int64_t parent_stride, int32_t width,
+                   const int32_t* cu_seqlens_q, int32_t num_seqs, int64_t* mask, int32_t words,
+                   int64_t rows, hipStream_t stream) {
+  if (width < 0 || num_seqs < 0 || words < 1 || rows < 0 || (num_seqs > 1 && parent_stride < width))
+    return RLT_ERR_ARGUMENT;
+  if (rows == 0) return RLT_OK;
+  if (!cu_seqlens_q || !mask || (width && num_seqs && !parents)) return RLT_ERR_ARGUMENT;
+  if (rows > 0x7fffffffLL * kThreads) return RLT_ERR_UNSUPPORTED;
+  hipLaunchKernelGGL(rlt_tree_masks_kernel, dim3((unsigned)((rows + kThreads - 1) / kThreads)),
+                     dim3(kThreads), 0, stream, parents, parent_stride, width, cu_seqlens_q,
+                     num_seqs, (uint64_t*)mask, words, rows);
   return rlt_launch_status();
 }
 

@@ -717,6 +717,189 @@ Tensor tree_attention(const Tensor& q, const Tensor& key_cache, const Tensor& va
   return output;
 }
 
+void check_tree(const Tensor& draft_tokens, const Tensor& parents, const Tensor& drafts) {
+  TORCH_CHECK_VALUE(draft_tokens.dim() == 2 && parents.sizes() == draft_tokens.sizes(),
+                    "draft_tokens and parents must be [n, W]");
+  TORCH_CHECK_VALUE(drafts.sizes() == at::IntArrayRef{draft_tokens.size(0)}, "drafts must be [n]");
+  TORCH_CHECK_VALUE(draft_tokens.size(1) <= 255, "at most 255 drafts per tree are supported");
+}
+
+constexpr int64_t kTreeVocab = 1 << 20;
+
+// Greedy acceptance along draft trees (rlt_greedy_tree_accept).
+std::tuple<Tensor, Tensor, Tensor, Tensor> greedy_tree_accept(const Tensor& draft_tokens,
+                                                              const Tensor& parents,
+                                                              const Tensor& drafts,
+                                                              const Tensor& target_logits) {
+  check_tree(draft_tokens, parents, drafts);
+  const int64_t n = draft_tokens.size(0), w = draft_tokens.size(1);
+  TORCH_CHECK_VALUE(target_logits.dim() == 3 && target_logits.size(0) == n &&
+                        target_logits.size(1) == w + 1,
+                    "target_logits must be [n, W + 1, V]");
+  const int64_t vocab = target_logits.size(2);
+  TORCH_CHECK_VALUE(vocab >= 1 && vocab <= kTreeVocab, "V must be between 1 and 2^20");
+  same_device(target_logits, draft_tokens, parents, drafts);
+  logit_rows(target_logits, "target_logits");
+  TORCH_CHECK_VALUE(n <= 1 || target_logits.stride(0) == (w + 1) * target_logits.stride(1),
+                    "target_logits rows of a request must be evenly strided ([n * (W + 1), V] view)");
+  TORCH_CHECK_VALUE(n * (w + 1) <= 1 || target_logits.stride(1) >= vocab,
+                    "target_logits rows must not overlap");
+  need(draft_tokens, at::kLong, "draft_tokens");
+  need(parents, at::kLong, "parents");
+  need(drafts, at::kLong, "drafts");
+  const auto i64 = draft_tokens.options();
+  const c10::hip::HIPGuardMasqueradingAsCUDA guard(target_logits.device());
+  Tensor targets = at::empty({n, w + 1}, i64), path = at::empty({n, w + 1}, i64);
+  Tensor accepted = at::empty({n}, i64), next = at::empty({n}, i64);
+  if (n == 0) return {targets, path, accepted, next};
+  const Tensor ws = workspace(rlt_greedy_tree_accept_workspace_size(n, (int32_t)w, vocab), drafts);
+  const int status = rlt_greedy_tree_accept(
+      (const int64_t*)ptr(draft_tokens), (const int64_t*)ptr(parents), (const int64_t*)ptr(drafts),
+      ptr(target_logits), dtype_code(target_logits.scalar_type()),
+      n * (w + 1) > 1 ? target_logits.stride(1) : vocab, n, (int32_t)w, vocab,
+      (int64_t*)ptr(targets), (int64_t*)ptr(path), (int64_t*)ptr(accepted), (int64_t*)ptr(next),
+      ptr(ws), ws.numel(), stream_of(target_logits));
+  check_status(status, "rlt_greedy_tree_accept");
+  return {targets, path, accepted, next};
+}
+
+// Sampled acceptance along draft trees (rlt_tree_accept).
+std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> tree_accept(
+    const Tensor& draft_tokens, const Tensor& parents, const Tensor& drafts, const Tensor& q,
+    const Tensor& p, const Tensor& u_accept, const Tensor& u_final) {
+  check_tree(draft_tokens, parents, drafts);
+  const int64_t n = draft_tokens.size(0), w = draft_tokens.size(1), vocab = p.size(-1);
+  TORCH_CHECK_VALUE(p.sizes() == at::IntArrayRef({n, w + 1, vocab}) &&
+                        q.sizes() == at::IntArrayRef({n, w, vocab}),
+                    "q must be [n, W, V] and p [n, W + 1, V]");
+  TORCH_CHECK_VALUE(u_accept.sizes() == at::IntArrayRef({n, w}) &&
+                        u_final.sizes() == at::IntArrayRef{n},
+                    "u_accept must be [n, W] and u_final [n]");
+  TORCH_CHECK_VALUE(vocab >= 1 && vocab <= kTreeVocab, "V must be between 1 and 2^20");
+  same_device(p, draft_tokens, parents, drafts, q, u_accept, u_final);
+  need(draft_tokens, at::kLong, "draft_tokens");
+  need(parents, at::kLong, "parents");
+  need(drafts, at::kLong, "drafts");
+  need(q, at::kFloat, "q");
+  need(p, at::kFloat, "p");
+  need(u_accept, at::kFloat, "u_accept");
+  need(u_final, at::kFloat, "u_final");
+  const auto i64 = draft_tokens.options();
+  const c10::hip::HIPGuardMasqueradingAsCUDA guard(p.device());
+  Tensor path = at::empty({n, w + 1}, i64), tokens = at::empty({n, w + 1}, i64);
+  Tensor accepted = at::empty({n}, i64), final_token = at::empty({n}, i64);
+  Tensor error = at::empty({n}, i64.dtype(at::kBool));
+  if (n == 0) return {path, tokens, accepted, final_token, error};
+  const Tensor ws = workspace(rlt_tree_accept_workspace_size(n, (int32_t)w, vocab), p);
+  const int status = rlt_tree_accept(
+      (const int64_t*)ptr(draft_tokens), (const int64_t*)ptr(parents), (const int64_t*)ptr(drafts),
+      (const float*)ptr(q), (const float*)ptr(p), (const float*)ptr(u_accept),
+      (const float*)ptr(u_final), n, (int32_t)w, vocab, (int64_t*)ptr(path), (int64_t*)ptr(tokens),
+      (int64_t*)ptr(accepted), (int64_t*)ptr(final_token), (uint8_t*)ptr(error), ptr(ws),
+      ws.numel(), stream_of(p));
+  check_status(status, "rlt_tree_accept");
+  return {path, tokens, accepted, final_token, error};
+}
+
+// Log probabilities of given tokens (rlt_token_logprobs).
+std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> token_logprobs(const Tensor& logits,
+                                                                  const Tensor& tokens,
+                                                                  const OptTensor& rows,
+                                                                  int64_t top_n) {
+  TORCH_CHECK_VALUE(logits.dim() == 2 && tokens.dim() == 1, "logits must be [m, V] and tokens [r]");
+  const int64_t m = logits.size(0), vocab = logits.size(1), count = tokens.size(0);
+  TORCH_CHECK_VALUE(vocab >= 1 && vocab <= kTreeVocab, "V must be between 1 and 2^20");
+  TORCH_CHECK_VALUE(top_n >= 0 && top_n <= 64 && top_n <= vocab,
+                    "top_n must be between 0 and min(64, V)");
+  TORCH_CHECK_VALUE(rows.has_value() ? rows->dim() == 1 && rows->size(0) == count : count == m,
+                    "rows must be [r]; without it there is one token per logit row");
+  same_device(logits, tokens, rows);
+  logit_rows(logits, "logits");
+  TORCH_CHECK_VALUE(m <= 1 || logits.stride(0) >= vocab, "logits rows must not overlap");
+  need(tokens, at::kLong, "tokens");
+  need(rows, at::kLong, "rows");
+  const auto i64 = tokens.options(), f32 = tokens.options().dtype(at::kFloat);
+  const c10::hip::HIPGuardMasqueradingAsCUDA guard(logits.device());
+  Tensor logprob = at::empty({count}, f32), rank = at::empty({count}, i64);
+  Tensor entropy = at::empty({count}, f32), top_logprob = at::empty({count, top_n}, f32);
+  Tensor top_tokens = at::empty({count, top_n}, i64);
+  // (a launch takes 65535 rows)
+  for (int64_t at = 0; at < count; at += 65535) {
+    const int64_t part = std::min<int64_t>(count - at, 65535);
+    const Tensor ws = workspace(rlt_token_logprobs_workspace_size(part, vocab, (int32_t)top_n), tokens);
+    const int64_t elt = logits.element_size();
+    const int status = rlt_token_logprobs(
+        rows.has_value() ? ptr(logits) : (char*)ptr(logits) + at * logits.stride(0) * elt,
+        dtype_code(logits.scalar_type()), m > 1 ? logits.stride(0) : vocab,
+        rows.has_value() ? m : part, vocab,
+        rows.has_value() ? (const int64_t*)ptr(rows) + at : nullptr,
+        (const int64_t*)ptr(tokens) + at, part, (int32_t)top_n, (float*)ptr(logprob) + at,
+        (int64_t*)ptr(rank) + at, (float*)ptr(entropy) + at, (float*)ptr(top_logprob) + at * top_n,
+        (int64_t*)ptr(top_tokens) + at * top_n, ptr(ws), ws.numel(), stream_of(logits));
+    check_status(status, "rlt_token_logprobs");
+  }
+  return {logprob, rank, entropy, top_logprob, top_tokens};
+}
+
+// The accepted paths' keys and values to their places (rlt_kv_commit_path).
+void commit_tree_kv(const Tensor& key_pool, const Tensor& value_pool, const Tensor& tables,
+                    const Tensor& starts, const Tensor& path, const Tensor& accepted,
+                    int64_t block_size) {
+  TORCH_CHECK_VALUE(key_pool.dim() >= 3 && key_pool.sizes() == value_pool.sizes() &&
+                        key_pool.strides() == value_pool.strides() &&
+                        key_pool.scalar_type() == value_pool.scalar_type(),
+                    "key and value pools must be [block, layer, token, ...] of one layout and dtype");
+  TORCH_CHECK_VALUE(block_size >= 1 && key_pool.size(2) == block_size,
+                    "the pools' blocks must hold block_size tokens");
+  int64_t per_token = 1;
+  for (int64_t d = key_pool.dim() - 1; d >= 3; --d) {
+    TORCH_CHECK_VALUE(key_pool.size(d) <= 1 || key_pool.stride(d) == per_token,
+                      "the per-token channels of the pools must be contiguous");
+    per_token *= key_pool.size(d);
+  }
+  TORCH_CHECK_VALUE((tables.dim() == 2 || tables.dim() == 3) && tables.size(0) == path.size(0),
+                    "tables must be [n, width] or [n, planes, width]");
+  TORCH_CHECK_VALUE(path.dim() == 2 && path.size(1) <= 256 && starts.dim() == 1 &&
+                        accepted.dim() == 1 && starts.size(0) == path.size(0) &&
+                        accepted.size(0) == path.size(0),
+                    "path must be [n, W + 1] with W <= 255, starts and accepted [n]");
+  same_device(key_pool, value_pool, tables, starts, path, accepted);
+  need(tables, at::kInt, "tables");
+  need(starts, at::kLong, "starts");
+  need(path, at::kLong, "path");
+  need(accepted, at::kLong, "accepted");
+  const int64_t n = path.size(0), planes = tables.dim() == 3 ? tables.size(1) : 1;
+  if (n == 0 || planes == 0 || per_token == 0 || key_pool.size(1) == 0 || tables.size(-1) == 0) return;
+  const c10::hip::HIPGuardMasqueradingAsCUDA guard(key_pool.device());
+  const int status = rlt_kv_commit_path(
+      (const int32_t*)ptr(tables), n, (int32_t)planes, (int32_t)tables.size(-1),
+      (int32_t)block_size, (const int64_t*)ptr(starts), (const int64_t*)ptr(path), path.size(1),
+      (int32_t)path.size(1), (const int64_t*)ptr(accepted), (int32_t)key_pool.size(1),
+      key_pool.size(0), ptr(key_pool), ptr(value_pool), key_pool.stride(0), key_pool.stride(1),
+      key_pool.stride(2), per_token * key_pool.element_size(), (int32_t)key_pool.element_size(),
+      stream_of(key_pool));
+  check_status(status, "rlt_kv_commit_path");
+}
+
+// Ancestor masks of draft trees (rlt_tree_masks).
+Tensor tree_masks(const Tensor& parents, const Tensor& cu_seqlens_q, int64_t rows) {
+  TORCH_CHECK_VALUE(parents.dim() == 2 && parents.size(1) <= 255, "parents must be [n, W], W <= 255");
+  TORCH_CHECK_VALUE(cu_seqlens_q.dim() == 1 && cu_seqlens_q.size(0) == parents.size(0) + 1,
+                    "cu_seqlens_q must be [n + 1]");
+  TORCH_CHECK_VALUE(rows >= 0, "rows must be nonnegative");
+  same_device(parents, cu_seqlens_q);
+  need(parents, at::kLong, "parents");
+  need(cu_seqlens_q, at::kInt, "cu_seqlens_q");
+  const int64_t width = parents.size(1), words = (width + 64) / 64;
+  const c10::hip::HIPGuardMasqueradingAsCUDA guard(parents.device());
+  Tensor mask = at::empty({rows, words}, parents.options());
+  const int status = rlt_tree_masks((const int64_t*)ptr(parents), width, (int32_t)width,
+                                    (const int32_t*)ptr(cu_seqlens_q), (int32_t)parents.size(0),
+                                    (int64_t*)ptr(mask), (int32_t)words, rows, stream_of(parents));
+  check_status(status, "rlt_tree_masks");
+  return mask;
+}
+
 }  // namespace
 
 TORCH_LIBRARY(rlt_mi355x, m) {
@@ -744,6 +927,15 @@ TORCH_LIBRARY(rlt_mi355x, m) {
   m.def("tree_attention(Tensor q, Tensor key_cache, Tensor value_cache, Tensor block_tables, "
         "Tensor context_lengths, Tensor cu_seqlens_q, int max_seqlen_q, Tensor tree_mask, "
         "Tensor? key_scale=None, Tensor? value_scale=None, int window=0) -> Tensor");
+  m.def("tree_masks(Tensor parents, Tensor cu_seqlens_q, int rows) -> Tensor");
+  m.def("greedy_tree_accept(Tensor draft_tokens, Tensor parents, Tensor drafts, "
+        "Tensor target_logits) -> (Tensor, Tensor, Tensor, Tensor)");
+  m.def("tree_accept(Tensor draft_tokens, Tensor parents, Tensor drafts, Tensor q, Tensor p, "
+        "Tensor u_accept, Tensor u_final) -> (Tensor, Tensor, Tensor, Tensor, Tensor)");
+  m.def("token_logprobs(Tensor logits, Tensor tokens, Tensor? rows=None, int top_n=0) "
+        "-> (Tensor, Tensor, Tensor, Tensor, Tensor)");
+  m.def("commit_tree_kv(Tensor(a!) key_pool, Tensor(b!) value_pool, Tensor tables, Tensor starts, "
+        "Tensor path, Tensor accepted, int block_size) -> ()");
 }
 
 TORCH_LIBRARY_IMPL(rlt_mi355x, CUDA, m) {
@@ -757,4 +949,9 @@ TORCH_LIBRARY_IMPL(rlt_mi355x, CUDA, m) {
   m.impl("verify_accept", &verify_accept);
   m.impl("paged_attention_store", &paged_attention_store);
   m.impl("tree_attention", &tree_attention);
+  m.impl("tree_masks", &tree_masks);
+  m.impl("greedy_tree_accept", &greedy_tree_accept);
+  m.impl("tree_accept", &tree_accept);
+  m.impl("token_logprobs", &token_logprobs);
+  m.impl("commit_tree_kv", &commit_tree_kv);
 }

@@ -1,0 +1,411 @@
+// Acceptance along a tree of drafted tokens, greedy and sampled, for MI355X (gfx950).
+//
+// Node 0 of a request is its last committed token, node j + 1 draft j, whose parent is an
+// earlier node.  Both walks start at node 0 and end where no child is accepted.  A child has
+// a larger index than its parent and siblings come in index order, so one scan of the drafts
+// in index order is the whole walk.
+//
+// Greedy: the child that holds the node's argmax token (the first, of several).  All logit
+// rows' argmaxes are formed by row slices (the targets are an output), then one workgroup per
+// request joins its slices and walks.
+//
+// Sampled: at a node the children are tried in order, each drawn from the draft distribution
+// q of the node.  With y the weights left of the target distribution p (at first y = p) and
+// R = sum y (p counts as 1), a child of token t is accepted when u R q(t) < y(t); a rejected
+// one leaves y' = max(y - R q, 0).  Since y only shrinks where it is positive, after k
+// rejections y = max(p - C q, 0) with C = R_0 + .. + R_(k-1): no residual is stored, and a
+// rejection costs one sum over the node's two rows.  Where no child is left the next token is
+// drawn from y by inverse CDF.  The emitted tokens follow p whatever q and the tree are.
+// Sums, weights and the CDF are float64: one workgroup per request, each thread 16
+// consecutive columns at a time; the wave sums of the last pass are the CDF's coarse table.
+
+#include "vocab_rows.h"
+
+#include "rlt_mi355x.h"
+
+#include <math.h>
+
+namespace {
+
+using namespace vocab;
+
+constexpr int kMaxDrafts = 255;
+constexpr int64_t kMaxVocab = 1 << 20;
+constexpr int kSliceEpt = 32;
+
+// ---------------------------------------------------------------- greedy
+
+template <int DT>
+__global__ __launch_bounds__(kThreads) void rlt_tree_argmax_kernel(const void* logits, int64_t row_stride,
+                                                                  int64_t vocab, int slices,
+                                                                  unsigned long long* best) {
+  __shared__ unsigned long long sh[4];
+  using S = Slice<DT, kSliceEpt>;
+  constexpr int ELT = DT == RLT_F32 ? 4 : 2;
+  const int64_t row = blockIdx.x / slices;
+  const int slice = (int)(blockIdx.x % slices);
+  const int64_t begin = (int64_t)slice * kSliceEpt * kThreads;
+  S x;
+  x.load((const uint8_t*)logits + row * row_stride * ELT, begin, vocab);
+  // columns ascend within a thread: the first of the largest keys
+  uint32_t key = 0, at = 0;
+#pragma unroll
+  for (int i = 0; i < S::NP; ++i) {
+    const int64_t c = S::column(begin, i);
+#pragma unroll
+    for (int e = 0; e < S::VE; ++e) {
+      const uint32_t k = c + e < vocab ? order_key(x.at(i, e)) : 0u;
+      at = k > key ? (uint32_t)(c + e) : at;
+      key = k > key ? k : key;
+    }
+  }
+  unsigned long long m = wave_max(key ? composite(key, at) : 0ull);
+  if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = m;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int i = 1; i < 4; ++i) m = sh[i] > m ? sh[i] : m;
+    best[blockIdx.x] = m;
+  }
+}
+
+__global__ __launch_bounds__(kThreads) void rlt_greedy_tree_kernel(
+    const unsigned long long* best, int slices, const int64_t* draft_tokens, const int64_t* parents,
+    const int64_t* drafts, int width, int64_t* targets, int64_t* path, int64_t* accepted,
+    int64_t* next_token) {
+  __shared__ int64_t target[kMaxDrafts + 1];
+  __shared__ int walk[kMaxDrafts + 1];
+  const int64_t r = blockIdx.x;
+  const int t = threadIdx.x, lane = t & 63, nodes = width + 1;
+  // node i's argmax: one lane group of 16 per node
+  for (int i = t >> 4; i < nodes; i += kThreads / 16) {
+    unsigned long long m = 0;
+    for (int s = t & 15; s < slices; s += 16) {
+      const unsigned long long c = best[(r * nodes + i) * slices + s];
+      m = c > m ? c : m;
+    }
+#pragma unroll
+    for (int o = 8; o >= 1; o >>= 1) {
+      const unsigned long long c = __shfl_xor(m, o, RLT_WAVE);
+      m = c > m ? c : m;
+    }
+    if ((t & 15) == 0) {
+      target[i] = composite_col(m);
+      targets[r * nodes + i] = target[i];
+    }
+  }
+  __syncthreads();
+  if (t >= 64) return;
+  // one wave walks: lane holds drafts lane, lane + 64, ..
+  const int64_t d = drafts[r];
+  const int live = (int)(d < 0 ? 0 : d > width ? width : d);
+  int64_t token[4], parent[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const int j = lane + 64 * k;
+    token[k] = j < live ? draft_tokens[r * width + j] : -1;
+    parent[k] = j < live ? parents[r * width + j] : -1;
+  }
+  int node = 0, count = 0;
+  for (;;) {
+    int next = -1;
+#pragma unroll
+    for (int k = 3; k >= 0; --k) {
+      // (a child comes after its parent: a larger index)
+      const bool hit = lane + 64 * k >= node && parent[k] == node && token[k] == target[node];
+      const uint64_t b = __builtin_amdgcn_ballot_w64(hit);
+      if (b) next = 64 * k + __builtin_ctzll(b);
+    }
+    if (next < 0) break;
+    node = next + 1;
+    ++count;
+    if (lane == 0) walk[count] = node;
+  }
+  if (lane == 0) walk[0] = 0;
+  __builtin_amdgcn_wave_barrier();
+  for (int i = lane; i < nodes; i += 64) path[r * nodes + i] = i <= count ? walk[i] : -1;
+  if (lane == 0) {
+    accepted[r] = count;
+    next_token[r] = target[node];
+  }
+}
+
+// ---------------------------------------------------------------- sampled
+
+constexpr int kAccThreads = 1024;
+constexpr int kAccWaves = kAccThreads / 64;
+constexpr int kRun = 16;                           // consecutive columns of a thread
+constexpr int64_t kStep = (int64_t)kAccThreads * kRun;
+constexpr int kMaxSegments = (int)(kMaxVocab / kStep) * kAccWaves;
+
+struct AcceptShared {
+  double seg[kMaxSegments];  // weight of every wave's kRun * 64 columns, in column order
+  float px[kMaxDrafts], qx[kMaxDrafts];
+  int32_t parent[kMaxDrafts];
+  int64_t token[kMaxDrafts];
+  int32_t walk[kMaxDrafts + 1];  // the accepted path
+  int64_t last;
+};
+
+// y = max(p - C q, 0), NaN kept
+__device__ __forceinline__ double left_of(float p, float q, double C) {
+  const double y = (double)p - C * (double)q;
+  return y < 0.0 ? 0.0 : y;
+}
+
+struct __attribute__((packed, aligned(4))) Quad {
+  float v[4];
+};
+
+// Segment weights of a node's rows for C; q is not read for C = 0.
+__device__ __forceinline__ void weigh(AcceptShared& sh, const float* p, const float* q, double C,
+                                      int64_t vocab) {
+  const int t = threadIdx.x, w = t >> 6;
+  const bool plain = C == 0.0;
+  int step = 0;
+  for (int64_t base = 0; base < vocab; base += kStep, ++step) {
+    const int64_t c = base + (int64_t)t * kRun;
+    double s = 0.0;
+    if (c + kRun <= vocab) {
+      Quad a[kRun / 4], b[kRun / 4];
+#pragma unroll
+      for (int i = 0; i < kRun / 4; ++i) a[i] = *(const Quad*)(p + c + 4 * i);
+      if (!plain) {
+#pragma unroll
+        for (int i = 0; i < kRun / 4; ++i) b[i] = *(const Quad*)(q + c + 4 * i);
+      } else {
+#pragma unroll
+        for (int i = 0; i < kRun / 4; ++i) b[i] = Quad{{0.f, 0.f, 0.f, 0.f}};
+      }
+#pragma unroll
+      for (int i = 0; i < kRun / 4; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s += left_of(a[i].v[e], b[i].v[e], C);
+    } else {
+      for (int i = 0; i < kRun; ++i)
+        if (c + i < vocab) s += left_of(p[c + i], plain ? 0.f : q[c + i], C);
+    }
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) s += __shfl_xor(s, o, RLT_WAVE);
+    if ((t & 63) == 0) sh.seg[step * kAccWaves + w] = s;
+  }
+  __syncthreads();
+}
+
+__device__ __forceinline__ double wave_incl(double x) {
+  const int lane = threadIdx.x & 63;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const double y = __shfl_up(x, o, RLT_WAVE);
+    if (lane >= o) x += y;
+  }
+  return x;
+}
+
+// Exclusive weights before each lane's run of segments, and their total (every wave alike).
+__device__ __forceinline__ double segment_scan(const AcceptShared& sh, int segments, double& before) {
+  const int lane = threadIdx.x & 63, per = (segments + 63) / 64;
+  double mine = 0.0;
+  for (int i = 0; i < per; ++i)
+    if (lane * per + i < segments) mine += sh.seg[lane * per + i];
+  const double incl = wave_incl(mine);
+  before = __shfl_up(incl, 1, RLT_WAVE);
+  if (lane == 0) before = 0.0;
+  return __shfl(incl, 63, RLT_WAVE);
+}
+
+// The first column whose running weight passes `target` (one wave).
+__device__ __forceinline__ int64_t draw(const AcceptShared& sh, const float* p, const float* q, double C,
+                                        int64_t vocab, int segments, double before, double target) {
+  const int lane = threadIdx.x & 63, per = (segments + 63) / 64;
+  // the last segment with weight at or before the target's: rounding may leave the running
+  // weight's end short of it
+  int seg = -1;
+  double at = 0.0, run = before;
+  for (int i = 0; i < per; ++i) {
+    const int s = lane * per + i;
+    if (s >= segments) break;
+    if (sh.seg[s] > 0.0 && run <= target) {
+      seg = s;
+      at = run;
+    }
+    run += sh.seg[s];
+  }
+  const uint64_t has = __builtin_amdgcn_ballot_w64(seg >= 0);
+  if (!has) return 0;
+  const int owner = 63 - __builtin_clzll(has);
+  seg = __shfl(seg, owner, RLT_WAVE);
+  at = __shfl(at, owner, RLT_WAVE);
+  const int64_t c = (int64_t)(seg / kAccWaves) * kStep + (int64_t)(seg % kAccWaves) * 64 * kRun + lane * kRun;
+  const bool plain = C == 0.0;
+  double y[kRun], mine = 0.0;
+#pragma unroll
+  for (int i = 0; i < kRun; ++i) {
+    y[i] = c + i < vocab ? left_of(p[c + i], plain ? 0.f : q[c + i], C) : 0.0;
+    mine += y[i];
+  }
+  const double incl = wave_incl(mine);
+  double lane_before = __shfl_up(incl, 1, RLT_WAVE);
+  if (lane == 0) lane_before = 0.0;
+  run = at + lane_before;
+  int col = -1;
+#pragma unroll
+  for (int i = 0; i < kRun; ++i) {
+    if (y[i] > 0.0 && run <= target) col = i;
+    run += y[i];
+  }
+  const uint64_t lanes = __builtin_amdgcn_ballot_w64(col >= 0);
+  if (!lanes) return 0;
+  const int who = 63 - __builtin_clzll(lanes);
+  return __shfl(c + col, who, RLT_WAVE);
+}
+
+__global__ __launch_bounds__(kAccThreads) void rlt_tree_accept_kernel(
+    const int64_t* draft_tokens, const int64_t* parents, const int64_t* drafts, const float* q_all,
+    const float* p_all, const float* u_accept, const float* u_final, int width, int64_t vocab,
+    int64_t* path, int64_t* tokens, int64_t* accepted, int64_t* final_token, uint8_t* error) {
+  __shared__ AcceptShared sh;
+  const int64_t r = blockIdx.x;
+  const int t = threadIdx.x, nodes = width + 1;
+  const float* const p = p_all + r * nodes * vocab;
+  const float* const q = q_all + r * width * vocab;
+  const int64_t d = drafts[r];
+  const int live = (int)(d < 0 ? 0 : d > width ? width : d);
+  bool bad = d != live;
+  // every draft's two probabilities at its parent, in one round of loads
+  for (int j = t; j < live; j += kAccThreads) {
+    const int64_t parent = parents[r * width + j], token = draft_tokens[r * width + j];
+    const bool child = parent >= 0 && parent <= j;
+    sh.parent[j] = child ? (int32_t)parent : -1;
+    sh.token[j] = token;
+    const bool in = child && token >= 0 && token < vocab;
+    sh.px[j] = in ? p[parent * vocab + token] : 0.f;
+    sh.qx[j] = in ? q[parent * vocab + token] : 0.f;  // 0: cannot have been drawn
+  }
+  if (t == 0) {
+    sh.walk[0] = 0;
+    sh.last = 0;
+  }
+  __syncthreads();
+  const int segments = (int)((vocab + kStep - 1) / kStep) * kAccWaves;
+  int node = 0, count = 0;
+  double C = 0.0, R = 1.0;
+  // every thread walks alike
+  for (int j = 0; j < live && !bad; ++j) {
+    if (sh.parent[j] != node) continue;
+    const double px = sh.px[j], qx = sh.qx[j];
+    if (!(qx > 0.0) || !(fabs(px) < INFINITY) || !(qx < INFINITY)) {
+      bad = true;
+    } else if ((double)u_accept[r * width + j] * R * qx < px - C * qx) {
+      ++count;
+      node = j + 1;
+      if (t == 0) sh.walk[count] = node;
+      C = 0.0;
+      R = 1.0;
+    } else {
+      C += R;
+      __syncthreads();  // the table of an earlier pass is read
+      weigh(sh, p + (int64_t)node * vocab, q + (int64_t)node * vocab, C, vocab);
+      double before;
+      R = segment_scan(sh, segments, before);
+      bad = !(R > 0.0) || !(R < INFINITY);
+    }
+  }
+  if (!bad) {
+    if (C == 0.0) {
+      __syncthreads();
+      weigh(sh, p + (int64_t)node * vocab, q, 0.0, vocab);
+    }
+    if (t < 64) {
+      double before;
+      const double total = segment_scan(sh, segments, before);
+      bad = !(total > 0.0) || !(total < INFINITY);
+      if (!bad) {
+        const double u = (double)u_final[r] * total;
+        // the draw stays below the total
+        const double top = __longlong_as_double(__double_as_longlong(total) - 1);
+        const int64_t token = draw(sh, p + (int64_t)node * vocab, q + (int64_t)node * vocab, C, vocab,
+                                   segments, before, u < top ? u : top);
+        if (t == 0) sh.last = token;
+      }
+    }
+  }
+  if (t == 0) {
+    accepted[r] = count;
+    error[r] = bad ? 1 : 0;  // (thread 0 is in the drawing wave)
+  }
+  __syncthreads();
+  if (t == 0) final_token[r] = sh.last;
+  for (int i = t; i < nodes; i += kAccThreads) {
+    path[r * nodes + i] = i <= count ? sh.walk[i] : -1;
+    tokens[r * nodes + i] = i < count ? sh.token[sh.walk[i + 1] - 1] : i == count ? sh.last : 0;
+  }
+}
+
+int64_t argmax_slices(int64_t vocab) {
+  return (vocab + kSliceEpt * kThreads - 1) / (kSliceEpt * kThreads);
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t rlt_tree_accept_workspace_size(int64_t n, int32_t width, int64_t vocab) { return 0; }
+
+int rlt_tree_accept(const int64_t* draft_tokens, const int64_t* parents, const int64_t* drafts,
+                    const float* q, const float* p, const float* u_accept, const float* u_final,
+                    int64_t n, int32_t width, int64_t vocab, int64_t* path, int64_t* tokens,
+                    int64_t* accepted, int64_t* final_token, uint8_t* error, void* workspace,
+                    size_t workspace_bytes, hipStream_t stream) {
+  if (n < 0 || width < 0 || vocab < 1) return RLT_ERR_ARGUMENT;
+  if (width > kMaxDrafts || vocab > kMaxVocab || n > 0x7fffffff) return RLT_ERR_UNSUPPORTED;
+  if (n == 0) return RLT_OK;
+  if (!drafts || !p || !u_final || !path || !tokens || !accepted || !final_token || !error ||
+      (width && (!draft_tokens || !parents || !q || !u_accept)))
+    return RLT_ERR_ARGUMENT;
+  hipLaunchKernelGGL(rlt_tree_accept_kernel, dim3((unsigned)n), dim3(kAccThreads), 0, stream,
+                     draft_tokens, parents, drafts, q, p, u_accept, u_final, width, vocab, path,
+                     tokens, accepted, final_token, error);
+  return rlt_launch_status();
+}
+
+size_t rlt_greedy_tree_accept_workspace_size(int64_t n, int32_t width, int64_t vocab) {
+  if (n <= 0 || width < 0 || width > kMaxDrafts || vocab < 1 || vocab > kMaxVocab) return 0;
+  return (size_t)(n * (width + 1) * argmax_slices(vocab)) * sizeof(unsigned long long);
+}
+
+int rlt_greedy_tree_accept(const int64_t* draft_tokens, const int64_t* parents,
+                           const int64_t* drafts, const void* target_logits, int32_t logits_dtype,
+                           int64_t row_stride, int64_t n, int32_t width, int64_t vocab,
+                           int64_t* targets, int64_t* path, int64_t* accepted, int64_t* next_token,
+                           void* workspace, size_t workspace_bytes, hipStream_t stream) {
+  if (n < 0 || width < 0 || vocab < 1) return RLT_ERR_ARGUMENT;
+  if (n > 0 && n * (width + 1) > 1 && row_stride < vocab) return RLT_ERR_ARGUMENT;
+  if (width > kMaxDrafts || vocab > kMaxVocab) return RLT_ERR_UNSUPPORTED;
+  if (logits_dtype != RLT_F32 && logits_dtype != RLT_BF16 && logits_dtype != RLT_F16)
+    return RLT_ERR_UNSUPPORTED;
+  if (n == 0) return RLT_OK;
+  const int64_t slices = argmax_slices(vocab), wgs = n * (width + 1) * slices;
+  if (n > 0x7fffffff || wgs > 0x7fffffff) return RLT_ERR_UNSUPPORTED;
+  if (!drafts || !target_logits || !targets || !path || !accepted || !next_token ||
+      (width && (!draft_tokens || !parents)))
+    return RLT_ERR_ARGUMENT;
+  if (!workspace || (uintptr_t)workspace % 8 ||
+      workspace_bytes < rlt_greedy_tree_accept_workspace_size(n, width, vocab))
+    return RLT_ERR_WORKSPACE;
+  unsigned long long* const best = (unsigned long long*)workspace;
+#define RLT_TREE_ARGMAX(DT)                                                                     \
+  hipLaunchKernelGGL((rlt_tree_argmax_kernel<DT>), dim3((unsigned)wgs), dim3(kThreads), 0, stream, \
+                     target_logits, row_stride, vocab, (int)slices, best)
+  switch (logits_dtype) {
+    case RLT_F32: RLT_TREE_ARGMAX(RLT_F32); break;
+    case RLT_BF16: RLT_TREE_ARGMAX(RLT_BF16); break;
+    default: RLT_TREE_ARGMAX(RLT_F16); break;
+  }
+#undef RLT_TREE_ARGMAX
+  hipLaunchKernelGGL(rlt_greedy_tree_kernel, dim3((unsigned)n), dim3(kThreads), 0, stream, best,
+                     (int)slices, draft_tokens, parents, drafts, width, targets, path, accepted,
+                     next_token);
+  return rlt_launch_status();
+}
+
+}  // extern "C"

@@ -9,7 +9,8 @@ Same arguments and semantics as
 * vllm_rlt/kernels/routing.py:147-180 ``finalize_kernel`` (``finalize_rows`` here, the
   LAST_EXITED copy into deeper planes),
 plus ``store_kv``, the unmasked index-put writer
-(vllm_rlt/core/kv_cache_manager.py:893-895).  Every call enqueues one gfx950 launch on
+(vllm_rlt/core/kv_cache_manager.py:893-895), and ``commit_tree_kv``, which moves the accepted
+path of a draft tree behind the prefix (the reference's drafts are chains).  Every call enqueues one gfx950 launch on
 the current stream without host synchronization.  Rows whose block or offset lies
 outside the pool are skipped (the reference's kernels would write out of bounds).
 """
@@ -169,3 +170,26 @@ def finalize_rows(descriptor, tables, key_pool, value_pool, block_size):
         key_pool.stride(0), key_pool.stride(1), key_pool.stride(2), per_token,
         key_pool.element_size(), _lib.stream_of(key_pool.device))
     _lib.check(status, "rlt_kv_finalize")
+
+
+def commit_tree_kv(key_pool, value_pool, tables, starts, path, accepted, block_size):
+    """Move the accepted path of draft trees behind the prefix, in place.
+
+    Request r's node j lies at position ``starts[r] + j``; for j = 1 .. ``accepted[r]`` the K/V
+    at position ``starts[r] + path[r, j]`` move to position ``starts[r] + j``, in every layer of
+    the pools ``[block, layer, token, ...]`` (code / value pools, or the fp32 scale pools of an
+    FP8 cache).  ``tables`` int32 ``[n, width]``, or ``[n, planes, width]`` to move in every
+    plane; ``path`` int64 ``[n, W + 1]`` ascending from 0 and ``accepted`` int64 ``[n]`` as
+    ``tree_accept`` / ``greedy_tree_accept`` return them.  The blocks that hold drafts must not
+    be shared between requests or planes.  Positions past the table or blocks outside the pool
+    copy nothing.  Runs ``torch.ops.rlt_mi355x.commit_tree_kv``.
+    """
+    _lib.require_gpu(key_pool, value_pool, tables, starts, path, accepted)
+    if path.ndim != 2:
+        raise ValueError("path must be [n, W + 1]")
+    n = path.shape[0]
+    tables = tables if tables.dtype == torch.int32 else tables.to(torch.int32)
+    path = path if path.dtype == torch.int64 else path.long()
+    _lib.ops().commit_tree_kv(key_pool, value_pool, tables.contiguous(),
+                              _index(starts, n, "starts"), path.contiguous(),
+                              _index(accepted, n, "accepted"), int(block_size))

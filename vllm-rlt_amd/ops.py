@@ -5,7 +5,9 @@ The reference binds its native code as a ``TORCH_LIBRARY`` schema
 (vllm_rlt/kernels/activation.py:34-39).  This package does the same for the gfx950
 kernels: the per-step entry points -- ``paged_attention``, ``paged_attention_store``,
 ``store_kv``, ``spec_probs``, ``categorical``, ``spec_accept``, ``greedy_accept``,
-``verify_distributions``, ``verify_accept`` -- are C++ operators
+``verify_distributions``, ``verify_accept``, and those of the draft-tree round
+(``tree_attention``, ``tree_masks``, ``tree_accept``, ``greedy_tree_accept``,
+``commit_tree_kv``, ``token_logprobs``) -- are C++ operators
 (``csrc/torch_bindings.cpp`` -> ``_C.so``: schema, argument checks, workspace and
 launch, one dispatcher call per step); the rest are Python ``torch.library``
 custom ops over the same library.  Every operator has an implementation for ROCm
@@ -104,6 +106,37 @@ def _(target_logits, temperature, top_k, top_p, draft_tokens, drafts, q, u_accep
 
 
 
+@torch.library.register_fake("rlt_mi355x::tree_masks")
+def _(parents, cu_seqlens_q, rows):
+    return parents.new_empty((rows, (parents.shape[1] + 64) // 64))
+
+
+@torch.library.register_fake("rlt_mi355x::greedy_tree_accept")
+def _(draft_tokens, parents, drafts, target_logits):
+    n, w = draft_tokens.shape
+    return (drafts.new_empty((n, w + 1)), drafts.new_empty((n, w + 1)), drafts.new_empty((n,)),
+            drafts.new_empty((n,)))
+
+
+@torch.library.register_fake("rlt_mi355x::tree_accept")
+def _(draft_tokens, parents, drafts, q, p, u_accept, u_final):
+    n, w = draft_tokens.shape
+    return (drafts.new_empty((n, w + 1)), drafts.new_empty((n, w + 1)), drafts.new_empty((n,)),
+            drafts.new_empty((n,)), drafts.new_empty((n,), dtype=torch.bool))
+
+
+@torch.library.register_fake("rlt_mi355x::token_logprobs")
+def _(logits, tokens, rows=None, top_n=0):
+    r, f32 = tokens.shape[0], dict(dtype=torch.float32)
+    return (tokens.new_empty((r,), **f32), tokens.new_empty((r,)), tokens.new_empty((r,), **f32),
+            tokens.new_empty((r, top_n), **f32), tokens.new_empty((r, top_n)))
+
+
+@torch.library.register_fake("rlt_mi355x::commit_tree_kv")
+def _(key_pool, value_pool, tables, starts, path, accepted, block_size):
+    return None
+
+
 @torch.library.custom_op("rlt_mi355x::merge_random_round", mutates_args=(), device_types="cuda")
 def merge_random_round(target: torch.Tensor, accepted: torch.Tensor, next_tokens: torch.Tensor,
                        starts: torch.Tensor, input_tokens: torch.Tensor, tokens: torch.Tensor,
@@ -172,7 +205,8 @@ def finalize_rows(descriptor: torch.Tensor, tables: torch.Tensor, key_pool: torc
     _kv.finalize_rows(descriptor, tables, key_pool, value_pool, block_size)
 
 
-OPS = ("paged_attention", "paged_attention_store", "tree_attention", "spec_probs", "categorical", "spec_accept", "greedy_accept",
+OPS = ("paged_attention", "paged_attention_store", "tree_attention", "tree_masks",
+       "greedy_tree_accept", "tree_accept", "token_logprobs", "commit_tree_kv", "spec_probs", "categorical", "spec_accept", "greedy_accept",
        "propose_drafts", "verify_distributions", "verify_accept", "merge_random_round",
        "rejection_rows", "store_kv",
        "store_fp8", "finalize_rows")

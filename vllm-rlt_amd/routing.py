@@ -230,3 +230,19 @@ def depth_tables(tables, depth, positions, block_size, active=None):
         _lib.ptr(blocks), _lib.ptr(offsets), _lib.ptr(lengths), n, _lib.stream_of(dev))
     _lib.check(status, "rlt_depth_tables")
     return table, blocks, offsets, lengths
+
+
+def tree_masks(parents, cu_seqlens_q, rows):
+    """Mask rows of draft trees for ``MI355XPagedAttention.tree``: int64 ``[rows, words]``.
+
+    Q row ``cu_seqlens_q[s] + i`` is node i of sequence s and sees itself and its ancestors;
+    node i's parent is ``parents[s, i - 1]`` (int64 ``[n, W]``, W <= 255), node 0 the root.  A
+    parent outside [0, i) ends the walk.  ``rows`` is the number of q rows; rows of no sequence
+    see nothing.  Runs ``torch.ops.rlt_mi355x.tree_masks``.
+    """
+    _lib.require_gpu(parents, cu_seqlens_q)
+    if parents.ndim != 2:
+        raise ValueError("parents must be [n, W]")
+    parents = parents if parents.dtype == torch.int64 else parents.long()
+    cu = cu_seqlens_q if cu_seqlens_q.dtype == torch.int32 else cu_seqlens_q.to(torch.int32)
+    return _lib.ops().tree_masks(parents.contiguous(), cu.contiguous(), int(rows))

@@ -242,6 +242,96 @@ def verify_distributions(logits, random_rows, temperature, top_k, top_p, *, max_
     return target, p_out
 
 
+class TreeAcceptResult(NamedTuple):
+    """Device-side result of a sampled draft-tree round.
+
+    ``path[r, 0 .. accepted[r]]`` are the nodes of the walk (0, then the accepted drafts'; -1
+    behind them), ``tokens[r]`` the accepted tokens, then the final one, then zeros;
+    ``tokens[r, i]`` was decided at node ``path[r, i]``.
+    """
+
+    path: torch.Tensor
+    tokens: torch.Tensor
+    accepted: torch.Tensor
+    final: torch.Tensor
+    error: torch.Tensor
+
+
+class TokenLogprobs(NamedTuple):
+    """Per given token; ``top_logprob`` / ``top_tokens`` are ``[r, top_n]``."""
+
+    logprob: torch.Tensor
+    rank: torch.Tensor
+    entropy: torch.Tensor
+    top_logprob: torch.Tensor
+    top_tokens: torch.Tensor
+
+
+def tree_accept(draft_tokens, parents, drafts, q, p, u_accept, u_final):
+    """Sampled acceptance of draft trees: ``speculative_accept`` along a tree.
+
+    Node 0 of a request is its last committed token, node ``j + 1`` its draft j, whose parent
+    is node ``parents[r, j]`` (0 .. j; a draft with any other parent is never reached); only
+    ``drafts[r]`` drafts count.  ``q[r, i]`` is the distribution that node i's children were
+    drawn from, each independently; ``p[r, i]`` the target distribution after node i.  A
+    node's children are tried in index order: child t is accepted when ``u_accept * R * q[t] <
+    y[t]``, where y is what is left of p (at first p, R = 1) and a rejection leaves
+    ``max(y - R q, 0)`` with its sum R; where none is left the final token is drawn from y with
+    ``u_final``.  The emitted tokens follow p.  Rows count as distributions as they stand, all
+    sums are float64.  ``error`` is set (and the final token 0) for a draft count outside
+    ``[0, W]``, a tried draft that q cannot have proposed, and weights without a finite
+    positive sum.
+
+    ``draft_tokens``, ``parents`` int64 ``[n, W]`` (W <= 255), ``drafts`` int64 ``[n]``, ``q``
+    float32 ``[n, W, V]``, ``p`` float32 ``[n, W + 1, V]``, ``u_accept`` ``[n, W]``,
+    ``u_final`` ``[n]``; returns ``TreeAcceptResult``.  With ``parents[r, j] = j`` it is the
+    chain's round (vllm_rlt/worker/speculative_sampling.py:104-181) on normalized rows.  Runs
+    ``torch.ops.rlt_mi355x.tree_accept``.
+    """
+    _lib.require_gpu(draft_tokens, parents, drafts, q, p, u_accept, u_final)
+    if p.ndim != 3:
+        raise ValueError("q must be [n, W, V] and p [n, W + 1, V]")
+    return TreeAcceptResult(*_lib.ops().tree_accept(
+        _i64(draft_tokens), _i64(parents), _i64(drafts), _f32(q), _f32(p), _f32(u_accept),
+        _f32(u_final)))
+
+
+def greedy_tree_accept(draft_tokens, parents, drafts, target_logits):
+    """Greedy acceptance of draft trees: ``greedy_accept_batched`` along a tree.
+
+    Nodes, parents and draft counts as in ``tree_accept``; ``target_logits`` is ``[n, W + 1,
+    V]``.  Returns ``(targets int64 [n, W + 1], path int64 [n, W + 1], accepted int64 [n],
+    next_token int64 [n])``: every node's argmax (first maximal column), the walk from node 0
+    to the first child that holds its node's target until there is none (-1 behind it), and
+    the last node's target.  The emitted tokens are ``targets[r, path[r, i]]`` for ``i <=
+    accepted[r]``.  Runs ``torch.ops.rlt_mi355x.greedy_tree_accept``.
+    """
+    _lib.require_gpu(draft_tokens, parents, drafts, target_logits)
+    if target_logits.ndim != 3:
+        raise ValueError("target_logits must be [n, W + 1, V]")
+    return tuple(_lib.ops().greedy_tree_accept(_i64(draft_tokens), _i64(parents), _i64(drafts),
+                                               _request_rows(target_logits)))
+
+
+def token_logprobs(logits, tokens, *, rows=None, top_n=0):
+    """Log probabilities of given tokens, with rank, entropy and their rows' alternatives.
+
+    ``logits`` ``[m, V]``, ``tokens`` int64 ``[r]``, ``rows`` int64 ``[r]`` (the logit row of
+    each token; without it r = m and token i belongs to row i).  Returns ``TokenLogprobs``:
+    ``logprob`` float32 ``[r]``, ``rank`` int64 ``[r]`` (1 for the row's first column in
+    descending order, equal logits by ascending column), ``entropy`` float32 ``[r]`` in nats,
+    and the first ``top_n`` (at most 64) columns with their log probabilities.  A row index
+    outside the logits gives NaN, rank 0 and tokens -1, so the -1 of an acceptance path may be
+    passed on.  Logits of -inf weigh nothing; a row with a NaN or +inf, or without a logit above
+    -inf, gives NaN.  Runs ``torch.ops.rlt_mi355x.token_logprobs``.
+    """
+    _lib.require_gpu(logits, tokens, rows)
+    if logits.ndim != 2:
+        raise ValueError("logits must be a 2-D [m, V] tensor")
+    return TokenLogprobs(*_lib.ops().token_logprobs(
+        _rows(logits), _i64(tokens), None if rows is None else _i64(rows), int(top_n)))
+
+
 def categorical(weights, u):
     """Inverse-CDF draw from ``[m, V]`` nonnegative weights with ``[m]`` uniforms.
 
