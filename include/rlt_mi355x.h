@@ -216,7 +216,8 @@ int rlt_paged_attention_uses_prefill(int32_t q_dtype, int32_t kv_dtype, int32_t 
  * rounding.  No counterpart in the reference, whose drafts are chains.  The grid is static:
  * safe under graph capture.
  */
-size_t rlt_tree_attention_workspace_size(int32_t num_seqs, int32_t head_dim);
+size_t rlt_tree_attention_workspace_size(int32_t num_seqs, int32_t max_q_len, int32_t num_q_heads,
+                                         int32_t num_kv_heads, int32_t head_dim, int32_t kv_dtype);
 
 int rlt_tree_attention(const void* q, int64_t q_row_stride, int64_t q_head_stride,
                        const void* key_cache, const void* value_cache, int64_t k_block_stride,

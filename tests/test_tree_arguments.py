@@ -44,7 +44,8 @@ def test_tree_attention_statuses(pkg):
     assert attend(pkg, width=1 << 28) == 2
     assert attend(pkg, ws_bytes=16) == 3
     size = lib(pkg).rlt_tree_attention_workspace_size
-    assert size(2, 128) > 0 and size(2, 80) == 0 and size(-1, 128) == 0
+    assert size(2, 5, 16, 4, 128, 2) > 0 and size(2, 5, 16, 4, 80, 2) == 0
+    assert size(2, -1, 4, 4, 128, 2) == 0
 
 
 def test_round_statuses(pkg):

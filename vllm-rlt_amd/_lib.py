@@ -88,7 +88,7 @@ _SIGNATURES = {
         _p, _i64, _i64,                 # out
         _p, _sz, _p,                    # workspace, bytes, stream
     ]),
-    "rlt_tree_attention_workspace_size": (_sz, [_i32, _i32]),
+    "rlt_tree_attention_workspace_size": (_sz, [_i32, _i32, _i32, _i32, _i32, _i32]),
     "rlt_tree_attention": (ctypes.c_int, [
         _p, _i64, _i64,                 # q
         _p, _p, _i64, _i64, _i64, _i64, _i64, _i64, _i32,  # pools, strides, blocks

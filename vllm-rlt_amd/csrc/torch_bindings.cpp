@@ -697,7 +697,11 @@ Tensor tree_attention(const Tensor& q, const Tensor& key_cache, const Tensor& va
   const c10::hip::HIPGuardMasqueradingAsCUDA guard(q.device());
   Tensor output = at::empty({rows, heads, head_dim}, q.options());
   if (rows == 0 || num_seqs == 0 || max_seqlen_q == 0) return output;
-  const Tensor ws = workspace(rlt_tree_attention_workspace_size((int32_t)num_seqs, (int32_t)head_dim), q);
+  const Tensor ws = workspace(
+      rlt_tree_attention_workspace_size((int32_t)num_seqs, (int32_t)max_seqlen_q, (int32_t)heads,
+                                        (int32_t)kv_heads, (int32_t)head_dim,
+                                        dtype_code(key_cache.scalar_type())),
+      q);
   const int64_t mask_stride = std::max(tree_mask.stride(0), tree_mask.size(1));
   TORCH_CHECK_VALUE(rows == 1 || tree_mask.stride(0) >= tree_mask.size(1),
                     "tree_mask rows must not overlap");

@@ -8,12 +8,14 @@
 // them -- share every key and value, so a pass is R flops per byte of a 16-bit pool (2 R of an
 // fp8 one): the KV stream bounds it up to R ~ 200.
 //
-// Tiling.  A workgroup is four waves on one CU: RW row waves times KW = 4 / RW kv waves.  A
-// row wave holds NT column tiles of 32 rows (v_mfma_f32_32x32x16: S^T = K Q^T, O^T += V^T P^T);
-// each kv wave (group of RW waves) streams its own 32-position tiles, every KW-th of the
-// workgroup's span, through a ring of S stages in LDS filled by direct global -> LDS loads.
-// With RW = 1 no wave ever waits for another inside the stream, and a key is read from LDS
-// once for up to 64 rows; more rows take two row waves that share the tiles.
+// Tiling.  A workgroup is four waves, two workgroups share a CU: two waves per SIMD hide each
+// other's chains of LDS reads, matrix instructions and exponentials.  The waves are RW row
+// waves times KW = 4 / RW kv waves.  A row wave holds 32 rows (v_mfma_f32_32x32x16: S^T = K
+// Q^T, O^T += V^T P^T); each kv wave (group of RW row waves) streams its own 32-position
+// tiles, every KW-th of the workgroup's share, through LDS by direct global -> LDS loads.
+// With RW = 1 (up to 32 rows) no wave waits for another inside the stream: a tile's keys are
+// refilled as soon as its scores are taken, its values as soon as they are added.  More rows
+// take 2 or 4 row waves that share the tiles, one barrier per tile.
 //
 // Schedule.  The keys of all (sequence, kv head, row block) pairs are one line of macro tiles
 // (KW tiles each), of which every workgroup takes an equal share, whatever the mix of lengths.
@@ -29,12 +31,23 @@
 
 namespace tree {
 
+// Where a pair's partials are: slot `first` of the workgroup that holds its first macro tile, then
+// the slots 2 b of the workgroups b up to `last`; last < 0: normalized where it was computed.
+struct Split {
+  int32_t first, last;
+};
+
 constexpr int kWaves = 4;
 constexpr int kTile = 32;          // key positions per LDS tile
-constexpr int kGrid = 256;         // persistent workgroups: one per CU
+constexpr int kGrid = 512;         // persistent workgroups, at most: two per CU
+// (256 dims: the states of a workgroup take more than half of a CU's LDS and registers)
+template <int D>
+constexpr int per_cu() { return D == 256 ? 1 : 2; }
+template <int D>
+constexpr int grid_of() { return kGrid / 2 * per_cu<D>(); }
 constexpr int kMaxNodes = 256;     // nodes of one sequence's tree
 constexpr int kWords = kMaxNodes / 64;
-constexpr int kRingBytes = 128 << 10;
+constexpr int kRingBytes = 64 << 10;
 constexpr int kBadWords = kMaxNodes / kTile + 3;  // tiles that a range of kMaxNodes meets
 constexpr float kLazy = 8.f;       // log2 headroom before the running max moves
 
@@ -62,7 +75,8 @@ struct Params {
   int32_t scale_mode;
   void* out;
   int64_t out_row_stride, out_head_stride;
-  int64_t* starts;        // [num_seqs + 1]: first macro tile of each sequence; [num_seqs]: share
+  int32_t max_blocks;     // row blocks of the longest tree
+  struct Split* splits;   // [num_seqs][hkv][max_blocks]
   float* part;            // [2 * kGrid][rows per block * (head_dim + 2)]
 };
 
@@ -226,6 +240,15 @@ __device__ __forceinline__ Span span_of(const Params& P, const Seq& v) {
   return x;
 }
 
+template <int RB, int MACRO>
+__device__ __forceinline__ Span uniform_span(const Params& P, const Seq& v) {
+  Span x = span_of<RB, MACRO>(P, v);
+  x.m0 = uniform(x.m0);
+  x.count = uniform(x.count);
+  x.blocks = uniform(x.blocks);
+  return x;
+}
+
 // 32 visibility bits of a node at positions tb .. tb + 31: the prefix from `lo` on, then the
 // node's mask words (bits past the tree are clear).
 __device__ __forceinline__ uint32_t tile_bits(const uint64_t* words, int base, int lo, int tb) {
@@ -279,12 +302,12 @@ __device__ __forceinline__ int node_mask(const Params& P, const Seq& v, int node
 
 // ---------------------------------------------------------------- MFMA kernel
 
-template <int QT, int KVT, int D, int NT, int RW>
+template <int QT, int KVT, int D, int RW>
 struct Geometry {
   static constexpr bool FP8 = KVT != QT;
   static constexpr int ELT = FP8 ? 1 : 2;
   static constexpr int KW = kWaves / RW;
-  static constexpr int RB = 32 * NT * RW;            // rows per block
+  static constexpr int RB = 32 * RW;                 // rows per block
   static constexpr int MACRO = kTile * KW;           // positions per macro tile
   static constexpr int ROW = (D == 96 ? 128 : D) * ELT;  // bytes of an LDS row
   static constexpr int SLOTS = ROW / 16;
@@ -293,20 +316,22 @@ struct Geometry {
   static constexpr int LOADS = kTile / RPL;          // such loads per K (V) tile
   static constexpr int TILE = kTile * ROW;           // bytes of a K (V) tile
   static constexpr int FIT = kRingBytes / (KW * 2 * TILE);
-  static constexpr int S = FIT > 6 ? 6 : FIT;        // stages
-  static_assert(S >= 2, "at least two stages");
-  static_assert(LOADS % RW == 0, "the row waves share a tile's loads");
+  static constexpr int S = FIT > 4 ? 4 : FIT;        // stages
+  static_assert(S >= (RW == 1 ? 1 : 2), "row waves that share tiles need a second stage");
+  // a row wave's loads of a K (V) tile (of fewer loads than waves some are done twice)
+  static constexpr int LV = LOADS >= RW ? LOADS / RW : 1;
+  static_assert(LOADS % RW == 0 || RW % LOADS == 0, "the row waves share a tile's loads");
   static constexpr int RING = KW * S * 2 * TILE;
   static constexpr int OSTRIDE = D + 4;              // floats per row of the combine buffer
   static constexpr int COMBINE = KW * RB * OSTRIDE * 4;
   static constexpr int BODY = RING > COMBINE ? RING : COMBINE;
 };
 
-template <int QT, int KVT, int D, int NT, int RW>
+template <int QT, int KVT, int D, int RW>
 struct Shared {
-  using G = Geometry<QT, KVT, D, NT, RW>;
+  using G = Geometry<QT, KVT, D, RW>;
   alignas(16) uint8_t body[G::BODY];                 // the ring, then the combine buffer
-  alignas(16) float scale[kWaves][G::S][64];         // per wave: 32 key, 32 value scales
+  alignas(16) float scale[kWaves][G::S + 1][64];     // per wave: 32 key, 32 value scales
   uint64_t words[G::RB][kWords];                     // mask words of the row block's nodes
   int lo[G::RB];
   float ml[G::KW][G::RB][2];
@@ -327,16 +352,16 @@ __device__ __forceinline__ int v_swz(int r) {
   return SLOTS >= 16 ? 4 * (r & 3) : 4 * ((r >> 1) & 1);
 }
 
-template <int QT, int KVT, int D, int SM, int NT, int RW>
-__global__ __launch_bounds__(64 * kWaves, 1) void rlt_tree_kernel(Params P) {
-  using G = Geometry<QT, KVT, D, NT, RW>;
+template <int QT, int KVT, int D, int SM, int RW>
+__global__ __launch_bounds__(64 * kWaves, per_cu<D>()) void rlt_tree_kernel(Params P) {
+  using G = Geometry<QT, KVT, D, RW>;
   constexpr bool FP8 = G::FP8;
   constexpr int ELT = G::ELT, KW = G::KW, RB = G::RB, MACRO = G::MACRO, S = G::S;
   constexpr int SLOTS = G::SLOTS, PIECES = G::PIECES, RPL = G::RPL;
   constexpr int NQ = D / 16;  // contraction slices of S^T
   constexpr int ND = D / 32;  // dim tiles of O^T
-  constexpr int LPT = 2 * G::LOADS / RW + (SM == 2 ? 1 : 0);  // a wave's loads per tile
-  __shared__ Shared<QT, KVT, D, NT, RW> sh;
+  constexpr int LV = G::LV, LK = LV + (SM == 2 ? 1 : 0);  // a wave's loads per tile
+  __shared__ Shared<QT, KVT, D, RW> sh;
   const int t = threadIdx.x, lane = t & 63, l32 = lane & 31, h = lane >> 5;
   const int w = __builtin_amdgcn_readfirstlane(t >> 6);
   const int kg = w / RW, rw = w % RW;  // kv group, row wave
@@ -363,18 +388,9 @@ __global__ __launch_bounds__(64 * kWaves, 1) void rlt_tree_kernel(Params P) {
     total += sh.totals[i];
   }
   total = uniform(total);
-  const int64_t share = (total + kGrid - 1) / kGrid;
+  const int64_t share = (total + grid_of<D>() - 1) / grid_of<D>();
   const int64_t f_begin = (int64_t)blockIdx.x * share;
   const int64_t f_end = min(f_begin + share, total);
-  if (blockIdx.x == 0) {
-    int64_t at = before;
-    for (int s = s_lo; s < s_hi; ++s) {
-      P.starts[s] = at;
-      const Span x = span_of<RB, MACRO>(P, seq_of(P, s));
-      at += (int64_t)x.count * x.blocks * P.hkv;
-    }
-    if (t == 0) P.starts[P.num_seqs] = share;
-  }
   if (f_begin >= f_end) return;  // uniform over the workgroup
   if (before <= f_begin && f_begin < before + run) {
     int64_t at = before;
@@ -393,12 +409,14 @@ __global__ __launch_bounds__(64 * kWaves, 1) void rlt_tree_kernel(Params P) {
   int seq = uniform(sh.find_seq);
   int64_t seq_start = uniform(sh.find_start);
   Seq sv = uniform_seq(P, seq);
-  Span sp = span_of<RB, MACRO>(P, sv);
+  Span sp = uniform_span<RB, MACRO>(P, sv);
 
   // ---- lane constants of the loads: lane L of load j fills row RPL j + L / SLOTS, slot L % SLOTS
   const int ld_row = lane / SLOTS, ld_slot = lane % SLOTS;
   const uint32_t k_tok = (uint32_t)P.k_token_stride * ELT, v_tok = (uint32_t)P.v_token_stride * ELT;
-  uint8_t* const ring = sh.body + kg * (S * 2 * G::TILE);
+  uint8_t* const ring = sh.body + kg * (S * 2 * G::TILE);  // the group's S key tiles, then S value tiles
+  // (block, offset) of a tile's first position: advanced without a division
+  const int step_q = uniform(MACRO / P.block_size), step_r = MACRO - step_q * P.block_size;
 
   float qk_scale = P.qk_scale_log2, v_mul = 1.f;
   if (SM == 1) {
@@ -426,24 +444,26 @@ __global__ __launch_bounds__(64 * kWaves, 1) void rlt_tree_kernel(Params P) {
       seq_start += (int64_t)sp.count * sp.blocks * P.hkv;
       ++seq;
       sv = uniform_seq(P, seq);
-      sp = span_of<RB, MACRO>(P, sv);
+      sp = uniform_span<RB, MACRO>(P, sv);
     }
-    const int64_t in_seq = f - seq_start;
-    const int pair = (int)(in_seq / sp.count);
-    const int a = (int)(in_seq - (int64_t)pair * sp.count);
-    const int b = (int)min((int64_t)sp.count, a + (f_end - f));
-    const int rb = pair % sp.blocks, kvh = pair / sp.blocks;
+    const uint32_t in_seq = (uint32_t)(f - seq_start);
+    const int pair = uniform((int)(in_seq / (uint32_t)sp.count));
+    const int a = (int)(in_seq - (uint32_t)pair * sp.count);
+    const int n = (int)min((int64_t)(sp.count - a), f_end - f);
+    const int kvh = uniform(pair / sp.blocks), rb = pair - kvh * sp.blocks;
     const int rows = min(RB, sv.nodes * P.group - rb * RB);
     const int node0 = rb * RB / P.group;
 
-    // ---- loads of the tile at position tb into a stage
+    // ---- loads of the next tile of the group
     const auto* table = (const __attribute__((address_space(4))) int32_t*)(
         P.tables + (int64_t)seq * P.table_stride);
-    auto issue = [&](int macro, int stage) {
-      const int tb = ((sp.m0 + macro) * KW + kg) * kTile;
-      // blocks hold whole 8-position groups: four scalar (block, offset) pairs per tile
-      int blk[4], off[4];
-      int idx = tb / P.block_size, o = tb - idx * P.block_size;
+    const uint8_t* const k_head = (const uint8_t*)P.k + (int64_t)kvh * P.k_head_stride * ELT;
+    const uint8_t* const v_head = (const uint8_t*)P.v + (int64_t)kvh * P.v_head_stride * ELT;
+    const int first_tb = ((sp.m0 + a) * KW + kg) * kTile;
+    int next_idx = uniform(first_tb / P.block_size), next_off = first_tb - next_idx * P.block_size;
+    int blk[4], off[4];  // of the tile's four 8-position groups (blocks hold whole groups)
+    auto next_tile = [&]() {
+      int idx = next_idx, o = next_off;
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
         const int32_t e = table[min(idx, P.table_width - 1)];
@@ -455,118 +475,117 @@ __global__ __launch_bounds__(64 * kWaves, 1) void rlt_tree_kernel(Params P) {
           ++idx;
         }
       }
-      uint8_t* const st = ring + stage * (2 * G::TILE);
-      auto rows_of = [&](const void* pool, int64_t bs, int64_t ts, int64_t hs, uint32_t tok,
-                         uint8_t* dst, auto swz) {
-        const uint8_t* const head = (const uint8_t*)pool + (int64_t)kvh * hs * ELT;
+      next_idx += step_q;
+      next_off += step_r;
+      if (next_off >= P.block_size) {
+        next_off -= P.block_size;
+        ++next_idx;
+      }
+    };
+    auto load_rows = [&](const uint8_t* head, int64_t bs, uint32_t tok, uint8_t* dst, auto swz) {
+      const uint8_t* base[4];
 #pragma unroll
-        for (int i = 0; i < G::LOADS / RW; ++i) {
-          const int j = i * RW + rw;  // wave-uniform
-          const int r0 = RPL * j;
-          const int piece = ld_slot ^ swz(r0 + ld_row);
-          if (PIECES == SLOTS || piece < PIECES) {
-            const uint32_t lds = uniform((int)(lds_offset(dst) + r0 * G::ROW));
-            if constexpr (RPL <= 8) {
-              const int g = r0 >> 3;
-              const int64_t bk = g == 0 ? blk[0] : g == 1 ? blk[1] : g == 2 ? blk[2] : blk[3];
-              const int og = g == 0 ? off[0] : g == 1 ? off[1] : g == 2 ? off[2] : off[3];
-              const uint8_t* base = head + (bk * bs + (int64_t)(og + (r0 & 7)) * ts) * ELT;
-              load_lds16(base, (uint32_t)ld_row * tok + piece * 16, lds);
-            } else {
-              // 16 rows per load: two groups
-              const bool up = ld_row >= 8;
-              const int64_t bk = r0 == 0 ? (up ? blk[1] : blk[0]) : (up ? blk[3] : blk[2]);
-              const int og = r0 == 0 ? (up ? off[1] : off[0]) : (up ? off[3] : off[2]);
-              load_lds16(head + (bk * bs + (int64_t)(og + (ld_row & 7)) * ts) * ELT + piece * 16, lds);
-            }
+      for (int g = 0; g < 4; ++g)
+        base[g] = head + uniform((int64_t)blk[g] * (bs * ELT) + (int64_t)((uint64_t)((uint32_t)off[g]) * tok));
+#pragma unroll
+      for (int i = 0; i < LV; ++i) {
+        const int j = (i * RW + rw) % G::LOADS;  // wave-uniform
+        const int r0 = RPL * j;
+        const int piece = ld_slot ^ swz(r0 + ld_row);
+        if (PIECES == SLOTS || piece < PIECES) {
+          const uint32_t lds = uniform((int)(lds_offset(dst) + r0 * G::ROW));
+          if constexpr (RPL <= 8) {
+            const int g = r0 >> 3;
+            const uint8_t* const at = g == 0 ? base[0] : g == 1 ? base[1] : g == 2 ? base[2] : base[3];
+            load_lds16(at, (uint32_t)((r0 & 7) + ld_row) * tok + piece * 16, lds);
+          } else {
+            // 16 rows per load: two groups
+            const bool up = ld_row >= 8;
+            const uint8_t* const at = r0 == 0 ? (up ? base[1] : base[0]) : (up ? base[3] : base[2]);
+            load_lds16(at + (uint32_t)(ld_row & 7) * tok + piece * 16, lds);
           }
         }
-      };
-      rows_of(P.k, P.k_block_stride, P.k_token_stride, P.k_head_stride, k_tok, st,
-              [](int r) { return k_swz<SLOTS>(r); });
-      rows_of(P.v, P.v_block_stride, P.v_token_stride, P.v_head_stride, v_tok, st + G::TILE,
-              [](int r) { return v_swz<SLOTS, FP8>(r); });
+      }
+    };
+    auto load_k = [&](int stage, int scale_stage) {
+      load_rows(k_head, P.k_block_stride, k_tok, ring + stage * G::TILE,
+                [](int r) { return k_swz<SLOTS>(r); });
       if constexpr (SM == 2) {
         const int g = l32 >> 3;
         const int64_t bk = g == 0 ? blk[0] : g == 1 ? blk[1] : g == 2 ? blk[2] : blk[3];
         const int og = g == 0 ? off[0] : g == 1 ? off[1] : g == 2 ? off[2] : off[3];
         load_lds4((h ? P.v_scale : P.k_scale) + bk * P.s_block_stride +
                       (int64_t)(og + (l32 & 7)) * P.s_token_stride + (int64_t)kvh * P.s_head_stride,
-                  uniform((int)lds_offset(sh.scale[w][stage])));
+                  uniform((int)lds_offset(sh.scale[w][scale_stage])));
       }
     };
-    const int n = b - a;
+    auto load_v = [&](int stage) {
+      load_rows(v_head, P.v_block_stride, v_tok, ring + (S + stage) * G::TILE,
+                [](int r) { return v_swz<SLOTS, FP8>(r); });
+    };
+
+    // this wave's tiles: a row wave's barriers are the workgroup's, so those of KW groups alike
+    const int tiles = RW > 1 ? n : max(0, min(n, (sv.len - first_tb + MACRO - 1) / MACRO));
+    if constexpr (RW == 1) {
+#pragma unroll
+      for (int i = 0; i < S; ++i)
+        if (i < tiles) {
+          next_tile();
+          load_k(i, i);
+          load_v(i);
+        }
+    } else {
 #pragma unroll 1
-    for (int i = 0; i < S - 1 && i < n; ++i) issue(a + i, i);
+      for (int i = 0; i < S - 1 && i < tiles; ++i) {
+        next_tile();
+        load_k(i, i);
+        load_v(i);
+      }
+    }
 
     // ---- this wave's rows: B operands of S^T, and the masks of the block's nodes
-    u32x4 qreg[NT][NQ];
-    int local[NT];  // node within the block
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      const int r = (rw * NT + nt) * 32 + l32;
+    u32x4 qreg[NQ];
+    int local;  // node within the block
+    {
+      const int r = rw * 32 + l32;
       const int rho = rb * RB + r;
       const int node = rho / P.group, head = kvh * P.group + rho % P.group;
-      local[nt] = r < rows ? node - node0 : 0;
+      local = r < rows ? node - node0 : 0;
       const uint16_t* qp = (const uint16_t*)P.q + (int64_t)(sv.q_begin + node) * P.q_row_stride +
                            (int64_t)head * P.q_head_stride;
 #pragma unroll
       for (int c = 0; c < NQ; ++c) {
         // (codes: slices 2 j and 2 j + 1 take a lane's 16 elements 32 j + 16 h ..)
         const int e = FP8 ? 32 * (c / 2) + 16 * h + 8 * (c % 2) : 16 * c + 8 * h;
-        qreg[nt][c] = r < rows ? *(const u32x4*)(qp + e) : u32x4{0, 0, 0, 0};
+        qreg[c] = r < rows ? *(const u32x4*)(qp + e) : u32x4{0, 0, 0, 0};
       }
     }
     const int nodes_here = min(sv.nodes - node0, (rows + rb * RB - node0 * P.group + P.group - 1) / P.group);
-    for (int i = t; i < nodes_here; i += 64 * kWaves) sh.lo[i] = node_mask(P, sv, node0 + i, sh.words[i]);
+    if (t < nodes_here) sh.lo[t] = node_mask(P, sv, node0 + t, sh.words[t]);
     if (t < 2 * kBadWords) sh.bad[t] = 0;
     // the masked tiles: of the tree, and where a sliding window begins
     const int tree_tile = max(sv.base, 0) / kTile, first_tile = first_position(P, sv) / kTile;
     __syncthreads();
 
-    f32x16 oacc[NT][ND];
-    float m_run[NT], m_use[NT], l_run[NT];
+    f32x16 oacc[ND];
+    float m_run = -INFINITY, m_use = 0.f, l_run = 0.f;
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      m_run[nt] = -INFINITY;
-      m_use[nt] = 0.f;
-      l_run[nt] = 0.f;
+    for (int dt = 0; dt < ND; ++dt)
 #pragma unroll
-      for (int dt = 0; dt < ND; ++dt)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) oacc[nt][dt][i] = 0.f;
-    }
+      for (int i = 0; i < 16; ++i) oacc[dt][i] = 0.f;
 
-    int stage = 0;
-    for (int it = 0; it < n; ++it, stage = stage + 1 == S ? 0 : stage + 1) {
-      if (it + S - 1 < n) {
-        wait_loads<(S - 2) * LPT>();
-        if (RW > 1) stage_barrier();
-        issue(a + it + S - 1, stage == 0 ? S - 1 : stage - 1);
-      } else {
-        wait_loads<0>();
-        if (RW > 1) stage_barrier();
-      }
-      const int tb = ((sp.m0 + a + it) * KW + kg) * kTile;
-      if (tb >= sv.len) continue;  // wave-uniform: a macro tile's last tiles
-      const uint8_t* const kt = ring + stage * (2 * G::TILE);
-      uint8_t* const vt = ring + stage * (2 * G::TILE) + G::TILE;
-      // no row hides any of the tile's positions
-      const bool full = tb + kTile <= sv.base && (P.window <= 0 || tb >= sv.len - P.window);
-
-      // ---- S^T = K Q^T
-      f32x16 sc[NT];
+    // no row hides any of the positions of the tile at tb
+    auto is_full = [&](int tb) {
+      return tb + kTile <= sv.base && (P.window <= 0 || tb >= sv.len - P.window);
+    };
+    // ---- S^T = K Q^T of the tile in stage `kt`
+    auto scores = [&](f32x16& sc, const uint8_t* kt) {
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) sc[nt][i] = 0.f;
+      for (int i = 0; i < 16; ++i) sc[i] = 0.f;
       if constexpr (!FP8) {
 #pragma unroll
-        for (int c = 0; c < NQ; ++c) {
-          const u32x4 ka = *(const u32x4*)(kt + k_lane + ((32 * c) ^ k_x));
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt) sc[nt] = mfma<QT>(ka, qreg[nt][c], sc[nt]);
-        }
+        for (int c = 0; c < NQ; ++c)
+          sc = mfma<QT>(*(const u32x4*)(kt + k_lane + ((32 * c) ^ k_x)), qreg[c], sc);
       } else {
 #pragma unroll
         for (int j = 0; j < NQ / 2; ++j) {
@@ -574,98 +593,94 @@ __global__ __launch_bounds__(64 * kWaves, 1) void rlt_tree_kernel(Params P) {
 #pragma unroll
           for (int x = 0; x < 2; ++x) {
             const uint2 lo = widen<QT>(raw[2 * x]), hi = widen<QT>(raw[2 * x + 1]);
-            const u32x4 ka = {lo.x, lo.y, hi.x, hi.y};
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt) sc[nt] = mfma<QT>(ka, qreg[nt][2 * j + x], sc[nt]);
+            sc = mfma<QT>(u32x4{lo.x, lo.y, hi.x, hi.y}, qreg[2 * j + x], sc);
           }
         }
       }
+    };
+    // ---- weights in the log2 domain, packed as the P^T operands.  The running maximum moves
+    // only when a tile's exceeds it by kLazy (weights stay below 2^kLazy), so the accumulators
+    // are rarely rescaled.
+    auto weigh = [&](f32x16& sc, uint32_t (&p)[8], int tb, bool full, const float* scale) {
       if constexpr (SM == 2) {
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
-          const f32x4 x = *(const f32x4*)(sh.scale[w][stage] + 8 * g + 4 * h);
+          const f32x4 x = *(const f32x4*)(scale + 8 * g + 4 * h);
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) sc[nt][4 * g + i] *= x[i];
+          for (int i = 0; i < 4; ++i) sc[4 * g + i] *= x[i];
         }
       }
       if (!full) {
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          // bit 8 g + i: position 8 g + 4 h + i of the tile
-          const uint32_t sees = tile_bits(sh.words[local[nt]], sv.base, sh.lo[local[nt]], tb) >> (4 * h);
-#pragma unroll
-          for (int i = 0; i < 16; ++i)
-            sc[nt][i] = (sees >> (8 * (i >> 2) + (i & 3))) & 1 ? sc[nt][i] : -INFINITY;
-        }
-      }
-      // ---- weights in the log2 domain.  The running maximum moves only when a tile's exceeds
-      // it by kLazy (weights stay below 2^kLazy), so the accumulators are rarely rescaled.
-      uint32_t p[NT][8];
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        float mx = sc[nt][0];
-#pragma unroll
-        for (int i = 1; i < 16; ++i) mx = fmaxf(mx, sc[nt][i]);
-        mx = half_max(mx) * qk_scale;
-        const bool grow = mx > m_run[nt] + kLazy;
-        if (__builtin_amdgcn_ballot_w64(grow) != 0) {
-          const float m_new = grow ? mx : m_run[nt];
-          const float use = m_new == -INFINITY ? 0.f : m_new;
-          const float corr = grow ? __builtin_amdgcn_exp2f(m_run[nt] - use) : 1.f;
-          l_run[nt] *= corr;
-#pragma unroll
-          for (int dt = 0; dt < ND; ++dt) oacc[nt][dt] *= corr;
-          m_run[nt] = m_new;
-          m_use[nt] = use;
-        }
-        float x[16];
+        // bit 8 g + i: position 8 g + 4 h + i of the tile
+        const uint32_t sees = tile_bits(sh.words[local], sv.base, sh.lo[local], tb) >> (4 * h);
 #pragma unroll
         for (int i = 0; i < 16; ++i)
-          x[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[nt][i], qk_scale, -m_use[nt]));
-#pragma unroll
-        for (int g = 0; g < 4; ++g) l_run[nt] += (x[4 * g] + x[4 * g + 1]) + (x[4 * g + 2] + x[4 * g + 3]);
-        if constexpr (SM == 2) {
-#pragma unroll
-          for (int g = 0; g < 4; ++g) {
-            const f32x4 y = *(const f32x4*)(sh.scale[w][stage] + 32 + 8 * g + 4 * h);
-            // (a hidden position's scale may be anything, and its weight is 0)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) x[4 * g + i] = x[4 * g + i] == 0.f ? 0.f : x[4 * g + i] * y[i];
-          }
-        }
-#pragma unroll
-        for (int i = 0; i < 8; ++i) p[nt][i] = pack2<QT>(x[2 * i], x[2 * i + 1]);
+          sc[i] = (sees >> (8 * (i >> 2) + (i & 3))) & 1 ? sc[i] : -INFINITY;
       }
-      // ---- O^T += V^T P^T.  In masked tiles a value may be hidden from some rows, and 0 times
-      // a non-finite value would spoil them: such values are cleared (idempotent: the row waves
-      // may both do it) and marked, and rows that see them get them behind the stream.  Rows
-      // past the sequence belong to no row.
-      if (!full) {
-        const int tile = tb / kTile;
-        const int word = tile >= tree_tile ? min(tile - tree_tile, kBadWords - 1)
-                                           : kBadWords + min(max(tile - first_tile, 0), kBadWords - 1);
+      float mx = sc[0];
 #pragma unroll
-        for (int j = 0; j < G::LOADS; ++j) {
-          const int r = RPL * j + ld_row;
-          if (PIECES == SLOTS || (ld_slot ^ v_swz<SLOTS, FP8>(r)) < PIECES) {
-            u32x4* const at = (u32x4*)(vt + r * G::ROW + ld_slot * 16);
-            if (tb + r >= sv.len) {
-              *at = u32x4{0, 0, 0, 0};
-            } else {
-              const u32x4 x = *at;
-              const u32x4 y = {finite_part<QT, FP8>(x[0]), finite_part<QT, FP8>(x[1]),
-                               finite_part<QT, FP8>(x[2]), finite_part<QT, FP8>(x[3])};
-              if (x[0] != y[0] || x[1] != y[1] || x[2] != y[2] || x[3] != y[3]) {
-                atomicOr(&sh.bad[word], 1u << r);
-                *at = y;
-              }
+      for (int i = 1; i < 16; ++i) mx = fmaxf(mx, sc[i]);
+      mx = half_max(mx) * qk_scale;
+      const bool grow = mx > m_run + kLazy;
+      if (__builtin_amdgcn_ballot_w64(grow) != 0) {
+        const float m_new = grow ? mx : m_run;
+        const float use = m_new == -INFINITY ? 0.f : m_new;
+        const float corr = grow ? __builtin_amdgcn_exp2f(m_run - use) : 1.f;
+        l_run *= corr;
+#pragma unroll
+        for (int dt = 0; dt < ND; ++dt) oacc[dt] *= corr;
+        m_run = m_new;
+        m_use = use;
+      }
+      float x[16];
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        x[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[i], qk_scale, -m_use));
+      float part[4];
+#pragma unroll
+      for (int g = 0; g < 4; ++g) part[g] = (x[4 * g] + x[4 * g + 1]) + (x[4 * g + 2] + x[4 * g + 3]);
+      l_run += (part[0] + part[1]) + (part[2] + part[3]);
+      if constexpr (SM == 2) {
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          const f32x4 y = *(const f32x4*)(scale + 32 + 8 * g + 4 * h);
+          // (a hidden position's scale may be anything, and its weight is 0)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) x[4 * g + i] = x[4 * g + i] == 0.f ? 0.f : x[4 * g + i] * y[i];
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) p[i] = pack2<QT>(x[2 * i], x[2 * i + 1]);
+    };
+    // In masked tiles a value may be hidden from some rows, and 0 times a non-finite value would
+    // spoil them: such values are cleared (idempotent: the row waves may all do it) and marked,
+    // and rows that see them get them behind the stream.  Rows past the sequence belong to no row.
+    auto clean = [&](uint8_t* vt, int tb) {
+      const int tile = tb / kTile;
+      const int word = tile >= tree_tile ? min(tile - tree_tile, kBadWords - 1)
+                                         : kBadWords + min(max(tile - first_tile, 0), kBadWords - 1);
+#pragma unroll
+      for (int j = 0; j < G::LOADS; ++j) {
+        const int r = RPL * j + ld_row;
+        if (PIECES == SLOTS || (ld_slot ^ v_swz<SLOTS, FP8>(r)) < PIECES) {
+          u32x4* const at = (u32x4*)(vt + r * G::ROW + ld_slot * 16);
+          if (tb + r >= sv.len) {
+            *at = u32x4{0, 0, 0, 0};
+          } else {
+            const u32x4 x = *at;
+            const u32x4 y = {finite_part<QT, FP8>(x[0]), finite_part<QT, FP8>(x[1]),
+                             finite_part<QT, FP8>(x[2]), finite_part<QT, FP8>(x[3])};
+            if (x[0] != y[0] || x[1] != y[1] || x[2] != y[2] || x[3] != y[3]) {
+              atomicOr(&sh.bad[word], 1u << r);
+              *at = y;
             }
           }
         }
-        asm volatile("" ::: "memory");
       }
+      asm volatile("" ::: "memory");
+    };
+    // ---- O^T += V^T P^T of the tile in stage `vt`
+    auto product = [&](const uint8_t* vt, const uint32_t (&p)[8]) {
 #pragma unroll
       for (int c = 0; c < 2; ++c)
 #pragma unroll
@@ -690,25 +705,78 @@ __global__ __launch_bounds__(64 * kWaves, 1) void rlt_tree_kernel(Params P) {
             const uint2 lo = widen<QT>((uint32_t)x[0]), hi = widen<QT>((uint32_t)x[1]);
             va = u32x4{lo.x, lo.y, hi.x, hi.y};
           }
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt) {
-            const u32x4 pc = {p[nt][4 * c], p[nt][4 * c + 1], p[nt][4 * c + 2], p[nt][4 * c + 3]};
-            oacc[nt][dt] = mfma<QT>(va, pc, oacc[nt][dt]);
-          }
+          oacc[dt] = mfma<QT>(va, u32x4{p[4 * c], p[4 * c + 1], p[4 * c + 2], p[4 * c + 3]}, oacc[dt]);
         }
-      wait_lds();
+    };
+
+    int tb = first_tb;
+    if constexpr (RW == 1) {
+      int stage = 0, sstage = 0;
+      for (int it = 0; it < tiles; ++it) {
+        uint8_t* const kt = ring + stage * G::TILE;
+        uint8_t* const vt = ring + (S + stage) * G::TILE;
+        const float* const scale = sh.scale[w][sstage];
+        const bool more = it + S < tiles;
+        const bool full = is_full(tb);
+        // (ahead of this tile's keys: its values and the next S - 1 tiles)
+        if (more) wait_loads<LV + (S - 1) * (LK + LV)>();
+        else wait_loads<0>();
+        f32x16 sc;
+        scores(sc, kt);
+        wait_lds();
+        if (more) {
+          next_tile();
+          load_k(stage, sstage == 0 ? S : sstage - 1);
+        }
+        uint32_t p[8];
+        weigh(sc, p, tb, full, scale);
+        if (more) wait_loads<S * LK + (S - 1) * LV>();
+        if (!full) clean(vt, tb);
+        product(vt, p);
+        wait_lds();
+        if (more) load_v(stage);
+        tb += MACRO;
+        stage = stage + 1 == S ? 0 : stage + 1;
+        sstage = sstage == S ? 0 : sstage + 1;
+      }
+    } else {
+      int stage = 0;
+      for (int it = 0; it < tiles; ++it) {
+        if (it + S - 1 < tiles) {
+          wait_loads<(S - 2) * (LK + LV)>();
+          stage_barrier();
+          const int to = stage == 0 ? S - 1 : stage - 1;
+          next_tile();
+          load_k(to, to);
+          load_v(to);
+        } else {
+          wait_loads<0>();
+          stage_barrier();
+        }
+        if (tb < sv.len) {  // wave-uniform: not the last tiles of a macro tile
+          uint8_t* const vt = ring + (S + stage) * G::TILE;
+          const bool full = is_full(tb);
+          f32x16 sc;
+          scores(sc, ring + stage * G::TILE);
+          uint32_t p[8];
+          weigh(sc, p, tb, full, sh.scale[w][stage]);
+          if (!full) clean(vt, tb);
+          product(vt, p);
+        }
+        tb += MACRO;
+        stage = stage + 1 == S ? 0 : stage + 1;
+      }
     }
     wait_loads<0>();
     __syncthreads();  // every wave is done with the ring: the combine buffer takes its place
 
     // ---- the kv groups' states side by side in LDS, then combined in order
     float* const ob = (float*)sh.body;
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      const int r = (rw * NT + nt) * 32 + l32;
-      const float l = half_sum(l_run[nt]);
+    {
+      const int r = rw * 32 + l32;
+      const float l = half_sum(l_run);
       if (h == 0) {
-        sh.ml[kg][r][0] = m_run[nt];
+        sh.ml[kg][r][0] = m_run;
         sh.ml[kg][r][1] = l;
       }
       float* const row = ob + (kg * RB + r) * G::OSTRIDE + 4 * h;
@@ -716,7 +784,7 @@ __global__ __launch_bounds__(64 * kWaves, 1) void rlt_tree_kernel(Params P) {
       for (int dt = 0; dt < ND; ++dt)
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
-          const f32x16& o = oacc[nt][dt];
+          const f32x16& o = oacc[dt];
           *(f32x4*)(row + 32 * dt + 8 * g) = f32x4{o[4 * g], o[4 * g + 1], o[4 * g + 2], o[4 * g + 3]};
         }
     }
@@ -726,6 +794,9 @@ __global__ __launch_bounds__(64 * kWaves, 1) void rlt_tree_kernel(Params P) {
     for (int i = 0; i < 2 * kBadWords; ++i) any_bad |= sh.bad[i];
     const bool whole = n == sp.count;
     const int slot = 2 * blockIdx.x + (f == f_begin ? 0 : 1);
+    if (a == 0 && t == 0)
+      P.splits[((int64_t)seq * P.hkv + kvh) * P.max_blocks + rb] =
+          Split{slot, whole ? -1 : (int)((f + sp.count - 1) / share)};
     float* const part = P.part + (int64_t)slot * RB * (D + 2);
     for (int e = t; e < rows * (D / 4); e += 64 * kWaves) {
       const int r = e / (D / 4), d = 4 * (e % (D / 4));
@@ -736,25 +807,24 @@ __global__ __launch_bounds__(64 * kWaves, 1) void rlt_tree_kernel(Params P) {
       f32x4 o = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int g = 0; g < KW; ++g) {
-        const float mg = sh.ml[g][r][0];
-        const float x = mg == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mg - m);
-        // (a group whose sum is NaN spoils the row, as it should)
-        const float lg = sh.ml[g][r][1];
-        l += mg == -INFINITY && lg == 0.f ? 0.f : lg * x;
+        const float mg = sh.ml[g][r][0], lg = sh.ml[g][r][1];
+        // (a group that saw no key adds nothing; one whose sum is NaN spoils the row)
+        const float x = mg == -INFINITY ? (lg == 0.f ? 0.f : lg) : __builtin_amdgcn_exp2f(mg - m);
         const f32x4 og = *(const f32x4*)(ob + (g * RB + r) * G::OSTRIDE + d);
-        if (mg != -INFINITY || lg != 0.f) o += og * x;
+        l += lg * x;
+        o += og * x;
       }
       const int rho = rb * RB + r;
       if (any_bad) {
         const int local_node = rho / P.group - node0;
         for (int i = 0; i < 2 * kBadWords; ++i) {
-          const int tb = (i < kBadWords ? tree_tile + i : first_tile + i - kBadWords) * kTile;
+          const int at_tile = (i < kBadWords ? tree_tile + i : first_tile + i - kBadWords) * kTile;
           uint32_t left = sh.bad[i];
-          if (left) left &= tile_bits(sh.words[local_node], sv.base, sh.lo[local_node], tb);
+          if (left) left &= tile_bits(sh.words[local_node], sv.base, sh.lo[local_node], at_tile);
           for (; left; left &= left - 1) {
-            const int pos = tb + __builtin_ctz(left);
-            const int32_t e = table[min(pos / P.block_size, P.table_width - 1)];
-            const int64_t at = (int64_t)(e >= 0 && e < P.num_blocks ? e : 0) * P.v_block_stride +
+            const int pos = at_tile + __builtin_ctz(left);
+            const int32_t e2 = table[min(pos / P.block_size, P.table_width - 1)];
+            const int64_t at = (int64_t)(e2 >= 0 && e2 < P.num_blocks ? e2 : 0) * P.v_block_stride +
                                (int64_t)(pos % P.block_size) * P.v_token_stride +
                                (int64_t)kvh * P.v_head_stride + d;
 #pragma unroll
@@ -772,10 +842,7 @@ __global__ __launch_bounds__(64 * kWaves, 1) void rlt_tree_kernel(Params P) {
         *(uint2*)op = make_uint2(pack2<QT>(o[0] * inv, o[1] * inv), pack2<QT>(o[2] * inv, o[3] * inv));
       } else {
         *(f32x4*)(part + r * D + d) = o;
-        if (d == 0) {
-          part[RB * D + 2 * r] = m;
-          part[RB * D + 2 * r + 1] = l;
-        }
+        if (d == 0) *(float2*)(part + RB * D + 2 * r) = make_float2(m, l);
       }
     }
     __syncthreads();  // the ring, the masks and the sums are reused by the next pair
@@ -783,63 +850,85 @@ __global__ __launch_bounds__(64 * kWaves, 1) void rlt_tree_kernel(Params P) {
   }
 }
 
-// The partials of pairs that cross shares, combined in order: one wave per (row, q head).
-// Rows of sequences without a key become zeros here.
-template <int QT, int RB, int MACRO>
-__global__ __launch_bounds__(256) void rlt_tree_merge_kernel(Params P) {
-  const int lane = threadIdx.x & 63;
-  const int seq = blockIdx.x;
-  const int item = blockIdx.y * 4 + (threadIdx.x >> 6);  // (node, q head)
+// The partials of a pair that crosses shares, combined in order: workgroup (pair, y) takes the
+// rows y R .. of it, R rows at a time over lanes of 4 dims, with CG groups of threads that
+// take a run of the contributions each.  Rows of sequences without a key are cleared here.
+constexpr int kMergeThreads = 1024;
+template <int D, int CG>
+constexpr int merge_rows() { return kMergeThreads / CG / (D == 64 ? 16 : D == 256 ? 64 : 32); }
+template <int QT, int D, int RB, int MACRO, int CG>
+__global__ __launch_bounds__(kMergeThreads) void rlt_tree_merge_kernel(Params P) {
+  constexpr int R = merge_rows<D, CG>(), LPR = kMergeThreads / CG / R;
+  __shared__ float sh[CG > 1 ? CG - 1 : 1][kMergeThreads / CG][6];
+  const int t = threadIdx.x, cg = t / (kMergeThreads / CG), u = t % (kMergeThreads / CG);
+  const int r = blockIdx.y * R + u / LPR, d = 4 * (u % LPR);
+  const int rb = blockIdx.x % P.max_blocks, sh_id = blockIdx.x / P.max_blocks;
+  const int kvh = sh_id % P.hkv, seq = sh_id / P.hkv;
+  const Split x = P.splits[blockIdx.x];
   const Seq sv = seq_of(P, seq);
-  const int node = item / P.hq, head = item % P.hq;
-  if (node >= sv.nodes) return;
-  const int D = P.head_dim;
   const Span sp = span_of<RB, MACRO>(P, sv);
-  uint16_t* const op = (uint16_t*)P.out + (int64_t)(sv.q_begin + node) * P.out_row_stride +
-                       (int64_t)head * P.out_head_stride;
+  const int rows = min(RB, sv.nodes * P.group - rb * RB);
+  if (rows <= 0 || (sp.count > 0 && x.last < 0)) return;  // uniform over the workgroup
+  const bool live = r < rows && d < D;
+  f32x4 o = {0.f, 0.f, 0.f, 0.f};
+  float m = -INFINITY, l = 0.f;
+  const int rho = rb * RB + r;
+  uint16_t* const op = (uint16_t*)P.out + (int64_t)(sv.q_begin + rho / P.group) * P.out_row_stride +
+                       (int64_t)(kvh * P.group + rho % P.group) * P.out_head_stride + d;
   if (sp.count == 0) {
-    for (int d = lane; d < D; d += 64) op[d] = 0;
+    if (live && cg == 0) *(uint2*)op = make_uint2(0, 0);
     return;
   }
-  const int rho = node * P.group + head % P.group;
-  const int rb = rho / RB, r = rho % RB;
-  const int64_t share = P.starts[P.num_seqs];
-  const int64_t f0 = P.starts[seq] + ((int64_t)(head / P.group) * sp.blocks + rb) * sp.count;
-  const int b0 = (int)(f0 / share), b1 = (int)((f0 + sp.count - 1) / share);
-  if (b0 == b1) return;  // normalized where it was computed
-  auto slot_of = [&](int b) { return 2 * b + (b == b0 && f0 != b * share ? 1 : 0); };
-  const int64_t stride = (int64_t)RB * (D + 2);
-  // the overall maximum: lanes take the contributions
-  float m = -INFINITY;
-  for (int b = b0 + lane; b <= b1; b += 64)
-    m = fmaxf(m, P.part[slot_of(b) * stride + RB * D + 2 * r]);
+  // state (m, l, o) joined with another one; a state without a key has m = -inf, l = 0
+  auto join = [&](float m2, float l2, const f32x4& o2) {
+    const float mo = fmaxf(m, m2);
+    const float a = m == -INFINITY ? (l == 0.f ? 0.f : l) : __builtin_amdgcn_exp2f(m - mo);
+    const float b = m2 == -INFINITY ? (l2 == 0.f ? 0.f : l2) : __builtin_amdgcn_exp2f(m2 - mo);
+    l = l * a + l2 * b;
+    o = o * a + o2 * b;
+    m = mo;
+  };
+  constexpr int64_t stride = (int64_t)RB * (D + 2);
+  const int b0 = x.first >> 1, count = x.last - b0 + 1, per = (count + CG - 1) / CG;
+  const int i0 = cg * per, i1 = min(i0 + per, count);
+  if (live) {
+    constexpr int AHEAD = 4;
+    for (int i = i0; i < i1; i += AHEAD) {
+      float2 ml[AHEAD];
+      f32x4 oo[AHEAD];
 #pragma unroll
-  for (int o = 1; o < 64; o <<= 1) m = fmaxf(m, __shfl_xor(m, o, RLT_WAVE));
-  float acc[4] = {0.f, 0.f, 0.f, 0.f};  // dims lane, lane + 64, ..
-  float l = 0.f;
-#pragma unroll 4
-  for (int b = b0; b <= b1; ++b) {
-    const float* const part = P.part + slot_of(b) * stride;
-    const float mb = part[RB * D + 2 * r], lb = part[RB * D + 2 * r + 1];
-    const bool live = mb != -INFINITY || lb != 0.f;
-    const float x = mb == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mb - m);
-    if (live) l += lb * x;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int d = lane + 64 * i;
-      if (d < D) {
-        const float o = part[r * D + d];
-        if (live) acc[i] += o * x;
+      for (int k = 0; k < AHEAD; ++k) {
+        const int at = min(i + k, i1 - 1);
+        const float* const part =
+            P.part + (at == 0 ? (int64_t)x.first : 2 * (int64_t)(b0 + at)) * stride;
+        ml[k] = *(const float2*)(part + RB * D + 2 * r);
+        oo[k] = *(const f32x4*)(part + r * D + d);
       }
+#pragma unroll
+      for (int k = 0; k < AHEAD; ++k)
+        if (i + k < i1) join(ml[k].x, ml[k].y, oo[k]);
     }
   }
+  if constexpr (CG > 1) {
+    if (cg > 0) {
+      float* const s = sh[cg - 1][u];
+      s[0] = m;
+      s[1] = l;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) s[2 + c] = o[c];
+    }
+    __syncthreads();
+    if (cg > 0) return;
+#pragma unroll
+    for (int g = 0; g < CG - 1; ++g) {
+      const float* const s = sh[g][u];
+      join(s[0], s[1], f32x4{s[2], s[3], s[4], s[5]});
+    }
+  }
+  if (!live) return;
   const float v_mul = P.scale_mode == 1 ? P.v_scale[0] : 1.f;
   const float inv = l == 0.f ? 0.f : v_mul / l;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int d = lane + 64 * i;
-    if (d < D) store_from_f32<QT>(op, d, acc[i] * inv);
-  }
+  *(uint2*)op = make_uint2(pack2<QT>(o[0] * inv, o[1] * inv), pack2<QT>(o[2] * inv, o[3] * inv));
 }
 
 }  // namespace tree

@@ -120,28 +120,39 @@ __global__ __launch_bounds__(256) void rlt_tree_vec_kernel(Params P) {
 
 // ---------------------------------------------------------------- launches
 
-template <int QT, int KVT, int D, int SM, int NT, int RW>
+template <int QT, int KVT, int D, int SM, int RW>
 void launch(const Params& P, hipStream_t stream) {
-  using G = Geometry<QT, KVT, D, NT, RW>;
-  hipLaunchKernelGGL((rlt_tree_kernel<QT, KVT, D, SM, NT, RW>), dim3(kGrid), dim3(64 * kWaves), 0, stream, P);
-  const dim3 grid((unsigned)P.num_seqs, (unsigned)((P.max_q * P.hq + 3) / 4));
-  hipLaunchKernelGGL((rlt_tree_merge_kernel<QT, G::RB, G::MACRO>), grid, dim3(256), 0, stream, P);
+  using G = Geometry<QT, KVT, D, RW>;
+  hipLaunchKernelGGL((rlt_tree_kernel<QT, KVT, D, SM, RW>), dim3(grid_of<D>()), dim3(64 * kWaves), 0, stream, P);
+  // few pairs have many contributions each: more workgroups a pair, more threads a row
+  const int64_t pairs = (int64_t)P.num_seqs * P.hkv * P.max_blocks;
+  const int rows = P.max_q * P.group < G::RB ? P.max_q * P.group : G::RB;
+  auto merge = [&](auto cg) {
+    constexpr int CG = decltype(cg)::value, R = merge_rows<D, CG>();
+    hipLaunchKernelGGL((rlt_tree_merge_kernel<QT, D, G::RB, G::MACRO, CG>),
+                       dim3((unsigned)pairs, (unsigned)((rows + R - 1) / R)), dim3(kMergeThreads), 0,
+                       stream, P);
+  };
+  if (pairs < 64) merge(std::integral_constant<int, 4>{});
+  else merge(std::integral_constant<int, 1>{});
 }
 
-// Row tiles per wave and row waves: the fewest that hold the rows of a kv head.
+// Row waves: the fewest that hold the rows of a kv head, at most four (further rows are further
+// blocks).
+int row_waves(int rows, int head_dim, bool fp8) {
+  if (head_dim == 256 && !fp8) return 4;  // two stages of its tiles fit one kv group only
+  return rows <= 32 ? 1 : rows <= 64 ? 2 : 4;
+}
+
 template <int QT, int KVT, int D, int SM>
 void launch_rows(const Params& P, hipStream_t stream) {
-  const int rows = P.max_q * P.group;
-  if constexpr (D == 256) {
-    if constexpr (KVT != QT) {
-      if (rows <= 32) return launch<QT, KVT, D, SM, 1, 1>(P, stream);
-    }
-    return launch<QT, KVT, D, SM, 1, 2>(P, stream);
-  } else {
-    if (rows <= 32) return launch<QT, KVT, D, SM, 1, 1>(P, stream);
-    if (rows <= 64) return launch<QT, KVT, D, SM, 2, 1>(P, stream);
-    return launch<QT, KVT, D, SM, 2, 2>(P, stream);
+  constexpr bool fp8 = KVT != QT;
+  const int rw = row_waves(P.max_q * P.group, D, fp8);
+  if constexpr (D != 256 || fp8) {
+    if (rw == 1) return launch<QT, KVT, D, SM, 1>(P, stream);
+    if (rw == 2) return launch<QT, KVT, D, SM, 2>(P, stream);
   }
+  return launch<QT, KVT, D, SM, 4>(P, stream);
 }
 
 template <int QT, int KVT, int SM>
@@ -173,18 +184,20 @@ int launch_vec(const Params& P, int kv_dtype, hipStream_t stream) {
 
 bool mfma_dim(int d) { return d == 64 || d == 96 || d == 128 || d == 256; }
 
-// rows of a block, at most (the partials' size)
-int block_rows(int head_dim) { return head_dim == 256 ? 64 : 128; }
-
 }  // namespace tree
 
 extern "C" {
 
-size_t rlt_tree_attention_workspace_size(int32_t num_seqs, int32_t head_dim) {
-  if (num_seqs < 0 || head_dim <= 0) return 0;
-  if (!tree::mfma_dim(head_dim)) return 0;
-  return rlt_align_up((size_t)(num_seqs + 1) * sizeof(int64_t), 256) +
-         (size_t)2 * tree::kGrid * tree::block_rows(head_dim) * (head_dim + 2) * sizeof(float);
+size_t rlt_tree_attention_workspace_size(int32_t num_seqs, int32_t max_q_len, int32_t num_q_heads,
+                                         int32_t num_kv_heads, int32_t head_dim, int32_t kv_dtype) {
+  if (num_seqs <= 0 || max_q_len <= 0 || num_q_heads <= 0 || num_kv_heads <= 0 ||
+      !tree::mfma_dim(head_dim))
+    return 0;
+  const int64_t rows = (int64_t)max_q_len * (num_q_heads / num_kv_heads);
+  const int rb = 32 * tree::row_waves((int)(rows < 1024 ? rows : 1024), head_dim, kv_dtype == RLT_FP8_E4M3);
+  const int64_t pairs = (int64_t)num_seqs * num_kv_heads * ((rows + rb - 1) / rb);
+  return rlt_align_up((size_t)pairs * sizeof(tree::Split), 256) +
+         (size_t)2 * tree::kGrid * rb * (head_dim + 2) * sizeof(float);
 }
 
 int rlt_tree_attention(const void* q, int64_t q_row_stride, int64_t q_head_stride,
@@ -220,8 +233,14 @@ int rlt_tree_attention(const void* q, int64_t q_row_stride, int64_t q_head_strid
   if (mask_words <= 0 || (int64_t)mask_words * 64 < max_q_len || mask_stride < mask_words ||
       (uintptr_t)tree_mask % 8)
     return RLT_ERR_ARGUMENT;
-  if ((int64_t)table_width * block_size > INT32_MAX - 4096) return RLT_ERR_UNSUPPORTED;
-  if (workspace_bytes < rlt_tree_attention_workspace_size(num_seqs, head_dim)) return RLT_ERR_WORKSPACE;
+  // positions, and a sequence's macro tiles over its kv heads and row blocks, in 32 bits
+  const int64_t cap = (int64_t)table_width * block_size;
+  const int64_t blocks = ((int64_t)max_q_len * (num_q_heads / num_kv_heads) + 31) / 32;
+  if (cap > INT32_MAX - 4096 || (cap / kTile + 1) * num_kv_heads * blocks > INT32_MAX)
+    return RLT_ERR_UNSUPPORTED;
+  const size_t need = rlt_tree_attention_workspace_size(
+      num_seqs, max_q_len, num_q_heads, num_kv_heads, head_dim, kv_dtype);
+  if (workspace_bytes < need || (need && (!workspace || (uintptr_t)workspace % 16))) return RLT_ERR_WORKSPACE;
 
   Params P;
   P.q = q;
@@ -251,7 +270,7 @@ int rlt_tree_attention(const void* q, int64_t q_row_stride, int64_t q_head_strid
   P.s_head_stride = s_head_stride;
   P.num_seqs = num_seqs;
   P.num_rows = num_q_rows;
-  P.max_q = max_q_len < num_q_rows ? max_q_len : num_q_rows;
+  P.max_q = max_q_len;
   P.hq = num_q_heads;
   P.hkv = num_kv_heads;
   P.group = num_q_heads / num_kv_heads;
@@ -277,13 +296,18 @@ int rlt_tree_attention(const void* q, int64_t q_row_stride, int64_t q_head_strid
       (uintptr_t)out % 8 == 0 && ((out_row_stride | out_head_stride) * 2) % 8 == 0 &&
       k_token_stride >= 0 && k_token_stride < far && v_token_stride >= 0 && v_token_stride < far;
   if (mfma) {
-    P.starts = (int64_t*)workspace;
-    P.part = (float*)((char*)workspace + rlt_align_up((size_t)(num_seqs + 1) * sizeof(int64_t), 256));
+    const int rb = 32 * row_waves(P.max_q * P.group, head_dim, kv_dtype == RLT_FP8_E4M3);
+    P.max_blocks = (P.max_q * P.group + rb - 1) / rb;
+    const int64_t pairs = (int64_t)num_seqs * num_kv_heads * P.max_blocks;
+    if (pairs > INT32_MAX) return RLT_ERR_UNSUPPORTED;
+    P.splits = (Split*)workspace;
+    P.part = (float*)((char*)workspace + rlt_align_up((size_t)pairs * sizeof(Split), 256));
     if (q_dtype == RLT_BF16) launch_mfma<RLT_BF16>(P, kv_dtype, stream);
     else launch_mfma<RLT_F16>(P, kv_dtype, stream);
     return rlt_launch_status();
   }
-  P.starts = nullptr;
+  P.splits = nullptr;
+  P.max_blocks = 0;
   P.part = nullptr;
   if ((int64_t)P.max_q * num_q_heads > 65535) return RLT_ERR_UNSUPPORTED;
   switch (q_dtype) {
