@@ -35,9 +35,11 @@ namespace tree {
 // the slots 2 b of the workgroups b up to `last`; last < 0: normalized where it was computed.
 struct Split {
   int32_t first, last;
+  int32_t row;  // of the slots' rows, the pair's first
 };
 
 constexpr int kWaves = 4;
+constexpr int kPartRows = 32 * kWaves;  // rows of a partial, at most
 constexpr int kTile = 32;          // key positions per LDS tile
 constexpr int kGrid = 512;         // persistent workgroups, at most: two per CU
 // (256 dims: the states of a workgroup take more than half of a CU's LDS and registers)
@@ -49,6 +51,7 @@ constexpr int kMaxNodes = 256;     // nodes of one sequence's tree
 constexpr int kWords = kMaxNodes / 64;
 constexpr int kRingBytes = 64 << 10;
 constexpr int kBadWords = kMaxNodes / kTile + 3;  // tiles that a range of kMaxNodes meets
+constexpr int kApartTiles = 8;     // tiles per workgroup from which kv groups take heads apart
 constexpr float kLazy = 8.f;       // log2 headroom before the running max moves
 
 struct Params {
@@ -77,7 +80,7 @@ struct Params {
   int64_t out_row_stride, out_head_stride;
   int32_t max_blocks;     // row blocks of the longest tree
   struct Split* splits;   // [num_seqs][hkv][max_blocks]
-  float* part;            // [2 * kGrid][rows per block * (head_dim + 2)]
+  float* part;            // [2 * kGrid][kPartRows * (head_dim + 2)]
 };
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
@@ -226,23 +229,22 @@ __device__ __forceinline__ int first_position(const Params& P, const Seq& v) {
   return P.window > 0 ? max(0, v.base - P.window) : 0;
 }
 
-// Macro tiles [m0, m0 + count) of one (kv head, row block) pair of the sequence, and its
-// row blocks.
+// Macro tiles [m0, m0 + count) of `macro` positions (a power of two of tiles) of one pair of
+// the sequence, and its row blocks.
 struct Span {
   int m0, count, blocks;
 };
-template <int RB, int MACRO>
-__device__ __forceinline__ Span span_of(const Params& P, const Seq& v) {
+template <int RB>
+__device__ __forceinline__ Span span_of(const Params& P, const Seq& v, int macro) {
   Span x;
   x.blocks = (v.nodes * P.group + RB - 1) / RB;
-  x.m0 = first_position(P, v) / MACRO;
-  x.count = x.blocks ? max(0, (v.len + MACRO - 1) / MACRO - x.m0) : 0;
+  x.m0 = first_position(P, v) / macro;
+  x.count = x.blocks ? max(0, (v.len + macro - 1) / macro - x.m0) : 0;
   return x;
 }
-
-template <int RB, int MACRO>
-__device__ __forceinline__ Span uniform_span(const Params& P, const Seq& v) {
-  Span x = span_of<RB, MACRO>(P, v);
+template <int RB>
+__device__ __forceinline__ Span uniform_span(const Params& P, const Seq& v, int macro) {
+  Span x = span_of<RB>(P, v, macro);
   x.m0 = uniform(x.m0);
   x.count = uniform(x.count);
   x.blocks = uniform(x.blocks);
@@ -308,7 +310,6 @@ struct Geometry {
   static constexpr int ELT = FP8 ? 1 : 2;
   static constexpr int KW = kWaves / RW;
   static constexpr int RB = 32 * RW;                 // rows per block
-  static constexpr int MACRO = kTile * KW;           // positions per macro tile
   static constexpr int ROW = (D == 96 ? 128 : D) * ELT;  // bytes of an LDS row
   static constexpr int SLOTS = ROW / 16;
   static constexpr int PIECES = D * ELT / 16;        // 16-byte pieces of a row in the pool
@@ -331,12 +332,13 @@ template <int QT, int KVT, int D, int RW>
 struct Shared {
   using G = Geometry<QT, KVT, D, RW>;
   alignas(16) uint8_t body[G::BODY];                 // the ring, then the combine buffer
-  alignas(16) float scale[kWaves][G::S + 1][64];     // per wave: 32 key, 32 value scales
+  // per kv group and stage, for each row wave: its positions' key scales, then value scales
+  alignas(16) float scale[G::KW][G::S + 1][64];
   uint64_t words[G::RB][kWords];                     // mask words of the row block's nodes
   int lo[G::RB];
   float ml[G::KW][G::RB][2];
   uint32_t bad[2 * kBadWords];  // positions with a non-finite value in masked tiles
-  int64_t totals[kWaves];
+  int64_t totals[2][kWaves];
   int find_seq;
   int64_t find_start;
 };
@@ -356,7 +358,7 @@ template <int QT, int KVT, int D, int SM, int RW>
 __global__ __launch_bounds__(64 * kWaves, per_cu<D>()) void rlt_tree_kernel(Params P) {
   using G = Geometry<QT, KVT, D, RW>;
   constexpr bool FP8 = G::FP8;
-  constexpr int ELT = G::ELT, KW = G::KW, RB = G::RB, MACRO = G::MACRO, S = G::S;
+  constexpr int ELT = G::ELT, KW = G::KW, RB = G::RB, S = G::S;
   constexpr int SLOTS = G::SLOTS, PIECES = G::PIECES, RPL = G::RPL;
   constexpr int NQ = D / 16;  // contraction slices of S^T
   constexpr int ND = D / 32;  // dim tiles of O^T
@@ -366,26 +368,43 @@ __global__ __launch_bounds__(64 * kWaves, per_cu<D>()) void rlt_tree_kernel(Para
   const int w = __builtin_amdgcn_readfirstlane(t >> 6);
   const int kg = w / RW, rw = w % RW;  // kv group, row wave
 
-  // ---- this workgroup's share of the macro tiles
+  // ---- this workgroup's share of the macro tiles, in both forms: the kv groups on one head's
+  // neighbouring tiles, or (`apart`) each on its own one of KW neighbouring heads
   const int per = (P.num_seqs + 64 * kWaves - 1) / (64 * kWaves);
   const int s_lo = min(t * per, P.num_seqs), s_hi = min(s_lo + per, P.num_seqs);
-  int64_t run = 0;
+  const int head_groups = (P.hkv + KW - 1) / KW;
+  int64_t run = 0, run_apart = 0;
   for (int s = s_lo; s < s_hi; ++s) {
-    const Span x = span_of<RB, MACRO>(P, seq_of(P, s));
+    const Seq v = seq_of(P, s);
+    const Span x = span_of<RB>(P, v, kTile * KW), y = span_of<RB>(P, v, kTile);
     run += (int64_t)x.count * x.blocks * P.hkv;
+    run_apart += (int64_t)y.count * y.blocks * head_groups;
   }
-  int64_t incl = run;
+  int64_t incl = run, incl_apart = run_apart;
 #pragma unroll
   for (int o = 1; o < 64; o <<= 1) {
-    const int64_t y = __shfl_up(incl, o, RLT_WAVE);
-    if (lane >= o) incl += y;
+    const int64_t y = __shfl_up(incl, o, RLT_WAVE), z = __shfl_up(incl_apart, o, RLT_WAVE);
+    if (lane >= o) {
+      incl += y;
+      incl_apart += z;
+    }
   }
-  if (lane == 63) sh.totals[w] = incl;
+  if (lane == 63) {
+    sh.totals[0][w] = incl;
+    sh.totals[1][w] = incl_apart;
+  }
   __syncthreads();
-  int64_t before = incl - run, total = 0;
+  int64_t total_apart = 0;
+  for (int i = 0; i < kWaves; ++i) total_apart += sh.totals[1][i];
+  const bool apart = KW > 1 && P.hkv > 1 && uniform(total_apart) >= (int64_t)kApartTiles * grid_of<D>();
+  const int macro = apart ? kTile : kTile * KW;
+  const int units = apart ? head_groups : P.hkv;
+  int64_t before = apart ? incl_apart - run_apart : incl - run, total = 0;
+  if (apart) run = run_apart;
   for (int i = 0; i < kWaves; ++i) {
-    if (i < w) before += sh.totals[i];
-    total += sh.totals[i];
+    const int64_t x = sh.totals[apart ? 1 : 0][i];
+    if (i < w) before += x;
+    total += x;
   }
   total = uniform(total);
   const int64_t share = (total + grid_of<D>() - 1) / grid_of<D>();
@@ -395,8 +414,8 @@ __global__ __launch_bounds__(64 * kWaves, per_cu<D>()) void rlt_tree_kernel(Para
   if (before <= f_begin && f_begin < before + run) {
     int64_t at = before;
     for (int s = s_lo; s < s_hi; ++s) {
-      const Span x = span_of<RB, MACRO>(P, seq_of(P, s));
-      const int64_t n = (int64_t)x.count * x.blocks * P.hkv;
+      const Span x = span_of<RB>(P, seq_of(P, s), macro);
+      const int64_t n = (int64_t)x.count * x.blocks * units;
       if (f_begin < at + n) {
         sh.find_seq = s;
         sh.find_start = at;
@@ -409,14 +428,21 @@ __global__ __launch_bounds__(64 * kWaves, per_cu<D>()) void rlt_tree_kernel(Para
   int seq = uniform(sh.find_seq);
   int64_t seq_start = uniform(sh.find_start);
   Seq sv = uniform_seq(P, seq);
-  Span sp = uniform_span<RB, MACRO>(P, sv);
+  Span sp = uniform_span<RB>(P, sv, macro);
 
-  // ---- lane constants of the loads: lane L of load j fills row RPL j + L / SLOTS, slot L % SLOTS
+  // ---- lane constants of the loads: a wave's LV loads fill RPL rows each from row ld_first of a
+  // tile on, lane L row L / SLOTS and slot L % SLOTS of them (of fewer loads than row waves
+  // some are done twice); of the per-vector scales it takes positions SP rw .. SP rw + SP - 1
+  constexpr int DUP = G::LOADS >= RW ? 1 : RW / G::LOADS;
+  constexpr int NG = LV * RPL / 8;
+  constexpr int SP = kTile / RW;
   const int ld_row = lane / SLOTS, ld_slot = lane % SLOTS;
+  const int ld_first = rw / DUP * (LV * RPL);
+  const int sc_first = SP * rw - ld_first;
   const uint32_t k_tok = (uint32_t)P.k_token_stride * ELT, v_tok = (uint32_t)P.v_token_stride * ELT;
   uint8_t* const ring = sh.body + kg * (S * 2 * G::TILE);  // the group's S key tiles, then S value tiles
   // (block, offset) of a tile's first position: advanced without a division
-  const int step_q = uniform(MACRO / P.block_size), step_r = MACRO - step_q * P.block_size;
+  const int step_q = uniform(macro / P.block_size), step_r = macro - step_q * P.block_size;
 
   float qk_scale = P.qk_scale_log2, v_mul = 1.f;
   if (SM == 1) {
@@ -440,33 +466,41 @@ __global__ __launch_bounds__(64 * kWaves, per_cu<D>()) void rlt_tree_kernel(Para
   int64_t f = f_begin;
   while (f < f_end) {
     // ---- the pair and the part [a, b) of its macro tiles that this share holds
-    while (f >= seq_start + (int64_t)sp.count * sp.blocks * P.hkv) {
-      seq_start += (int64_t)sp.count * sp.blocks * P.hkv;
+    while (f >= seq_start + (int64_t)sp.count * sp.blocks * units) {
+      seq_start += (int64_t)sp.count * sp.blocks * units;
       ++seq;
       sv = uniform_seq(P, seq);
-      sp = uniform_span<RB, MACRO>(P, sv);
+      sp = uniform_span<RB>(P, sv, macro);
     }
     const uint32_t in_seq = (uint32_t)(f - seq_start);
     const int pair = uniform((int)(in_seq / (uint32_t)sp.count));
     const int a = (int)(in_seq - (uint32_t)pair * sp.count);
     const int n = (int)min((int64_t)(sp.count - a), f_end - f);
-    const int kvh = uniform(pair / sp.blocks), rb = pair - kvh * sp.blocks;
+    const int unit = uniform(pair / sp.blocks), rb = pair - unit * sp.blocks;
+    const int head0 = apart ? unit * KW : unit, heads = apart ? min(KW, P.hkv - head0) : 1;
+    const bool alive = !apart || kg < heads;  // (the last heads may be fewer than the kv groups)
+    const int kvh = alive ? head0 + (apart ? kg : 0) : head0;
     const int rows = min(RB, sv.nodes * P.group - rb * RB);
     const int node0 = rb * RB / P.group;
 
     // ---- loads of the next tile of the group
-    const auto* table = (const __attribute__((address_space(4))) int32_t*)(
-        P.tables + (int64_t)seq * P.table_stride);
+    // (constant address space and scalar addresses: scalar loads, which the vector loads'
+    // counter does not see -- a wait for a vector load would wait for all tiles in flight)
+    const auto* table = (const __attribute__((address_space(4))) int32_t*)uniform(
+        (int64_t)(P.tables + (int64_t)seq * P.table_stride));
     const uint8_t* const k_head = (const uint8_t*)P.k + (int64_t)kvh * P.k_head_stride * ELT;
     const uint8_t* const v_head = (const uint8_t*)P.v + (int64_t)kvh * P.v_head_stride * ELT;
-    const int first_tb = ((sp.m0 + a) * KW + kg) * kTile;
-    int next_idx = uniform(first_tb / P.block_size), next_off = first_tb - next_idx * P.block_size;
-    int blk[4], off[4];  // of the tile's four 8-position groups (blocks hold whole groups)
+    const int first_tb = (sp.m0 + a) * macro + (apart ? 0 : kg * kTile);
+    // this wave's rows of a tile are whole 8-position groups, and so are the pool's blocks: a
+    // scalar (block, offset) per group
+    const int cur = first_tb + ld_first;
+    int next_idx = uniform(cur / P.block_size), next_off = cur - next_idx * P.block_size;
+    int blk[NG], off[NG];
     auto next_tile = [&]() {
       int idx = next_idx, o = next_off;
 #pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const int32_t e = table[min(idx, P.table_width - 1)];
+      for (int g = 0; g < NG; ++g) {
+        const int32_t e = table[uniform(min(idx, P.table_width - 1))];
         blk[g] = e >= 0 && e < P.num_blocks ? e : 0;
         off[g] = o;
         o += 8;
@@ -483,25 +517,21 @@ __global__ __launch_bounds__(64 * kWaves, per_cu<D>()) void rlt_tree_kernel(Para
       }
     };
     auto load_rows = [&](const uint8_t* head, int64_t bs, uint32_t tok, uint8_t* dst, auto swz) {
-      const uint8_t* base[4];
+      const uint8_t* base[NG];
 #pragma unroll
-      for (int g = 0; g < 4; ++g)
+      for (int g = 0; g < NG; ++g)
         base[g] = head + uniform((int64_t)blk[g] * (bs * ELT) + (int64_t)((uint64_t)((uint32_t)off[g]) * tok));
+      const uint32_t to = lds_offset(dst) + ld_first * G::ROW;
 #pragma unroll
       for (int i = 0; i < LV; ++i) {
-        const int j = (i * RW + rw) % G::LOADS;  // wave-uniform
-        const int r0 = RPL * j;
-        const int piece = ld_slot ^ swz(r0 + ld_row);
+        const int piece = ld_slot ^ swz(ld_first + RPL * i + ld_row);
         if (PIECES == SLOTS || piece < PIECES) {
-          const uint32_t lds = uniform((int)(lds_offset(dst) + r0 * G::ROW));
+          const uint32_t lds = uniform((int)(to + RPL * i * G::ROW));
           if constexpr (RPL <= 8) {
-            const int g = r0 >> 3;
-            const uint8_t* const at = g == 0 ? base[0] : g == 1 ? base[1] : g == 2 ? base[2] : base[3];
-            load_lds16(at, (uint32_t)((r0 & 7) + ld_row) * tok + piece * 16, lds);
+            load_lds16(base[RPL * i >> 3], (uint32_t)((RPL * i & 7) + ld_row) * tok + piece * 16, lds);
           } else {
             // 16 rows per load: two groups
-            const bool up = ld_row >= 8;
-            const uint8_t* const at = r0 == 0 ? (up ? base[1] : base[0]) : (up ? base[3] : base[2]);
+            const uint8_t* const at = ld_row >= 8 ? base[2 * i + 1] : base[2 * i];
             load_lds16(at + (uint32_t)(ld_row & 7) * tok + piece * 16, lds);
           }
         }
@@ -511,12 +541,20 @@ __global__ __launch_bounds__(64 * kWaves, per_cu<D>()) void rlt_tree_kernel(Para
       load_rows(k_head, P.k_block_stride, k_tok, ring + stage * G::TILE,
                 [](int r) { return k_swz<SLOTS>(r); });
       if constexpr (SM == 2) {
-        const int g = l32 >> 3;
-        const int64_t bk = g == 0 ? blk[0] : g == 1 ? blk[1] : g == 2 ? blk[2] : blk[3];
-        const int og = g == 0 ? off[0] : g == 1 ? off[1] : g == 2 ? off[2] : off[3];
-        load_lds4((h ? P.v_scale : P.k_scale) + bk * P.s_block_stride +
-                      (int64_t)(og + (l32 & 7)) * P.s_token_stride + (int64_t)kvh * P.s_head_stride,
-                  uniform((int)lds_offset(sh.scale[w][scale_stage])));
+        // the wave's share of the tile's scales: SP key scales, then SP value scales
+        if (lane < 2 * SP) {
+          const int at = sc_first + (lane & (SP - 1)), g = at >> 3;
+          int64_t bk = blk[0];
+          int og = off[0];
+#pragma unroll
+          for (int x = 1; x < NG; ++x) {
+            bk = g == x ? blk[x] : bk;
+            og = g == x ? off[x] : og;
+          }
+          load_lds4((lane >= SP ? P.v_scale : P.k_scale) + bk * P.s_block_stride +
+                        (int64_t)(og + (at & 7)) * P.s_token_stride + (int64_t)kvh * P.s_head_stride,
+                    uniform((int)lds_offset(&sh.scale[kg][scale_stage][2 * SP * rw])));
+        }
       }
     };
     auto load_v = [&](int stage) {
@@ -525,7 +563,7 @@ __global__ __launch_bounds__(64 * kWaves, per_cu<D>()) void rlt_tree_kernel(Para
     };
 
     // this wave's tiles: a row wave's barriers are the workgroup's, so those of KW groups alike
-    const int tiles = RW > 1 ? n : max(0, min(n, (sv.len - first_tb + MACRO - 1) / MACRO));
+    const int tiles = RW > 1 ? n : alive ? max(0, min(n, (sv.len - first_tb + macro - 1) / macro)) : 0;
     if constexpr (RW == 1) {
 #pragma unroll
       for (int i = 0; i < S; ++i)
@@ -536,7 +574,7 @@ __global__ __launch_bounds__(64 * kWaves, per_cu<D>()) void rlt_tree_kernel(Para
         }
     } else {
 #pragma unroll 1
-      for (int i = 0; i < S - 1 && i < tiles; ++i) {
+      for (int i = 0; i < S - 1 && i < tiles && alive; ++i) {
         next_tile();
         load_k(i, i);
         load_v(i);
@@ -559,6 +597,9 @@ __global__ __launch_bounds__(64 * kWaves, per_cu<D>()) void rlt_tree_kernel(Para
         const int e = FP8 ? 32 * (c / 2) + 16 * h + 8 * (c % 2) : 16 * c + 8 * h;
         qreg[c] = r < rows ? *(const u32x4*)(qp + e) : u32x4{0, 0, 0, 0};
       }
+      // (arrived here: a wait at their use would wait for every tile in flight, in every step)
+#pragma unroll
+      for (int c = 0; c < NQ; ++c) asm volatile("" : "+v"(qreg[c]));
     }
     const int nodes_here = min(sv.nodes - node0, (rows + rb * RB - node0 * P.group + P.group - 1) / P.group);
     if (t < nodes_here) sh.lo[t] = node_mask(P, sv, node0 + t, sh.words[t]);
@@ -578,34 +619,35 @@ __global__ __launch_bounds__(64 * kWaves, per_cu<D>()) void rlt_tree_kernel(Para
     auto is_full = [&](int tb) {
       return tb + kTile <= sv.base && (P.window <= 0 || tb >= sv.len - P.window);
     };
-    // ---- S^T = K Q^T of the tile in stage `kt`
+    // ---- S^T = K Q^T of the tile in stage `kt`; all operand reads in flight together
     auto scores = [&](f32x16& sc, const uint8_t* kt) {
+      constexpr int NR = FP8 ? NQ / 2 : NQ;
+      u32x4 raw[NR];
+#pragma unroll
+      for (int c = 0; c < NR; ++c) raw[c] = *(const u32x4*)(kt + k_lane + ((32 * c) ^ k_x));
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int i = 0; i < 16; ++i) sc[i] = 0.f;
       if constexpr (!FP8) {
 #pragma unroll
-        for (int c = 0; c < NQ; ++c)
-          sc = mfma<QT>(*(const u32x4*)(kt + k_lane + ((32 * c) ^ k_x)), qreg[c], sc);
+        for (int c = 0; c < NQ; ++c) sc = mfma<QT>(raw[c], qreg[c], sc);
       } else {
 #pragma unroll
-        for (int j = 0; j < NQ / 2; ++j) {
-          const u32x4 raw = *(const u32x4*)(kt + k_lane + ((32 * j) ^ k_x));
-#pragma unroll
-          for (int x = 0; x < 2; ++x) {
-            const uint2 lo = widen<QT>(raw[2 * x]), hi = widen<QT>(raw[2 * x + 1]);
-            sc = mfma<QT>(u32x4{lo.x, lo.y, hi.x, hi.y}, qreg[2 * j + x], sc);
-          }
+        for (int c = 0; c < NQ; ++c) {
+          const uint2 lo = widen<QT>(raw[c / 2][2 * (c % 2)]), hi = widen<QT>(raw[c / 2][2 * (c % 2) + 1]);
+          sc = mfma<QT>(u32x4{lo.x, lo.y, hi.x, hi.y}, qreg[c], sc);
         }
       }
     };
     // ---- weights in the log2 domain, packed as the P^T operands.  The running maximum moves
     // only when a tile's exceeds it by kLazy (weights stay below 2^kLazy), so the accumulators
     // are rarely rescaled.
+    auto scale_at = [](int pos) { return pos / SP * (2 * SP) + pos % SP; };
     auto weigh = [&](f32x16& sc, uint32_t (&p)[8], int tb, bool full, const float* scale) {
       if constexpr (SM == 2) {
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
-          const f32x4 x = *(const f32x4*)(scale + 8 * g + 4 * h);
+          const f32x4 x = *(const f32x4*)(scale + scale_at(8 * g + 4 * h));
 #pragma unroll
           for (int i = 0; i < 4; ++i) sc[4 * g + i] *= x[i];
         }
@@ -643,7 +685,7 @@ __global__ __launch_bounds__(64 * kWaves, per_cu<D>()) void rlt_tree_kernel(Para
       if constexpr (SM == 2) {
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
-          const f32x4 y = *(const f32x4*)(scale + 32 + 8 * g + 4 * h);
+          const f32x4 y = *(const f32x4*)(scale + scale_at(8 * g + 4 * h) + SP);
           // (a hidden position's scale may be anything, and its weight is 0)
 #pragma unroll
           for (int i = 0; i < 4; ++i) x[4 * g + i] = x[4 * g + i] == 0.f ? 0.f : x[4 * g + i] * y[i];
@@ -679,34 +721,46 @@ __global__ __launch_bounds__(64 * kWaves, per_cu<D>()) void rlt_tree_kernel(Para
       }
       asm volatile("" ::: "memory");
     };
-    // ---- O^T += V^T P^T of the tile in stage `vt`
-    auto product = [&](const uint8_t* vt, const uint32_t (&p)[8]) {
+    // ---- O^T += V^T P^T of the tile in stage `vt`: operand c ND + dt is dim tile dt of chunk c
+    constexpr int VW = FP8 ? 2 : 4;  // words of an operand as read
+    auto read_v = [&](uint32_t (&va)[2 * ND][VW], const uint8_t* vt) {
 #pragma unroll
-      for (int c = 0; c < 2; ++c)
-#pragma unroll
-        for (int dt = 0; dt < ND; ++dt) {
-          u32x4 va;
-          if constexpr (!FP8) {
-            const int piece = 2 * ((lane >> 4) & 1) + ((i16 >> 1) & 1);  // within the dim tile
-            const uint8_t* vr = vt + (16 * c + vr16) * G::ROW +
-                                ((4 * dt + piece) ^ v_swz<SLOTS, false>(vr16)) * 16 + (i16 & 1) * 8;
-            const s16x4 x0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                (__attribute__((address_space(3))) s16x4*)(lds_void*)vr);
-            const s16x4 x1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                (__attribute__((address_space(3))) s16x4*)(lds_void*)(vr + 8 * G::ROW));
-            __builtin_memcpy(&va, &x0, 8);
-            __builtin_memcpy((char*)&va + 8, &x1, 8);
-          } else {
-            const int r = 16 * c + vr8;
-            const uint8_t* vr = vt + r * G::ROW +
-                                ((2 * dt + ((lane >> 4) & 1)) ^ v_swz<SLOTS, true>(r)) * 16 + (i16 & 1) * 8;
-            const i32x2 x = __builtin_amdgcn_ds_read_tr8_b64_v2i32(
-                (__attribute__((address_space(3))) i32x2*)(lds_void*)vr);
-            const uint2 lo = widen<QT>((uint32_t)x[0]), hi = widen<QT>((uint32_t)x[1]);
-            va = u32x4{lo.x, lo.y, hi.x, hi.y};
-          }
-          oacc[dt] = mfma<QT>(va, u32x4{p[4 * c], p[4 * c + 1], p[4 * c + 2], p[4 * c + 3]}, oacc[dt]);
+      for (int n = 0; n < 2 * ND; ++n) {
+        const int c = n / ND, dt = n % ND;
+        if constexpr (!FP8) {
+          const int piece = 2 * ((lane >> 4) & 1) + ((i16 >> 1) & 1);  // within the dim tile
+          const uint8_t* vr = vt + (16 * c + vr16) * G::ROW +
+                              ((4 * dt + piece) ^ v_swz<SLOTS, false>(vr16)) * 16 + (i16 & 1) * 8;
+          const s16x4 x0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+              (__attribute__((address_space(3))) s16x4*)(lds_void*)vr);
+          const s16x4 x1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+              (__attribute__((address_space(3))) s16x4*)(lds_void*)(vr + 8 * G::ROW));
+          __builtin_memcpy(&va[n][0], &x0, 8);
+          __builtin_memcpy(&va[n][2], &x1, 8);
+        } else {
+          const int r = 16 * c + vr8;
+          const uint8_t* vr = vt + r * G::ROW +
+                              ((2 * dt + ((lane >> 4) & 1)) ^ v_swz<SLOTS, true>(r)) * 16 + (i16 & 1) * 8;
+          const i32x2 x = __builtin_amdgcn_ds_read_tr8_b64_v2i32(
+              (__attribute__((address_space(3))) i32x2*)(lds_void*)vr);
+          va[n][0] = (uint32_t)x[0];
+          va[n][1] = (uint32_t)x[1];
         }
+      }
+    };
+    auto product = [&](const uint32_t (&va)[2 * ND][VW], const uint32_t (&p)[8]) {
+#pragma unroll
+      for (int n = 0; n < 2 * ND; ++n) {
+        const int c = n / ND, dt = n % ND;
+        u32x4 a4;
+        if constexpr (!FP8) {
+          a4 = u32x4{va[n][0], va[n][1], va[n][2], va[n][3]};
+        } else {
+          const uint2 lo = widen<QT>(va[n][0]), hi = widen<QT>(va[n][1]);
+          a4 = u32x4{lo.x, lo.y, hi.x, hi.y};
+        }
+        oacc[dt] = mfma<QT>(a4, u32x4{p[4 * c], p[4 * c + 1], p[4 * c + 2], p[4 * c + 3]}, oacc[dt]);
+      }
     };
 
     int tb = first_tb;
@@ -715,7 +769,7 @@ __global__ __launch_bounds__(64 * kWaves, per_cu<D>()) void rlt_tree_kernel(Para
       for (int it = 0; it < tiles; ++it) {
         uint8_t* const kt = ring + stage * G::TILE;
         uint8_t* const vt = ring + (S + stage) * G::TILE;
-        const float* const scale = sh.scale[w][sstage];
+        const float* const scale = sh.scale[kg][sstage];
         const bool more = it + S < tiles;
         const bool full = is_full(tb);
         // (ahead of this tile's keys: its values and the next S - 1 tiles)
@@ -728,14 +782,18 @@ __global__ __launch_bounds__(64 * kWaves, per_cu<D>()) void rlt_tree_kernel(Para
           next_tile();
           load_k(stage, sstage == 0 ? S : sstage - 1);
         }
-        uint32_t p[8];
-        weigh(sc, p, tb, full, scale);
+        // with a second stage the values are here by now: their reads run beside the weights
+        uint32_t p[8], va[2 * ND][VW];
+        if (S == 1) weigh(sc, p, tb, full, scale);
         if (more) wait_loads<S * LK + (S - 1) * LV>();
         if (!full) clean(vt, tb);
-        product(vt, p);
+        read_v(va, vt);
+        __builtin_amdgcn_sched_barrier(0);
+        if (S > 1) weigh(sc, p, tb, full, scale);
         wait_lds();
         if (more) load_v(stage);
-        tb += MACRO;
+        product(va, p);
+        tb += macro;
         stage = stage + 1 == S ? 0 : stage + 1;
         sstage = sstage == S ? 0 : sstage + 1;
       }
@@ -746,24 +804,28 @@ __global__ __launch_bounds__(64 * kWaves, per_cu<D>()) void rlt_tree_kernel(Para
           wait_loads<(S - 2) * (LK + LV)>();
           stage_barrier();
           const int to = stage == 0 ? S - 1 : stage - 1;
-          next_tile();
-          load_k(to, to);
-          load_v(to);
+          if (alive) {
+            next_tile();
+            load_k(to, to);
+            load_v(to);
+          }
         } else {
           wait_loads<0>();
           stage_barrier();
         }
-        if (tb < sv.len) {  // wave-uniform: not the last tiles of a macro tile
+        if (tb < sv.len && alive) {  // wave-uniform: not the last tiles of a macro tile
           uint8_t* const vt = ring + (S + stage) * G::TILE;
           const bool full = is_full(tb);
           f32x16 sc;
           scores(sc, ring + stage * G::TILE);
-          uint32_t p[8];
-          weigh(sc, p, tb, full, sh.scale[w][stage]);
+          uint32_t p[8], va[2 * ND][VW];
           if (!full) clean(vt, tb);
-          product(vt, p);
+          read_v(va, vt);
+          __builtin_amdgcn_sched_barrier(0);
+          weigh(sc, p, tb, full, sh.scale[kg][stage]);
+          product(va, p);
         }
-        tb += MACRO;
+        tb += macro;
         stage = stage + 1 == S ? 0 : stage + 1;
       }
     }
@@ -794,25 +856,31 @@ __global__ __launch_bounds__(64 * kWaves, per_cu<D>()) void rlt_tree_kernel(Para
     for (int i = 0; i < 2 * kBadWords; ++i) any_bad |= sh.bad[i];
     const bool whole = n == sp.count;
     const int slot = 2 * blockIdx.x + (f == f_begin ? 0 : 1);
-    if (a == 0 && t == 0)
-      P.splits[((int64_t)seq * P.hkv + kvh) * P.max_blocks + rb] =
-          Split{slot, whole ? -1 : (int)((f + sp.count - 1) / share)};
-    float* const part = P.part + (int64_t)slot * RB * (D + 2);
-    for (int e = t; e < rows * (D / 4); e += 64 * kWaves) {
-      const int r = e / (D / 4), d = 4 * (e % (D / 4));
-      float m = -INFINITY;
-#pragma unroll
-      for (int g = 0; g < KW; ++g) m = fmaxf(m, sh.ml[g][r][0]);
-      float l = 0.f;
+    if (a == 0 && t < heads)
+      P.splits[((int64_t)seq * P.hkv + head0 + t) * P.max_blocks + rb] =
+          Split{slot, whole ? -1 : (int)((f + sp.count - 1) / share), t * RB};
+    float* const part = P.part + (int64_t)slot * kPartRows * (D + 2);
+    for (int e = t; e < heads * rows * (D / 4); e += 64 * kWaves) {
+      const int hr = e / (D / 4), d = 4 * (e % (D / 4));
+      const int hx = hr / rows, r = hr - hx * rows;  // head of the unit, row of the block
+      float m = -INFINITY, l = 0.f;
       f32x4 o = {0.f, 0.f, 0.f, 0.f};
+      if (apart) {
+        m = sh.ml[hx][r][0];
+        l = sh.ml[hx][r][1];
+        o = *(const f32x4*)(ob + (hx * RB + r) * G::OSTRIDE + d);
+      } else {
 #pragma unroll
-      for (int g = 0; g < KW; ++g) {
-        const float mg = sh.ml[g][r][0], lg = sh.ml[g][r][1];
-        // (a group that saw no key adds nothing; one whose sum is NaN spoils the row)
-        const float x = mg == -INFINITY ? (lg == 0.f ? 0.f : lg) : __builtin_amdgcn_exp2f(mg - m);
-        const f32x4 og = *(const f32x4*)(ob + (g * RB + r) * G::OSTRIDE + d);
-        l += lg * x;
-        o += og * x;
+        for (int g = 0; g < KW; ++g) m = fmaxf(m, sh.ml[g][r][0]);
+#pragma unroll
+        for (int g = 0; g < KW; ++g) {
+          const float mg = sh.ml[g][r][0], lg = sh.ml[g][r][1];
+          // (a group that saw no key adds nothing; one whose sum is NaN spoils the row)
+          const float x = mg == -INFINITY ? (lg == 0.f ? 0.f : lg) : __builtin_amdgcn_exp2f(mg - m);
+          const f32x4 og = *(const f32x4*)(ob + (g * RB + r) * G::OSTRIDE + d);
+          l += lg * x;
+          o += og * x;
+        }
       }
       const int rho = rb * RB + r;
       if (any_bad) {
@@ -826,7 +894,7 @@ __global__ __launch_bounds__(64 * kWaves, per_cu<D>()) void rlt_tree_kernel(Para
             const int32_t e2 = table[min(pos / P.block_size, P.table_width - 1)];
             const int64_t at = (int64_t)(e2 >= 0 && e2 < P.num_blocks ? e2 : 0) * P.v_block_stride +
                                (int64_t)(pos % P.block_size) * P.v_token_stride +
-                               (int64_t)kvh * P.v_head_stride + d;
+                               (int64_t)(head0 + hx) * P.v_head_stride + d;
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
               const float x = load_as_f32<KVT>(P.v, at + c);
@@ -838,11 +906,11 @@ __global__ __launch_bounds__(64 * kWaves, per_cu<D>()) void rlt_tree_kernel(Para
       if (whole) {
         const float inv = l == 0.f ? 0.f : v_mul / l;
         uint16_t* const op = (uint16_t*)P.out + (int64_t)(sv.q_begin + rho / P.group) * P.out_row_stride +
-                             (int64_t)(kvh * P.group + rho % P.group) * P.out_head_stride + d;
+                             (int64_t)((head0 + hx) * P.group + rho % P.group) * P.out_head_stride + d;
         *(uint2*)op = make_uint2(pack2<QT>(o[0] * inv, o[1] * inv), pack2<QT>(o[2] * inv, o[3] * inv));
       } else {
-        *(f32x4*)(part + r * D + d) = o;
-        if (d == 0) *(float2*)(part + RB * D + 2 * r) = make_float2(m, l);
+        *(f32x4*)(part + (hx * RB + r) * D + d) = o;
+        if (d == 0) *(float2*)(part + kPartRows * D + 2 * (hx * RB + r)) = make_float2(m, l);
       }
     }
     __syncthreads();  // the ring, the masks and the sums are reused by the next pair
@@ -856,7 +924,7 @@ __global__ __launch_bounds__(64 * kWaves, per_cu<D>()) void rlt_tree_kernel(Para
 constexpr int kMergeThreads = 1024;
 template <int D, int CG>
 constexpr int merge_rows() { return kMergeThreads / CG / (D == 64 ? 16 : D == 256 ? 64 : 32); }
-template <int QT, int D, int RB, int MACRO, int CG>
+template <int QT, int D, int RB, int CG>
 __global__ __launch_bounds__(kMergeThreads) void rlt_tree_merge_kernel(Params P) {
   constexpr int R = merge_rows<D, CG>(), LPR = kMergeThreads / CG / R;
   __shared__ float sh[CG > 1 ? CG - 1 : 1][kMergeThreads / CG][6];
@@ -866,7 +934,7 @@ __global__ __launch_bounds__(kMergeThreads) void rlt_tree_merge_kernel(Params P)
   const int kvh = sh_id % P.hkv, seq = sh_id / P.hkv;
   const Split x = P.splits[blockIdx.x];
   const Seq sv = seq_of(P, seq);
-  const Span sp = span_of<RB, MACRO>(P, sv);
+  const Span sp = span_of<RB>(P, sv, kTile);
   const int rows = min(RB, sv.nodes * P.group - rb * RB);
   if (rows <= 0 || (sp.count > 0 && x.last < 0)) return;  // uniform over the workgroup
   const bool live = r < rows && d < D;
@@ -888,7 +956,7 @@ __global__ __launch_bounds__(kMergeThreads) void rlt_tree_merge_kernel(Params P)
     o = o * a + o2 * b;
     m = mo;
   };
-  constexpr int64_t stride = (int64_t)RB * (D + 2);
+  constexpr int64_t stride = (int64_t)kPartRows * (D + 2);
   const int b0 = x.first >> 1, count = x.last - b0 + 1, per = (count + CG - 1) / CG;
   const int i0 = cg * per, i1 = min(i0 + per, count);
   if (live) {
@@ -901,8 +969,8 @@ __global__ __launch_bounds__(kMergeThreads) void rlt_tree_merge_kernel(Params P)
         const int at = min(i + k, i1 - 1);
         const float* const part =
             P.part + (at == 0 ? (int64_t)x.first : 2 * (int64_t)(b0 + at)) * stride;
-        ml[k] = *(const float2*)(part + RB * D + 2 * r);
-        oo[k] = *(const f32x4*)(part + r * D + d);
+        ml[k] = *(const float2*)(part + kPartRows * D + 2 * (x.row + r));
+        oo[k] = *(const f32x4*)(part + (x.row + r) * D + d);
       }
 #pragma unroll
       for (int k = 0; k < AHEAD; ++k)

@@ -129,7 +129,7 @@ void launch(const Params& P, hipStream_t stream) {
   const int rows = P.max_q * P.group < G::RB ? P.max_q * P.group : G::RB;
   auto merge = [&](auto cg) {
     constexpr int CG = decltype(cg)::value, R = merge_rows<D, CG>();
-    hipLaunchKernelGGL((rlt_tree_merge_kernel<QT, D, G::RB, G::MACRO, CG>),
+    hipLaunchKernelGGL((rlt_tree_merge_kernel<QT, D, G::RB, CG>),
                        dim3((unsigned)pairs, (unsigned)((rows + R - 1) / R)), dim3(kMergeThreads), 0,
                        stream, P);
   };
@@ -197,7 +197,7 @@ size_t rlt_tree_attention_workspace_size(int32_t num_seqs, int32_t max_q_len, in
   const int rb = 32 * tree::row_waves((int)(rows < 1024 ? rows : 1024), head_dim, kv_dtype == RLT_FP8_E4M3);
   const int64_t pairs = (int64_t)num_seqs * num_kv_heads * ((rows + rb - 1) / rb);
   return rlt_align_up((size_t)pairs * sizeof(tree::Split), 256) +
-         (size_t)2 * tree::kGrid * rb * (head_dim + 2) * sizeof(float);
+         (size_t)2 * tree::kGrid * tree::kPartRows * (head_dim + 2) * sizeof(float);
 }
 
 int rlt_tree_attention(const void* q, int64_t q_row_stride, int64_t q_head_stride,
