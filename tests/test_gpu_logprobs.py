@@ -12,10 +12,12 @@ def plain(x, tokens, top_n):
     """(logprob, rank, entropy, top_logprob, top_tokens) and tolerances of the first three
     kinds of numbers, in float64.
 
-    With d = x - m taken in float32 (off by 2^-24 |d|), a weight e^d by an exponential and a
-    product (three half steps) is off by (3 + |d|) 2^-24 of itself; S and T are float64 sums of
-    them.  log S is then off by E (3 + |d|) 2^-24 with E the mean under the row's distribution,
-    T / S by E |d| (4 + |d|) + E |d| E (3 + |d|), and an output is rounded once.
+    With d = x - m taken in float32 (off by 2^-24 |d|), the exponent d log2(e) in float32 (its
+    constant and its product off by 1.3 2^-24 of it) and an exponential of two half steps, a
+    weight e^d is off by (2 + 2.3 |d|) 2^-24 of itself; two float32 additions of weights add two
+    half steps before the float64 sums S and T.  log S is then off by E (4 + 2.3 |d|) 2^-24 with E
+    the mean under the row's distribution, T / S (one more product) by E |d| (5 + 2.3 |d|) + E |d|
+    E (4 + 2.3 |d|), and an output is rounded once.
     """
     x = x.double()
     lp = torch.log_softmax(x, -1)
@@ -24,8 +26,8 @@ def plain(x, tokens, top_n):
     w = torch.where(p > 0, d, torch.zeros_like(d))
     mean = lambda f: (p * f).sum(-1)  # noqa: E731
     u = 2.0 ** -24
-    e_lse = u * mean(3 + w) * 1.1
-    e_t = u * (mean(w * (4 + w)) + mean(w) * mean(3 + w)) * 1.1
+    e_lse = u * mean(4 + 2.3 * w) * 1.1
+    e_t = u * (mean(w * (5 + 2.3 * w)) + mean(w) * mean(4 + 2.3 * w)) * 1.1
     at = torch.arange(x.shape[0])
     order = x.sort(dim=-1, descending=True, stable=True).indices
     rank = (order == tokens[:, None]).nonzero()[:, 1] + 1

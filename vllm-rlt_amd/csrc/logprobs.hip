@@ -9,16 +9,23 @@
 // workgroup per row, joins them.  S and T are float64 sums: next to a dominant token the
 // entropy is what is left of S after 1, which float32 sums would lose.
 //
-// The n first columns of a slice are taken without a sort: the n-th largest of the 256
-// threads' largest columns is a lower bound that at least n columns reach, and only threads
-// whose largest reaches it hold such columns, so at most n times a thread's columns are left
-// to be ranked against each other (a few more than n in practice).
+// The n first columns of a slice are taken without a sort.  The n-th largest of a wave's 64
+// lanes' largest columns is a lower bound that n columns of the wave reach, so the largest of
+// the four waves' bounds is one for the slice; the columns that reach it (a few more than n)
+// are listed and ranked by counting.  Where ties make them too many, the bound is taken over
+// the threads' largest (value, column) pairs, which are all different: then at most n threads
+// hold such columns.
+//
+// float64 sums cost more than the loads, so four weights at a time are added in float32 first;
+// weights of exactly 1 (the maximum) are counted instead, and nothing is lost next to them.
 
 #include "vocab_rows.h"
 
 #include "rlt_mi355x.h"
 
 #include <math.h>
+
+#include <type_traits>
 
 namespace {
 
@@ -57,8 +64,23 @@ struct TopShared {
   unsigned long long best[kThreads];
   unsigned long long list[kList];
   unsigned long long bound;
+  uint32_t wave_bound[kThreads / 64];
   int count;
 };
+
+// Ranks the `found` different composites of sh.list by counting; out(rank, composite) for the
+// first n, 0 behind the last.
+template <class Out>
+__device__ __forceinline__ void rank_list(const TopShared& sh, int found, int n, Out out) {
+  for (int e = threadIdx.x; e < found; e += kThreads) {
+    const unsigned long long c = sh.list[e];
+    int r = 0;
+#pragma unroll 8
+    for (int i = 0; i < found; ++i) r += sh.list[i] > c;
+    if (r < n) out(r, c);
+  }
+  for (int r = found + (int)threadIdx.x; r < n; r += kThreads) out(r, 0ull);
+}
 
 // The n largest of the workgroup's composites (item(i), i < items, of every thread) go to
 // out(rank, composite); ranks without a composite get 0.
@@ -106,31 +128,18 @@ __device__ __forceinline__ void select_top(TopShared& sh, int n, int items, Item
     }
   }
   __syncthreads();
-  const int found = min(sh.count, kList);
-  for (int e = t; e < found; e += kThreads) {
-    const unsigned long long c = sh.list[e];
-    int r = 0;
-    for (int i = 0; i < found; ++i) r += sh.list[i] > c;
-    if (r < n) out(r, c);
-  }
-  for (int r = found + t; r < n; r += kThreads) out(r, 0ull);
+  rank_list(sh, min(sh.count, kList), n, out);
 }
 
-__device__ __forceinline__ double block_sum(double x, double* sh) {
-#pragma unroll
-  for (int o = 32; o >= 1; o >>= 1) x += __shfl_xor(x, o, RLT_WAVE);
-  __syncthreads();
-  if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = x;
-  __syncthreads();
-  return (sh[0] + sh[1]) + (sh[2] + sh[3]);
-}
-__device__ __forceinline__ float block_max(float x, float* sh) {
-#pragma unroll
-  for (int o = 32; o >= 1; o >>= 1) x = fmaxf(x, __shfl_xor(x, o, RLT_WAVE));
-  __syncthreads();
-  if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = x;
-  __syncthreads();
-  return fmaxf(fmaxf(sh[0], sh[1]), fmaxf(sh[2], sh[3]));
+// The n-th largest of the wave's 64 values (0: fewer than n are positive).
+__device__ __forceinline__ uint32_t wave_nth(uint32_t x, int n) {
+  uint32_t bound = 0;
+#pragma unroll 4
+  for (int bit = 31; bit >= 0; --bit) {
+    const uint32_t next = bound | (1u << bit);
+    if (__popcll(__builtin_amdgcn_ballot_w64(x >= next)) >= n) bound = next;
+  }
+  return bound;
 }
 
 __device__ __forceinline__ int64_t source_row(const LogprobParams& P, int64_t r) {
@@ -138,98 +147,225 @@ __device__ __forceinline__ int64_t source_row(const LogprobParams& P, int64_t r)
   return row >= 0 && row < P.num_rows ? row : -1;
 }
 
-template <int DT, int EPT>
-__global__ __launch_bounds__(kThreads) void rlt_logprob_slices_kernel(LogprobParams P) {
-  __shared__ TopShared top;
-  __shared__ double dsh[4];
-  __shared__ float fsh[4];
+// The lower bound of the n largest keys among all threads' largest ones: wave w's part, in LDS
+// (a barrier follows before it is used).
+__device__ __forceinline__ void put_bound(TopShared& sh, uint32_t largest, int n) {
+  const uint32_t bound = wave_nth(largest, n);
+  if ((threadIdx.x & 63) == 0) sh.wave_bound[threadIdx.x >> 6] = bound;
+  if (threadIdx.x == 0) sh.count = 0;
+}
+__device__ __forceinline__ uint32_t get_bound(const TopShared& sh) {
+  return max(max(sh.wave_bound[0], sh.wave_bound[1]), max(sh.wave_bound[2], sh.wave_bound[3]));
+}
+__device__ __forceinline__ void list_column(TopShared& sh, unsigned long long c) {
+  const int at = atomicAdd(&sh.count, 1);
+  if (at < kThreads) sh.list[at] = c;
+}
+
+// The next lower number; of -inf NaN, which nothing lies at or below.
+__device__ __forceinline__ float below(float x) {
+  const uint32_t b = __float_as_uint(x + 0.f);  // (-0 is 0)
+  if (b == 0xff800000u) return __uint_as_float(0x7fc00000u);
+  return __uint_as_float(b == 0 ? 0x80000001u : b & 0x80000000u ? b + 1 : b - 1);
+}
+
+// A slice's statistics and first columns.  FULL: no column of it lies past the row.
+template <int DT, int EPT, bool FULL>
+__device__ __forceinline__ void scan_slice(const LogprobParams& P, const uint8_t* src, int64_t r, int slice, int token,
+                                           TopShared& top, double (&sums)[kThreads / 64][2],
+                                           uint32_t (&counts)[kThreads / 64][2], float (&maxima)[kThreads / 64]) {
   using S = Slice<DT, EPT>;
-  constexpr int ELT = DT == RLT_F32 ? 4 : 2;
-  const int64_t r = blockIdx.y;
-  const int slice = blockIdx.x;
-  const int64_t row = source_row(P, r);
-  if (row < 0) return;
-  const uint8_t* const src = (const uint8_t*)P.logits + row * P.row_stride * ELT;
-  const int64_t begin = (int64_t)slice * EPT * kThreads;
+  const int t = threadIdx.x, w = t >> 6;
+  const int begin = slice * EPT * kThreads, vocab = (int)P.vocab;
   S x;
-  x.load(src, begin, P.vocab);
-  const int64_t token = P.tokens[r];
-  unsigned long long mine = ~0ull;  // nothing comes before no token
-  if (token >= 0 && token < P.vocab)
-    mine = composite(order_key(load_as_f32<DT>(src, token)), (uint32_t)token);
+  x.load(src, begin, FULL ? begin + EPT * kThreads : vocab);
+  auto column = [&](int i) { return (int)S::column(begin, i); };
+  auto inside = [&](int c) { return FULL || c < vocab; };
+  const float xt = load_as_f32<DT>(src, token);
+  // columns past the row become -inf, which weighs nothing
+  if (!FULL) {
+#pragma unroll
+    for (int i = 0; i < S::NP; ++i)
+#pragma unroll
+      for (int e = 0; e < S::VE; ++e)
+        if (column(i) + e >= vocab) x.set(i, e, -INFINITY);
+  }
   float m = -INFINITY;
-  uint32_t before = 0;
+  bool nan = false;
 #pragma unroll
-  for (int i = 0; i < S::NP; ++i) {
-    const int64_t c = S::column(begin, i);
+  for (int i = 0; i < S::NP; ++i)
 #pragma unroll
-    for (int e = 0; e < S::VE; ++e) {
-      const bool ok = c + e < P.vocab;
-      const float v = x.at(i, e);
-      m = ok ? fmaxf(m, v) : m;
-      before += ok && composite(order_key(v), (uint32_t)(c + e)) > mine;
+    for (int e = 0; e < S::VE; e += 2) {
+      const float v0 = x.at(i, e), v1 = x.at(i, e + 1);
+      m = fmaxf(fmaxf(m, v0), v1);
+      nan |= __builtin_isunordered(v0, v1);
     }
-  }
-  m = block_max(m, fsh);
-  // e^d as 2^(d log2 e), the product's rounding made up for
-  constexpr float kL2e = 1.4426950408889634f, kL2eLo = 1.925963033500011e-8f, kLn2 = 0.6931471805599453f;
+  // the thread's largest column (NaN comes first; 0: none above -inf)
+  const uint32_t mine = nan ? 0xffffffffu : m == -INFINITY ? 0u : order_key(m);
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, RLT_WAVE));
+  const float wave_top = m;
+  if (P.top_n > 0) put_bound(top, mine, P.top_n);
+  if ((t & 63) == 0) maxima[w] = m;
+  __syncthreads();
+  m = fmaxf(fmaxf(maxima[0], maxima[1]), fmaxf(maxima[2], maxima[3]));
+  // (a slice without a finite maximum counts no ones: +inf or NaN spoils its sums, and with
+  // nothing but -inf they are 0)
+  const float from = m == -INFINITY ? 0.f : m;
+  constexpr float kL2e = 1.4426950408889634f;
   double s = 0.0, q = 0.0;
+  uint32_t ones = 0, before = 0;
+  // (the instructions of a column bound the kernel: the maximum is looked for in its wave only)
+  auto weigh = [&](auto counted) {
 #pragma unroll
-  for (int i = 0; i < S::NP; ++i) {
-    const int64_t c = S::column(begin, i);
+    for (int i = 0; i < S::NP; ++i)
 #pragma unroll
-    for (int e = 0; e < S::VE; ++e) {
-      const float d = x.at(i, e) - m;
-      const float hi = d * kL2e;
-      const float lo = __builtin_fmaf(d, kL2eLo, __builtin_fmaf(d, kL2e, -hi));
-      const float y = __builtin_amdgcn_exp2f(hi);
-      float w = __builtin_fmaf(y, lo * kLn2, y);
-      // columns past the row weigh nothing, nor do masked logits: -inf, and finite ones so far
-      // down that hi or lo overflow
-      if (!(c + e < P.vocab) || x.at(i, e) == -INFINITY || hi < -160.f) w = 0.f;
-      s += (double)w;
-      q += w == 0.f ? 0.0 : (double)w * (double)d;
+      for (int f = 0; f < S::VE; f += 4) {
+        float ws[4], qs[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const float d = x.at(i, f + k) - from;
+          float z = __builtin_amdgcn_exp2f(d * kL2e);
+          if constexpr (decltype(counted)::value) {
+            const bool one = d == 0.f;
+            z = one ? 0.f : z;
+            ones += one ? 1u : 0u;
+          }
+          ws[k] = z;
+          qs[k] = z * fmaxf(d, -200.f);  // (d may be -inf where z is 0)
+        }
+        s += (double)((ws[0] + ws[1]) + (ws[2] + ws[3]));
+        q += (double)((qs[0] + qs[1]) + (qs[2] + qs[3]));
+        __builtin_amdgcn_sched_barrier(0);
+      }
+  };
+  if (wave_top == m && fabsf(m) < INFINITY) weigh(std::true_type{});
+  else weigh(std::false_type{});
+  // Columns ahead of the token: greater (or NaN), or equal in an earlier column.  A slice
+  // before the token's takes "not below the token's" as "above the next lower number" (for
+  // -inf: everything), one behind it "above"; the token's own looks at the columns.
+  const int end = begin + EPT * kThreads;
+  if (xt != xt) {
+    // (of a NaN token, the NaN columns before it)
+#pragma unroll
+    for (int i = 0; i < S::NP; ++i)
+#pragma unroll
+      for (int e = 0; e < S::VE; ++e) {
+        const float v = x.at(i, e);
+        before += ((v != v) & (column(i) + e < token)) ? 1u : 0u;
+      }
+  } else if (token >= begin && token < end) {
+#pragma unroll
+    for (int i = 0; i < S::NP; ++i)
+#pragma unroll
+      for (int e = 0; e < S::VE; ++e) {
+        const float v = x.at(i, e);
+        before += ((!(v <= xt)) | ((v == xt) & (column(i) + e < token))) ? 1u : 0u;
+      }
+  } else {
+    const float least = token >= end ? below(xt) : xt;
+#pragma unroll
+    for (int i = 0; i < S::NP; ++i)
+#pragma unroll
+      for (int e = 0; e < S::VE; ++e) before += !(x.at(i, e) <= least) ? 1u : 0u;
+  }
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) {
+    s += __shfl_xor(s, o, RLT_WAVE);
+    q += __shfl_xor(q, o, RLT_WAVE);
+    before += __shfl_xor(before, o, RLT_WAVE);
+    ones += __shfl_xor(ones, o, RLT_WAVE);
+  }
+  if ((t & 63) == 0) {
+    sums[w][0] = s;
+    sums[w][1] = q;
+    counts[w][0] = before;
+    counts[w][1] = ones;
+  }
+  if (P.top_n > 0) {
+    // (bound 0, fewer than n columns above -inf in each wave: every column reaches it, as any
+    // does not lie below the NaN that is its value)
+    const uint32_t bound = get_bound(top);
+    const float least = key_value(bound);
+    if (mine >= bound) {
+#pragma unroll
+      for (int i = 0; i < S::NP; ++i) {
+        bool any = false;
+#pragma unroll
+        for (int e = 0; e < S::VE; ++e) any |= !(x.at(i, e) < least);
+        if (!any) continue;
+#pragma unroll
+        for (int e = 0; e < S::VE; ++e) {
+          const int c = column(i) + e;
+          const float v = x.at(i, e);
+          if ((!(v < least)) & inside(c)) list_column(top, composite(order_key(v), (uint32_t)c));
+        }
+      }
     }
   }
-  s = block_sum(s, dsh);
-  q = block_sum(q, dsh);
-#pragma unroll
-  for (int o = 32; o >= 1; o >>= 1) before += __shfl_xor(before, o, RLT_WAVE);
   __syncthreads();
-  uint32_t* const counts = (uint32_t*)fsh;
-  if ((threadIdx.x & 63) == 0) counts[threadIdx.x >> 6] = before;
-  __syncthreads();
-  if (threadIdx.x == 0) {
+  if (t == 0) {
     SliceStat st;
-    st.s = s;
-    st.t = q;
+    st.s = ((sums[0][0] + sums[1][0]) + (sums[2][0] + sums[3][0])) +
+           (double)(counts[0][1] + counts[1][1] + counts[2][1] + counts[3][1]);
+    st.t = (sums[0][1] + sums[1][1]) + (sums[2][1] + sums[3][1]);
     st.m = m;
-    st.before = counts[0] + counts[1] + counts[2] + counts[3];
+    st.before = counts[0][0] + counts[1][0] + counts[2][0] + counts[3][0];
     P.stats[r * P.slices + slice] = st;
   }
   if (P.top_n > 0) {
     unsigned long long* const dst = P.candidates + (r * P.slices + slice) * P.top_n;
-    select_top<EPT>(
-        top, P.top_n, EPT,
-        [&](int k) {
-          const int i = k / S::VE, e = k % S::VE;
-          const int64_t c = S::column(begin, i) + e;
-          return c < P.vocab ? composite(order_key(x.at(i, e)), (uint32_t)c) : 0ull;
-        },
-        [&](int rank, unsigned long long c) { dst[rank] = c; });
+    auto put = [&](int rank, unsigned long long c) { dst[rank] = c; };
+    const int found = top.count;  // (the same in every thread)
+    if (found <= kThreads) {
+      rank_list(top, found, P.top_n, put);
+    } else {
+      __syncthreads();
+      select_top<EPT>(
+          top, P.top_n, EPT,
+          [&](int k) {
+            const int c = column(k / S::VE) + k % S::VE;
+            return inside(c) ? composite(order_key(x.at(k / S::VE, k % S::VE)), (uint32_t)c) : 0ull;
+          },
+          put);
+    }
   }
+}
+
+template <int DT, int EPT>
+__global__ __launch_bounds__(kThreads, EPT == kWideEpt ? 4 : 8) void rlt_logprob_slices_kernel(LogprobParams P) {
+  __shared__ TopShared top;
+  __shared__ double sums[kThreads / 64][2];
+  __shared__ uint32_t counts[kThreads / 64][2];
+  __shared__ float maxima[kThreads / 64];
+  const int64_t r = blockIdx.y;
+  const int slice = blockIdx.x;
+  const int64_t wanted = P.tokens[r];
+  const int64_t row = source_row(P, r);
+  if (row < 0) return;
+  const int token = wanted >= 0 && wanted < P.vocab ? (int)wanted : 0;
+  const uint8_t* const src = (const uint8_t*)P.logits + row * P.row_stride * (DT == RLT_F32 ? 4 : 2);
+  if ((int64_t)(slice + 1) * EPT * kThreads <= P.vocab)
+    scan_slice<DT, EPT, true>(P, src, r, slice, token, top, sums, counts, maxima);
+  else
+    scan_slice<DT, EPT, false>(P, src, r, slice, token, top, sums, counts, maxima);
 }
 
 template <int DT>
 __global__ __launch_bounds__(kThreads) void rlt_logprob_rows_kernel(LogprobParams P) {
   __shared__ TopShared top;
-  __shared__ double dsh[4];
-  __shared__ float fsh[4];
+  __shared__ double sh[2];  // the row's maximum, and the log of its sum over it
   constexpr int ELT = DT == RLT_F32 ? 4 : 2;
   const int64_t r = blockIdx.x;
   const int t = threadIdx.x;
-  const int64_t row = source_row(P, r);
   const float nan = __uint_as_float(0x7fc00000u);
+  // (the partial results of a row index outside the logits were not written: read for nothing)
+  const unsigned long long* const c = P.candidates + r * P.slices * P.top_n;
+  const int total = P.slices * P.top_n, items = (total + kThreads - 1) / kThreads;
+  auto item = [&](int i) { return i * kThreads + t < total ? c[i * kThreads + t] : 0ull; };
+  unsigned long long best = 0;
+  for (int i = 0; i < items; ++i) best = max(best, item(i));
+  const int64_t row = source_row(P, r);
   if (row < 0) {
     if (t == 0) {
       P.logprob[r] = P.entropy[r] = nan;
@@ -241,44 +377,64 @@ __global__ __launch_bounds__(kThreads) void rlt_logprob_rows_kernel(LogprobParam
     }
     return;
   }
-  const SliceStat* const st = P.stats + r * P.slices;
-  float m = -INFINITY;
-  for (int i = t; i < P.slices; i += kThreads) m = fmaxf(m, st[i].m);
-  m = block_max(m, fsh);
-  double s = 0.0, q = 0.0, before = 0.0;
-  for (int i = t; i < P.slices; i += kThreads) {
-    const SliceStat x = st[i];
-    before += x.before;
-    if (x.m == -INFINITY && x.s == 0.0) continue;  // nothing but masked logits
-    const double d = (double)x.m - (double)m, w = exp(d);
-    s += x.s * w;
-    q += (x.t + d * x.s) * w;
-  }
-  s = block_sum(s, dsh);
-  q = block_sum(q, dsh);
-  before = block_sum(before, dsh);
-  const double lse = log(s);  // over the maximum; a row without a finite one gives NaN
-  const bool ok = m > -INFINITY;
-  if (t == 0) {
+  if (t < 64) {
+    // one wave joins the slices while the others wait with their candidates
+    const SliceStat* const st = P.stats + r * P.slices;
     const int64_t token = P.tokens[r];
     const bool in = token >= 0 && token < P.vocab;
-    const uint8_t* const src = (const uint8_t*)P.logits + row * P.row_stride * ELT;
-    P.logprob[r] = ok && in ? (float)(((double)load_as_f32<DT>(src, token) - (double)m) - lse) : nan;
-    P.entropy[r] = ok ? (float)(lse - q / s) : nan;
-    P.rank[r] = in ? 1 + (int64_t)before : 0;
+    const float xt = load_as_f32<DT>((const uint8_t*)P.logits + row * P.row_stride * ELT, in ? token : 0);
+    float m = -INFINITY;
+    for (int i = t; i < P.slices; i += 64) m = fmaxf(m, st[i].m);
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, RLT_WAVE));
+    double s = 0.0, q = 0.0;
+    uint32_t before = 0;
+    for (int i = t; i < P.slices; i += 64) {
+      const SliceStat x = st[i];
+      before += x.before;
+      if (x.m == -INFINITY && x.s == 0.0) continue;  // nothing but masked logits
+      const double d = (double)x.m - (double)m, w = exp(d);
+      s += x.s * w;
+      q += (x.t + d * x.s) * w;
+    }
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) {
+      s += __shfl_xor(s, o, RLT_WAVE);
+      q += __shfl_xor(q, o, RLT_WAVE);
+      before += __shfl_xor(before, o, RLT_WAVE);
+    }
+    const double lse = log(s);  // over the maximum; a row without a finite one gives NaN
+    if (t == 0) {
+      const bool ok = m > -INFINITY;
+      sh[0] = ok ? (double)m : (double)nan;
+      sh[1] = lse;
+      P.logprob[r] = ok && in ? (float)(((double)xt - (double)m) - lse) : nan;
+      P.entropy[r] = ok ? (float)(lse - q / s) : nan;
+      P.rank[r] = in ? 1 + (int64_t)before : 0;
+    }
   }
   if (P.top_n > 0) {
-    const unsigned long long* const c = P.candidates + r * P.slices * P.top_n;
-    const int total = P.slices * P.top_n, items = (total + kThreads - 1) / kThreads;
-    select_top<0>(
-        top, P.top_n, items,
-        [&](int i) { return i * kThreads + t < total ? c[i * kThreads + t] : 0ull; },
-        [&](int rank, unsigned long long x) {
-          const int64_t at = r * P.top_n + rank;
-          P.top_tokens[at] = x ? (int64_t)composite_col(x) : -1;
-          P.top_logprob[at] =
-              x && ok ? (float)(((double)key_value((uint32_t)(x >> 32)) - (double)m) - lse) : nan;
-        });
+    // (a candidate's key is 0 where a slice had fewer columns)
+    put_bound(top, (uint32_t)(best >> 32), P.top_n);
+    __syncthreads();
+    const uint32_t bound = max(get_bound(top), 1u);
+    if ((uint32_t)(best >> 32) >= bound)
+      for (int i = 0; i < items; ++i)
+        if ((uint32_t)(item(i) >> 32) >= bound) list_column(top, item(i));
+    __syncthreads();
+    const double m = sh[0], lse = sh[1];
+    auto put = [&](int rank, unsigned long long x) {
+      const int64_t at = r * P.top_n + rank;
+      P.top_tokens[at] = x ? (int64_t)composite_col(x) : -1;
+      P.top_logprob[at] = x ? (float)(((double)key_value((uint32_t)(x >> 32)) - m) - lse) : nan;
+    };
+    const int found = top.count;  // (the same in every thread)
+    if (found <= kThreads) {
+      rank_list(top, found, P.top_n, put);
+    } else {
+      __syncthreads();
+      select_top<0>(top, P.top_n, items, item, put);
+    }
   }
 }
 

@@ -86,6 +86,15 @@ struct Slice {
     }
   }
   __device__ __forceinline__ float at(int i, int e) const { return piece_at<DT>(p[i], e); }
+  // (a value that the type holds)
+  __device__ __forceinline__ void set(int i, int e, float v) {
+    if constexpr (DT == RLT_F32) {
+      p[i].w[e] = __float_as_uint(v);
+    } else {
+      const uint32_t b = DT == RLT_BF16 ? f32_to_bf16_bits(v) : f32_to_f16_bits(v);
+      p[i].w[e >> 1] = e & 1 ? (p[i].w[e >> 1] & 0xffffu) | b << 16 : (p[i].w[e >> 1] & 0xffff0000u) | b;
+    }
+  }
 };
 
 __device__ __forceinline__ unsigned long long wave_max(unsigned long long x) {
