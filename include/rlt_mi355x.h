@@ -461,7 +461,7 @@ int rlt_greedy_tree_accept(const int64_t* draft_tokens, const int64_t* parents,
  * rlt_categorical.  All in float64; rows of p and q count as distributions as they stand.
  * error[r] is set, and the final token 0, where drafts[r] is outside [0, width], a tried draft
  * has a token outside the vocabulary, no q mass or weights that are not finite, or where the
- * weights left have no finite positive mass.
+ * weights left have no finite positive mass (a NaN or an infinity in a row that is summed).
  *   draft_tokens, parents int64 [n, width], drafts int64 [n], q fp32 [n, width, V] (row i:
  *   the distribution that node i's children were drawn from; the last node has none), p fp32
  *   [n, width + 1, V], u_accept fp32 [n, width], u_final fp32 [n] (contiguous)

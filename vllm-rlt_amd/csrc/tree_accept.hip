@@ -16,14 +16,16 @@
 // rejections y = max(p - C q, 0) with C = R_0 + .. + R_(k-1): no residual is stored, and a
 // rejection costs one sum over the node's two rows.  Where no child is left the next token is
 // drawn from y by inverse CDF.  The emitted tokens follow p whatever q and the tree are.
-// Sums, weights and the CDF are float64: one workgroup per request, each thread 16
-// consecutive columns at a time; the wave sums of the last pass are the CDF's coarse table.
+// Sums, weights and the CDF are float64: one workgroup per request, each wave 1024 columns at a
+// time, the next ones in flight; the wave sums of the last pass are the CDF's coarse table.
 
 #include "vocab_rows.h"
 
 #include "rlt_mi355x.h"
 
 #include <math.h>
+
+#include <type_traits>
 
 namespace {
 
@@ -133,61 +135,104 @@ __global__ __launch_bounds__(kThreads) void rlt_greedy_tree_kernel(
 
 constexpr int kAccThreads = 1024;
 constexpr int kAccWaves = kAccThreads / 64;
-constexpr int kRun = 16;                           // consecutive columns of a thread
+constexpr int kRun = 16;                           // columns of a thread and step
 constexpr int64_t kStep = (int64_t)kAccThreads * kRun;
 constexpr int kMaxSegments = (int)(kMaxVocab / kStep) * kAccWaves;
 
 struct AcceptShared {
   double seg[kMaxSegments];  // weight of every wave's kRun * 64 columns, in column order
-  float px[kMaxDrafts], qx[kMaxDrafts];
+  float px[kMaxDrafts], qx[kMaxDrafts], u[kMaxDrafts];
   int32_t parent[kMaxDrafts];
   int64_t token[kMaxDrafts];
   int32_t walk[kMaxDrafts + 1];  // the accepted path
   int64_t last;
 };
 
-// y = max(p - C q, 0), NaN kept
+// y = max(p - C q, 0); NaN becomes 0 here and is looked for apart
 __device__ __forceinline__ double left_of(float p, float q, double C) {
-  const double y = (double)p - C * (double)q;
-  return y < 0.0 ? 0.0 : y;
+  return fmax(__builtin_fma(-C, (double)q, (double)p), 0.0);
 }
 
 struct __attribute__((packed, aligned(4))) Quad {
   float v[4];
 };
 
-// Segment weights of a node's rows for C; q is not read for C = 0.
+// A wave's 1024 columns of one step from c on (a lane takes every 256th four, so that a load is
+// contiguous); zeros past the row's last whole four.
+struct Run {
+  Quad a[kRun / 4], b[kRun / 4];
+  __device__ __forceinline__ void load(const float* p, const float* q, int64_t c, int64_t vocab) {
+    const int lane = threadIdx.x & 63;
+#pragma unroll
+    for (int i = 0; i < kRun / 4; ++i) {
+      const int64_t at = c + 256 * i + 4 * lane;
+      a[i] = b[i] = Quad{{0.f, 0.f, 0.f, 0.f}};
+      if (at + 4 <= vocab) {
+        a[i] = *(const Quad*)(p + at);
+        b[i] = *(const Quad*)(q + at);
+      }
+    }
+  }
+};
+
+// Sum over the wave by lane exchanges of the vector unit (quads, halves, rows of 16, then the
+// row pairs): through LDS these exchanges took longer than the columns.
+__device__ __forceinline__ double pair_sum(uint32_t lo0, uint32_t hi0, uint32_t lo1, uint32_t hi1) {
+  return __hiloint2double((int)hi0, (int)lo0) + __hiloint2double((int)hi1, (int)lo1);
+}
+__device__ __forceinline__ double wave_sum(double x) {
+  auto add = [&](auto ctrl) {
+    const int lo = __builtin_amdgcn_update_dpp(0, __double2loint(x), decltype(ctrl)::value, 0xf, 0xf, true);
+    const int hi = __builtin_amdgcn_update_dpp(0, __double2hiint(x), decltype(ctrl)::value, 0xf, 0xf, true);
+    x += __hiloint2double(hi, lo);
+  };
+  add(std::integral_constant<int, 0xB1>{});   // quad_perm: lane ^ 1
+  add(std::integral_constant<int, 0x4E>{});   // quad_perm: lane ^ 2
+  add(std::integral_constant<int, 0x141>{});  // row_half_mirror: the other quad of eight
+  add(std::integral_constant<int, 0x140>{});  // row_mirror: the other eight of the row
+  auto lo = __builtin_amdgcn_permlane16_swap(__double2loint(x), __double2loint(x), false, false);
+  auto hi = __builtin_amdgcn_permlane16_swap(__double2hiint(x), __double2hiint(x), false, false);
+  x = pair_sum(lo[0], hi[0], lo[1], hi[1]);
+  lo = __builtin_amdgcn_permlane32_swap(__double2loint(x), __double2loint(x), false, false);
+  hi = __builtin_amdgcn_permlane32_swap(__double2hiint(x), __double2hiint(x), false, false);
+  return pair_sum(lo[0], hi[0], lo[1], hi[1]);
+}
+
+// Segment weights of a node's rows for C (0 with q = p: the target's own).
 __device__ __forceinline__ void weigh(AcceptShared& sh, const float* p, const float* q, double C,
                                       int64_t vocab) {
-  const int t = threadIdx.x, w = t >> 6;
-  const bool plain = C == 0.0;
-  int step = 0;
-  for (int64_t base = 0; base < vocab; base += kStep, ++step) {
-    const int64_t c = base + (int64_t)t * kRun;
-    double s = 0.0;
-    if (c + kRun <= vocab) {
-      Quad a[kRun / 4], b[kRun / 4];
+  const int t = threadIdx.x, w = t >> 6, lane = t & 63;
+  const int steps = (int)((vocab + kStep - 1) / kStep);
+  float odd = 0.f;  // NaN where a column is
+  int64_t c = (int64_t)w * (64 * kRun);
+  Run cur, next;
+  cur.load(p, q, c, vocab);
+#pragma unroll 1
+  for (int step = 0; step < steps; ++step, c += kStep) {
+    if (step + 1 < steps) next.load(p, q, c + kStep, vocab);
+    double s[4] = {0.0, 0.0, 0.0, 0.0};
 #pragma unroll
-      for (int i = 0; i < kRun / 4; ++i) a[i] = *(const Quad*)(p + c + 4 * i);
-      if (!plain) {
+    for (int i = 0; i < kRun / 4; ++i)
 #pragma unroll
-        for (int i = 0; i < kRun / 4; ++i) b[i] = *(const Quad*)(q + c + 4 * i);
-      } else {
-#pragma unroll
-        for (int i = 0; i < kRun / 4; ++i) b[i] = Quad{{0.f, 0.f, 0.f, 0.f}};
+      for (int e = 0; e < 4; ++e) {
+        // (x - x is NaN for NaN and infinities: no distribution)
+        odd += (cur.a[i].v[e] - cur.a[i].v[e]) + (cur.b[i].v[e] - cur.b[i].v[e]);
+        s[e] += left_of(cur.a[i].v[e], cur.b[i].v[e], C);
       }
-#pragma unroll
-      for (int i = 0; i < kRun / 4; ++i)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) s += left_of(a[i].v[e], b[i].v[e], C);
-    } else {
-      for (int i = 0; i < kRun; ++i)
-        if (c + i < vocab) s += left_of(p[c + i], plain ? 0.f : q[c + i], C);
-    }
-#pragma unroll
-    for (int o = 32; o >= 1; o >>= 1) s += __shfl_xor(s, o, RLT_WAVE);
-    if ((t & 63) == 0) sh.seg[step * kAccWaves + w] = s;
+    double sum = (s[0] + s[1]) + (s[2] + s[3]);
+    // the row's last columns, fewer than four
+    const int64_t rest = vocab & ~(int64_t)3;
+    if (rest < vocab && rest >= c && rest < c + 64 * kRun && lane == 0)
+      for (int64_t at = rest; at < vocab; ++at) {
+        odd += (p[at] - p[at]) + (q[at] - q[at]);
+        sum += left_of(p[at], q[at], C);
+      }
+    sum = wave_sum(sum);
+    if (lane == 0) sh.seg[step * kAccWaves + w] = sum;
+    cur = next;
   }
+  if (__builtin_amdgcn_ballot_w64(odd != 0.f) != 0 && lane == 0)
+    sh.seg[w] = __longlong_as_double(0x7ff8000000000000ll);
   __syncthreads();
 }
 
@@ -236,11 +281,27 @@ __device__ __forceinline__ int64_t draw(const AcceptShared& sh, const float* p, 
   seg = __shfl(seg, owner, RLT_WAVE);
   at = __shfl(at, owner, RLT_WAVE);
   const int64_t c = (int64_t)(seg / kAccWaves) * kStep + (int64_t)(seg % kAccWaves) * 64 * kRun + lane * kRun;
-  const bool plain = C == 0.0;
+  // (here a lane's columns are consecutive)
+  Quad a[kRun / 4], b[kRun / 4];
+#pragma unroll
+  for (int i = 0; i < kRun / 4; ++i) {
+    const int64_t from = c + 4 * i;
+    a[i] = b[i] = Quad{{0.f, 0.f, 0.f, 0.f}};
+    if (from + 4 <= vocab) {
+      a[i] = *(const Quad*)(p + from);
+      b[i] = *(const Quad*)(q + from);
+    } else {
+      for (int e = 0; e < 3; ++e)
+        if (from + e < vocab) {
+          a[i].v[e] = p[from + e];
+          b[i].v[e] = q[from + e];
+        }
+    }
+  }
   double y[kRun], mine = 0.0;
 #pragma unroll
   for (int i = 0; i < kRun; ++i) {
-    y[i] = c + i < vocab ? left_of(p[c + i], plain ? 0.f : q[c + i], C) : 0.0;
+    y[i] = left_of(a[i / 4].v[i % 4], b[i / 4].v[i % 4], C);
     mine += y[i];
   }
   const double incl = wave_incl(mine);
@@ -271,10 +332,12 @@ __global__ __launch_bounds__(kAccThreads) void rlt_tree_accept_kernel(
   const int64_t d = drafts[r];
   const int live = (int)(d < 0 ? 0 : d > width ? width : d);
   bool bad = d != live;
+  const float last_u = u_final[r];
   // every draft's two probabilities at its parent, in one round of loads
   for (int j = t; j < live; j += kAccThreads) {
     const int64_t parent = parents[r * width + j], token = draft_tokens[r * width + j];
     const bool child = parent >= 0 && parent <= j;
+    sh.u[j] = u_accept[r * width + j];
     sh.parent[j] = child ? (int32_t)parent : -1;
     sh.token[j] = token;
     const bool in = child && token >= 0 && token < vocab;
@@ -295,7 +358,7 @@ __global__ __launch_bounds__(kAccThreads) void rlt_tree_accept_kernel(
     const double px = sh.px[j], qx = sh.qx[j];
     if (!(qx > 0.0) || !(fabs(px) < INFINITY) || !(qx < INFINITY)) {
       bad = true;
-    } else if ((double)u_accept[r * width + j] * R * qx < px - C * qx) {
+    } else if ((double)sh.u[j] * R * qx < px - C * qx) {
       ++count;
       node = j + 1;
       if (t == 0) sh.walk[count] = node;
@@ -313,18 +376,19 @@ __global__ __launch_bounds__(kAccThreads) void rlt_tree_accept_kernel(
   if (!bad) {
     if (C == 0.0) {
       __syncthreads();
-      weigh(sh, p + (int64_t)node * vocab, q, 0.0, vocab);
+      weigh(sh, p + (int64_t)node * vocab, p + (int64_t)node * vocab, 0.0, vocab);
     }
     if (t < 64) {
       double before;
       const double total = segment_scan(sh, segments, before);
       bad = !(total > 0.0) || !(total < INFINITY);
       if (!bad) {
-        const double u = (double)u_final[r] * total;
+        const double u = (double)last_u * total;
         // the draw stays below the total
         const double top = __longlong_as_double(__double_as_longlong(total) - 1);
-        const int64_t token = draw(sh, p + (int64_t)node * vocab, q + (int64_t)node * vocab, C, vocab,
-                                   segments, before, u < top ? u : top);
+        const float* const row = p + (int64_t)node * vocab;
+        const int64_t token = draw(sh, row, C == 0.0 ? row : q + (int64_t)node * vocab, C, vocab, segments,
+                                   before, u < top ? u : top);
         if (t == 0) sh.last = token;
       }
     }
