@@ -467,16 +467,13 @@ int rlt_greedy_tree_accept(const int64_t* draft_tokens, const int64_t* parents,
  *   [n, width + 1, V], u_accept fp32 [n, width], u_final fp32 [n] (contiguous)
  *   -> path (as above), tokens int64 [n, width + 1] (the accepted tokens, the final one,
  *   zeros), accepted, final_token int64 [n], error uint8 (bool) [n].
- * width <= 255, V <= 2^20.  Workspace: rlt_tree_accept_workspace_size.  The chain's round is
+ * width <= 255, V <= 2^20.  No workspace.  The chain's round is
  * vllm_rlt/worker/speculative_sampling.py:104-181.
  */
-size_t rlt_tree_accept_workspace_size(int64_t n, int32_t width, int64_t vocab);
-
 int rlt_tree_accept(const int64_t* draft_tokens, const int64_t* parents, const int64_t* drafts,
                     const float* q, const float* p, const float* u_accept, const float* u_final,
                     int64_t n, int32_t width, int64_t vocab, int64_t* path, int64_t* tokens,
-                    int64_t* accepted, int64_t* final_token, uint8_t* error, void* workspace,
-                    size_t workspace_bytes, hipStream_t stream);
+                    int64_t* accepted, int64_t* final_token, uint8_t* error, hipStream_t stream);
 
 /*
  * Log probabilities of given tokens, with rank, entropy and the top alternatives of their

@@ -64,7 +64,7 @@ def test_round_statuses(pkg):
 
     def sampled(n=2, w=4, vocab=100, p=FAKE, q=FAKE):
         return L.rlt_tree_accept(FAKE, FAKE, FAKE, q, p, FAKE, FAKE, n, w, vocab, FAKE, FAKE, FAKE,
-                                 FAKE, FAKE, NULL, 0, NULL)
+                                 FAKE, FAKE, NULL)
 
     assert sampled(n=0) == 0
     assert sampled(w=-1) == 1 and sampled(p=NULL) == 1 and sampled(q=NULL) == 1

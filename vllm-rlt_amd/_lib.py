@@ -142,9 +142,8 @@ _SIGNATURES = {
     "rlt_greedy_tree_accept_workspace_size": (_sz, [_i64, _i32, _i64]),
     "rlt_greedy_tree_accept": (ctypes.c_int, [
         _p, _p, _p, _p, _i32, _i64, _i64, _i32, _i64, _p, _p, _p, _p, _p, _sz, _p]),
-    "rlt_tree_accept_workspace_size": (_sz, [_i64, _i32, _i64]),
     "rlt_tree_accept": (ctypes.c_int, [
-        _p, _p, _p, _p, _p, _p, _p, _i64, _i32, _i64, _p, _p, _p, _p, _p, _p, _sz, _p]),
+        _p, _p, _p, _p, _p, _p, _p, _i64, _i32, _i64, _p, _p, _p, _p, _p, _p]),
     "rlt_token_logprobs_workspace_size": (_sz, [_i64, _i64, _i32]),
     "rlt_token_logprobs": (ctypes.c_int, [
         _p, _i32, _i64, _i64, _i64, _p, _p, _i64, _i32, _p, _p, _p, _p, _p, _p, _sz, _p]),
@@ -237,7 +236,7 @@ def check(status, what):
 
 def require_gpu(*tensors):
     for t in tensors:
-        if t is not None and t.device.type != "cuda":
+        if t is not None and not t.is_cuda:
             raise ValueError("the MI355X kernels require ROCm device tensors")
 
 

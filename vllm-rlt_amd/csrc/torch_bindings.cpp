@@ -623,6 +623,28 @@ Tensor paged_attention_store(const Tensor& q, const Tensor& k_new_in, const Tens
 
 // ---------------------------------------------------------------- draft trees
 
+// The outputs of one call as views of one allocation (an allocation takes about a microsecond
+// of the host, which the small calls of a round are bound by).
+class Outputs {
+ public:
+  Outputs(int64_t bytes, const Tensor& like) : buffer_(at::empty({bytes}, like.options().dtype(at::kByte))) {}
+  static int64_t room(int64_t elements, int64_t size) { return (elements * size + 255) / 256 * 256; }
+  Tensor take(at::IntArrayRef sizes, at::ScalarType dtype) {
+    auto impl = c10::make_intrusive<c10::TensorImpl>(c10::Storage(buffer_.storage()), buffer_.key_set(),
+                                                     c10::scalarTypeToTypeMeta(dtype));
+    const int64_t size = (int64_t)c10::elementSize(dtype);
+    impl->set_storage_offset(at_ / size);
+    impl->set_sizes_contiguous(sizes);
+    Tensor t(std::move(impl));
+    at_ += room(t.numel(), size);
+    return t;
+  }
+
+ private:
+  Tensor buffer_;
+  int64_t at_ = 0;
+};
+
 // Attention of the nodes of draft trees (rlt_tree_attention): packed rows, an ancestor mask in
 // place of the causal window.
 Tensor tree_attention(const Tensor& q, const Tensor& key_cache, const Tensor& value_cache,
@@ -751,10 +773,10 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> greedy_tree_accept(const Tensor& draf
   need(draft_tokens, at::kLong, "draft_tokens");
   need(parents, at::kLong, "parents");
   need(drafts, at::kLong, "drafts");
-  const auto i64 = draft_tokens.options();
   const c10::hip::HIPGuardMasqueradingAsCUDA guard(target_logits.device());
-  Tensor targets = at::empty({n, w + 1}, i64), path = at::empty({n, w + 1}, i64);
-  Tensor accepted = at::empty({n}, i64), next = at::empty({n}, i64);
+  Outputs outs(2 * Outputs::room(n * (w + 1), 8) + 2 * Outputs::room(n, 8), drafts);
+  Tensor targets = outs.take({n, w + 1}, at::kLong), path = outs.take({n, w + 1}, at::kLong);
+  Tensor accepted = outs.take({n}, at::kLong), next = outs.take({n}, at::kLong);
   if (n == 0) return {targets, path, accepted, next};
   const Tensor ws = workspace(rlt_greedy_tree_accept_workspace_size(n, (int32_t)w, vocab), drafts);
   const int status = rlt_greedy_tree_accept(
@@ -788,19 +810,17 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> tree_accept(
   need(p, at::kFloat, "p");
   need(u_accept, at::kFloat, "u_accept");
   need(u_final, at::kFloat, "u_final");
-  const auto i64 = draft_tokens.options();
   const c10::hip::HIPGuardMasqueradingAsCUDA guard(p.device());
-  Tensor path = at::empty({n, w + 1}, i64), tokens = at::empty({n, w + 1}, i64);
-  Tensor accepted = at::empty({n}, i64), final_token = at::empty({n}, i64);
-  Tensor error = at::empty({n}, i64.dtype(at::kBool));
+  Outputs outs(2 * Outputs::room(n * (w + 1), 8) + 2 * Outputs::room(n, 8) + Outputs::room(n, 1), p);
+  Tensor path = outs.take({n, w + 1}, at::kLong), tokens = outs.take({n, w + 1}, at::kLong);
+  Tensor accepted = outs.take({n}, at::kLong), final_token = outs.take({n}, at::kLong);
+  Tensor error = outs.take({n}, at::kBool);
   if (n == 0) return {path, tokens, accepted, final_token, error};
-  const Tensor ws = workspace(rlt_tree_accept_workspace_size(n, (int32_t)w, vocab), p);
   const int status = rlt_tree_accept(
       (const int64_t*)ptr(draft_tokens), (const int64_t*)ptr(parents), (const int64_t*)ptr(drafts),
       (const float*)ptr(q), (const float*)ptr(p), (const float*)ptr(u_accept),
       (const float*)ptr(u_final), n, (int32_t)w, vocab, (int64_t*)ptr(path), (int64_t*)ptr(tokens),
-      (int64_t*)ptr(accepted), (int64_t*)ptr(final_token), (uint8_t*)ptr(error), ptr(ws),
-      ws.numel(), stream_of(p));
+      (int64_t*)ptr(accepted), (int64_t*)ptr(final_token), (uint8_t*)ptr(error), stream_of(p));
   check_status(status, "rlt_tree_accept");
   return {path, tokens, accepted, final_token, error};
 }
@@ -822,11 +842,13 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> token_logprobs(const Tensor& 
   TORCH_CHECK_VALUE(m <= 1 || logits.stride(0) >= vocab, "logits rows must not overlap");
   need(tokens, at::kLong, "tokens");
   need(rows, at::kLong, "rows");
-  const auto i64 = tokens.options(), f32 = tokens.options().dtype(at::kFloat);
   const c10::hip::HIPGuardMasqueradingAsCUDA guard(logits.device());
-  Tensor logprob = at::empty({count}, f32), rank = at::empty({count}, i64);
-  Tensor entropy = at::empty({count}, f32), top_logprob = at::empty({count, top_n}, f32);
-  Tensor top_tokens = at::empty({count, top_n}, i64);
+  Outputs outs(2 * Outputs::room(count, 4) + Outputs::room(count, 8) + Outputs::room(count * top_n, 4) +
+                   Outputs::room(count * top_n, 8),
+               tokens);
+  Tensor logprob = outs.take({count}, at::kFloat), rank = outs.take({count}, at::kLong);
+  Tensor entropy = outs.take({count}, at::kFloat), top_logprob = outs.take({count, top_n}, at::kFloat);
+  Tensor top_tokens = outs.take({count, top_n}, at::kLong);
   // (a launch takes 65535 rows)
   for (int64_t at = 0; at < count; at += 65535) {
     const int64_t part = std::min<int64_t>(count - at, 65535);

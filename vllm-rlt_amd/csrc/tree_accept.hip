@@ -413,13 +413,10 @@ int64_t argmax_slices(int64_t vocab) {
 
 extern "C" {
 
-size_t rlt_tree_accept_workspace_size(int64_t n, int32_t width, int64_t vocab) { return 0; }
-
 int rlt_tree_accept(const int64_t* draft_tokens, const int64_t* parents, const int64_t* drafts,
                     const float* q, const float* p, const float* u_accept, const float* u_final,
                     int64_t n, int32_t width, int64_t vocab, int64_t* path, int64_t* tokens,
-                    int64_t* accepted, int64_t* final_token, uint8_t* error, void* workspace,
-                    size_t workspace_bytes, hipStream_t stream) {
+                    int64_t* accepted, int64_t* final_token, uint8_t* error, hipStream_t stream) {
   if (n < 0 || width < 0 || vocab < 1) return RLT_ERR_ARGUMENT;
   if (width > kMaxDrafts || vocab > kMaxVocab || n > 0x7fffffff) return RLT_ERR_UNSUPPORTED;
   if (n == 0) return RLT_OK;
