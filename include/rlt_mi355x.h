@@ -207,7 +207,8 @@ int rlt_paged_attention_uses_prefill(int32_t q_dtype, int32_t kv_dtype, int32_t 
  * [0, context_lengths[s] - N) and the nodes j of its own tree whose bit is set: bit j % 64 of
  * word j / 64 of its tree_mask row (int64 [num_q_rows, mask_words], mask_stride words
  * between rows; rlt_tree_masks makes the ancestors' bits from the parents).  Bits past the
- * tree are ignored; a row that sees nothing gives zeros.  With window > 0 a row sees the
+ * tree are ignored; a row that sees nothing gives zeros, rows of no sequence are not written.
+ * With window > 0 a row sees the
  * last `window` of those positions.  Keys, values and scales at positions that a row does
  * not see have no effect on it, whatever they hold.  Other arguments as
  * rlt_paged_attention; the pool is of q's type (no scales) or fp8-e4m3 (scale_mode 1 or 2).
@@ -709,8 +710,9 @@ int rlt_merge_random_round(const int64_t* target, int64_t num_rows, const int64_
 
 /* Mask rows of draft trees for rlt_tree_attention: q row cu_seqlens_q[s] + i is node i of
  * sequence s and sees itself and its ancestors; node i's parent is parents[s, i - 1] (int64
- * [num_seqs, width], parent_stride between rows), node 0 the root.  A parent outside [0, i), or a
- * node past width, ends the walk.  mask int64 [rows, words]; rows of no sequence are cleared.
+ * [num_seqs, width], parent_stride between rows, width <= 255), node 0 the root.  A parent
+ * outside [0, i), or a node past width, ends the walk; nodes past 255 see nothing.
+ * cu_seqlens_q must not descend.  mask int64 [rows, words]; rows of no sequence are cleared.
  * No counterpart in the reference. */
 int rlt_tree_masks(const int64_t* parents, int64_t parent_stride, int32_t width,
                    const int32_t* cu_seqlens_q, int32_t num_seqs, int64_t* mask, int32_t words,

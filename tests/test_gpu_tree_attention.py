@@ -24,8 +24,8 @@ def call(pkg, dev, c, window=0, **over):
                        **{k: v for k, v in a.items() if k != "max_seqlen_q"})
 
 
-def check(got, c, window=0, rows=None):
-    want, tol = reference(c, window)
+def check(got, c, window=0, rows=None, fine=False):
+    want, tol = reference(c, window, fine)
     got = got.double().cpu()
     if rows is not None:
         got, want, tol = got[rows], want[rows], tol[rows]
@@ -318,3 +318,43 @@ def test_empty_calls(pkg, dev):
                cu_seqlens_q=torch.zeros(2, dtype=torch.int32))
     assert got.shape == (0, 2, 64)
     assert FP8  # (the fp8 cases are among SHAPES)
+
+
+@pytest.mark.parametrize("hq,hkv,dim,nodes", [(2, 2, 128, [16, 7]), (4, 1, 64, [40, 12]),
+                                              (8, 2, 96, [9, 16])])
+@pytest.mark.parametrize("low,high", [(-26, -22), (-20, 4), (2, 6)])
+def test_value_scales_of_any_size(pkg, dev, hq, hkv, dim, nodes, low, high):
+    """fp16 rows over per-vector scales far from 1, and over scales that differ widely."""
+    c = make_case(nodes, [515, 96], hq, hkv, dim, HF, "fp8_vector", seed=50 + dim)
+    g = torch.Generator().manual_seed(dim)
+    exps = low + (high - low) * torch.rand(c.v_scale.shape, generator=g)
+    c.v_scale = torch.where(c.v_scale.isnan(), c.v_scale, torch.exp2(exps))
+    check(call(pkg, dev, c), c, fine=True)
+
+
+def flat_keys(c, weight):
+    """Keys and values of sequence 0: position 0 has score 0 and value 0, each other one the
+    weight ``weight`` next to it and value 1."""
+    c.q.fill_(0)
+    c.q[..., 0] = 8
+    c.k.fill_(0)
+    c.k[..., 0] = math.log(weight) * math.sqrt(c.q.shape[-1]) / 8
+    c.v.fill_(1)
+    blk = int(c.tables[0, 0])
+    c.k[blk, 0], c.v[blk, 0] = 0, 0
+
+
+@pytest.mark.parametrize("nodes", [[3], [40]])
+def test_many_small_weights(pkg, dev, nodes):
+    """fp16: 20000 keys of weight 1.4 2^-25 next to one of 1 are a part of the row."""
+    c = make_case(nodes, [20000], 2, 1, 64, HF, seed=3, bits=[[1 << i for i in range(nodes[0])]])
+    flat_keys(c, 1.4 * 2.0 ** -25)
+    check(call(pkg, dev, c), c, fine=True)
+
+
+@pytest.mark.parametrize("dtype,dim", [(BF, 128), (HF, 64), (BF, 80)])
+@pytest.mark.parametrize("scale", [0.0, -1 / 60.0])
+def test_key_scale_zero_or_negative(pkg, dev, dtype, dim, scale):
+    c = make_case([16, 40], [515, 96], 4, 2, dim, dtype, "fp8", seed=60)
+    c.k_scale = torch.tensor(scale)
+    check(call(pkg, dev, c), c)

@@ -83,6 +83,18 @@ def test_commit_leaves_what_it_cannot_place(pkg, dev):
     assert torch.equal(kd.cpu(), want) and torch.equal(vd.cpu(), -want)
 
 
+def test_commit_of_far_positions(pkg, dev):
+    """Starts that no table reaches, up to the largest integer: nothing moves."""
+    g = torch.Generator().manual_seed(4)
+    k = torch.randn(6, 2, 4, 2, 16, generator=g)
+    tables = torch.tensor([[0, 1], [2, 3], [4, 5]], dtype=torch.int32)
+    starts = torch.tensor([(1 << 63) - 1, (1 << 63) - 3, 8])
+    path, accepted = torch.tensor([[0, 3, 5, 6]] * 3), torch.full((3,), 3)
+    kd, vd = k.to(dev), (-k).to(dev)
+    pkg.commit_tree_kv(kd, vd, *to_dev(dev, tables, starts, path, accepted), 4)
+    assert torch.equal(kd.cpu(), k) and torch.equal(vd.cpu(), -k)
+
+
 def to_dev(dev, *xs):
     return [x.to(dev) for x in xs]
 

@@ -95,6 +95,19 @@ def test_round_statuses(pkg):
     assert ctypes.sizeof(ctypes.c_void_p) == 8
 
 
+def test_launches_of_more_threads_than_an_axis_holds(pkg):
+    L = lib(pkg)
+    assert attend(pkg, seqs=1 << 21, ws_bytes=1 << 40) == 2
+    assert attend(pkg, seqs=1 << 25, d=80, ws_bytes=1 << 40) == 2
+    assert L.rlt_tree_accept(FAKE, FAKE, FAKE, FAKE, FAKE, FAKE, FAKE, 1 << 22, 4, 10, FAKE, FAKE,
+                             FAKE, FAKE, FAKE, NULL) == 2
+    assert L.rlt_greedy_tree_accept(FAKE, FAKE, FAKE, FAKE, 0, 10, 1 << 16, 255, 10, FAKE, FAKE, FAKE,
+                                    FAKE, FAKE, 1 << 40, NULL) == 2
+    assert L.rlt_kv_commit_path(FAKE, 1 << 23, 2, 4, 16, FAKE, FAKE, 5, 5, FAKE, 2, 10, FAKE, FAKE,
+                                4096, 2048, 128, 256, 2, NULL) == 2
+    assert L.rlt_tree_masks(FAKE, 256, 256, FAKE, 2, FAKE, 5, 5, NULL) == 2
+
+
 def test_host_tensors_are_refused(pkg):
     i64 = dict(dtype=torch.int64)
     t, d = torch.zeros(2, 3, **i64), torch.zeros(2, **i64)

@@ -107,7 +107,7 @@ def gathered(c, s):
     return out
 
 
-def reference(c, window=0):
+def reference(c, window=0, fine=False):
     """(output, tolerance) in float64, [rows, heads, dim].
 
     The tolerance counts the roundings of a kernel that takes scores in float32, weights in q's
@@ -117,6 +117,11 @@ def reference(c, window=0):
     the denominator by that much each; float32 sums over the keys, L 2^-24 A; and fp16 weights
     below 2^-14 are multiples of 2^-24 next to a sum of at least 1, so they add 2^-25 of the
     values as the product holds them (codes where a scale is in the weight).
+
+    ``fine`` counts what a kernel leaves that keeps the largest fp16 weight at 2^7 or more:
+    2^-32 of the values; and with a scale in the weight, the largest product of weight and scale
+    there too (up to 2^4 lower where the running maximum has moved since it was taken): 2^-28
+    of it times the codes.
     """
     rows, hq, dim = c.q.shape
     hkv = c.k.shape[2]
@@ -140,12 +145,18 @@ def reference(c, window=0):
                 es = 2 * dim * 2.0 ** -24 * size
                 t = a * (u + es + (c.ctx[s] + 8) * 2.0 ** -24) * 1.01 + u * o.abs()
                 if c.q.dtype == torch.float16:
-                    held = vv.abs()
+                    held = vv
                     if c.v_scale is not None and c.v_scale.ndim == 3:
                         pos = torch.arange(c.ctx[s])
                         held = held / c.v_scale[c.tables[s, pos // c.block].long(),
                                                 pos % c.block][:, h // group, None].double()
-                    t = t + 2.0 ** -25 * (sees.double() @ held.nan_to_num(0, 0, 0)) + 2.0 ** -25
+                    unit = 2.0 ** -25
+                    if fine and held is not vv:
+                        y = c.v_scale[c.tables[s, pos // c.block].long(), pos % c.block][:, h // group]
+                        unit = 2.0 ** -28 * (p * y.double().abs()).amax(-1, keepdim=True)
+                    elif fine:
+                        unit = 2.0 ** -32
+                    t = t + unit * (sees.double() @ held.abs().nan_to_num(0, 0, 0)) + 2.0 ** -25
                 out[begin:begin + m, h] = o
                 tol[begin:begin + m, h] = t
         begin += m

@@ -195,7 +195,7 @@ __global__ __launch_bounds__(256) void rlt_kv_commit_kernel(
     const int32_t* const table = tables + (r * planes + plane) * (int64_t)width;
     int64_t f = -1, g = -1;
     const int64_t src = start + node, dst = start + t + 1;
-    if (start >= 0 && node > t + 1 && node <= kMaxPath && dst / block_size < width &&
+    if (start >= 0 && start < (int64_t)width * block_size && node > t + 1 && node <= kMaxPath &&
         src / block_size < width) {
       const int64_t sb = table[src / block_size], db = table[dst / block_size];
       if (sb >= 0 && sb < num_blocks && db >= 0 && db < num_blocks) {
@@ -333,7 +333,7 @@ int rlt_kv_commit_path(const int32_t* tables, int64_t n, int32_t planes, int32_t
   if (n < 0 || planes < 1 || width < 0 || block_size < 1 || path_width < 0 || layers < 1 ||
       num_blocks < 0 || bytes_per_token < 1 || elt_bytes < 1 || (n > 1 && path_stride < path_width))
     return RLT_ERR_ARGUMENT;
-  if (path_width > kMaxPath + 1 || layers > 32767 || n * planes > 0x7fffffff)
+  if (path_width > kMaxPath + 1 || layers > 32767 || n > UINT32_MAX / 256 / planes)  // (threads of a launch)
     return RLT_ERR_UNSUPPORTED;
   if (n == 0 || path_width < 2 || width == 0) return RLT_OK;
   if (!tables || !starts || !path || !accepted || !key_pool || !value_pool) return RLT_ERR_ARGUMENT;

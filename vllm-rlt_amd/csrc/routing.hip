@@ -179,31 +179,45 @@ inline bool grid_ok(int64_t x, int64_t y, int64_t z = 1) {
 }
 
 // Mask rows of draft trees: node i of sequence s (q row cu[s] + i) sees itself and its
-// ancestors.  One thread per row walks the parents up to the root, node 0.
+// ancestors.  One wave per sequence: its parents go to LDS, then every lane walks from its
+// nodes up to the root, node 0 (a walk through global memory pays a load's latency per step).
+constexpr int kTreeDrafts = 255;
+constexpr int kTreeWords = 4;
 __global__ __launch_bounds__(kThreads) void rlt_tree_masks_kernel(
     const int64_t* __restrict__ parents, int64_t parent_stride, int width,
     const int32_t* __restrict__ cu, int num_seqs, uint64_t* __restrict__ mask, int words,
     int64_t rows) {
-  const int64_t row = (int64_t)blockIdx.x * kThreads + threadIdx.x;
-  if (row >= rows) return;
-  uint64_t* const out = mask + row * words;
-  for (int w = 0; w < words; ++w) out[w] = 0;
-  // the last sequence that begins at or before the row (empty ones begin there too)
-  int lo = 0, hi = num_seqs;  // cu[lo] <= row is kept, cu[hi] > row or hi == num_seqs
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (cu[mid] <= row) lo = mid;
-    else hi = mid;
+  __shared__ int16_t up[kThreads / 64][kTreeDrafts + 1];  // of node i; -1: its walk ends there
+  const int w = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const int64_t s = (int64_t)blockIdx.x * (kThreads / 64) + w;
+  const bool live = s < num_seqs;
+  const int64_t begin = live ? max(cu[s], 0) : 0, end = live ? min((int64_t)cu[s + 1], rows) : 0;
+  if (live)
+    for (int i = lane; i <= kTreeDrafts; i += 64) {
+      const int64_t p = i > 0 && i <= width ? parents[s * parent_stride + i - 1] : -1;
+      up[w][i] = (int16_t)(p >= 0 && p < i ? p : -1);
+    }
+  __syncthreads();
+  for (int64_t row = begin + lane; row < end; row += 64) {
+    uint64_t x[kTreeWords] = {0, 0, 0, 0};
+    for (int64_t node = row - begin; node >= 0 && node <= kTreeDrafts; node = up[w][node]) {
+      const uint64_t bit = 1ull << (node & 63);
+#pragma unroll
+      for (int i = 0; i < kTreeWords; ++i) x[i] |= node >> 6 == i ? bit : 0ull;
+    }
+    uint64_t* const out = mask + row * words;
+#pragma unroll
+    for (int i = 0; i < kTreeWords; ++i)
+      if (i < words) out[i] = x[i];
+    for (int i = kTreeWords; i < words; ++i) out[i] = 0;
   }
-  if (num_seqs == 0 || row < cu[lo] || row >= cu[lo + 1]) return;  // in no sequence
-  const int64_t* const up = parents + lo * parent_stride;
-  int64_t node = row - cu[lo];
-  for (;;) {
-    if (node < 64 * (int64_t)words) out[node >> 6] |= 1ull << (node & 63);
-    if (node == 0 || node > width) break;
-    const int64_t p = up[node - 1];
-    if (p < 0 || p >= node) break;  // no earlier node: the walk ends
-    node = p;
+  // rows of no sequence
+  const int64_t first = num_seqs ? cu[0] : 0, last = num_seqs ? cu[num_seqs] : 0;
+  const int64_t ahead = min(max(first, (int64_t)0), rows), past = max(last, ahead);
+  for (int64_t at = (int64_t)blockIdx.x * kThreads + threadIdx.x; at < rows - past + ahead;
+       at += (int64_t)gridDim.x * kThreads) {
+    uint64_t* const out = mask + (at < ahead ? at : at - ahead + past) * words;
+    for (int i = 0; i < words; ++i) out[i] = 0;
   }
 }
 
@@ -366,10 +380,11 @@ int rlt_tree_masks(const int64_t* parents, int64_t parent_stride, int32_t width,
     return RLT_ERR_ARGUMENT;
   if (rows == 0) return RLT_OK;
   if (!cu_seqlens_q || !mask || (width && num_seqs && !parents)) return RLT_ERR_ARGUMENT;
-  if (rows > 0x7fffffffLL * kThreads) return RLT_ERR_UNSUPPORTED;
-  hipLaunchKernelGGL(rlt_tree_masks_kernel, dim3((unsigned)((rows + kThreads - 1) / kThreads)),
-                     dim3(kThreads), 0, stream, parents, parent_stride, width, cu_seqlens_q,
-                     num_seqs, (uint64_t*)mask, words, rows);
+  if (width > kTreeDrafts) return RLT_ERR_UNSUPPORTED;
+  const int64_t wgs = num_seqs ? (num_seqs + kThreads / 64 - 1) / (kThreads / 64) : 1;
+  if (wgs > UINT32_MAX / kThreads) return RLT_ERR_UNSUPPORTED;  // (threads of a launch)
+  hipLaunchKernelGGL(rlt_tree_masks_kernel, dim3((unsigned)wgs), dim3(kThreads), 0, stream, parents,
+                     parent_stride, width, cu_seqlens_q, num_seqs, (uint64_t*)mask, words, rows);
   return rlt_launch_status();
 }
 

@@ -667,7 +667,7 @@ Tensor tree_attention(const Tensor& q, const Tensor& key_cache, const Tensor& va
   TORCH_CHECK_VALUE(kv_heads >= 1 && heads >= 1 && heads % kv_heads == 0 &&
                         key_cache.size(3) == head_dim,
                     "q heads must be a positive multiple of KV heads with equal head_dim");
-  TORCH_CHECK_VALUE(num_blocks >= 1 && block_size >= 1 && num_blocks <= INT32_MAX,
+  TORCH_CHECK_VALUE(num_blocks >= 1 && block_size >= 1 && num_blocks <= INT32_MAX && block_size <= INT32_MAX,
                     "the KV pool must hold at least one block");
   TORCH_CHECK_VALUE(key_cache.stride(3) == 1 && value_cache.stride(3) == 1 && q.stride(2) == 1,
                     "paged attention requires a contiguous head dimension");

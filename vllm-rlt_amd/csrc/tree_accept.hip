@@ -34,6 +34,7 @@ using namespace vocab;
 constexpr int kMaxDrafts = 255;
 constexpr int64_t kMaxVocab = 1 << 20;
 constexpr int kSliceEpt = 32;
+constexpr int64_t kMaxLaunch = UINT32_MAX;  // threads of a launch along one axis
 
 // ---------------------------------------------------------------- greedy
 
@@ -418,7 +419,7 @@ int rlt_tree_accept(const int64_t* draft_tokens, const int64_t* parents, const i
                     int64_t n, int32_t width, int64_t vocab, int64_t* path, int64_t* tokens,
                     int64_t* accepted, int64_t* final_token, uint8_t* error, hipStream_t stream) {
   if (n < 0 || width < 0 || vocab < 1) return RLT_ERR_ARGUMENT;
-  if (width > kMaxDrafts || vocab > kMaxVocab || n > 0x7fffffff) return RLT_ERR_UNSUPPORTED;
+  if (width > kMaxDrafts || vocab > kMaxVocab || n > kMaxLaunch / kAccThreads) return RLT_ERR_UNSUPPORTED;
   if (n == 0) return RLT_OK;
   if (!drafts || !p || !u_final || !path || !tokens || !accepted || !final_token || !error ||
       (width && (!draft_tokens || !parents || !q || !u_accept)))
@@ -446,7 +447,7 @@ int rlt_greedy_tree_accept(const int64_t* draft_tokens, const int64_t* parents,
     return RLT_ERR_UNSUPPORTED;
   if (n == 0) return RLT_OK;
   const int64_t slices = argmax_slices(vocab), wgs = n * (width + 1) * slices;
-  if (n > 0x7fffffff || wgs > 0x7fffffff) return RLT_ERR_UNSUPPORTED;
+  if (n > 0x7fffffff || wgs > kMaxLaunch / kThreads) return RLT_ERR_UNSUPPORTED;
   if (!drafts || !target_logits || !targets || !path || !accepted || !next_token ||
       (width && (!draft_tokens || !parents)))
     return RLT_ERR_ARGUMENT;

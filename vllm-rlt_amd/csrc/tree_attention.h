@@ -53,6 +53,7 @@ constexpr int kRingBytes = 64 << 10;
 constexpr int kBadWords = kMaxNodes / kTile + 3;  // tiles that a range of kMaxNodes meets
 constexpr int kApartTiles = 8;     // tiles per workgroup from which kv groups take heads apart
 constexpr float kLazy = 8.f;       // log2 headroom before the running max moves
+constexpr float kLowExp = -100.f;  // lowest exponent that weights times value scales are held over
 
 struct Params {
   const void* q;
@@ -363,6 +364,8 @@ __global__ __launch_bounds__(64 * kWaves, per_cu<D>()) void rlt_tree_kernel(Para
   constexpr int NQ = D / 16;  // contraction slices of S^T
   constexpr int ND = D / 32;  // dim tiles of O^T
   constexpr int LV = G::LV, LK = LV + (SM == 2 ? 1 : 0);  // a wave's loads per tile
+  constexpr bool REFER = QT == RLT_F16 && SM == 2;
+  constexpr float LIFT = QT == RLT_F16 ? 7.f : 0.f;
   __shared__ Shared<QT, KVT, D, RW> sh;
   const int t = threadIdx.x, lane = t & 63, l32 = lane & 31, h = lane >> 5;
   const int w = __builtin_amdgcn_readfirstlane(t >> 6);
@@ -444,9 +447,12 @@ __global__ __launch_bounds__(64 * kWaves, per_cu<D>()) void rlt_tree_kernel(Para
   // (block, offset) of a tile's first position: advanced without a division
   const int step_q = uniform(macro / P.block_size), step_r = macro - step_q * P.block_size;
 
-  float qk_scale = P.qk_scale_log2, v_mul = 1.f;
+  // (the scale is not folded into qk_scale, which maxima and masked scores are multiplied by: it
+  // may be 0 or negative)
+  const float qk_scale = P.qk_scale_log2;
+  float k_mul = 1.f, v_mul = 1.f;
   if (SM == 1) {
-    qk_scale *= P.k_scale[0];
+    k_mul = P.k_scale[0];
     v_mul = P.v_scale[0];
   }
 
@@ -610,6 +616,7 @@ __global__ __launch_bounds__(64 * kWaves, per_cu<D>()) void rlt_tree_kernel(Para
 
     f32x16 oacc[ND];
     float m_run = -INFINITY, m_use = 0.f, l_run = 0.f;
+    float v_exp = kLowExp;  // REFER: oacc is the sum over 2^v_exp
 #pragma unroll
     for (int dt = 0; dt < ND; ++dt)
 #pragma unroll
@@ -641,9 +648,16 @@ __global__ __launch_bounds__(64 * kWaves, per_cu<D>()) void rlt_tree_kernel(Para
     };
     // ---- weights in the log2 domain, packed as the P^T operands.  The running maximum moves
     // only when a tile's exceeds it by kLazy (weights stay below 2^kLazy), so the accumulators
-    // are rarely rescaled.
+    // are rarely rescaled.  The product takes them in q's 16-bit type, as precise as the output.
+    // fp16 has few exponents: there weights lie 2^LIFT above their place, below its largest
+    // number, and weights times value scales, which may be of any size, are held over a power
+    // of two that follows the row's largest such product (REFER).
     auto scale_at = [](int pos) { return pos / SP * (2 * SP) + pos % SP; };
     auto weigh = [&](f32x16& sc, uint32_t (&p)[8], int tb, bool full, const float* scale) {
+      if constexpr (SM == 1) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) sc[i] *= k_mul;
+      }
       if constexpr (SM == 2) {
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
@@ -666,13 +680,19 @@ __global__ __launch_bounds__(64 * kWaves, per_cu<D>()) void rlt_tree_kernel(Para
       const bool grow = mx > m_run + kLazy;
       if (__builtin_amdgcn_ballot_w64(grow) != 0) {
         const float m_new = grow ? mx : m_run;
-        const float use = m_new == -INFINITY ? 0.f : m_new;
-        const float corr = grow ? __builtin_amdgcn_exp2f(m_run - use) : 1.f;
-        l_run *= corr;
+        const float step = grow ? m_new - m_run : 0.f;
+        l_run *= __builtin_amdgcn_exp2f(-step);
+        float o_step = step;
+        if constexpr (REFER) {
+          const float down = fminf(floorf(step), v_exp - kLowExp);
+          o_step -= down;
+          v_exp -= down;
+        }
+        const float corr = __builtin_amdgcn_exp2f(-o_step);
 #pragma unroll
         for (int dt = 0; dt < ND; ++dt) oacc[dt] *= corr;
         m_run = m_new;
-        m_use = use;
+        m_use = m_new == -INFINITY ? 0.f : m_new - LIFT;
       }
       float x[16];
 #pragma unroll
@@ -690,6 +710,24 @@ __global__ __launch_bounds__(64 * kWaves, per_cu<D>()) void rlt_tree_kernel(Para
 #pragma unroll
           for (int i = 0; i < 4; ++i) x[4 * g + i] = x[4 * g + i] == 0.f ? 0.f : x[4 * g + i] * y[i];
         }
+      }
+      if constexpr (REFER) {
+        float top = fabsf(x[0]);
+#pragma unroll
+        for (int i = 1; i < 16; ++i) top = fmaxf(top, fabsf(x[i]));
+        top = half_max(top);
+        const bool up = top > __builtin_amdgcn_ldexpf(32768.f, (int)v_exp);
+        if (__builtin_amdgcn_ballot_w64(up) != 0) {
+          // (the largest product becomes 2^7 .. 2^8; not finite: it stays so)
+          const float e = up ? (float)(__builtin_amdgcn_frexp_expf(top) - 8) : v_exp;
+          const float corr = __builtin_amdgcn_exp2f(v_exp - e);
+#pragma unroll
+          for (int dt = 0; dt < ND; ++dt) oacc[dt] *= corr;
+          v_exp = e;
+        }
+        const float down = __builtin_amdgcn_exp2f(-v_exp);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) x[i] *= down;
       }
 #pragma unroll
       for (int i = 0; i < 8; ++i) p[i] = pack2<QT>(x[2 * i], x[2 * i + 1]);
@@ -842,6 +880,11 @@ __global__ __launch_bounds__(64 * kWaves, per_cu<D>()) void rlt_tree_kernel(Para
         sh.ml[kg][r][1] = l;
       }
       float* const row = ob + (kg * RB + r) * G::OSTRIDE + 4 * h;
+      if constexpr (REFER) {
+        const float back = __builtin_amdgcn_exp2f(v_exp);
+#pragma unroll
+        for (int dt = 0; dt < ND; ++dt) oacc[dt] *= back;
+      }
 #pragma unroll
       for (int dt = 0; dt < ND; ++dt)
 #pragma unroll

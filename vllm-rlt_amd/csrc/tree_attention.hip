@@ -12,6 +12,7 @@ namespace tree {
 // ---------------------------------------------------------------- vector form
 
 constexpr int kVecDims = 256;
+constexpr int64_t kMaxLaunch = UINT32_MAX;  // threads of a launch along one axis
 
 // float32 q, other head sizes, unaligned pools or blocks that split an 8-position group: one
 // workgroup per (node, q head), its four waves taking 64-position tiles in turn.  Lane = key
@@ -299,7 +300,7 @@ int rlt_tree_attention(const void* q, int64_t q_row_stride, int64_t q_head_strid
     const int rb = 32 * row_waves(P.max_q * P.group, head_dim, kv_dtype == RLT_FP8_E4M3);
     P.max_blocks = (P.max_q * P.group + rb - 1) / rb;
     const int64_t pairs = (int64_t)num_seqs * num_kv_heads * P.max_blocks;
-    if (pairs > INT32_MAX) return RLT_ERR_UNSUPPORTED;
+    if (pairs > kMaxLaunch / kMergeThreads) return RLT_ERR_UNSUPPORTED;
     P.splits = (Split*)workspace;
     P.part = (float*)((char*)workspace + rlt_align_up((size_t)pairs * sizeof(Split), 256));
     if (q_dtype == RLT_BF16) launch_mfma<RLT_BF16>(P, kv_dtype, stream);
@@ -309,7 +310,7 @@ int rlt_tree_attention(const void* q, int64_t q_row_stride, int64_t q_head_strid
   P.splits = nullptr;
   P.max_blocks = 0;
   P.part = nullptr;
-  if ((int64_t)P.max_q * num_q_heads > 65535) return RLT_ERR_UNSUPPORTED;
+  if ((int64_t)P.max_q * num_q_heads > 65535 || num_seqs > kMaxLaunch / 256) return RLT_ERR_UNSUPPORTED;
   switch (q_dtype) {
     case RLT_F32: launch_vec<RLT_F32>(P, kv_dtype, stream); break;
     case RLT_F16: launch_vec<RLT_F16>(P, kv_dtype, stream); break;
