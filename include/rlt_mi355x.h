@@ -459,7 +459,9 @@ int rlt_greedy_tree_accept(const int64_t* draft_tokens, const int64_t* parents,
  * from q[node]: accepted when u_accept[r, j] * R * q[node, t] < y[t] (t its token), else
  * y = max(y - R q[node], 0) and R = sum y.  The walk goes on at an accepted draft's node; where
  * none is left, the final token is drawn from y by inverse CDF with u_final[r] as in
- * rlt_categorical.  All in float64; rows of p and q count as distributions as they stand.
+ * rlt_categorical.  y is p - C q clipped at 0, C the sum of the node's R so far in float64, each
+ * column rounded once to float32; sums and decisions in float64.  Rows of p and q count as
+ * distributions as they stand.
  * error[r] is set, and the final token 0, where drafts[r] is outside [0, width], a tried draft
  * has a token outside the vocabulary, no q mass or weights that are not finite, or where the
  * weights left have no finite positive mass (a NaN or an infinity in a row that is summed).

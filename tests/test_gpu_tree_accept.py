@@ -40,6 +40,25 @@ def test_sampled_rounds_of_other_distributions(pkg, dev, sharp, noise):
     same(pkg.tree_accept(*to(dev, args)), tree_accept(*args))
 
 
+@pytest.mark.parametrize("vocab", [8191, 8193, 32768, 32770, 40961, 49152, 49155, 100003])
+def test_many_rejections_at_one_node(pkg, dev, vocab):
+    """Passes over rows that are kept on the chip from the first one, wholly and in part; the
+    same after an accepted draft."""
+    args = list(sampled_inputs(4, 9, vocab, seed=vocab, noise=2.0))
+    args[1][:] = torch.tensor([0, 0, 0, 0, 0, 5, 5, 5, 5])
+    args[5][:] = 1 - 2.0 ** -20
+    args[5][2:, 4] = 0  # the fifth draft is accepted, if anything is left for it
+    args[2][:] = torch.tensor([9, 3, 9, 7])
+    for r in range(4):
+        for j in range(9):
+            node = int(args[1][r, j])
+            args[0][r, j] = int((args[3][r, node] - args[4][r, node] * (j != 4) * 3).argmax()) if j != 4 \
+                else int((args[4][r, node] - 9 * args[3][r, node]).argmax())
+    want = tree_accept(*args)
+    same(pkg.tree_accept(*to(dev, args)), want)
+    assert want[2][1] == 0 and want[2].max() == 1 and not want[4].any()
+
+
 def test_uniforms_at_their_ends(pkg, dev):
     args = list(sampled_inputs(6, 9, 500, seed=5))
     top = 1 - 2.0 ** -24

@@ -16,8 +16,17 @@
 // rejections y = max(p - C q, 0) with C = R_0 + .. + R_(k-1): no residual is stored, and a
 // rejection costs one sum over the node's two rows.  Where no child is left the next token is
 // drawn from y by inverse CDF.  The emitted tokens follow p whatever q and the tree are.
-// Sums, weights and the CDF are float64: one workgroup per request, each wave 1024 columns at a
-// time, the next ones in flight; the wave sums of the last pass are the CDF's coarse table.
+// C, sums and the CDF are float64; a column's y is rounded once to float32 (two fused steps with
+// the two halves of C, so that what cancels stays exact), four of them are added, and these
+// sums in float64: float64 weights took 1.7x the instructions that a pass is bound by.
+//
+// One workgroup per request, each wave 1024 columns at a time.  A node's first pass is bound by
+// the rows' bytes: 83 GB/s of one CU, 6.6 TB/s of the chip at 128 requests.  It keeps what fits of
+// the two rows on the CU: 4 steps (32768 columns) in registers and 2 in LDS, so that each
+// further pass at the node costs 2.2 us at 49152 columns instead of 4.7.  The wave sums of the
+// last pass are the CDF's coarse table.
+// Measured: 4 requests, 49152 columns 14 us; 128 requests, 65536 columns, up to five passes 36 us
+// (rereading the rows in every pass: 50).
 
 #include "vocab_rows.h"
 
@@ -134,14 +143,20 @@ __global__ __launch_bounds__(kThreads) void rlt_greedy_tree_kernel(
 
 // ---------------------------------------------------------------- sampled
 
-constexpr int kAccThreads = 1024;
+constexpr int kAccThreads = 512;
 constexpr int kAccWaves = kAccThreads / 64;
 constexpr int kRun = 16;                           // columns of a thread and step
 constexpr int64_t kStep = (int64_t)kAccThreads * kRun;
+constexpr int kHeldSteps = 4, kLdsSteps = 2;         // of a node's rows, kept for its further passes
 constexpr int kMaxSegments = (int)(kMaxVocab / kStep) * kAccWaves;
 
+struct __attribute__((packed, aligned(4))) Quad {
+  float v[4];
+};
+
 struct AcceptShared {
-  double seg[kMaxSegments];  // weight of every wave's kRun * 64 columns, in column order
+  float4 kept[kLdsSteps][2][kRun / 4][kAccThreads];  // p and q of the steps from kHeldSteps on
+  double seg[2][kMaxSegments];  // passes in turn: weight of every wave's kRun * 64 columns, in column order
   float px[kMaxDrafts], qx[kMaxDrafts], u[kMaxDrafts];
   int32_t parent[kMaxDrafts];
   int64_t token[kMaxDrafts];
@@ -154,16 +169,20 @@ __device__ __forceinline__ double left_of(float p, float q, double C) {
   return fmax(__builtin_fma(-C, (double)q, (double)p), 0.0);
 }
 
-struct __attribute__((packed, aligned(4))) Quad {
-  float v[4];
-};
-
-// A wave's 1024 columns of one step from c on (a lane takes every 256th four, so that a load is
+// A wave's 1024 columns of one step from c on (a lane takes every 64th four, so that a load is
 // contiguous); zeros past the row's last whole four.
 struct Run {
   Quad a[kRun / 4], b[kRun / 4];
   __device__ __forceinline__ void load(const float* p, const float* q, int64_t c, int64_t vocab) {
     const int lane = threadIdx.x & 63;
+    if (c + 64 * kRun <= vocab) {
+#pragma unroll
+      for (int i = 0; i < kRun / 4; ++i) {
+        a[i] = *(const Quad*)(p + c + 256 * i + 4 * lane);
+        b[i] = *(const Quad*)(q + c + 256 * i + 4 * lane);
+      }
+      return;
+    }
 #pragma unroll
     for (int i = 0; i < kRun / 4; ++i) {
       const int64_t at = c + 256 * i + 4 * lane;
@@ -173,6 +192,23 @@ struct Run {
         b[i] = *(const Quad*)(q + at);
       }
     }
+  }
+  // (LOOK: `odd` becomes NaN where a column is no number)
+  template <bool LOOK>
+  __device__ __forceinline__ double weight(float c_hi, float c_lo, float& odd) const {
+    double sum = 0.0;
+#pragma unroll
+    for (int i = 0; i < kRun / 4; ++i) {
+      float y[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        // (0 x is NaN for NaN and infinities: no distribution)
+        if (LOOK) odd = __builtin_fmaf(0.f, a[i].v[e], __builtin_fmaf(0.f, b[i].v[e], odd));
+        y[e] = fmaxf(__builtin_fmaf(-c_lo, b[i].v[e], __builtin_fmaf(-c_hi, b[i].v[e], a[i].v[e])), 0.f);
+      }
+      sum += (double)((y[0] + y[1]) + (y[2] + y[3]));
+    }
+    return sum;
   }
 };
 
@@ -199,41 +235,86 @@ __device__ __forceinline__ double wave_sum(double x) {
   return pair_sum(lo[0], hi[0], lo[1], hi[1]);
 }
 
-// Segment weights of a node's rows for C (0 with q = p: the target's own).
-__device__ __forceinline__ void weigh(AcceptShared& sh, const float* p, const float* q, double C,
-                                      int64_t vocab) {
-  const int t = threadIdx.x, w = t >> 6, lane = t & 63;
+// Segment weights of a node's rows for C (0 with q = p: the target's own).  The first pass over a
+// node (`fresh`) keeps its first steps in registers and in LDS, for the passes of the node's
+// further rejections.
+struct Held {
+  Run step[kHeldSteps];
+};
+__device__ __forceinline__ void weigh(AcceptShared& sh, double* seg, Held& held, bool fresh, const float* p,
+                                      const float* q, double C, int64_t vocab) {
+  constexpr int kKept = kHeldSteps + kLdsSteps;
+  const int t = threadIdx.x, w = __builtin_amdgcn_readfirstlane(t >> 6), lane = t & 63;
   const int steps = (int)((vocab + kStep - 1) / kStep);
+  const int64_t first = (int64_t)w * (64 * kRun);
+  const float c_hi = (float)C, c_lo = (float)(C - (double)c_hi);
   float odd = 0.f;  // NaN where a column is
-  int64_t c = (int64_t)w * (64 * kRun);
-  Run cur, next;
-  cur.load(p, q, c, vocab);
-#pragma unroll 1
-  for (int step = 0; step < steps; ++step, c += kStep) {
-    if (step + 1 < steps) next.load(p, q, c + kStep, vocab);
-    double s[4] = {0.0, 0.0, 0.0, 0.0};
-#pragma unroll
-    for (int i = 0; i < kRun / 4; ++i)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        // (x - x is NaN for NaN and infinities: no distribution)
-        odd += (cur.a[i].v[e] - cur.a[i].v[e]) + (cur.b[i].v[e] - cur.b[i].v[e]);
-        s[e] += left_of(cur.a[i].v[e], cur.b[i].v[e], C);
-      }
-    double sum = (s[0] + s[1]) + (s[2] + s[3]);
-    // the row's last columns, fewer than four
-    const int64_t rest = vocab & ~(int64_t)3;
-    if (rest < vocab && rest >= c && rest < c + 64 * kRun && lane == 0)
-      for (int64_t at = rest; at < vocab; ++at) {
-        odd += (p[at] - p[at]) + (q[at] - q[at]);
-        sum += left_of(p[at], q[at], C);
-      }
+  auto close = [&](int step, double sum) {
     sum = wave_sum(sum);
-    if (lane == 0) sh.seg[step * kAccWaves + w] = sum;
+    if (lane == 0) seg[step * kAccWaves + w] = sum;
+  };
+  auto kept = [&](int s) { return &sh.kept[s][0][0][t]; };
+  if (fresh) {
+#pragma unroll
+    for (int s = 0; s < kHeldSteps; ++s) held.step[s].load(p, q, first + s * kStep, vocab);
+  }
+  // the first step that is streamed is on its way meanwhile
+  Run cur, next;
+  int step = fresh ? kHeldSteps : kKept;
+  if (step < steps) cur.load(p, q, first + step * kStep, vocab);
+  double sums[kHeldSteps] = {0.0, 0.0, 0.0, 0.0};
+  if (fresh) {
+#pragma unroll
+    for (int s = 0; s < kHeldSteps; ++s)
+      if (s < steps) sums[s] = held.step[s].weight<true>(c_hi, c_lo, odd);
+  } else {
+#pragma unroll
+    for (int s = 0; s < kHeldSteps; ++s)
+      if (s < steps) sums[s] = held.step[s].weight<false>(c_hi, c_lo, odd);
+  }
+  // (their exchanges side by side; steps past the row's are no segments)
+#pragma unroll
+  for (int s = 0; s < kHeldSteps; ++s) close(s, sums[s]);
+  if (!fresh) {
+#pragma unroll 1
+    for (int s = kHeldSteps; s < min(steps, kKept); ++s) {
+      const float4* const from = kept(s - kHeldSteps);
+#pragma unroll
+      for (int i = 0; i < kRun / 4; ++i) {
+        const float4 a = from[i * kAccThreads], b = from[(kRun / 4 + i) * kAccThreads];
+        next.a[i] = Quad{{a.x, a.y, a.z, a.w}};
+        next.b[i] = Quad{{b.x, b.y, b.z, b.w}};
+      }
+      close(s, next.weight<false>(c_hi, c_lo, odd));
+    }
+  }
+#pragma unroll 1
+  for (; step < steps; ++step) {
+    if (step + 1 < steps) next.load(p, q, first + (step + 1) * kStep, vocab);
+    if (fresh && step < kKept) {
+      float4* const to = kept(step - kHeldSteps);
+#pragma unroll
+      for (int i = 0; i < kRun / 4; ++i) {
+        const Quad &a = cur.a[i], &b = cur.b[i];
+        to[i * kAccThreads] = make_float4(a.v[0], a.v[1], a.v[2], a.v[3]);
+        to[(kRun / 4 + i) * kAccThreads] = make_float4(b.v[0], b.v[1], b.v[2], b.v[3]);
+      }
+    }
+    close(step, cur.weight<true>(c_hi, c_lo, odd));
     cur = next;
   }
+  // the row's last columns, fewer than four, belong to the segment that they end
+  const int64_t rest = vocab & ~(int64_t)3;
+  if (rest < vocab && (rest / (64 * kRun)) % kAccWaves == w && lane == 0) {
+    double sum = 0.0;
+    for (int64_t at = rest; at < vocab; ++at) {
+      odd += (p[at] - p[at]) + (q[at] - q[at]);
+      sum += left_of(p[at], q[at], C);
+    }
+    seg[rest / (64 * kRun)] += sum;
+  }
   if (__builtin_amdgcn_ballot_w64(odd != 0.f) != 0 && lane == 0)
-    sh.seg[w] = __longlong_as_double(0x7ff8000000000000ll);
+    seg[w] = __longlong_as_double(0x7ff8000000000000ll);
   __syncthreads();
 }
 
@@ -247,20 +328,17 @@ __device__ __forceinline__ double wave_incl(double x) {
   return x;
 }
 
-// Exclusive weights before each lane's run of segments, and their total (every wave alike).
-__device__ __forceinline__ double segment_scan(const AcceptShared& sh, int segments, double& before) {
+// The total of a lane's run of segments, and of all (every wave alike).
+__device__ __forceinline__ double lane_segments(const double* seg, int segments) {
   const int lane = threadIdx.x & 63, per = (segments + 63) / 64;
   double mine = 0.0;
   for (int i = 0; i < per; ++i)
-    if (lane * per + i < segments) mine += sh.seg[lane * per + i];
-  const double incl = wave_incl(mine);
-  before = __shfl_up(incl, 1, RLT_WAVE);
-  if (lane == 0) before = 0.0;
-  return __shfl(incl, 63, RLT_WAVE);
+    if (lane * per + i < segments) mine += seg[lane * per + i];
+  return mine;
 }
 
 // The first column whose running weight passes `target` (one wave).
-__device__ __forceinline__ int64_t draw(const AcceptShared& sh, const float* p, const float* q, double C,
+__device__ __forceinline__ int64_t draw(const double* weights, const float* p, const float* q, double C,
                                         int64_t vocab, int segments, double before, double target) {
   const int lane = threadIdx.x & 63, per = (segments + 63) / 64;
   // the last segment with weight at or before the target's: rounding may leave the running
@@ -270,11 +348,11 @@ __device__ __forceinline__ int64_t draw(const AcceptShared& sh, const float* p, 
   for (int i = 0; i < per; ++i) {
     const int s = lane * per + i;
     if (s >= segments) break;
-    if (sh.seg[s] > 0.0 && run <= target) {
+    if (weights[s] > 0.0 && run <= target) {
       seg = s;
       at = run;
     }
-    run += sh.seg[s];
+    run += weights[s];
   }
   const uint64_t has = __builtin_amdgcn_ballot_w64(seg >= 0);
   if (!has) return 0;
@@ -327,7 +405,7 @@ __global__ __launch_bounds__(kAccThreads) void rlt_tree_accept_kernel(
     int64_t* path, int64_t* tokens, int64_t* accepted, int64_t* final_token, uint8_t* error) {
   __shared__ AcceptShared sh;
   const int64_t r = blockIdx.x;
-  const int t = threadIdx.x, nodes = width + 1;
+  const int t = threadIdx.x, lane = t & 63, nodes = width + 1;
   const float* const p = p_all + r * nodes * vocab;
   const float* const q = q_all + r * width * vocab;
   const int64_t d = drafts[r];
@@ -353,42 +431,63 @@ __global__ __launch_bounds__(kAccThreads) void rlt_tree_accept_kernel(
   const int segments = (int)((vocab + kStep - 1) / kStep) * kAccWaves;
   int node = 0, count = 0;
   double C = 0.0, R = 1.0;
-  // every thread walks alike
-  for (int j = 0; j < live && !bad; ++j) {
-    if (sh.parent[j] != node) continue;
-    const double px = sh.px[j], qx = sh.qx[j];
-    if (!(qx > 0.0) || !(fabs(px) < INFINITY) || !(qx < INFINITY)) {
-      bad = true;
-    } else if ((double)sh.u[j] * R * qx < px - C * qx) {
-      ++count;
-      node = j + 1;
-      if (t == 0) sh.walk[count] = node;
-      C = 0.0;
-      R = 1.0;
-    } else {
-      C += R;
-      __syncthreads();  // the table of an earlier pass is read
-      weigh(sh, p + (int64_t)node * vocab, q + (int64_t)node * vocab, C, vocab);
-      double before;
-      R = segment_scan(sh, segments, before);
-      bad = !(R > 0.0) || !(R < INFINITY);
+  Held held;
+  double* seg = sh.seg[1];
+  // every wave walks alike: a lane holds the parents of drafts lane, lane + 64, ..
+  int parent[(kMaxDrafts + 63) / 64];
+#pragma unroll
+  for (int k = 0; k < (kMaxDrafts + 63) / 64; ++k)
+    parent[k] = lane + 64 * k < live ? sh.parent[lane + 64 * k] : -1;
+  bool last = false;  // the pass over p alone, behind the walk
+  for (int j = 0; !bad && !last;) {
+    int child = live;
+#pragma unroll
+    for (int k = (kMaxDrafts + 63) / 64 - 1; k >= 0; --k) {
+      const uint64_t b = __builtin_amdgcn_ballot_w64(lane + 64 * k >= j && parent[k] == node);
+      if (b) child = 64 * k + __builtin_ctzll(b);
     }
+    j = child;
+    if (j < live) {
+      const double px = sh.px[j], qx = sh.qx[j], u = sh.u[j];
+      ++j;
+      if (!(qx > 0.0) || !(fabs(px) < INFINITY) || !(qx < INFINITY)) {
+        bad = true;
+        break;
+      }
+      if (u * R * qx < px - C * qx) {
+        ++count;
+        node = j;
+        if (t == 0) sh.walk[count] = node;
+        C = 0.0;
+        R = 1.0;
+        continue;
+      }
+    } else if (C == 0.0) {
+      last = true;
+    } else {
+      break;
+    }
+    const int64_t row = (int64_t)__builtin_amdgcn_readfirstlane(node) * vocab;
+    const bool fresh = __builtin_amdgcn_readfirstlane(C == 0.0), alone = __builtin_amdgcn_readfirstlane(last);
+    if (!last) C += R;
+    seg = seg == sh.seg[0] ? sh.seg[1] : sh.seg[0];  // (the last pass's may still be read)
+    weigh(sh, seg, held, fresh, p + row, (alone ? p : q) + row, C, vocab);
+    if (last) break;
+    R = wave_sum(lane_segments(seg, segments));
+    bad = !(R > 0.0) || !(R < INFINITY);
   }
   if (!bad) {
-    if (C == 0.0) {
-      __syncthreads();
-      weigh(sh, p + (int64_t)node * vocab, p + (int64_t)node * vocab, 0.0, vocab);
-    }
     if (t < 64) {
-      double before;
-      const double total = segment_scan(sh, segments, before);
+      const double incl = wave_incl(lane_segments(seg, segments)), total = __shfl(incl, 63, RLT_WAVE);
+      double before = __shfl_up(incl, 1, RLT_WAVE);  // each lane's run
+      if (lane == 0) before = 0.0;
       bad = !(total > 0.0) || !(total < INFINITY);
       if (!bad) {
         const double u = (double)last_u * total;
         // the draw stays below the total
         const double top = __longlong_as_double(__double_as_longlong(total) - 1);
         const float* const row = p + (int64_t)node * vocab;
-        const int64_t token = draw(sh, row, C == 0.0 ? row : q + (int64_t)node * vocab, C, vocab, segments,
+        const int64_t token = draw(seg, row, C == 0.0 ? row : q + (int64_t)node * vocab, C, vocab, segments,
                                    before, u < top ? u : top);
         if (t == 0) sh.last = token;
       }

@@ -277,8 +277,8 @@ def tree_accept(draft_tokens, parents, drafts, q, p, u_accept, u_final):
     node's children are tried in index order: child t is accepted when ``u_accept * R * q[t] <
     y[t]``, where y is what is left of p (at first p, R = 1) and a rejection leaves
     ``max(y - R q, 0)`` with its sum R; where none is left the final token is drawn from y with
-    ``u_final``.  The emitted tokens follow p.  Rows count as distributions as they stand, all
-    sums are float64.  ``error`` is set (and the final token 0) for a draft count outside
+    ``u_final``.  The emitted tokens follow p.  Rows count as distributions as they stand; sums and
+    decisions are float64.  ``error`` is set (and the final token 0) for a draft count outside
     ``[0, W]``, a tried draft that q cannot have proposed, and weights without a finite
     positive sum.
 
