@@ -73,6 +73,25 @@ def test_ties_and_orders(pkg, dev, vocab):
     check(pkg.token_logprobs(x.to(dev), tokens.to(dev), top_n=30), x, tokens, 30)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("top_n", [1, 5, 20, 64])
+def test_uneven_rows(pkg, dev, dtype, top_n):
+    """The largest columns side by side, at the row's start, its end and within a wave's columns;
+    a row's end inside the first wave's columns; fewer columns above -inf than asked for."""
+    g = torch.Generator().manual_seed(top_n)
+    for vocab in (2048 * 5 + 384, 8192 * 3 + 100, 70):
+        x = torch.randn(6, vocab, generator=g)
+        x[0, :min(200, vocab)] += 20
+        x[1, -40:] += 20
+        x[2, vocab // 2:vocab // 2 + 30] += 20
+        x[3, :] = -math.inf
+        x[3, 3::vocab // 7] = 1.0
+        x[4, :vocab - 300 if vocab > 300 else 1] = -50.0
+        x = x.to(dtype)
+        tokens = torch.tensor([0, vocab - 1, vocab // 2, 3, 0, 1])
+        check(pkg.token_logprobs(x.to(dev), tokens.to(dev), top_n=top_n), x, tokens, top_n)
+
+
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
 def test_masked_logits(pkg, dev, dtype):
     """-inf and the type's lowest value as masks; a dominant token; one token left."""

@@ -9,14 +9,16 @@
 // workgroup per row, joins them.  S and T are float64 sums: next to a dominant token the
 // entropy is what is left of S after 1, which float32 sums would lose.
 //
-// The n first columns of a slice are taken without a sort.  The n-th largest of a wave's 64
-// lanes' largest columns is a lower bound that n columns of the wave reach, so the largest of
-// the four waves' bounds is one for the slice; the columns that reach it (a few more than n)
-// are listed and ranked by counting.  Where ties make them too many, the bound is taken over
-// the threads' largest (value, column) pairs, which are all different: then at most n threads
-// hold such columns.
+// The n first columns of a slice are taken without a sort.  Bounds on the waves' lanes' largest
+// columns give one that n columns of the slice reach; those that reach it (a few more than n)
+// are listed wave by wave and ranked by counting.  Where ties or an uneven slice make a list too
+// long, the bound is taken over all threads' largest (value, column) pairs, which are all
+// different: then at most n threads hold such columns.
 //
-// float64 sums cost more than the loads, so four weights at a time are added in float32 first;
+// The instructions of a column bound the kernel (160 rows of 49152 float32 columns with 20
+// alternatives: 14 us for the slices, 2.2 TB/s, and 5 us to join them); of a workgroup's 9 us the
+// loads take 1.6, the bound 1, the weights 0.8, the columns ahead 0.6, the listing and the ranks
+// 1.3 each.  float64 sums cost more than the loads, so four weights at a time are added in float32 first;
 // weights of exactly 1 (the maximum) are counted instead, and nothing is lost next to them.
 
 #include "vocab_rows.h"
@@ -24,8 +26,6 @@
 #include "rlt_mi355x.h"
 
 #include <math.h>
-
-#include <type_traits>
 
 namespace {
 
@@ -64,8 +64,9 @@ struct TopShared {
   unsigned long long best[kThreads];
   unsigned long long list[kList];
   unsigned long long bound;
-  uint32_t wave_bound[kThreads / 64];
-  int count;
+  uint2 wave_bound[kThreads / 64];  // of n, of n / 4
+  int wave_count[kThreads / 64];
+  int count;  // select_top
 };
 
 // Ranks the `found` different composites of sh.list by counting; out(rank, composite) for the
@@ -131,13 +132,16 @@ __device__ __forceinline__ void select_top(TopShared& sh, int n, int items, Item
   rank_list(sh, min(sh.count, kList), n, out);
 }
 
-// The n-th largest of the wave's 64 values (0: fewer than n are positive).
-__device__ __forceinline__ uint32_t wave_nth(uint32_t x, int n) {
-  uint32_t bound = 0;
-#pragma unroll 4
-  for (int bit = 31; bit >= 0; --bit) {
-    const uint32_t next = bound | (1u << bit);
-    if (__popcll(__builtin_amdgcn_ballot_w64(x >= next)) >= n) bound = next;
+// Lower bounds that n and `part` of the wave's 64 values reach: the n-th largest, its low bits
+// cleared (0: fewer than n are positive).  16-bit logits' keys have no low bits; a float32 one's
+// bound lies up to 2^-9 below it, for half the steps.
+__device__ __forceinline__ uint2 wave_nth(uint32_t x, int n, int part) {
+  uint2 bound = make_uint2(0, 0);
+#pragma unroll 6
+  for (int bit = 31; bit >= 14; --bit) {
+    const uint2 next = make_uint2(bound.x | (1u << bit), bound.y | (1u << bit));
+    if (__popcll(__builtin_amdgcn_ballot_w64(x >= next.x)) >= n) bound.x = next.x;
+    if (__popcll(__builtin_amdgcn_ballot_w64(x >= next.y)) >= part) bound.y = next.y;
   }
   return bound;
 }
@@ -147,19 +151,58 @@ __device__ __forceinline__ int64_t source_row(const LogprobParams& P, int64_t r)
   return row >= 0 && row < P.num_rows ? row : -1;
 }
 
-// The lower bound of the n largest keys among all threads' largest ones: wave w's part, in LDS
-// (a barrier follows before it is used).
+// A lower bound that n columns of the workgroup reach: the threads' largest columns reach the
+// least of the waves' bounds for n / 4, and the largest of their bounds for n (the better one
+// where the row ends inside the first wave's columns).  Wave w's part, in LDS; the waves' lists
+// are cleared (a barrier follows before they are used).
+constexpr int kWaveList = 64;
 __device__ __forceinline__ void put_bound(TopShared& sh, uint32_t largest, int n) {
-  const uint32_t bound = wave_nth(largest, n);
+  const uint2 bound = wave_nth(largest, n, (n + kThreads / 64 - 1) / (kThreads / 64));
   if ((threadIdx.x & 63) == 0) sh.wave_bound[threadIdx.x >> 6] = bound;
-  if (threadIdx.x == 0) sh.count = 0;
+  sh.list[threadIdx.x] = 0;
 }
 __device__ __forceinline__ uint32_t get_bound(const TopShared& sh) {
-  return max(max(sh.wave_bound[0], sh.wave_bound[1]), max(sh.wave_bound[2], sh.wave_bound[3]));
+  uint2 x = sh.wave_bound[0];
+#pragma unroll
+  for (int v = 1; v < kThreads / 64; ++v)
+    x = make_uint2(max(x.x, sh.wave_bound[v].x), min(x.y, sh.wave_bound[v].y));
+  return max(x.x, x.y);
 }
-__device__ __forceinline__ void list_column(TopShared& sh, unsigned long long c) {
-  const int at = atomicAdd(&sh.count, 1);
-  if (at < kThreads) sh.list[at] = c;
+// Columns that reach the bound go to their wave's list, without atomics; `count` is the same in
+// every lane and goes on past a full list.
+__device__ __forceinline__ void list_column(TopShared& sh, int& count, bool hit, unsigned long long c) {
+  const uint64_t hits = __builtin_amdgcn_ballot_w64(hit);
+  if (!hits) return;
+  const int lane = threadIdx.x & 63;
+  const int at = count + (int)__popcll(hits & ((1ull << lane) - 1));
+  if (hit && at < kWaveList) sh.list[(threadIdx.x >> 6) * kWaveList + at] = c;
+  count += (int)__popcll(hits);
+}
+// Ranks the waves' lists by counting; out(rank, composite) for the first n, 0 behind the last.
+// False (of every thread alike): a list is not complete.
+template <class Out>
+__device__ __forceinline__ bool rank_lists(const TopShared& sh, int n, Out out) {
+  const int t = threadIdx.x, lane = t & 63;
+  int counts[kThreads / 64], found = 0, longest = 0;
+#pragma unroll
+  for (int v = 0; v < kThreads / 64; ++v) {
+    counts[v] = sh.wave_count[v];
+    found += counts[v];
+    longest = max(longest, counts[v]);
+  }
+  if (longest > kWaveList) return false;
+  if (lane < sh.wave_count[t >> 6]) {
+    const unsigned long long c = sh.list[t];
+    int r = 0;
+#pragma unroll
+    for (int v = 0; v < kThreads / 64; ++v)
+      for (int i = 0; i < counts[v]; i += 8)  // (zeros behind a list's end)
+#pragma unroll
+        for (int k = 0; k < 8; ++k) r += sh.list[v * kWaveList + i + k] > c;
+    if (r < n) out(r, c);
+  }
+  for (int r = found + t; r < n; r += kThreads) out(r, 0ull);
+  return true;
 }
 
 // The next lower number; of -inf NaN, which nothing lies at or below.
@@ -202,8 +245,7 @@ __device__ __forceinline__ void scan_slice(const LogprobParams& P, const uint8_t
     }
   // the thread's largest column (NaN comes first; 0: none above -inf)
   const uint32_t mine = nan ? 0xffffffffu : m == -INFINITY ? 0u : order_key(m);
-#pragma unroll
-  for (int o = 32; o >= 1; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, RLT_WAVE));
+  m = wave_max(m);
   const float wave_top = m;
   if (P.top_n > 0) put_bound(top, mine, P.top_n);
   if ((t & 63) == 0) maxima[w] = m;
@@ -269,39 +311,32 @@ __device__ __forceinline__ void scan_slice(const LogprobParams& P, const uint8_t
 #pragma unroll
       for (int e = 0; e < S::VE; ++e) before += !(x.at(i, e) <= least) ? 1u : 0u;
   }
-#pragma unroll
-  for (int o = 32; o >= 1; o >>= 1) {
-    s += __shfl_xor(s, o, RLT_WAVE);
-    q += __shfl_xor(q, o, RLT_WAVE);
-    before += __shfl_xor(before, o, RLT_WAVE);
-    ones += __shfl_xor(ones, o, RLT_WAVE);
-  }
+  s = wave_sum(s);
+  q = wave_sum(q);
+  const uint32_t both = wave_sum(before << 16 | ones);  // (at most 64 EPT of each)
   if ((t & 63) == 0) {
     sums[w][0] = s;
     sums[w][1] = q;
-    counts[w][0] = before;
-    counts[w][1] = ones;
+    counts[w][0] = both >> 16;
+    counts[w][1] = both & 0xffffu;
   }
   if (P.top_n > 0) {
     // (bound 0, fewer than n columns above -inf in each wave: every column reaches it, as any
     // does not lie below the NaN that is its value)
     const uint32_t bound = get_bound(top);
     const float least = key_value(bound);
-    if (mine >= bound) {
+    int listed = 0;
+    if (__builtin_amdgcn_ballot_w64(mine >= bound) != 0) {
 #pragma unroll
-      for (int i = 0; i < S::NP; ++i) {
-        bool any = false;
-#pragma unroll
-        for (int e = 0; e < S::VE; ++e) any |= !(x.at(i, e) < least);
-        if (!any) continue;
+      for (int i = 0; i < S::NP; ++i)
 #pragma unroll
         for (int e = 0; e < S::VE; ++e) {
           const int c = column(i) + e;
           const float v = x.at(i, e);
-          if ((!(v < least)) & inside(c)) list_column(top, composite(order_key(v), (uint32_t)c));
+          list_column(top, listed, (!(v < least)) & inside(c), composite(order_key(v), (uint32_t)c));
         }
-      }
     }
+    if ((t & 63) == 0) top.wave_count[w] = listed;
   }
   __syncthreads();
   if (t == 0) {
@@ -316,10 +351,7 @@ __device__ __forceinline__ void scan_slice(const LogprobParams& P, const uint8_t
   if (P.top_n > 0) {
     unsigned long long* const dst = P.candidates + (r * P.slices + slice) * P.top_n;
     auto put = [&](int rank, unsigned long long c) { dst[rank] = c; };
-    const int found = top.count;  // (the same in every thread)
-    if (found <= kThreads) {
-      rank_list(top, found, P.top_n, put);
-    } else {
+    if (!rank_lists(top, P.top_n, put)) {
       __syncthreads();
       select_top<EPT>(
           top, P.top_n, EPT,
@@ -385,8 +417,7 @@ __global__ __launch_bounds__(kThreads) void rlt_logprob_rows_kernel(LogprobParam
     const float xt = load_as_f32<DT>((const uint8_t*)P.logits + row * P.row_stride * ELT, in ? token : 0);
     float m = -INFINITY;
     for (int i = t; i < P.slices; i += 64) m = fmaxf(m, st[i].m);
-#pragma unroll
-    for (int o = 32; o >= 1; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, RLT_WAVE));
+    m = wave_max(m);
     double s = 0.0, q = 0.0;
     uint32_t before = 0;
     for (int i = t; i < P.slices; i += 64) {
@@ -397,12 +428,9 @@ __global__ __launch_bounds__(kThreads) void rlt_logprob_rows_kernel(LogprobParam
       s += x.s * w;
       q += (x.t + d * x.s) * w;
     }
-#pragma unroll
-    for (int o = 32; o >= 1; o >>= 1) {
-      s += __shfl_xor(s, o, RLT_WAVE);
-      q += __shfl_xor(q, o, RLT_WAVE);
-      before += __shfl_xor(before, o, RLT_WAVE);
-    }
+    s = wave_sum(s);
+    q = wave_sum(q);
+    before = wave_sum(before);
     const double lse = log(s);  // over the maximum; a row without a finite one gives NaN
     if (t == 0) {
       const bool ok = m > -INFINITY;
@@ -418,9 +446,13 @@ __global__ __launch_bounds__(kThreads) void rlt_logprob_rows_kernel(LogprobParam
     put_bound(top, (uint32_t)(best >> 32), P.top_n);
     __syncthreads();
     const uint32_t bound = max(get_bound(top), 1u);
-    if ((uint32_t)(best >> 32) >= bound)
-      for (int i = 0; i < items; ++i)
-        if ((uint32_t)(item(i) >> 32) >= bound) list_column(top, item(i));
+    int listed = 0;
+    if (__builtin_amdgcn_ballot_w64((uint32_t)(best >> 32) >= bound) != 0)
+      for (int i = 0; i < items; ++i) {
+        const unsigned long long x = item(i);
+        list_column(top, listed, (uint32_t)(x >> 32) >= bound, x);
+      }
+    if ((t & 63) == 0) top.wave_count[t >> 6] = listed;
     __syncthreads();
     const double m = sh[0], lse = sh[1];
     auto put = [&](int rank, unsigned long long x) {
@@ -428,18 +460,16 @@ __global__ __launch_bounds__(kThreads) void rlt_logprob_rows_kernel(LogprobParam
       P.top_tokens[at] = x ? (int64_t)composite_col(x) : -1;
       P.top_logprob[at] = x ? (float)(((double)key_value((uint32_t)(x >> 32)) - m) - lse) : nan;
     };
-    const int found = top.count;  // (the same in every thread)
-    if (found <= kThreads) {
-      rank_list(top, found, P.top_n, put);
-    } else {
+    if (!rank_lists(top, P.top_n, put)) {
       __syncthreads();
       select_top<0>(top, P.top_n, items, item, put);
     }
   }
 }
 
-// Columns per thread: wide slices where they fill the chip (fewer candidates to join), narrow
-// ones for a few rows, whose time is one slice's.
+// Columns per thread: wide slices where they fill the chip (fewer candidates to join: 160 rows of
+// 49152 columns 16 us, 22 in narrow ones), narrow ones for a few rows, whose time is one
+// slice's (4 rows of 151936 bf16 columns: 6 us).
 int slice_ept(int64_t count, int64_t vocab) {
   const int64_t wide = (vocab + kWideEpt * kThreads - 1) / (kWideEpt * kThreads);
   return count * wide < 256 && vocab <= 262144 ? kNarrowEpt : kWideEpt;

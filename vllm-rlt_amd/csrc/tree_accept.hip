@@ -34,8 +34,6 @@
 
 #include <math.h>
 
-#include <type_traits>
-
 namespace {
 
 using namespace vocab;
@@ -211,29 +209,6 @@ struct Run {
     return sum;
   }
 };
-
-// Sum over the wave by lane exchanges of the vector unit (quads, halves, rows of 16, then the
-// row pairs): through LDS these exchanges took longer than the columns.
-__device__ __forceinline__ double pair_sum(uint32_t lo0, uint32_t hi0, uint32_t lo1, uint32_t hi1) {
-  return __hiloint2double((int)hi0, (int)lo0) + __hiloint2double((int)hi1, (int)lo1);
-}
-__device__ __forceinline__ double wave_sum(double x) {
-  auto add = [&](auto ctrl) {
-    const int lo = __builtin_amdgcn_update_dpp(0, __double2loint(x), decltype(ctrl)::value, 0xf, 0xf, true);
-    const int hi = __builtin_amdgcn_update_dpp(0, __double2hiint(x), decltype(ctrl)::value, 0xf, 0xf, true);
-    x += __hiloint2double(hi, lo);
-  };
-  add(std::integral_constant<int, 0xB1>{});   // quad_perm: lane ^ 1
-  add(std::integral_constant<int, 0x4E>{});   // quad_perm: lane ^ 2
-  add(std::integral_constant<int, 0x141>{});  // row_half_mirror: the other quad of eight
-  add(std::integral_constant<int, 0x140>{});  // row_mirror: the other eight of the row
-  auto lo = __builtin_amdgcn_permlane16_swap(__double2loint(x), __double2loint(x), false, false);
-  auto hi = __builtin_amdgcn_permlane16_swap(__double2hiint(x), __double2hiint(x), false, false);
-  x = pair_sum(lo[0], hi[0], lo[1], hi[1]);
-  lo = __builtin_amdgcn_permlane32_swap(__double2loint(x), __double2loint(x), false, false);
-  hi = __builtin_amdgcn_permlane32_swap(__double2hiint(x), __double2hiint(x), false, false);
-  return pair_sum(lo[0], hi[0], lo[1], hi[1]);
-}
 
 // Segment weights of a node's rows for C (0 with q = p: the target's own).  The first pass over a
 // node (`fresh`) keeps its first steps in registers and in LDS, for the passes of the node's

@@ -4,6 +4,8 @@
 
 #include "common.h"
 
+#include <type_traits>
+
 namespace vocab {
 
 constexpr int kThreads = 256;
@@ -97,13 +99,56 @@ struct Slice {
   }
 };
 
+// A value combined over the wave by lane exchanges of the vector unit (quads, halves, rows of
+// 16, then the row pairs): the same exchanges through LDS took a large part of these kernels.
+template <class F>
+__device__ __forceinline__ uint32_t wave_join(uint32_t x, F f) {
+  auto step = [&](auto ctrl) {
+    x = f(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, decltype(ctrl)::value, 0xf, 0xf, true));
+  };
+  step(std::integral_constant<int, 0xB1>{});   // quad_perm: lane ^ 1
+  step(std::integral_constant<int, 0x4E>{});   // quad_perm: lane ^ 2
+  step(std::integral_constant<int, 0x141>{});  // row_half_mirror: the other quad of eight
+  step(std::integral_constant<int, 0x140>{});  // row_mirror: the other eight of the row
+  const auto a = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+  x = f(a[0], a[1]);
+  const auto b = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+  return f(b[0], b[1]);
+}
+__device__ __forceinline__ float wave_max(float x) {
+  return __uint_as_float(wave_join(__float_as_uint(x), [](uint32_t a, uint32_t b) {
+    return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b)));
+  }));
+}
+__device__ __forceinline__ uint32_t wave_sum(uint32_t x) {
+  return wave_join(x, [](uint32_t a, uint32_t b) { return a + b; });
+}
+// the same of 64-bit values, as (low, high) halves
+template <class F>
+__device__ __forceinline__ uint64_t wave_join(uint64_t x, F f) {
+  auto step = [&](auto ctrl) {
+    const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, decltype(ctrl)::value, 0xf, 0xf, true);
+    const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(x >> 32), decltype(ctrl)::value, 0xf, 0xf, true);
+    x = f(x, (uint64_t)hi << 32 | lo);
+  };
+  step(std::integral_constant<int, 0xB1>{});
+  step(std::integral_constant<int, 0x4E>{});
+  step(std::integral_constant<int, 0x141>{});
+  step(std::integral_constant<int, 0x140>{});
+  auto lo = __builtin_amdgcn_permlane16_swap((uint32_t)x, (uint32_t)x, false, false);
+  auto hi = __builtin_amdgcn_permlane16_swap((uint32_t)(x >> 32), (uint32_t)(x >> 32), false, false);
+  x = f((uint64_t)hi[0] << 32 | lo[0], (uint64_t)hi[1] << 32 | lo[1]);
+  lo = __builtin_amdgcn_permlane32_swap((uint32_t)x, (uint32_t)x, false, false);
+  hi = __builtin_amdgcn_permlane32_swap((uint32_t)(x >> 32), (uint32_t)(x >> 32), false, false);
+  return f((uint64_t)hi[0] << 32 | lo[0], (uint64_t)hi[1] << 32 | lo[1]);
+}
+__device__ __forceinline__ double wave_sum(double x) {
+  return __longlong_as_double((long long)wave_join((uint64_t)__double_as_longlong(x), [](uint64_t a, uint64_t b) {
+    return (uint64_t)__double_as_longlong(__longlong_as_double((long long)a) + __longlong_as_double((long long)b));
+  }));
+}
 __device__ __forceinline__ unsigned long long wave_max(unsigned long long x) {
-#pragma unroll
-  for (int o = 32; o >= 1; o >>= 1) {
-    const unsigned long long y = __shfl_xor(x, o, RLT_WAVE);
-    x = x > y ? x : y;
-  }
-  return x;
+  return wave_join((uint64_t)x, [](uint64_t a, uint64_t b) { return a > b ? a : b; });
 }
 
 }  // namespace vocab
