@@ -18,8 +18,9 @@
 // The instructions of a column bound the kernel (160 rows of 49152 float32 columns with 20
 // alternatives: 14 us for the slices, 2.2 TB/s, and 5 us to join them); of a workgroup's 9 us the
 // loads take 1.6, the bound 1, the weights 0.8, the columns ahead 0.6, the listing and the ranks
-// 1.3 each.  float64 sums cost more than the loads, so four weights at a time are added in float32 first;
-// weights of exactly 1 (the maximum) are counted instead, and nothing is lost next to them.
+// 1.3 each.  float64 sums cost more than the loads, so four weights at a time are added in
+// float32 first; weights of exactly 1 (the maximum) are counted instead, and nothing is lost
+// next to them.
 
 #include "vocab_rows.h"
 
@@ -467,9 +468,10 @@ __global__ __launch_bounds__(kThreads) void rlt_logprob_rows_kernel(LogprobParam
   }
 }
 
-// Columns per thread: wide slices where they fill the chip (fewer candidates to join: 160 rows of
-// 49152 columns 16 us, 22 in narrow ones), narrow ones for a few rows, whose time is one
-// slice's (4 rows of 151936 bf16 columns: 6 us).
+// Columns per thread: wide slices where they fill the chip (less to join, and a slice's fixed
+// phases over more columns: 160 rows of 49152 columns 14.2 + 4.8 us, 18.8 + 5.6 in narrow
+// ones), narrow ones for a few rows, whose time is one slice's (4 rows of 151936 bf16 columns
+// 6.1 + 5.6 us, 7.9 + 4.1 in wide ones).
 int slice_ept(int64_t count, int64_t vocab) {
   const int64_t wide = (vocab + kWideEpt * kThreads - 1) / (kWideEpt * kThreads);
   return count * wide < 256 && vocab <= 262144 ? kNarrowEpt : kWideEpt;

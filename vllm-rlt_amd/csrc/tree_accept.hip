@@ -7,7 +7,9 @@
 //
 // Greedy: the child that holds the node's argmax token (the first, of several).  All logit
 // rows' argmaxes are formed by row slices (the targets are an output), then one workgroup per
-// request joins its slices and walks.
+// request joins its slices and walks.  The logits' bytes bound it (32 requests of 32 nodes, 49152
+// float32 columns: 31 us for 201 MB, 6.5 TB/s, and 5 to join); for one request the two
+// launches (4.6 + 3.3 us).
 //
 // Sampled: at a node the children are tried in order, each drawn from the draft distribution
 // q of the node.  With y the weights left of the target distribution p (at first y = p) and

@@ -10,8 +10,8 @@ Same arguments and semantics as
   LAST_EXITED copy into deeper planes),
 plus ``store_kv``, the unmasked index-put writer
 (vllm_rlt/core/kv_cache_manager.py:893-895), and ``commit_tree_kv``, which moves the accepted
-path of a draft tree behind the prefix (the reference's drafts are chains).  Every call enqueues one gfx950 launch on
-the current stream without host synchronization.  Rows whose block or offset lies
+path of a draft tree behind the prefix (the reference's drafts are chains).  Every call
+enqueues one gfx950 launch on the current stream without host synchronization.  Rows whose block or offset lies
 outside the pool are skipped (the reference's kernels would write out of bounds).
 """
 

@@ -206,7 +206,7 @@ def finalize_rows(descriptor: torch.Tensor, tables: torch.Tensor, key_pool: torc
 
 
 OPS = ("paged_attention", "paged_attention_store", "tree_attention", "tree_masks",
-       "greedy_tree_accept", "tree_accept", "token_logprobs", "commit_tree_kv", "spec_probs", "categorical", "spec_accept", "greedy_accept",
-       "propose_drafts", "verify_distributions", "verify_accept", "merge_random_round",
+       "greedy_tree_accept", "tree_accept", "token_logprobs", "commit_tree_kv", "spec_probs",
+       "categorical", "spec_accept", "greedy_accept", "propose_drafts", "verify_distributions", "verify_accept", "merge_random_round",
        "rejection_rows", "store_kv",
        "store_fp8", "finalize_rows")
