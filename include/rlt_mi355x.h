@@ -470,7 +470,7 @@ int rlt_greedy_tree_accept(const int64_t* draft_tokens, const int64_t* parents,
  *   [n, width + 1, V], u_accept fp32 [n, width], u_final fp32 [n] (contiguous)
  *   -> path (as above), tokens int64 [n, width + 1] (the accepted tokens, the final one,
  *   zeros), accepted, final_token int64 [n], error uint8 (bool) [n].
- * width <= 255, V <= 2^20.  No workspace.  The chain's round is
+ * width <= 255, V <= 2^20, n < 2^22.  No workspace.  The chain's round is
  * vllm_rlt/worker/speculative_sampling.py:104-181.
  */
 int rlt_tree_accept(const int64_t* draft_tokens, const int64_t* parents, const int64_t* drafts,

@@ -43,6 +43,7 @@ using namespace vocab;
 constexpr int kMaxDrafts = 255;
 constexpr int64_t kMaxVocab = 1 << 20;
 constexpr int kSliceEpt = 32;
+constexpr int64_t kMaxRequests = 1 << 22;  // of a sampled round: a launch's threads fit 32 bits
 constexpr int64_t kMaxLaunch = UINT32_MAX;  // threads of a launch along one axis
 
 // ---------------------------------------------------------------- greedy
@@ -495,7 +496,7 @@ int rlt_tree_accept(const int64_t* draft_tokens, const int64_t* parents, const i
                     int64_t n, int32_t width, int64_t vocab, int64_t* path, int64_t* tokens,
                     int64_t* accepted, int64_t* final_token, uint8_t* error, hipStream_t stream) {
   if (n < 0 || width < 0 || vocab < 1) return RLT_ERR_ARGUMENT;
-  if (width > kMaxDrafts || vocab > kMaxVocab || n > kMaxLaunch / kAccThreads) return RLT_ERR_UNSUPPORTED;
+  if (width > kMaxDrafts || vocab > kMaxVocab || n >= kMaxRequests) return RLT_ERR_UNSUPPORTED;
   if (n == 0) return RLT_OK;
   if (!drafts || !p || !u_final || !path || !tokens || !accepted || !final_token || !error ||
       (width && (!draft_tokens || !parents || !q || !u_accept)))
