@@ -195,3 +195,19 @@ def test_in_a_graph_and_bit_for_bit(pkg, dev):
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(out, eager))
         assert math.isfinite(torch.randn(1 << 18, device=dev).sum().item())
+
+
+def test_one_row_for_many_tokens(pkg, dev):
+    """The same row index, and the same token, several times; on a stream of its own."""
+    g = torch.Generator().manual_seed(30)
+    x = torch.randn(3, 20000, generator=g) * 3
+    rows = torch.tensor([2, 2, 0, 2, 0])
+    tokens = torch.tensor([5, 5, 5, 19999, 7])
+    xd, rd, td = x.to(dev), rows.to(dev), tokens.to(dev)
+    side = torch.cuda.Stream(dev)
+    side.wait_stream(torch.cuda.current_stream(dev))
+    with torch.cuda.stream(side):
+        res = pkg.token_logprobs(xd, td, rows=rd, top_n=8)
+    torch.cuda.synchronize()
+    check(res, x[rows], tokens, 8)
+    assert res.logprob[0] == res.logprob[1]

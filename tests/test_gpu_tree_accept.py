@@ -261,3 +261,31 @@ def test_tree_masks(pkg, dev):
     got = pkg.tree_masks(bad.to(dev), torch.tensor([0, 5], dtype=torch.int32).to(dev), 5)
     assert got[:, 0].tolist() == [1, 3, 4, 12, 16]
     assert pkg.tree_masks(bad[:0].to(dev), cu[:1].to(dev), 3).eq(0).all()
+
+
+def test_tree_masks_of_single_nodes(pkg, dev):
+    """No drafts at all; sequences of one node; rows before the first sequence and behind the last."""
+    cu = torch.tensor([2, 3, 4, 4, 5], dtype=torch.int32)
+    got = pkg.tree_masks(torch.zeros(4, 0, dtype=torch.int64, device=dev), cu.to(dev), 9)
+    assert got.tolist() == [[0], [0], [1], [1], [1], [0], [0], [0], [0]]
+    got = pkg.tree_masks(torch.zeros(4, 70, dtype=torch.int64, device=dev), cu.to(dev), 3)
+    assert got.tolist() == [[0, 0], [0, 0], [1, 0]]
+
+
+def test_rounds_on_two_streams(pkg, dev):
+    """Calls in flight side by side."""
+    args = [to(dev, sampled_inputs(20, 9, 30000, seed=s)) for s in (1, 2)]
+    logits = [a[4].log() for a in args]
+    want = [(pkg.tree_accept(*a), pkg.greedy_tree_accept(*a[:3], x)) for a, x in zip(args, logits)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(dev) for _ in range(2)]
+    got = [[], []]
+    for _ in range(5):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append((pkg.tree_accept(*args[i]), pkg.greedy_tree_accept(*args[i][:3], logits[i])))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for pair in got[i]:
+            for x, y in zip(pair, want[i]):
+                assert all(torch.equal(a, b) for a, b in zip(x, y))

@@ -358,3 +358,33 @@ def test_key_scale_zero_or_negative(pkg, dev, dtype, dim, scale):
     c = make_case([16, 40], [515, 96], 4, 2, dim, dtype, "fp8", seed=60)
     c.k_scale = torch.tensor(scale)
     check(call(pkg, dev, c), c)
+
+
+def test_no_table_at_all(pkg, dev):
+    """Tables of width 0 hold no position: rows of zeros."""
+    c = make_case([3, 2], [40, 20], 4, 2, 128, BF)
+    got = call(pkg, dev, c, block_tables=c.tables[:, :0])
+    assert got.shape == c.q.shape and (got == 0).all()
+
+
+def test_calls_side_by_side(pkg, dev):
+    """Two streams, each with calls of its own: every call has its own partials."""
+    cases = [make_case([26, 9], [2600, 511], 16, 4, 128, BF, seed=30),
+             make_case([16, 7], [1515, 3096], 16, 8, 128, BF, "fp8", seed=31)]
+    want = [call(pkg, dev, c) for c in cases]
+    kernel = pkg.create_backend("auto", dev, BF, 128, 16)
+    args = []
+    for c in cases:
+        args.append([x.to(dev) if x is not None else None
+                     for x in (c.q, c.k, c.v, c.tables, c.lengths, c.cu, c.mask, c.k_scale, c.v_scale)])
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(dev) for _ in cases]
+    got = [[], []]
+    for _ in range(5):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                a = args[i]
+                got[i].append(kernel.tree(*a[:6], cases[i].max_q, *a[6:]))
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(x, want[i]) for x in got[i])

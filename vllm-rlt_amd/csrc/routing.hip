@@ -213,7 +213,7 @@ __global__ __launch_bounds__(kThreads) void rlt_tree_masks_kernel(
   }
   // rows of no sequence
   const int64_t first = num_seqs ? cu[0] : 0, last = num_seqs ? cu[num_seqs] : 0;
-  const int64_t ahead = min(max(first, (int64_t)0), rows), past = max(last, ahead);
+  const int64_t ahead = min(max(first, (int64_t)0), rows), past = min(max(last, ahead), rows);
   for (int64_t at = (int64_t)blockIdx.x * kThreads + threadIdx.x; at < rows - past + ahead;
        at += (int64_t)gridDim.x * kThreads) {
     uint64_t* const out = mask + (at < ahead ? at : at - ahead + past) * words;

@@ -231,8 +231,8 @@ int rlt_tree_attention(const void* q, int64_t q_row_stride, int64_t q_head_strid
       (kv_dtype == RLT_FP8_E4M3) != (scale_mode != 0))
     return RLT_ERR_ARGUMENT;
   if (num_seqs == 0 || num_q_rows == 0 || max_q_len == 0) return RLT_OK;
-  if (!q || !key_cache || !value_cache || !block_tables || !context_lengths || !cu_seqlens_q ||
-      !tree_mask || !out)
+  if (!q || !key_cache || !value_cache || (!block_tables && table_width) || !context_lengths ||
+      !cu_seqlens_q || !tree_mask || !out)
     return RLT_ERR_ARGUMENT;
   if (head_dim > kVecDims || max_q_len > kMaxNodes || num_q_heads > 1024) return RLT_ERR_UNSUPPORTED;
   if (mask_words <= 0 || (int64_t)mask_words * 64 < max_q_len || mask_stride < mask_words ||
