@@ -6,7 +6,7 @@ import pytest
 import torch
 
 from tests.tree_cases import FP8, make_case, pack_bits, reference
-from tests.tree_rounds import greedy_tree, random_trees
+from tests.tree_rounds import greedy_tree, random_trees, sampled_inputs
 
 pytestmark = pytest.mark.gpu
 
@@ -180,3 +180,24 @@ def test_a_whole_round(pkg, dev, kv):
                              max(counts), *scales)
     assert ((causal.double() - out[keep].double()).cpu().abs() <= 2 * tol[keep]).all()
     assert math.isfinite(float(again.float().sum()))
+
+
+def test_operators_keep_their_schemas(pkg, dev):
+    """torch.library.opcheck's schema and fake-tensor checks of every operator of the round."""
+    checks = ("test_schema", "test_faketensor")
+    ops = torch.ops.rlt_mi355x
+    c = make_case([9, 5], [70, 33], 4, 2, 64, torch.bfloat16, seed=50)
+    a = to_dev(dev, *sampled_inputs(3, 5, 300, seed=1))
+    path, accepted = paths(2, 10, torch.Generator().manual_seed(2))
+    pool = torch.randn(10, 2, 16, 2, 64, device=dev)
+    tables = torch.arange(10).view(2, 5).int()
+    for op, args in (
+            (ops.tree_attention, (*to_dev(dev, c.q, c.k, c.v, c.tables, c.lengths, c.cu), 9,
+                                  c.mask.to(dev))),
+            (ops.tree_masks, (a[1], torch.tensor([0, 6, 9, 12], dtype=torch.int32, device=dev), 12)),
+            (ops.tree_accept, a),
+            (ops.greedy_tree_accept, (*a[:3], a[4])),
+            (ops.token_logprobs, (a[4][0], torch.zeros(6, dtype=torch.int64, device=dev), None, 3)),
+            (ops.commit_tree_kv, (pool, pool.clone(), *to_dev(dev, tables, torch.tensor([5, 40]), path,
+                                                              accepted), 16))):
+        torch.library.opcheck(op, tuple(args), test_utils=checks)

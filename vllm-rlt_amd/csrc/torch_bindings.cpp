@@ -9,6 +9,7 @@
 // registered from Python (vllm-rlt_amd/ops.py).
 
 #include <ATen/ATen.h>
+#include <ATen/hip/EmptyTensor.h>
 #include <ATen/hip/impl/HIPGuardImplMasqueradingAsCUDA.h>
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 #include <torch/library.h>
@@ -623,27 +624,11 @@ Tensor paged_attention_store(const Tensor& q, const Tensor& k_new_in, const Tens
 
 // ---------------------------------------------------------------- draft trees
 
-// The outputs of one call as views of one allocation (an allocation takes about a microsecond
-// of the host, which the small calls of a round are bound by).
-class Outputs {
- public:
-  Outputs(int64_t bytes, const Tensor& like) : buffer_(at::empty({bytes}, like.options().dtype(at::kByte))) {}
-  static int64_t room(int64_t elements, int64_t size) { return (elements * size + 255) / 256 * 256; }
-  Tensor take(at::IntArrayRef sizes, at::ScalarType dtype) {
-    auto impl = c10::make_intrusive<c10::TensorImpl>(c10::Storage(buffer_.storage()), buffer_.key_set(),
-                                                     c10::scalarTypeToTypeMeta(dtype));
-    const int64_t size = (int64_t)c10::elementSize(dtype);
-    impl->set_storage_offset(at_ / size);
-    impl->set_sizes_contiguous(sizes);
-    Tensor t(std::move(impl));
-    at_ += room(t.numel(), size);
-    return t;
-  }
-
- private:
-  Tensor buffer_;
-  int64_t at_ = 0;
-};
+// An output of a small call, straight from the allocator (half of at::empty's host time): a
+// round's small calls are bound by the host.  Outputs share no storage, as the schemas say.
+Tensor fresh(at::IntArrayRef sizes, at::ScalarType dtype, const Tensor& like) {
+  return at::detail::empty_cuda(sizes, dtype, like.device(), std::nullopt);
+}
 
 // Attention of the nodes of draft trees (rlt_tree_attention): packed rows, an ancestor mask in
 // place of the causal window.
@@ -774,11 +759,11 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> greedy_tree_accept(const Tensor& draf
   need(parents, at::kLong, "parents");
   need(drafts, at::kLong, "drafts");
   const c10::hip::HIPGuardMasqueradingAsCUDA guard(target_logits.device());
-  Outputs outs(2 * Outputs::room(n * (w + 1), 8) + 2 * Outputs::room(n, 8), drafts);
-  Tensor targets = outs.take({n, w + 1}, at::kLong), path = outs.take({n, w + 1}, at::kLong);
-  Tensor accepted = outs.take({n}, at::kLong), next = outs.take({n}, at::kLong);
+  Tensor targets = fresh({n, w + 1}, at::kLong, drafts), path = fresh({n, w + 1}, at::kLong, drafts);
+  Tensor accepted = fresh({n}, at::kLong, drafts), next = fresh({n}, at::kLong, drafts);
   if (n == 0) return {targets, path, accepted, next};
-  const Tensor ws = workspace(rlt_greedy_tree_accept_workspace_size(n, (int32_t)w, vocab), drafts);
+  const Tensor ws =
+      fresh({(int64_t)rlt_greedy_tree_accept_workspace_size(n, (int32_t)w, vocab)}, at::kByte, drafts);
   const int status = rlt_greedy_tree_accept(
       (const int64_t*)ptr(draft_tokens), (const int64_t*)ptr(parents), (const int64_t*)ptr(drafts),
       ptr(target_logits), dtype_code(target_logits.scalar_type()),
@@ -811,10 +796,9 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> tree_accept(
   need(u_accept, at::kFloat, "u_accept");
   need(u_final, at::kFloat, "u_final");
   const c10::hip::HIPGuardMasqueradingAsCUDA guard(p.device());
-  Outputs outs(2 * Outputs::room(n * (w + 1), 8) + 2 * Outputs::room(n, 8) + Outputs::room(n, 1), p);
-  Tensor path = outs.take({n, w + 1}, at::kLong), tokens = outs.take({n, w + 1}, at::kLong);
-  Tensor accepted = outs.take({n}, at::kLong), final_token = outs.take({n}, at::kLong);
-  Tensor error = outs.take({n}, at::kBool);
+  Tensor path = fresh({n, w + 1}, at::kLong, drafts), tokens = fresh({n, w + 1}, at::kLong, drafts);
+  Tensor accepted = fresh({n}, at::kLong, drafts), final_token = fresh({n}, at::kLong, drafts);
+  Tensor error = fresh({n}, at::kBool, drafts);
   if (n == 0) return {path, tokens, accepted, final_token, error};
   const int status = rlt_tree_accept(
       (const int64_t*)ptr(draft_tokens), (const int64_t*)ptr(parents), (const int64_t*)ptr(drafts),
@@ -843,16 +827,14 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> token_logprobs(const Tensor& 
   need(tokens, at::kLong, "tokens");
   need(rows, at::kLong, "rows");
   const c10::hip::HIPGuardMasqueradingAsCUDA guard(logits.device());
-  Outputs outs(2 * Outputs::room(count, 4) + Outputs::room(count, 8) + Outputs::room(count * top_n, 4) +
-                   Outputs::room(count * top_n, 8),
-               tokens);
-  Tensor logprob = outs.take({count}, at::kFloat), rank = outs.take({count}, at::kLong);
-  Tensor entropy = outs.take({count}, at::kFloat), top_logprob = outs.take({count, top_n}, at::kFloat);
-  Tensor top_tokens = outs.take({count, top_n}, at::kLong);
+  Tensor logprob = fresh({count}, at::kFloat, tokens), rank = fresh({count}, at::kLong, tokens);
+  Tensor entropy = fresh({count}, at::kFloat, tokens), top_logprob = fresh({count, top_n}, at::kFloat, tokens);
+  Tensor top_tokens = fresh({count, top_n}, at::kLong, tokens);
   // (a launch takes 65535 rows)
   for (int64_t at = 0; at < count; at += 65535) {
     const int64_t part = std::min<int64_t>(count - at, 65535);
-    const Tensor ws = workspace(rlt_token_logprobs_workspace_size(part, vocab, (int32_t)top_n), tokens);
+    const Tensor ws =
+        fresh({(int64_t)rlt_token_logprobs_workspace_size(part, vocab, (int32_t)top_n)}, at::kByte, tokens);
     const int64_t elt = logits.element_size();
     const int status = rlt_token_logprobs(
         rows.has_value() ? ptr(logits) : (char*)ptr(logits) + at * logits.stride(0) * elt,
