@@ -281,7 +281,9 @@ int rlt_tree_attention(const void* q, int64_t q_row_stride, int64_t q_head_strid
   P.group = num_q_heads / num_kv_heads;
   P.head_dim = head_dim;
   P.block_size = block_size;
-  P.window = window;
+  // (one that covers the table hides nothing; a smaller one keeps 32-bit positions, down to the
+  // -256 of a tree longer than its cache, above -2^31)
+  P.window = window < cap ? window : 0;
   P.qk_scale_log2 = 1.4426950408889634f / sqrtf((float)head_dim);
   P.scale_mode = scale_mode;
   P.out = out;
