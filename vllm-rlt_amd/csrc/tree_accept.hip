@@ -18,9 +18,11 @@
 // rejections y = max(p - C q, 0) with C = R_0 + .. + R_(k-1): no residual is stored, and a
 // rejection costs one sum over the node's two rows.  Where no child is left the next token is
 // drawn from y by inverse CDF.  The emitted tokens follow p whatever q and the tree are.
-// C, sums and the CDF are float64; a column's y is rounded once to float32 (two fused steps with
-// the two halves of C, so that what cancels stays exact), four of them are added, and these
-// sums in float64: float64 weights took 1.7x the instructions that a pass is bound by.
+// C is the sum of two floats (48 bits).  A column's y is float32, from two fused steps with them:
+// exact in sign and off by at most 2 half steps, 2^-23 of itself.  Four of them are added in
+// float32 (two more half steps), these sums in float64: R and the CDF's coarse table are off by
+// at most 2^-22 of themselves and C's 2^-48.  float64 weights took 1.7x the instructions that a
+// pass is bound by.  Inside the drawn segment, and for a draft's own column, weights are float64.
 //
 // One workgroup per request, each wave 1024 columns at a time.  A node's first pass is bound by
 // the rows' bytes: 83 GB/s of one CU, 6.6 TB/s of the chip at 128 requests.  It keeps what fits of
@@ -164,6 +166,14 @@ struct AcceptShared {
   int32_t walk[kMaxDrafts + 1];  // the accepted path
   int64_t last;
 };
+
+// C as the two floats that a column's weight is formed with.  With no bit of it past them a float32
+// weight and a float64 one have the same sign: where p - C q cancels, p - c_hi q is exact.  A segment
+// that weighs anything then holds a column that does.
+__device__ __forceinline__ double two_floats(double C) {
+  const float hi = (float)C;
+  return (double)hi + (double)(float)(C - (double)hi);
+}
 
 // y = max(p - C q, 0); NaN becomes 0 here and is looked for apart
 __device__ __forceinline__ double left_of(float p, float q, double C) {
@@ -432,7 +442,7 @@ __global__ __launch_bounds__(kAccThreads) void rlt_tree_accept_kernel(
         bad = true;
         break;
       }
-      if (u * R * qx < px - C * qx) {
+      if (u * R * qx < __builtin_fma(-C, qx, px)) {
         ++count;
         node = j;
         if (t == 0) sh.walk[count] = node;
@@ -447,7 +457,7 @@ __global__ __launch_bounds__(kAccThreads) void rlt_tree_accept_kernel(
     }
     const int64_t row = (int64_t)__builtin_amdgcn_readfirstlane(node) * vocab;
     const bool fresh = __builtin_amdgcn_readfirstlane(C == 0.0), alone = __builtin_amdgcn_readfirstlane(last);
-    if (!last) C += R;
+    if (!last) C = two_floats(C + R);
     seg = seg == sh.seg[0] ? sh.seg[1] : sh.seg[0];  // (the last pass's may still be read)
     weigh(sh, seg, held, fresh, p + row, (alone ? p : q) + row, C, vocab);
     if (last) break;
