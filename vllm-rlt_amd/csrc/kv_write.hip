@@ -338,6 +338,10 @@ int rlt_kv_commit_path(const int32_t* tables, int64_t n, int32_t planes, int32_t
     return RLT_ERR_UNSUPPORTED;
   if (n == 0 || path_width < 2 || width == 0) return RLT_OK;
   if (!tables || !starts || !path || !accepted || !key_pool || !value_pool) return RLT_ERR_ARGUMENT;
+  // (moves of memory that two workgroups hold would race)
+  if (key_pool == value_pool || (layers > 1 && layer_stride == 0) || (num_blocks > 1 && block_stride == 0) ||
+      (block_size > 1 && token_stride == 0))
+    return RLT_ERR_ARGUMENT;
   const int64_t bs = block_stride * elt_bytes, ls = layer_stride * elt_bytes,
                 ts = token_stride * elt_bytes;
   const int64_t all = bs | ls | ts | bytes_per_token | (int64_t)(uintptr_t)key_pool |

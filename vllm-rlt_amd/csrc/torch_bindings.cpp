@@ -9,6 +9,7 @@
 // registered from Python (vllm-rlt_amd/ops.py).
 
 #include <ATen/ATen.h>
+#include <ATen/MemoryOverlap.h>
 #include <ATen/hip/EmptyTensor.h>
 #include <ATen/hip/impl/HIPGuardImplMasqueradingAsCUDA.h>
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
@@ -876,6 +877,13 @@ void commit_tree_kv(const Tensor& key_pool, const Tensor& value_pool, const Tens
   need(starts, at::kLong, "starts");
   need(path, at::kLong, "path");
   need(accepted, at::kLong, "accepted");
+  // (the workgroups of two pools or layers move side by side)
+  const at::MemOverlapStatus shared = at::get_overlap_status(key_pool, value_pool);
+  TORCH_CHECK_VALUE(key_pool.numel() == 0 ||
+                        (ptr(key_pool) != ptr(value_pool) && shared != at::MemOverlapStatus::Full &&
+                         shared != at::MemOverlapStatus::Partial &&
+                         at::has_internal_overlap(key_pool) != at::MemOverlap::Yes),
+                    "key and value pools must not overlap, nor their blocks, layers and tokens");
   const int64_t n = path.size(0), planes = tables.dim() == 3 ? tables.size(1) : 1;
   if (n == 0 || planes == 0 || per_token == 0 || key_pool.size(1) == 0 || tables.size(-1) == 0) return;
   const c10::hip::HIPGuardMasqueradingAsCUDA guard(key_pool.device());

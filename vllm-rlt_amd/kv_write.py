@@ -181,7 +181,7 @@ def commit_tree_kv(key_pool, value_pool, tables, starts, path, accepted, block_s
     FP8 cache).  ``tables`` int32 ``[n, width]``, or ``[n, planes, width]`` to move in every
     plane; ``path`` int64 ``[n, W + 1]`` ascending from 0 and ``accepted`` int64 ``[n]`` as
     ``tree_accept`` / ``greedy_tree_accept`` return them.  The blocks that hold drafts must not
-    be shared between requests or planes.  Positions past the table or blocks outside the pool
+    be shared between requests or planes, nor the pools overlap.  Positions past the table or blocks outside the pool
     copy nothing.  Runs ``torch.ops.rlt_mi355x.commit_tree_kv``.
     """
     _lib.require_gpu(key_pool, value_pool, tables, starts, path, accepted)
