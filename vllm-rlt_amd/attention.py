@@ -65,7 +65,11 @@ class AttentionBackend:
         return self.kernel.prefill_store(*args, **kwargs)
 
     def tree(self, *args, **kwargs):
-        return self.kernel.tree(*args, **kwargs)
+        method = getattr(self.kernel, "tree", None)
+        if method is None:
+            selected = self.info.get("selected_backend", "this attention backend")
+            raise NotImplementedError(f"{selected} does not implement draft-tree attention")
+        return method(*args, **kwargs)
 
     def windowed(self, *args, **kwargs):
         method = getattr(self.kernel, "windowed", None)
