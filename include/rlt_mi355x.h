@@ -235,6 +235,26 @@ int rlt_tree_attention(const void* q, int64_t q_row_stride, int64_t q_head_strid
                        void* out, int64_t out_row_stride, int64_t out_head_stride,
                        void* workspace, size_t workspace_bytes, hipStream_t stream);
 
+/*
+ * The same with `flags`: with RLT_ATTN_COMPENSATE the weights' rounding to q's 16-bit type is
+ * followed by a second product with what it dropped, at any block size (other bits:
+ * RLT_ERR_ARGUMENT).  float32 q and the shapes of the vector form have float32 weights either way.
+ */
+int rlt_tree_attention_flags(const void* q, int64_t q_row_stride, int64_t q_head_stride,
+                             const void* key_cache, const void* value_cache, int64_t k_block_stride,
+                             int64_t k_token_stride, int64_t k_head_stride, int64_t v_block_stride,
+                             int64_t v_token_stride, int64_t v_head_stride, int32_t num_blocks,
+                             const int32_t* block_tables, int64_t table_stride, int32_t table_width,
+                             const int32_t* context_lengths, const int32_t* cu_seqlens_q,
+                             const int64_t* tree_mask, int64_t mask_stride, int32_t mask_words,
+                             int32_t num_seqs, int32_t max_q_len, int32_t num_q_rows,
+                             const float* key_scale, const float* value_scale, int32_t scale_mode,
+                             int64_t s_block_stride, int64_t s_token_stride, int64_t s_head_stride,
+                             int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim,
+                             int32_t block_size, int32_t q_dtype, int32_t kv_dtype, int32_t window,
+                             int32_t flags, void* out, int64_t out_row_stride, int64_t out_head_stride,
+                             void* workspace, size_t workspace_bytes, hipStream_t stream);
+
 /* ---------------------------------------------------------------- sampler */
 
 /*

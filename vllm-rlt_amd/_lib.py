@@ -101,6 +101,18 @@ _SIGNATURES = {
         _p, _i64, _i64,                 # out
         _p, _sz, _p,                    # workspace, bytes, stream
     ]),
+    "rlt_tree_attention_flags": (ctypes.c_int, [
+        _p, _i64, _i64,                 # q
+        _p, _p, _i64, _i64, _i64, _i64, _i64, _i64, _i32,  # pools, strides, blocks
+        _p, _i64, _i32, _p, _p,         # tables, stride, width, lengths, cu
+        _p, _i64, _i32,                 # mask, stride, words
+        _i32, _i32, _i32,               # num_seqs, max_q_len, num_q_rows
+        _p, _p, _i32, _i64, _i64, _i64,  # scales
+        _i32, _i32, _i32, _i32,         # hq, hkv, head_dim, block_size
+        _i32, _i32, _i32, _i32,         # q dtype, kv dtype, window, flags
+        _p, _i64, _i64,                 # out
+        _p, _sz, _p,                    # workspace, bytes, stream
+    ]),
     "rlt_merge_random_round": (ctypes.c_int, [
         _p, _i64, _p, _p, _p, _p, _i64,  # target, rows, accepted, next, starts, inputs, n
         _p, _i32, _p, _p, _p, _p, _i64,  # tokens, width, accepted, final, error, requests, r

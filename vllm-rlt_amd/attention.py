@@ -104,7 +104,8 @@ class MI355XPagedAttention:
     weights for the P V product is followed by a second MFMA with the bits it dropped,
     so P V keeps ~16 bits of each weight instead of 8 (bf16).  Applies to bf16 / fp16
     q on pools whose block size is a multiple of 16; packed calls then stay on the
-    verify kernels at every window length (rows equal per-row rows bit for bit).
+    verify kernels at every window length (rows equal per-row rows bit for bit).  ``tree``
+    takes it at any block size.
     """
 
     generation = None
@@ -192,8 +193,8 @@ class MI355XPagedAttention:
         parents), with ``window > 0`` the last ``window`` of those positions.  A row that sees
         nothing gives zeros; what a row does not see has no effect on it, whatever it holds.
         The pool is of q's type, or float8_e4m3fn with per-tensor or per-vector scales.
-        A row's last bits depend on the lengths of the whole batch, since its keys are split
-        over the CUs by them.  No reference counterpart (its drafts are chains).
+        ``compensate`` holds for trees too, at any block size.  A row's last bits depend on the
+        lengths of the whole batch, since its keys are split over the CUs by them.  No reference counterpart (its drafts are chains).
         """
         if type(window) is not int or window < 0:
             raise ValueError("window must be a nonnegative integer")
@@ -202,7 +203,8 @@ class MI355XPagedAttention:
         # argument checks, workspace and launch: torch.ops.rlt_mi355x.tree_attention
         return _lib.ops().tree_attention(q, key_cache, value_cache, block_tables,
                                          context_lengths, cu_seqlens_q, int(max_seqlen_q),
-                                         tree_mask, key_scale, value_scale, window)
+                                         tree_mask, key_scale, value_scale, window,
+                                         self.compensate)
 
     def uses_mfma(self, q_dtype, kv_dtype, head_dim):
         lib = _lib.library()

@@ -636,7 +636,8 @@ Tensor fresh(at::IntArrayRef sizes, at::ScalarType dtype, const Tensor& like) {
 Tensor tree_attention(const Tensor& q, const Tensor& key_cache, const Tensor& value_cache,
                       const Tensor& block_tables, const Tensor& context_lengths,
                       const Tensor& cu_seqlens_q, int64_t max_seqlen_q, const Tensor& tree_mask,
-                      const OptTensor& key_scale, const OptTensor& value_scale, int64_t window) {
+                      const OptTensor& key_scale, const OptTensor& value_scale, int64_t window,
+                      bool compensate) {
   TORCH_CHECK_VALUE(window >= 0 && window <= INT32_MAX, "window must be a nonnegative integer");
   TORCH_CHECK_VALUE(q.dim() == 3 && key_cache.dim() == 4 && value_cache.dim() == 4,
                     "q must be [rows, heads, dim] and caches [block, token, kv_head, dim]");
@@ -713,7 +714,7 @@ Tensor tree_attention(const Tensor& q, const Tensor& key_cache, const Tensor& va
   const int64_t mask_stride = std::max(tree_mask.stride(0), tree_mask.size(1));
   TORCH_CHECK_VALUE(rows == 1 || tree_mask.stride(0) >= tree_mask.size(1),
                     "tree_mask rows must not overlap");
-  const int status = rlt_tree_attention(
+  const int status = rlt_tree_attention_flags(
       ptr(q), q.stride(0), q.stride(1), ptr(key_cache), ptr(value_cache), key_cache.stride(0),
       key_cache.stride(1), key_cache.stride(2), value_cache.stride(0), value_cache.stride(1),
       value_cache.stride(2), (int32_t)num_blocks, (const int32_t*)ptr(block_tables),
@@ -723,8 +724,8 @@ Tensor tree_attention(const Tensor& q, const Tensor& key_cache, const Tensor& va
       (const float*)ptr(key_scale), (const float*)ptr(value_scale), mode, s_strides[0],
       s_strides[1], s_strides[2], (int32_t)heads, (int32_t)kv_heads, (int32_t)head_dim,
       (int32_t)block_size, dtype_code(q.scalar_type()), dtype_code(key_cache.scalar_type()),
-      (int32_t)window, ptr(output), output.stride(0), output.stride(1), ptr(ws), ws.numel(),
-      stream_of(q));
+      (int32_t)window, compensate ? RLT_ATTN_COMPENSATE : 0, ptr(output), output.stride(0),
+      output.stride(1), ptr(ws), ws.numel(), stream_of(q));
   check_status(status, "rlt_tree_attention");
   return output;
 }
@@ -942,7 +943,8 @@ TORCH_LIBRARY(rlt_mi355x, m) {
         "Tensor(d!)? value_scale=None, Tensor? row_lengths=None, bool compensate=False) -> Tensor");
   m.def("tree_attention(Tensor q, Tensor key_cache, Tensor value_cache, Tensor block_tables, "
         "Tensor context_lengths, Tensor cu_seqlens_q, int max_seqlen_q, Tensor tree_mask, "
-        "Tensor? key_scale=None, Tensor? value_scale=None, int window=0) -> Tensor");
+        "Tensor? key_scale=None, Tensor? value_scale=None, int window=0, "
+        "bool compensate=False) -> Tensor");
   m.def("tree_masks(Tensor parents, Tensor cu_seqlens_q, int rows) -> Tensor");
   m.def("greedy_tree_accept(Tensor draft_tokens, Tensor parents, Tensor drafts, "
         "Tensor target_logits) -> (Tensor, Tensor, Tensor, Tensor)");

@@ -86,6 +86,7 @@ struct Params {
   int32_t hq, hkv, group, head_dim, block_size, window;
   float qk_scale_log2;    // log2(e) / sqrt(head_dim)
   int32_t scale_mode;
+  int32_t compensate;     // the product with the values also takes what rounding the weights dropped
   void* out;
   int64_t out_row_stride, out_head_stride;
   int32_t max_blocks;     // row blocks of the longest tree
@@ -154,6 +155,24 @@ __device__ __forceinline__ uint32_t finite_part(uint32_t w) {
     if (((w >> 16) & E) == E) w &= 0xffffu;
   }
   return w;
+}
+
+// What the rounding of (a, b) to the packed pair `w` dropped, as a pair of the type (INF: nothing
+// of a number that is infinite there).
+template <int QT, bool INF>
+__device__ __forceinline__ uint32_t dropped2(float a, float b, uint32_t w) {
+  if constexpr (QT == RLT_BF16) {
+    a -= __uint_as_float(w << 16);
+    b -= __uint_as_float(w & 0xffff0000u);
+  } else {
+    a -= f16_bits_to_f32((uint16_t)w);
+    b -= f16_bits_to_f32((uint16_t)(w >> 16));
+  }
+  if constexpr (INF) {
+    a = fabsf(a) < INFINITY ? a : 0.f;
+    b = fabsf(b) < INFINITY ? b : 0.f;
+  }
+  return pack2<QT>(a, b);
 }
 
 // Direct global -> LDS loads: lane L's 16 (4) bytes land at `lds` + 16 L (4 L).  In assembly,
@@ -364,7 +383,9 @@ __device__ __forceinline__ int v_swz(int r) {
   return SLOTS >= 16 ? 4 * (r & 3) : 4 * ((r >> 1) & 1);
 }
 
-template <int QT, int KVT, int D, int SM, int RW>
+// CP: what the weights' rounding to q's type dropped is a second operand of the product with the
+// values, which keeps ~16 bits of each weight (bf16; fp16 22) instead of 8 (11).
+template <int QT, int KVT, int D, int SM, int RW, bool CP>
 __global__ __launch_bounds__(64 * kWaves, per_cu<D>()) void rlt_tree_kernel(Params P) {
   using G = Geometry<QT, KVT, D, RW>;
   constexpr bool FP8 = G::FP8;
@@ -662,7 +683,8 @@ __global__ __launch_bounds__(64 * kWaves, per_cu<D>()) void rlt_tree_kernel(Para
     // number, and weights times value scales, which may be of any size, are held over a power
     // of two that follows the row's largest such product (REFER).
     auto scale_at = [](int pos) { return pos / SP * (2 * SP) + pos % SP; };
-    auto weigh = [&](f32x16& sc, uint32_t (&p)[8], int tb, bool full, const float* scale) {
+    constexpr int NP = CP ? 16 : 8;  // packed weights, then what their rounding dropped
+    auto weigh = [&](f32x16& sc, uint32_t (&p)[NP], int tb, bool full, const float* scale) {
       if constexpr (SM == 1) {
 #pragma unroll
         for (int i = 0; i < 16; ++i) sc[i] *= k_mul;
@@ -740,6 +762,11 @@ __global__ __launch_bounds__(64 * kWaves, per_cu<D>()) void rlt_tree_kernel(Para
       }
 #pragma unroll
       for (int i = 0; i < 8; ++i) p[i] = pack2<QT>(x[2 * i], x[2 * i + 1]);
+      if constexpr (CP) {
+        // (weights times value scales may be infinite)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) p[8 + i] = dropped2<QT, SM == 2>(x[2 * i], x[2 * i + 1], p[i]);
+      }
     };
     // In masked tiles a value may be hidden from some rows, and 0 times a non-finite value would
     // spoil them: such values are cleared (idempotent: the row waves may all do it) and marked,
@@ -795,7 +822,7 @@ __global__ __launch_bounds__(64 * kWaves, per_cu<D>()) void rlt_tree_kernel(Para
         }
       }
     };
-    auto product = [&](const uint32_t (&va)[2 * ND][VW], const uint32_t (&p)[8]) {
+    auto product = [&](const uint32_t (&va)[2 * ND][VW], const uint32_t (&p)[NP]) {
 #pragma unroll
       for (int n = 0; n < 2 * ND; ++n) {
         const int c = n / ND, dt = n % ND;
@@ -807,6 +834,8 @@ __global__ __launch_bounds__(64 * kWaves, per_cu<D>()) void rlt_tree_kernel(Para
           a4 = u32x4{lo.x, lo.y, hi.x, hi.y};
         }
         oacc[dt] = mfma<QT>(a4, u32x4{p[4 * c], p[4 * c + 1], p[4 * c + 2], p[4 * c + 3]}, oacc[dt]);
+        if constexpr (CP)
+          oacc[dt] = mfma<QT>(a4, u32x4{p[8 + 4 * c], p[9 + 4 * c], p[10 + 4 * c], p[11 + 4 * c]}, oacc[dt]);
       }
     };
 
@@ -830,7 +859,7 @@ __global__ __launch_bounds__(64 * kWaves, per_cu<D>()) void rlt_tree_kernel(Para
           load_k(stage, sstage == 0 ? S : sstage - 1);
         }
         // with a second stage the values are here by now: their reads run beside the weights
-        uint32_t p[8], va[2 * ND][VW];
+        uint32_t p[NP], va[2 * ND][VW];
         if (S == 1) weigh(sc, p, tb, full, scale);
         if (more) wait_loads<S * LK + (S - 1) * LV>();
         if (!full) clean(vt, tb);
@@ -865,7 +894,7 @@ __global__ __launch_bounds__(64 * kWaves, per_cu<D>()) void rlt_tree_kernel(Para
           const bool full = is_full(tb);
           f32x16 sc;
           scores(sc, ring + stage * G::TILE);
-          uint32_t p[8], va[2 * ND][VW];
+          uint32_t p[NP], va[2 * ND][VW];
           if (!full) clean(vt, tb);
           read_v(va, vt);
           __builtin_amdgcn_sched_barrier(0);

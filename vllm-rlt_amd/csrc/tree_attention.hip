@@ -124,7 +124,11 @@ __global__ __launch_bounds__(256) void rlt_tree_vec_kernel(Params P) {
 template <int QT, int KVT, int D, int SM, int RW>
 void launch(const Params& P, hipStream_t stream) {
   using G = Geometry<QT, KVT, D, RW>;
-  hipLaunchKernelGGL((rlt_tree_kernel<QT, KVT, D, SM, RW>), dim3(grid_of<D>()), dim3(64 * kWaves), 0, stream, P);
+  const dim3 grid(grid_of<D>()), block(64 * kWaves);
+  if (P.compensate)
+    hipLaunchKernelGGL((rlt_tree_kernel<QT, KVT, D, SM, RW, true>), grid, block, 0, stream, P);
+  else
+    hipLaunchKernelGGL((rlt_tree_kernel<QT, KVT, D, SM, RW, false>), grid, block, 0, stream, P);
   // few pairs have many contributions each: more workgroups a pair, more threads a row (8 / 32 / 56
   // pairs: 7.7 / 9.0 / 4.8 us against 19.4 / 20.9 / 6.0; 128 / 512 / 880 pairs with one group of
   // threads: 10.6 / 11.2 / 17.2 against 15.7 / 17.8 / 43 with four)
@@ -205,22 +209,23 @@ size_t rlt_tree_attention_workspace_size(int32_t num_seqs, int32_t max_q_len, in
          (size_t)2 * tree::kGrid * tree::kPartRows * (head_dim + 2) * sizeof(float);
 }
 
-int rlt_tree_attention(const void* q, int64_t q_row_stride, int64_t q_head_stride,
-                       const void* key_cache, const void* value_cache, int64_t k_block_stride,
-                       int64_t k_token_stride, int64_t k_head_stride, int64_t v_block_stride,
-                       int64_t v_token_stride, int64_t v_head_stride, int32_t num_blocks,
-                       const int32_t* block_tables, int64_t table_stride, int32_t table_width,
-                       const int32_t* context_lengths, const int32_t* cu_seqlens_q,
-                       const int64_t* tree_mask, int64_t mask_stride, int32_t mask_words,
-                       int32_t num_seqs, int32_t max_q_len, int32_t num_q_rows,
-                       const float* key_scale, const float* value_scale, int32_t scale_mode,
-                       int64_t s_block_stride, int64_t s_token_stride, int64_t s_head_stride,
-                       int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim,
-                       int32_t block_size, int32_t q_dtype, int32_t kv_dtype, int32_t window,
-                       void* out, int64_t out_row_stride, int64_t out_head_stride,
-                       void* workspace, size_t workspace_bytes, hipStream_t stream) {
+int rlt_tree_attention_flags(const void* q, int64_t q_row_stride, int64_t q_head_stride,
+                             const void* key_cache, const void* value_cache, int64_t k_block_stride,
+                             int64_t k_token_stride, int64_t k_head_stride, int64_t v_block_stride,
+                             int64_t v_token_stride, int64_t v_head_stride, int32_t num_blocks,
+                             const int32_t* block_tables, int64_t table_stride, int32_t table_width,
+                             const int32_t* context_lengths, const int32_t* cu_seqlens_q,
+                             const int64_t* tree_mask, int64_t mask_stride, int32_t mask_words,
+                             int32_t num_seqs, int32_t max_q_len, int32_t num_q_rows,
+                             const float* key_scale, const float* value_scale, int32_t scale_mode,
+                             int64_t s_block_stride, int64_t s_token_stride, int64_t s_head_stride,
+                             int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim,
+                             int32_t block_size, int32_t q_dtype, int32_t kv_dtype, int32_t window,
+                             int32_t flags, void* out, int64_t out_row_stride, int64_t out_head_stride,
+                             void* workspace, size_t workspace_bytes, hipStream_t stream) {
   using namespace tree;
-  if (num_seqs < 0 || num_q_rows < 0 || max_q_len < 0 || table_width < 0 || window < 0)
+  if (num_seqs < 0 || num_q_rows < 0 || max_q_len < 0 || table_width < 0 || window < 0 ||
+      (flags & ~RLT_ATTN_COMPENSATE))
     return RLT_ERR_ARGUMENT;
   if (num_q_heads <= 0 || num_kv_heads <= 0 || num_q_heads % num_kv_heads || head_dim <= 0 ||
       block_size <= 0 || num_blocks <= 0)
@@ -286,6 +291,7 @@ int rlt_tree_attention(const void* q, int64_t q_row_stride, int64_t q_head_strid
   P.window = window < cap ? window : 0;
   P.qk_scale_log2 = 1.4426950408889634f / sqrtf((float)head_dim);
   P.scale_mode = scale_mode;
+  P.compensate = (flags & RLT_ATTN_COMPENSATE) ? 1 : 0;
   P.out = out;
   P.out_row_stride = out_row_stride;
   P.out_head_stride = out_head_stride;
@@ -323,6 +329,29 @@ int rlt_tree_attention(const void* q, int64_t q_row_stride, int64_t q_head_strid
     default: launch_vec<RLT_BF16>(P, kv_dtype, stream); break;
   }
   return rlt_launch_status();
+}
+
+int rlt_tree_attention(const void* q, int64_t q_row_stride, int64_t q_head_stride,
+                       const void* key_cache, const void* value_cache, int64_t k_block_stride,
+                       int64_t k_token_stride, int64_t k_head_stride, int64_t v_block_stride,
+                       int64_t v_token_stride, int64_t v_head_stride, int32_t num_blocks,
+                       const int32_t* block_tables, int64_t table_stride, int32_t table_width,
+                       const int32_t* context_lengths, const int32_t* cu_seqlens_q,
+                       const int64_t* tree_mask, int64_t mask_stride, int32_t mask_words,
+                       int32_t num_seqs, int32_t max_q_len, int32_t num_q_rows,
+                       const float* key_scale, const float* value_scale, int32_t scale_mode,
+                       int64_t s_block_stride, int64_t s_token_stride, int64_t s_head_stride,
+                       int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim,
+                       int32_t block_size, int32_t q_dtype, int32_t kv_dtype, int32_t window,
+                       void* out, int64_t out_row_stride, int64_t out_head_stride,
+                       void* workspace, size_t workspace_bytes, hipStream_t stream) {
+  return rlt_tree_attention_flags(
+      q, q_row_stride, q_head_stride, key_cache, value_cache, k_block_stride, k_token_stride,
+      k_head_stride, v_block_stride, v_token_stride, v_head_stride, num_blocks, block_tables,
+      table_stride, table_width, context_lengths, cu_seqlens_q, tree_mask, mask_stride, mask_words,
+      num_seqs, max_q_len, num_q_rows, key_scale, value_scale, scale_mode, s_block_stride,
+      s_token_stride, s_head_stride, num_q_heads, num_kv_heads, head_dim, block_size, q_dtype,
+      kv_dtype, window, 0, out, out_row_stride, out_head_stride, workspace, workspace_bytes, stream);
 }
 
 }  // extern "C"

@@ -42,7 +42,7 @@ def _(q, k_new, v_new, key_cache, value_cache, block_tables, context_lengths, cu
 
 @torch.library.register_fake("rlt_mi355x::tree_attention")
 def _(q, key_cache, value_cache, block_tables, context_lengths, cu_seqlens_q, max_seqlen_q,
-      tree_mask, key_scale=None, value_scale=None, window=0):
+      tree_mask, key_scale=None, value_scale=None, window=0, compensate=False):
     return q.new_empty(q.shape)
 
 
