@@ -479,9 +479,11 @@ int rlt_greedy_tree_accept(const int64_t* draft_tokens, const int64_t* parents,
  * from q[node]: accepted when u_accept[r, j] * R * q[node, t] < y[t] (t its token), else
  * y = max(y - R q[node], 0) and R = sum y.  The walk goes on at an accepted draft's node; where
  * none is left, the final token is drawn from y by inverse CDF with u_final[r] as in
- * rlt_categorical.  y is p - C q clipped at 0, C the sum of the node's R so far in float64, each
- * column rounded once to float32; sums and decisions in float64.  Rows of p and q count as
- * distributions as they stand.
+ * rlt_categorical.  y is p - C q clipped at 0, C the sum of the node's R so far, held in 48 bits.
+ * In the sums a column's y is float32, off by at most 2^-23 of itself and exactly 0 where p - C q
+ * is not positive; four of them are added in float32, these in float64, so that R and the draw's
+ * running weights are within 2^-22 of themselves.  A draft's own y, the comparisons and the
+ * draw within its 1024 columns are float64.  Rows of p and q count as distributions as they stand.
  * error[r] is set, and the final token 0, where drafts[r] is outside [0, width], a tried draft
  * has a token outside the vocabulary, no q mass or weights that are not finite, or where the
  * weights left have no finite positive mass (a NaN or an infinity in a row that is summed).
@@ -505,7 +507,11 @@ int rlt_tree_accept(const int64_t* draft_tokens, const int64_t* parents, const i
  *   logprob[i] = x_t - log sum e^x, rank[i] = 1 + the columns before t in descending order
  *   (equal logits by ascending column, NaN first), entropy[i] = -sum p log p (nats),
  *   top_tokens / top_logprob [count, top_n] = the first top_n columns in that order.
- * Sums in float64, outputs rounded once.  Logits of -inf weigh nothing; a row with a NaN, with
+ * A column's weight e^d, d = x - max, is float32; four are added in float32, these in float64.  With E
+ * the mean under the row's distribution, log sum e^x is within E[4 + 2.3 |d|] 2^-24, the entropy
+ * within that and (E[|d| (5 + 2.3 |d|)] + E|d| E[4 + 2.3 |d|]) 2^-24, and each output is rounded
+ * once (next to a dominant logit, whose weight is counted exactly, nothing is lost).
+ * Logits of -inf weigh nothing; a row with a NaN, with
  * +inf or without a logit above -inf gives NaN log probabilities and entropy.  A row index outside
  * [0, num_rows) gives NaN, rank 0 and tokens -1; a token outside the vocabulary NaN and rank
  * 0 beside the row's entropy and alternatives.  top_n <= 64, V <= 2^20, count <= 65535.

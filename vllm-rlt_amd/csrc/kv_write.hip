@@ -161,9 +161,10 @@ inline int elt_size(int dtype) {
 // accepted[r], the bytes at position start + path[j] go to position start + j, in every layer
 // of both pools.  A path ascends, so path[j] >= j: a thread that takes one 16-byte column of a
 // layer through the moves in order never overwrites a source that it still needs, in place
-// and without a second buffer; eight moves are loaded before the first is stored.  At few
-// requests the chain of loads path -> table -> pool bounds it (16 drafts over 24 layers: 3.8 us),
-// then the moves in order (64 requests, 31 drafts, 32 layers, 24 MB: 8.7 us, 2.7 TB/s).
+// and without a second buffer; eight moves are loaded before the first is stored.  The chain of
+// loads count -> path -> table -> pool bounds it: once at few requests (16 drafts over 24 layers:
+// 4.0 us), twice where the grid takes two rounds of the chip (64 requests, 31 drafts, 32 layers of
+// 1 KB rows, of whose workgroups 64 threads copy: 24 MB in 8.5 us, 2.8 TB/s).
 constexpr int kMaxPath = 255;
 constexpr int kMovesAhead = 8;
 

@@ -8,8 +8,8 @@
 // Greedy: the child that holds the node's argmax token (the first, of several).  All logit
 // rows' argmaxes are formed by row slices (the targets are an output), then one workgroup per
 // request joins its slices and walks.  The logits' bytes bound it (32 requests of 32 nodes, 49152
-// float32 columns: 31 us for 201 MB, 6.5 TB/s, and 5 to join); for one request the two
-// launches (4.6 + 3.3 us).
+// float32 columns: 31 us for 201 MB, 6.5 TB/s, and 5.4 to join); for one request the two
+// launches (4.6 + 3.8 us).
 //
 // Sampled: at a node the children are tried in order, each drawn from the draft distribution
 // q of the node.  With y the weights left of the target distribution p (at first y = p) and
@@ -29,7 +29,7 @@
 // the two rows on the CU: 4 steps (32768 columns) in registers and 2 in LDS, so that each
 // further pass at the node costs 2.2 us at 49152 columns instead of 4.7.  The wave sums of the
 // last pass are the CDF's coarse table.
-// Measured: 4 requests, 49152 columns 14 us; 128 requests, 65536 columns, up to five passes 36 us
+// Measured: 4 requests, 49152 columns 15 us; 128 requests, 65536 columns, up to five passes 36.6 us
 // (rereading the rows in every pass: 50).
 
 #include "vocab_rows.h"

@@ -17,11 +17,13 @@
 // refilled as soon as its scores are taken, its values as soon as they are added.  More rows
 // take 2 or 4 row waves that share the tiles, one barrier per tile.
 //
-// Measured (main kernel + merge): 32 sequences of 20 to 32 nodes, GQA 4, up to 8192 positions, bf16
-// 75 + 11 us (3.8 TB/s; the loads alone 65); 64 nodes of 55 heads of 96 150 + 17 us (4.8 TB/s);
-// 64 sequences of 16k to 32k positions in fp8 600 + 11 us (5.5 TB/s: the loads bound it, which
-// alone take as long).  One sequence of 700 positions takes 11 + 4 us: 2 us to find the
-// share, 2 for tables and first loads, 1 for the tiles, 2 to combine; the launches the rest.
+// Measured (main kernel + merge, medians; bytes by counters): 32 sequences of 20 to 32 nodes, GQA 4,
+// up to 8192 positions, bf16 76 + 11 us (296 MB read, 33 of partials written: 4.3 TB/s); 16
+// sequences of 64 nodes, 55 heads of 96 163 + 18 us (835 MB read for 692 of keys and values, whose
+// heads straddle lines, 44 written: 5.4 TB/s); 64 sequences of 16k to 32k positions in fp8
+// 645 + 12 us (3.29 GB read: 5.2 TB/s).  One sequence of 700 positions takes 11.5 + 4 us: 2 us
+// to find the share, 2 for tables and first loads, 1 for the tiles, 2 to combine; the launches the
+// rest.  With the compensated product 86, 166, 646 and 11.6 us.
 //
 // Schedule.  The keys of all (sequence, kv head, row block) pairs are one line of macro tiles
 // (KW tiles each), of which every workgroup takes an equal share, whatever the mix of lengths.
@@ -58,7 +60,7 @@ constexpr int kWords = kMaxNodes / 64;
 constexpr int kRingBytes = 64 << 10;
 constexpr int kBadWords = kMaxNodes / kTile + 3;  // tiles that a range of kMaxNodes meets
 // Tiles per workgroup from which the kv groups take neighbouring heads apart: these share a
-// position's cache lines (fp8, 8 heads of 128: 600 us, 670 together; 55 heads of 96: 150 and 180),
+// position's cache lines (fp8, 8 heads of 128: 645 us, 710 together; 55 heads of 96: 163 and 197),
 // but a pair's tiles then come one by one, which leaves short shares to few waves.
 constexpr int kApartTiles = 8;
 constexpr float kLazy = 8.f;       // log2 headroom before the running max moves

@@ -130,8 +130,8 @@ void launch(const Params& P, hipStream_t stream) {
   else
     hipLaunchKernelGGL((rlt_tree_kernel<QT, KVT, D, SM, RW, false>), grid, block, 0, stream, P);
   // few pairs have many contributions each: more workgroups a pair, more threads a row (8 / 32 / 56
-  // pairs: 7.7 / 9.0 / 4.8 us against 19.4 / 20.9 / 6.0; 128 / 512 / 880 pairs with one group of
-  // threads: 10.6 / 11.2 / 17.2 against 15.7 / 17.8 / 43 with four)
+  // pairs: 8.0 / 9.6 / 5.1 us against 19.9 / 20.8 / 6.1; 128 / 512 / 880 pairs with one group of
+  // threads: 11.0 / 11.5 / 17.8 against 16.5 / 18.8 / 45 with four)
   const int64_t pairs = (int64_t)P.num_seqs * P.hkv * P.max_blocks;
   const int rows = P.max_q * P.group < G::RB ? P.max_q * P.group : G::RB;
   auto merge = [&](auto cg) {
@@ -145,9 +145,9 @@ void launch(const Params& P, hipStream_t stream) {
 }
 
 // Row waves: the fewest that hold the rows of a kv head, at most four (further rows are further
-// blocks, which read the keys again: 80 to 128 rows at up to 8192 positions 75 us with four, 98
-// with two; 64 rows of 55 heads 150 us with two, 241 with one).  More waves than rows need lose
-// the free run of single ones (32 rows in fp8: 605 us with one, 705 with two).
+// blocks, which read the keys again: 80 to 128 rows at up to 8192 positions 76 us with four, 98
+// with two; 64 rows of 55 heads 163 us with two, 248 with one).  More waves than rows need lose
+// the free run of single ones (32 rows in fp8: 645 us with one, 697 with two).
 int row_waves(int rows, int head_dim, bool fp8) {
   if (head_dim == 256 && !fp8) return 4;  // two stages of its tiles fit one kv group only
   return rows <= 32 ? 1 : rows <= 64 ? 2 : 4;

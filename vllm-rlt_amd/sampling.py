@@ -277,10 +277,13 @@ def tree_accept(draft_tokens, parents, drafts, q, p, u_accept, u_final):
     node's children are tried in index order: child t is accepted when ``u_accept * R * q[t] <
     y[t]``, where y is what is left of p (at first p, R = 1) and a rejection leaves
     ``max(y - R q, 0)`` with its sum R; where none is left the final token is drawn from y with
-    ``u_final``.  The emitted tokens follow p.  Rows count as distributions as they stand; sums and
-    decisions are float64.  ``error`` is set (and the final token 0) for a draft count outside
-    ``[0, W]``, a tried draft that q cannot have proposed, and weights without a finite
-    positive sum.
+    ``u_final``.  The emitted tokens follow p.  This holds for siblings that are drawn
+    independently from one q: children that are distinct by construction (the k likeliest tokens,
+    draws without replacement) are accepted with a bias.  Rows count as distributions as they
+    stand; a column's y is float32 in the sums (R is within 2^-22 of itself), the sums of more
+    than four columns, the comparisons and the draw are float64.  ``error`` is set (and the
+    final token 0) for a draft count outside ``[0, W]``, a tried draft that q cannot have
+    proposed, and weights without a finite positive sum.
 
     ``draft_tokens``, ``parents`` int64 ``[n, W]`` (W <= 255), ``drafts`` int64 ``[n]``, ``q``
     float32 ``[n, W, V]``, ``p`` float32 ``[n, W + 1, V]``, ``u_accept`` ``[n, W]``,
@@ -322,7 +325,9 @@ def token_logprobs(logits, tokens, *, rows=None, top_n=0):
     descending order, equal logits by ascending column), ``entropy`` float32 ``[r]`` in nats,
     and the first ``top_n`` (at most 64) columns with their log probabilities.  A row index
     outside the logits gives NaN, rank 0 and tokens -1, so the -1 of an acceptance path may be
-    passed on.  Logits of -inf weigh nothing; a row with a NaN or +inf, or without a logit above
+    passed on.  Weights are float32 under float64 sums: a log probability is within
+    ``E[4 + 2.3 |x - max|] 2^-24`` (the mean under its row's distribution) and one rounding.
+    Logits of -inf weigh nothing; a row with a NaN or +inf, or without a logit above
     -inf, gives NaN.  Runs ``torch.ops.rlt_mi355x.token_logprobs``.
     """
     _lib.require_gpu(logits, tokens, rows)
