@@ -591,8 +591,8 @@ int rlt_kv_finalize(const int64_t* descriptors, int64_t count, const int32_t* ta
  * path int64 [n, path_width] (path_stride between rows) ascends from path[r, 0] = 0, as the
  * tree rounds return it; entries with path[r, j] <= j stay.  In place and in order: blocks of
  * one table, and the blocks of different requests and planes that hold drafts, must be
- * distinct, and the two pools must not overlap (RLT_ERR_ARGUMENT for one pool given twice, and
- * for a stride of 0 between blocks, layers or tokens).  Positions beyond the table or entries outside the pool copy nothing.
+ * distinct, and the two pools must not overlap, nor rows of one pool (RLT_ERR_ARGUMENT where the
+ * strides say that they do).  Positions beyond the table or entries outside the pool copy nothing.
  * path_width <= 256.  No counterpart in the reference, where a chain's path lies in place.
  */
 int rlt_kv_commit_path(const int32_t* tables, int64_t n, int32_t planes, int32_t width,

@@ -26,6 +26,7 @@
 
 #include "common.h"
 #include "fp8_codec.h"
+#include "pool_overlap.h"
 #include "rlt_mi355x.h"
 
 #include <math.h>
@@ -339,12 +340,12 @@ int rlt_kv_commit_path(const int32_t* tables, int64_t n, int32_t planes, int32_t
     return RLT_ERR_UNSUPPORTED;
   if (n == 0 || path_width < 2 || width == 0) return RLT_OK;
   if (!tables || !starts || !path || !accepted || !key_pool || !value_pool) return RLT_ERR_ARGUMENT;
-  // (moves of memory that two workgroups hold would race)
-  if (key_pool == value_pool || (layers > 1 && layer_stride == 0) || (num_blocks > 1 && block_stride == 0) ||
-      (block_size > 1 && token_stride == 0))
-    return RLT_ERR_ARGUMENT;
   const int64_t bs = block_stride * elt_bytes, ls = layer_stride * elt_bytes,
                 ts = token_stride * elt_bytes;
+  // (moves of memory that two workgroups hold would race)
+  if (pools::overlap((int64_t)((uintptr_t)value_pool - (uintptr_t)key_pool),
+                     {{bs, num_blocks}, {ls, layers}, {ts, block_size}}, bytes_per_token))
+    return RLT_ERR_ARGUMENT;
   const int64_t all = bs | ls | ts | bytes_per_token | (int64_t)(uintptr_t)key_pool |
                       (int64_t)(uintptr_t)value_pool;
   const int unit = all % 16 == 0 ? 16 : all % 4 == 0 ? 4 : 1;

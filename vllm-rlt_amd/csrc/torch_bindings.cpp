@@ -9,7 +9,6 @@
 // registered from Python (vllm-rlt_amd/ops.py).
 
 #include <ATen/ATen.h>
-#include <ATen/MemoryOverlap.h>
 #include <ATen/hip/EmptyTensor.h>
 #include <ATen/hip/impl/HIPGuardImplMasqueradingAsCUDA.h>
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
@@ -18,6 +17,7 @@
 #include <optional>
 #include <tuple>
 
+#include "pool_overlap.h"
 #include "rlt_mi355x.h"
 
 namespace {
@@ -879,11 +879,13 @@ void commit_tree_kv(const Tensor& key_pool, const Tensor& value_pool, const Tens
   need(path, at::kLong, "path");
   need(accepted, at::kLong, "accepted");
   // (the workgroups of two pools or layers move side by side)
-  const at::MemOverlapStatus shared = at::get_overlap_status(key_pool, value_pool);
+  const int64_t elt = key_pool.element_size();
   TORCH_CHECK_VALUE(key_pool.numel() == 0 ||
-                        (ptr(key_pool) != ptr(value_pool) && shared != at::MemOverlapStatus::Full &&
-                         shared != at::MemOverlapStatus::Partial &&
-                         at::has_internal_overlap(key_pool) != at::MemOverlap::Yes),
+                        !pools::overlap((int64_t)((uintptr_t)ptr(value_pool) - (uintptr_t)ptr(key_pool)),
+                                        {{key_pool.stride(0) * elt, key_pool.size(0)},
+                                         {key_pool.stride(1) * elt, key_pool.size(1)},
+                                         {key_pool.stride(2) * elt, key_pool.size(2)}},
+                                        per_token * elt),
                     "key and value pools must not overlap, nor their blocks, layers and tokens");
   const int64_t n = path.size(0), planes = tables.dim() == 3 ? tables.size(1) : 1;
   if (n == 0 || planes == 0 || per_token == 0 || key_pool.size(1) == 0 || tables.size(-1) == 0) return;
