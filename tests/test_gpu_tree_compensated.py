@@ -101,3 +101,34 @@ def test_infinite_value_scales_stay_infinite(pkg, dev, dtype):
     assert torch.isposinf(got[:16, :2]).all()
     assert torch.isfinite(got[:16, 2:]).all() and torch.isfinite(got[16:]).all()
     assert torch.equal(torch.isposinf(attend(pkg, dev, c).float().cpu()), torch.isposinf(got))
+
+
+@pytest.mark.parametrize("hq,hkv,dim,nodes", [(2, 2, 128, [16, 7]), (4, 1, 64, [40, 12]), (8, 2, 96, [9, 16])])
+@pytest.mark.parametrize("low,high", [(-26, -22), (-20, 4), (2, 6)])
+def test_value_scales_of_any_size(pkg, dev, hq, hkv, dim, nodes, low, high):
+    """fp16 rows over per-vector scales far from 1, and over scales that differ widely: what the
+    rounding of weight times scale drops is held over the same power of two."""
+    c = make_case(nodes, [515, 96], hq, hkv, dim, HF, "fp8_vector", seed=50 + dim)
+    g = torch.Generator().manual_seed(dim)
+    exps = low + (high - low) * torch.rand(c.v_scale.shape, generator=g)
+    c.v_scale = torch.where(c.v_scale.isnan(), c.v_scale, torch.exp2(exps))
+    close(attend(pkg, dev, c, pkg.MI355XPagedAttention(compensate=True)), *dense(c, second=True))
+
+
+@pytest.mark.parametrize("dtype,kv,dim", [(BF, "same", 128), (BF, "fp8_vector", 64), (HF, "same", 96)])
+def test_hidden_values_with_compensation(pkg, dev, dtype, kv, dim):
+    """NaN at the last node's position: only that node's row of its kv head shows it, in its dim."""
+    nodes, ctx = [16, 40], [200, 131]
+    c = make_case(nodes, ctx, 4, 2, dim, dtype, kv, seed=3)
+    want, tol = dense(c, second=True)
+    rows = []
+    for s in range(2):
+        blk, off = int(c.tables[s, (ctx[s] - 1) // c.block]), (ctx[s] - 1) % c.block
+        c.v[blk, off, 0, dim // 2] = torch.tensor(math.nan).to(c.v.dtype)
+        rows.append(int(c.cu[s + 1]) - 1)
+    got = attend(pkg, dev, c, pkg.MI355XPagedAttention(compensate=True)).double().cpu()
+    hit = torch.zeros_like(want, dtype=torch.bool)
+    for r in rows:
+        hit[r, :2, dim // 2] = True
+    assert torch.isnan(got[hit]).all() and torch.isfinite(got[~hit]).all()
+    assert ((got - want).abs() <= tol)[~hit].all()
