@@ -1,4 +1,4 @@
-// Long-prompt prefill tiling of the paged attention (included by paged_attention.hip,
+// Long-prompt prefill tiling of the paged attention (included by paged_attention.h,
 // inside its namespace).
 //
 // Calls whose longest q window reaches kPfMinQ rows (prompt prefill, long chunks) take a
