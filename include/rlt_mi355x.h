@@ -9,7 +9,8 @@
  *   - returns 0 (RLT_OK) or an rlt_status error code; numerical failure of the
  *     sampler is reported through its `error` / `valid` outputs, not the status.
  *
- * Element types: RLT_F32 = 0, RLT_F16 = 1, RLT_BF16 = 2, RLT_FP8_E4M3 = 3 (OCP e4m3fn).
+ * Element types: RLT_F32 = 0, RLT_F16 = 1, RLT_BF16 = 2, RLT_FP8_E4M3 = 3 (OCP e4m3fn),
+ * RLT_INT8 = 4 (KV pools with block scales).
  * Status codes:  0 ok, 1 bad argument, 2 unsupported, 3 workspace, 4 launch failure.
  * Strides are in elements of the tensor they describe.
  */
@@ -601,6 +602,80 @@ int rlt_kv_commit_path(const int32_t* tables, int64_t n, int32_t planes, int32_t
                        int32_t layers, int64_t num_blocks, void* key_pool, void* value_pool,
                        int64_t block_stride, int64_t layer_stride, int64_t token_stride,
                        int64_t bytes_per_token, int32_t elt_bytes, hipStream_t stream);
+
+/* ---------------------------------------------------------------- rotary positions, appends */
+
+/*
+ * Rotary positions.  Row r of q [rows, num_q_heads, head_dim] and k [rows, num_kv_heads,
+ * head_dim] (row / head strides in elements, unit dim stride; either may have 0 heads) at
+ * positions[r] (int64): pair p of the first rotary_dim dims, (x[p], x[p + rotary_dim / 2]) or,
+ * interleaved, (x[2p], x[2p + 1]), goes from (a, b) to (a c - b s, a s + b c) with
+ * (c, s) = amplitude (cos, sin)(2 pi positions[r] turns[p]); the other dims are copied.
+ * turns: float64 [rotary_dim / 2], turns per position.  inverse: -s.  The angle is reduced
+ * in float64; float32 arithmetic, rounded once to dtype (RLT_F32 / RLT_F16 / RLT_BF16).  The
+ * outputs may be the inputs with their strides, else they must lie apart from them.
+ * head_dim <= 256.  The reference leaves the rotation to its model layers (vllm_rlt/layers/).
+ */
+int rlt_rotary(const void* q, int64_t q_row_stride, int64_t q_head_stride, const void* k,
+               int64_t k_row_stride, int64_t k_head_stride, const int64_t* positions, int64_t rows,
+               const double* turns, int32_t rotary_dim, float amplitude, int32_t interleaved,
+               int32_t inverse, int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim,
+               int32_t dtype, void* q_out, int64_t qo_row_stride, int64_t qo_head_stride,
+               void* k_out, int64_t ko_row_stride, int64_t ko_head_stride, hipStream_t stream);
+
+/*
+ * Windows of rows into the paged cache, keys and queries turned on the way (as rlt_rotary;
+ * rotary_dim 0: not at all).  Sequence s owns rows cu_seqlens_q[s] .. cu_seqlens_q[s + 1] - 1, at
+ * most max_q_len; row i of its n goes to position context_lengths[s] - n + i of its table
+ * and turns by it, or by positions[row] (int64, optional).  Rows before position 0, past the
+ * table or whose entry lies outside the pool are not written.  k, v [rows, num_kv_heads,
+ * head_dim] and q (optional) of `dtype`; q_out as in rlt_rotary.  Pools:
+ *   - kv_dtype == dtype, scale_mode 0: turned rows rounded once;
+ *   - RLT_FP8_E4M3, scale_mode 1 (one float each, read) or 2 ([block, token, kv_head],
+ *     written): codes and scales of the float32 rows as rlt_kv_store_fp8's;
+ *   - RLT_FP8_E4M3 or RLT_INT8, scale_mode 3 ([block, kv_head], written): max(amax (1 / M),
+ *     FLT_MIN) of the call's rows in the block (M = 448, int8 127; values that are not finite
+ *     do not count); where they go on behind earlier tokens of the block, the larger of that
+ *     and the block's scale, and if it grew the earlier codes' values are quantized again over
+ *     it.  Codes: x / scale (IEEE), clamped to +-M, to the nearest even; e4m3 keeps NaN, int8
+ *     takes it as 0.  A block is written by one sequence of a call only.
+ * The pools must not overlap, nor blocks, tokens and heads of one.  num_kv_heads <= 256,
+ * head_dim <= 256.  No workspace.  Replaces, behind the rotation, the writers
+ * vllm_rlt/kernels/graph_kv.py:52-67 and vllm_rlt/kernels/triton_attention.py:506-623 for
+ * packed windows; block scales have no counterpart in the reference.
+ */
+int rlt_kv_append(const void* k, int64_t k_row_stride, int64_t k_head_stride, const void* v,
+                  int64_t v_row_stride, int64_t v_head_stride, int32_t dtype, void* key_cache,
+                  void* value_cache, int64_t k_block_stride, int64_t k_token_stride,
+                  int64_t kc_head_stride, int64_t v_block_stride, int64_t v_token_stride,
+                  int64_t vc_head_stride, int32_t num_blocks, int32_t block_size, int32_t kv_dtype,
+                  float* key_scale, float* value_scale, int32_t scale_mode, int64_t s_block_stride,
+                  int64_t s_token_stride, int64_t s_head_stride, const int32_t* block_tables,
+                  int64_t table_stride, int32_t table_width, const int32_t* context_lengths,
+                  const int32_t* cu_seqlens_q, int32_t num_seqs, int32_t max_q_len, int64_t rows,
+                  int32_t num_kv_heads, int32_t head_dim, const int64_t* positions,
+                  const double* turns, int32_t rotary_dim, float amplitude, int32_t interleaved,
+                  const void* q, int64_t q_row_stride, int64_t q_head_stride, int32_t num_q_heads,
+                  void* q_out, int64_t qo_row_stride, int64_t qo_head_stride, hipStream_t stream);
+
+/*
+ * Cached positions as numbers: rows cu_seqlens[s] .. cu_seqlens[s + 1] - 1 (at most max_len)
+ * of k_out, v_out [rows, num_kv_heads, head_dim] (contiguous, out_dtype RLT_F32 / RLT_F16 /
+ * RLT_BF16) are the last n positions of sequence s, element or code times scale, rounded once.
+ * Pools and scale modes as rlt_kv_append (a pool of a row type may have another type than the
+ * outputs).  Positions before 0, past the table or in blocks outside the pool give zeros;
+ * rows of no sequence are not written.  No counterpart in the reference.
+ */
+int rlt_kv_load(const void* key_cache, const void* value_cache, int64_t k_block_stride,
+                int64_t k_token_stride, int64_t k_head_stride, int64_t v_block_stride,
+                int64_t v_token_stride, int64_t v_head_stride, int32_t num_blocks,
+                int32_t block_size, int32_t kv_dtype, const float* key_scale,
+                const float* value_scale, int32_t scale_mode, int64_t s_block_stride,
+                int64_t s_token_stride, int64_t s_head_stride, const int32_t* block_tables,
+                int64_t table_stride, int32_t table_width, const int32_t* context_lengths,
+                const int32_t* cu_seqlens, int32_t num_seqs, int32_t max_len, int64_t rows,
+                int32_t num_kv_heads, int32_t head_dim, int32_t out_dtype, void* k_out,
+                void* v_out, hipStream_t stream);
 
 /* ---------------------------------------------------------------- routing / metadata */
 

@@ -19,6 +19,10 @@ Drop-in host layer over ``librlt_mi355x.so`` (hand-written gfx950 HIP kernels):
 * draft trees in place of chains (no reference counterpart): ``MI355XPagedAttention.tree``
   with ``routing.tree_masks``, ``sampling.tree_accept`` / ``greedy_tree_accept``,
   ``kv_write.commit_tree_kv``; and ``sampling.token_logprobs`` for the emitted tokens.
+* what a layer does around its attention (no reference counterpart as kernels):
+  ``rotary.Rotary`` / ``apply_rotary`` (rotary positions), ``kv_write.append_kv`` (rows rotated
+  on the way into a paged cache of 16 bits, or of 8 with scales per tensor, vector, or block and
+  head) and ``kv_write.load_kv`` (the cache read back).
 * ``ops``: the same entry points as ``torch.ops.rlt_mi355x.*`` operators (ROCm device
   implementations and fake shape functions; the reference's torch_bindings pattern).
 * ``routing``: device metadata and request routing of the asynchronous verify step
@@ -29,7 +33,7 @@ The directory is named ``vllm-rlt_amd``; it is imported as ``vllm_rlt_amd``
 (see ``__graft_entry__.load_package``).
 """
 
-from . import attention, kv_write, ops, routing, sampling  # noqa: F401
+from . import attention, kv_write, ops, rotary, routing, sampling  # noqa: F401
 from .attention import (  # noqa: F401
     AttentionBackend,
     BackendCapabilities,
@@ -58,11 +62,14 @@ from .sampling import (  # noqa: F401
     verify_distributions,
 )
 from .kv_write import (  # noqa: F401
+    append_kv,
     commit_tree_kv,
     finalize_rows,
+    load_kv,
     masked_kv_store,
     store_fp8,
     store_kv,
     write_graph_kv,
 )
+from .rotary import Rotary, apply_rotary  # noqa: F401
 from .routing import tree_masks  # noqa: F401

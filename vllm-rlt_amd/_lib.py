@@ -15,7 +15,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "librlt_mi355x.so")
 OPS_PATH = os.path.join(HERE, "_C.so")
 
-RLT_F32, RLT_F16, RLT_BF16, RLT_FP8_E4M3 = 0, 1, 2, 3
+RLT_F32, RLT_F16, RLT_BF16, RLT_FP8_E4M3, RLT_INT8 = 0, 1, 2, 3, 4
 _DTYPE_CODE = {
     torch.float32: RLT_F32,
     torch.float16: RLT_F16,
@@ -163,6 +163,26 @@ _SIGNATURES = {
         _p, _i64, _i32, _i32, _i32, _p, _p, _i64, _i32, _p, _i32, _i64, _p, _p, _i64, _i64, _i64,
         _i64, _i32, _p]),
     "rlt_tree_masks": (ctypes.c_int, [_p, _i64, _i32, _p, _i32, _p, _i32, _i64, _p]),
+    "rlt_rotary": (ctypes.c_int, [
+        _p, _i64, _i64, _p, _i64, _i64,  # q, k, row / head strides
+        _p, _i64,                       # positions, rows
+        _p, _i32, ctypes.c_float, _i32, _i32,  # turns, rotary dim, amplitude, layout, inverse
+        _i32, _i32, _i32, _i32,         # hq, hkv, head_dim, dtype
+        _p, _i64, _i64, _p, _i64, _i64, _p]),  # outputs, stream
+    "rlt_kv_append": (ctypes.c_int, [
+        _p, _i64, _i64, _p, _i64, _i64, _i32,  # k, v, row / head strides, dtype
+        _p, _p, _i64, _i64, _i64, _i64, _i64, _i64, _i32, _i32, _i32,  # pools, blocks, dtype
+        _p, _p, _i32, _i64, _i64, _i64,  # scales
+        _p, _i64, _i32, _p, _p,         # tables, stride, width, lengths, cu
+        _i32, _i32, _i64, _i32, _i32,   # num_seqs, max_q_len, rows, hkv, head_dim
+        _p, _p, _i32, ctypes.c_float, _i32,  # positions, turns, rotary dim, amplitude, layout
+        _p, _i64, _i64, _i32, _p, _i64, _i64, _p]),  # q, heads, its output, stream
+    "rlt_kv_load": (ctypes.c_int, [
+        _p, _p, _i64, _i64, _i64, _i64, _i64, _i64, _i32, _i32, _i32,  # pools, blocks, dtype
+        _p, _p, _i32, _i64, _i64, _i64,  # scales
+        _p, _i64, _i32, _p, _p,         # tables, stride, width, lengths, cu
+        _i32, _i32, _i64, _i32, _i32,   # num_seqs, max_len, rows, hkv, head_dim
+        _i32, _p, _p, _p]),             # output dtype, outputs, stream
     "rlt_kv_store": (ctypes.c_int, [
         _p, _p, _i64, _i64, _i64, _i64, _p, _p, _i64, _i64, _i64, _i64, _i32,
         _p, _p, _p, _p, _i64, _i32, _i32, _i32, _p]),

@@ -21,6 +21,7 @@ enum rlt_dtype {
   RLT_F16 = 1,
   RLT_BF16 = 2,
   RLT_FP8_E4M3 = 3,  // OCP e4m3fn (torch.float8_e4m3fn), saturating
+  RLT_INT8 = 4,      // KV pools with block scales
 };
 
 static inline size_t rlt_align_up(size_t x, size_t a) { return (x + a - 1) / a * a; }

@@ -1,0 +1,794 @@
+// Rotary positions on MI355X (gfx950): queries and keys turned by their positions, on their own
+// (rlt_rotary) or on the way into the paged KV cache (rlt_kv_append); and the cache read back
+// as numbers (rlt_kv_load).
+//
+// Pair p of a head's first `rotary_dim` dims, (a, b) = (x[2p], x[2p + 1]) in the interleaved
+// layout or (x[p], x[p + rotary_dim / 2]) in the other, becomes
+//   (a c - b s, a s + b c),  (c, s) = amplitude (cos, sin)(2 pi position turns[p]),
+// and the inverse takes -s, which is the transpose and so the gradient.  position * turns[p]
+// and its reduction to an eighth of a turn are float64 (at position 2^20 a float32 angle is off
+// by 0.06), the sine and cosine of the rest float32 series; products and sums float32, rounded
+// once to the rows' type.
+//
+// 8-bit pools take x over its scale: per tensor, per vector (amax / 448, as rlt_kv_store_fp8), or one
+// scale per block of tokens and kv head, amax / M of the call's rows in the block (M = 448 for
+// e4m3, 127 for int8).  A block that the sequence's earlier tokens had begun keeps the larger of
+// its scale and that, and where it grew its earlier codes are held over the new one: the values
+// they stand for are quantized again, off by half a step of the new scale at most.
+//
+// Work: a workgroup takes 16 rows of a sequence (with block scales: one block of it, 16 rows at
+// a time), makes their sines and cosines once in LDS, and its four waves take the heads of q, k
+// and v in turn.  A lane holds both halves of its pairs (2 x 16 bytes), a group of LP lanes one
+// head vector, so that maxima are lane exchanges and a block's rows stay in registers between
+// its maximum and its codes.  What bounds it: each row is read and written once (HBM), and at a
+// few rows the chain lengths -> table -> rows -> scale -> codes of one launch.
+
+#include "common.h"
+#include "fp8_codec.h"
+#include "rlt_mi355x.h"
+
+#include <math.h>
+
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kWavesPerGroup = kThreads / 64;
+constexpr int kRows = 16;        // rows whose sines are in LDS at a time
+constexpr int kMaxPairs = 128;   // head_dim <= 256
+constexpr int kMaxKvItems = 512; // k and v heads, whose maxima over long blocks are kept in LDS
+
+// What the rows are written to.
+enum Mode {
+  kApply = 0,       // q_out and k_out
+  kSame = 1,        // a pool of the rows' type
+  kTensorFp8 = 2,   // e4m3, one scale for the pool (read)
+  kVectorFp8 = 3,   // e4m3, a scale per token and head (written)
+  kBlockFp8 = 4,    // e4m3, a scale per block and head (written)
+  kBlockInt8 = 5,   // int8, a scale per block and head (written)
+};
+constexpr bool in_blocks(int mode) { return mode == kBlockFp8 || mode == kBlockInt8; }
+
+struct Side {
+  const void* src;
+  int64_t src_row, src_head;
+  void* dst;  // rows (kApply, and q), or the pool
+  int64_t dst_block, dst_row, dst_head;
+  float* scale;
+};
+
+struct Params {
+  Side q, k, v;
+  int32_t hq, hkv, head_dim;
+  int64_t rows;
+  const int64_t* positions;  // of every row (nullptr: its place in the sequence)
+  const double* turns;       // turns per position of every pair
+  float amplitude;
+  int32_t rotary_dim, interleaved;
+  float sign;                // of the sine: -1 turns back
+  int64_t s_block, s_token, s_head;
+  const int32_t* tables;
+  int64_t table_stride;
+  int32_t table_width, num_blocks, block_size;
+  const int32_t* lengths;
+  const int32_t* cu;
+  int32_t num_seqs, max_rows, tiles;
+};
+
+// ---------------------------------------------------------------- sines
+
+// (cos, sin) of 2 pi t, |error| < 2^-23: t less its nearest eighth-turn multiple of 1/4 in float64,
+// then the Taylor series on [-pi/4, pi/4] (the terms left out are below 2e-9).
+__device__ __forceinline__ float2 turn(double t) {
+  const double quarter = rint(4.0 * t);
+  const float x = (float)((t - 0.25 * quarter) * 6.283185307179586);
+  const int n = (int)(quarter - 4.0 * rint(0.25 * quarter)) & 3;
+  const float y = x * x;
+  float s = fmaf(y, 2.7557319e-6f, -1.9841270e-4f);
+  s = fmaf(y, s, 8.3333333e-3f);
+  s = fmaf(y, s, -1.6666667e-1f);
+  s = fmaf(x * y, s, x);
+  float c = fmaf(y, -2.7557319e-7f, 2.4801587e-5f);
+  c = fmaf(y, c, -1.3888889e-3f);
+  c = fmaf(y, c, 4.1666667e-2f);
+  c = fmaf(y, c, -0.5f);
+  c = fmaf(y, c, 1.f);
+  const float a = n & 1 ? s : c, b = n & 1 ? c : s;
+  return make_float2((n == 1 || n == 2) ? -a : a, n >= 2 ? -b : b);
+}
+
+// ---------------------------------------------------------------- pieces of W elements
+
+template <int DT, int W>
+__device__ __forceinline__ void load_piece(const void* base, int64_t at, float (&x)[W]) {
+  if constexpr (W == 1) {
+    x[0] = load_as_f32<DT>(base, at);
+  } else if constexpr (DT == RLT_F32) {
+    static_assert(W == 4, "16-byte pieces");
+    const float4 v = *(const float4*)((const float*)base + at);
+    x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w;
+  } else {
+    static_assert(W == 8, "16-byte pieces");
+    const uint4 v = *(const uint4*)((const uint16_t*)base + at);
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      x[2 * i] = DT == RLT_BF16 ? bf16_bits_to_f32((uint16_t)w[i]) : f16_bits_to_f32((uint16_t)w[i]);
+      x[2 * i + 1] = DT == RLT_BF16 ? bf16_bits_to_f32((uint16_t)(w[i] >> 16))
+                                    : f16_bits_to_f32((uint16_t)(w[i] >> 16));
+    }
+  }
+}
+
+template <int DT>
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+  if constexpr (DT == RLT_BF16) {
+    typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+    const bf16x2 v = {(__bf16)a, (__bf16)b};
+    return __builtin_bit_cast(uint32_t, v);
+  } else {
+    typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+    const f16x2 v = {(_Float16)a, (_Float16)b};
+    return __builtin_bit_cast(uint32_t, v);
+  }
+}
+
+template <int DT, int W>
+__device__ __forceinline__ void store_piece(void* base, int64_t at, const float (&x)[W]) {
+  if constexpr (W == 1) {
+    store_from_f32<DT>(base, at, x[0]);
+  } else if constexpr (DT == RLT_F32) {
+    *(float4*)((float*)base + at) = make_float4(x[0], x[1], x[2], x[3]);
+  } else {
+    *(uint4*)((uint16_t*)base + at) = make_uint4(pack2<DT>(x[0], x[1]), pack2<DT>(x[2], x[3]),
+                                                 pack2<DT>(x[4], x[5]), pack2<DT>(x[6], x[7]));
+  }
+}
+
+// ---------------------------------------------------------------- codes
+
+template <int MODE>
+constexpr float top_of() { return MODE == kBlockInt8 ? 127.f : rlt_fp8::kMax; }
+
+// The code of x / scale (IEEE division, round to nearest even): e4m3 keeps NaN and clamps the
+// rest to +-448; int8 has no NaN and takes it as 0.
+template <int MODE>
+__device__ __forceinline__ uint32_t code_of(float x, float scale) {
+  if constexpr (MODE == kBlockInt8) {
+    const float y = x / scale;
+    const float c = fminf(fmaxf(y, -127.f), 127.f);
+    return (uint32_t)(int)(y != y ? 0.f : rintf(c)) & 0xffu;
+  } else {
+    return rlt_fp8::encode(x, scale);
+  }
+}
+template <int MODE>
+__device__ __forceinline__ float value_of(uint32_t code) {
+  if constexpr (MODE == kBlockInt8) return (float)(int8_t)code;
+  else return fp8x2_to_f32<false>(code).x;
+}
+
+template <int MODE, int W>
+__device__ __forceinline__ void store_codes(void* pool, int64_t at, const float (&x)[W], float scale) {
+  uint8_t* const p = (uint8_t*)pool + at;
+  if constexpr (W == 1) {
+    *p = (uint8_t)code_of<MODE>(x[0], scale);
+  } else {
+    uint32_t w[W / 4];
+#pragma unroll
+    for (int i = 0; i < W / 4; ++i) {
+      w[i] = 0;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) w[i] |= code_of<MODE>(x[4 * i + j], scale) << (8 * j);
+    }
+    if constexpr (W == 8) *(uint2*)p = make_uint2(w[0], w[1]);
+    else *(uint32_t*)p = w[0];
+  }
+}
+
+// |x| as a block's maximum takes it: what is not finite does not move a scale.
+__device__ __forceinline__ float finite_abs(float x) {
+  const float a = fabsf(x);
+  return a < INFINITY ? a : 0.f;
+}
+
+// ---------------------------------------------------------------- the kernel
+
+// One head's rows of a chunk: lane group g of LP lanes holds row RPW st + g in step st, a lane NS
+// slots of two W-element pieces (a and b).
+template <int W, int NS, int NSTEP>
+struct Held {
+  float x[NSTEP][NS][2][W];
+};
+
+template <int DT, int W, int LP, int MODE>
+__global__ __launch_bounds__(kThreads) void rlt_rotary_kernel(Params P) {
+  constexpr int NS = W == 1 ? 2 : 1;
+  constexpr int RPW = 64 / LP;
+  constexpr int NSTEP = kRows / RPW;
+  constexpr bool BLOCKS = in_blocks(MODE);
+  __shared__ float2 table[kRows * kMaxPairs];
+  __shared__ float tops[BLOCKS ? kMaxKvItems : 1];
+  const int t = threadIdx.x, lane = t & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
+  const int pairs = P.rotary_dim / 2;
+
+  // ---- the tile's rows [i0, i1) of its sequence
+  int64_t begin = 0;    // packed row of the sequence's first
+  int count, start = 0; // its rows, and the position of the first
+  int seq = 0, i0, i1, page = 0;
+  if constexpr (MODE == kApply) {
+    begin = (int64_t)blockIdx.x * kRows;
+    count = (int)min((int64_t)kRows, P.rows - begin);
+    i0 = 0;
+    i1 = count;
+  } else {
+    seq = (int)(blockIdx.x / (uint32_t)P.tiles);
+    const int tile = (int)(blockIdx.x - (uint32_t)seq * P.tiles);
+    const int64_t b = P.cu[seq], e = P.cu[seq + 1];
+    begin = b < 0 ? 0 : b > P.rows ? P.rows : b;
+    const int64_t n = (e > P.rows ? P.rows : e) - begin;
+    count = (int)(n < 0 ? 0 : n > P.max_rows ? P.max_rows : n);
+    start = P.lengths[seq] - count;
+    if constexpr (BLOCKS) {
+      const int first = start >= 0 ? start / P.block_size : -((-start + P.block_size - 1) / P.block_size);
+      page = first + tile;
+      const int64_t from = (int64_t)page * P.block_size - start;
+      i0 = (int)(from < 0 ? 0 : from);
+      i1 = (int)(from + P.block_size < count ? from + P.block_size : count);
+    } else {
+      i0 = tile * kRows;
+      i1 = min(count, i0 + kRows);
+    }
+  }
+  if (i0 >= i1) return;  // uniform over the workgroup
+
+  // the pool block of page `idx` of the sequence (-1: not in the pool, nothing is written)
+  auto block_at = [&](int idx) {
+    const int32_t e = idx >= 0 && idx < P.table_width ? P.tables[(int64_t)seq * P.table_stride + idx] : -1;
+    return e >= 0 && e < P.num_blocks ? e : -1;
+  };
+  const int entry = BLOCKS ? __builtin_amdgcn_readfirstlane(block_at(page)) : 0;
+  const int o0 = BLOCKS ? start + i0 - page * P.block_size : 0;  // offset of row i0 in its block
+
+  auto sines = [&](int c0, int c1) {
+    for (int e = t; e < (c1 - c0) * pairs; e += kThreads) {
+      const int r = e / pairs, p = e - r * pairs;
+      const int64_t row = begin + c0 + r;
+      const int64_t pos = P.positions ? P.positions[row] : (int64_t)start + c0 + r;
+      const float2 cs = turn((double)pos * P.turns[p]);
+      table[r * pairs + p] = make_float2(cs.x * P.amplitude, cs.y * P.amplitude * P.sign);
+    }
+  };
+
+  // ---- lane constants: slots of pieces (a, b)
+  const int in_group = lane % LP, group = lane / LP;
+  const int turning = P.interleaved || W == 1 ? P.rotary_dim / (2 * W) : pairs / W;
+  const int pieces = (P.head_dim + 2 * W - 1) / (2 * W);
+  int at_a[NS], at_b[NS];  // element of each piece, -1: none
+#pragma unroll
+  for (int n = 0; n < NS; ++n) {
+    const int i = in_group + LP * n;
+    at_a[n] = at_b[n] = -1;
+    if (i < pieces) {
+      if (i < turning && !P.interleaved) {
+        at_a[n] = W * i;
+        at_b[n] = pairs + W * i;
+      } else {
+        at_a[n] = 2 * W * i;
+        at_b[n] = 2 * W * i + W < P.head_dim ? 2 * W * i + W : -1;
+      }
+    }
+  }
+
+  // rows [c0, c1) of one head, turned if `turns`
+  auto fetch = [&](Held<W, NS, NSTEP>& held, const Side& s, int head, bool turns, int c0, int c1) {
+#pragma unroll
+    for (int st = 0; st < NSTEP; ++st) {
+      if (st * RPW >= c1 - c0) continue;  // uniform
+      const int r = st * RPW + group;
+      const int64_t at = (begin + c0 + r) * s.src_row + (int64_t)head * s.src_head;
+#pragma unroll
+      for (int n = 0; n < NS; ++n) {
+        float(&a)[W] = held.x[st][n][0];
+        float(&b)[W] = held.x[st][n][1];
+#pragma unroll
+        for (int e = 0; e < W; ++e) a[e] = b[e] = 0.f;
+        if (r < c1 - c0) {
+          if (at_a[n] >= 0) load_piece<DT, W>(s.src, at + at_a[n], a);
+          if (at_b[n] >= 0) load_piece<DT, W>(s.src, at + at_b[n], b);
+        }
+      }
+    }
+    if (!turns) return;
+#pragma unroll
+    for (int st = 0; st < NSTEP; ++st) {
+      if (st * RPW >= c1 - c0) continue;
+      const int r = st * RPW + group;
+#pragma unroll
+      for (int n = 0; n < NS; ++n) {
+        const int i = in_group + LP * n;
+        if (i >= turning || r >= c1 - c0) continue;
+        float(&a)[W] = held.x[st][n][0];
+        float(&b)[W] = held.x[st][n][1];
+        const float2* const cs = table + r * pairs + W * i;
+        if (W == 1 || !P.interleaved) {
+#pragma unroll
+          for (int e = 0; e < W; ++e) {
+            const float2 z = cs[e];
+            const float u = a[e] * z.x - b[e] * z.y, v = a[e] * z.y + b[e] * z.x;
+            a[e] = u;
+            b[e] = v;
+          }
+        } else {
+#pragma unroll
+          for (int e = 0; e + 1 < W; e += 2) {
+            const float2 y = cs[e / 2], z = cs[W / 2 + e / 2];
+            const float ua = a[e] * y.x - a[e + 1] * y.y, va = a[e] * y.y + a[e + 1] * y.x;
+            const float ub = b[e] * z.x - b[e + 1] * z.y, vb = b[e] * z.y + b[e + 1] * z.x;
+            a[e] = ua;
+            a[e + 1] = va;
+            b[e] = ub;
+            b[e + 1] = vb;
+          }
+        }
+      }
+    }
+  };
+  // the largest finite |x| of the held rows, in every lane
+  auto top = [&](const Held<W, NS, NSTEP>& held, int rows) {
+    float m = 0.f;
+#pragma unroll
+    for (int st = 0; st < NSTEP; ++st) {
+      if (st * RPW >= rows) continue;
+#pragma unroll
+      for (int n = 0; n < NS; ++n)
+#pragma unroll
+        for (int e = 0; e < W; ++e)
+          m = fmaxf(m, fmaxf(finite_abs(held.x[st][n][0][e]), finite_abs(held.x[st][n][1][e])));
+    }
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, RLT_WAVE));
+    return m;
+  };
+
+  // k and v first (their scales are a longer chain), then q
+  const int kv_items = MODE == kApply ? P.hkv : 2 * P.hkv;
+  const int items = kv_items + P.hq;
+  const int first_item = wave + kWavesPerGroup * blockIdx.y, step = kWavesPerGroup * gridDim.y;
+  const bool several = BLOCKS && i1 - i0 > kRows;
+  if constexpr (BLOCKS) {
+    if (several) {
+      // a block of more rows than are held: its maxima first
+      for (int i = t; i < kv_items; i += kThreads) tops[i] = 0.f;
+      for (int c0 = i0; c0 < i1; c0 += kRows) {
+        const int c1 = min(c0 + kRows, i1);
+        __syncthreads();
+        sines(c0, c1);
+        __syncthreads();
+        for (int item = first_item; item < kv_items; item += step) {
+          const bool key = item < P.hkv;
+          Held<W, NS, NSTEP> held;
+          fetch(held, key ? P.k : P.v, key ? item : item - P.hkv, key, c0, c1);
+          const float m = top(held, c1 - c0);
+          if (lane == 0) tops[item] = fmaxf(tops[item], m);
+        }
+      }
+    }
+  }
+  for (int c0 = i0; c0 < i1; c0 += kRows) {
+    const int c1 = min(c0 + kRows, i1);
+    if (several) __syncthreads();
+    sines(c0, c1);
+    __syncthreads();
+    for (int item = first_item; item < items; item += step) {
+      const bool is_q = item >= kv_items;
+      const bool key = item < P.hkv;
+      const int head = is_q ? item - kv_items : key ? item : item - P.hkv;
+      const Side& s = is_q ? P.q : key ? P.k : P.v;
+      Held<W, NS, NSTEP> held;
+      fetch(held, s, head, is_q || key, c0, c1);
+
+      if (MODE == kApply || is_q) {
+#pragma unroll
+        for (int st = 0; st < NSTEP; ++st) {
+          const int r = st * RPW + group;
+          if (r >= c1 - c0) continue;
+          const int64_t at = (begin + c0 + r) * s.dst_row + (int64_t)head * s.dst_head;
+#pragma unroll
+          for (int n = 0; n < NS; ++n) {
+            if (at_a[n] >= 0) store_piece<DT, W>(s.dst, at + at_a[n], held.x[st][n][0]);
+            if (at_b[n] >= 0) store_piece<DT, W>(s.dst, at + at_b[n], held.x[st][n][1]);
+          }
+        }
+        continue;
+      }
+      if constexpr (BLOCKS) {
+        if (entry < 0) continue;
+        float* const scale_at = s.scale + (int64_t)entry * P.s_block + (int64_t)head * P.s_head;
+        const float old = *scale_at;
+        const float m = several ? tops[item] : top(held, c1 - c0);
+        const float fresh = fmaxf(m * (1.f / top_of<MODE>()), rlt_fp8::kTiny);
+        const float scale = o0 > 0 && old > fresh ? old : fresh;
+        const int64_t base = (int64_t)entry * s.dst_block + (int64_t)head * s.dst_head;
+        if (c0 == i0 && o0 > 0 && scale > old) {
+          // the block's earlier codes, over the new scale
+          const int per_row = P.head_dim / W, n = o0 * per_row;
+          for (int e = lane; e < n; e += 64) {
+            const int r = e / per_row;
+            const int64_t at = base + (int64_t)r * s.dst_row + (e - r * per_row) * W;
+            float x[W];
+#pragma unroll
+            for (int u = 0; u < W; ++u) x[u] = value_of<MODE>(((const uint8_t*)s.dst)[at + u]) * old;
+            store_codes<MODE, W>(s.dst, at, x, scale);
+          }
+        }
+        if (lane == 0 && c1 == i1) *scale_at = scale;  // (the last chunk: all read the old one)
+#pragma unroll
+        for (int st = 0; st < NSTEP; ++st) {
+          const int r = st * RPW + group;
+          if (r >= c1 - c0) continue;
+          const int64_t at = base + (int64_t)(o0 + (c0 - i0) + r) * s.dst_row;
+#pragma unroll
+          for (int n = 0; n < NS; ++n) {
+            if (at_a[n] >= 0) store_codes<MODE, W>(s.dst, at + at_a[n], held.x[st][n][0], scale);
+            if (at_b[n] >= 0) store_codes<MODE, W>(s.dst, at + at_b[n], held.x[st][n][1], scale);
+          }
+        }
+      } else if constexpr (MODE != kApply) {
+#pragma unroll
+        for (int st = 0; st < NSTEP; ++st) {
+          if (st * RPW >= c1 - c0) continue;  // uniform
+          const int r = st * RPW + group;
+          const int pos = start + c0 + r;
+          const int e = r < c1 - c0 && pos >= 0 ? block_at(pos / P.block_size) : -1;
+          const int off = pos % P.block_size;
+          float scale = 1.f;
+          if constexpr (MODE == kTensorFp8) scale = s.scale[0];
+          if constexpr (MODE == kVectorFp8) {
+            // (NaN-propagating, as rlt_kv_store_fp8's)
+            float m = 0.f;
+#pragma unroll
+            for (int n = 0; n < NS; ++n)
+#pragma unroll
+              for (int u = 0; u < W; ++u)
+                m = rlt_fp8::nan_max(m, rlt_fp8::nan_max(fabsf(held.x[st][n][0][u]), fabsf(held.x[st][n][1][u])));
+#pragma unroll
+            for (int o = LP / 2; o >= 1; o >>= 1) m = rlt_fp8::nan_max(m, __shfl_xor(m, o, RLT_WAVE));
+            scale = rlt_fp8::dynamic_scale(m);
+          }
+          if (e < 0) continue;
+          const int64_t at = (int64_t)e * s.dst_block + (int64_t)off * s.dst_row + (int64_t)head * s.dst_head;
+          if (MODE == kVectorFp8 && in_group == 0)
+            s.scale[(int64_t)e * P.s_block + (int64_t)off * P.s_token + (int64_t)head * P.s_head] = scale;
+#pragma unroll
+          for (int n = 0; n < NS; ++n) {
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+              const int el = half ? at_b[n] : at_a[n];
+              if (el < 0) continue;
+              if constexpr (MODE == kSame) store_piece<DT, W>(s.dst, at + el, held.x[st][n][half]);
+              else store_codes<MODE, W>(s.dst, at + el, held.x[st][n][half], scale);
+            }
+          }
+        }
+      }
+    }
+  }
+}
+
+// ---------------------------------------------------------------- reading back
+
+struct LoadParams {
+  const void* k;
+  const void* v;
+  int64_t k_block, k_token, k_head, v_block, v_token, v_head;
+  const float* ks;
+  const float* vs;
+  int64_t s_block, s_token, s_head;  // 0 where the scales have no such axis
+  const int32_t* tables;
+  int64_t table_stride;
+  int32_t table_width, num_blocks, block_size;
+  const int32_t* lengths;
+  const int32_t* cu;
+  int64_t rows;
+  int32_t num_seqs, max_rows, tiles, hkv, head_dim;
+  void* k_out;
+  void* v_out;
+};
+
+template <int CT>
+__device__ __forceinline__ float pool_value(const void* base, int64_t at) {
+  if constexpr (CT == RLT_INT8) return (float)((const int8_t*)base)[at];
+  else return load_as_f32<CT>(base, at);
+}
+
+// kLoadRows rows of a sequence per workgroup, a thread W elements of a vector at a time.
+constexpr int kLoadRows = 16;
+template <int CT, int OT, int W>
+__global__ __launch_bounds__(kThreads) void rlt_kv_load_kernel(LoadParams P) {
+  const int seq = (int)(blockIdx.x / (uint32_t)P.tiles);
+  const int tile = (int)(blockIdx.x - (uint32_t)seq * P.tiles);
+  const int64_t b = P.cu[seq], e = P.cu[seq + 1];
+  const int64_t begin = b < 0 ? 0 : b > P.rows ? P.rows : b;
+  const int64_t n = (e > P.rows ? P.rows : e) - begin;
+  const int count = (int)(n < 0 ? 0 : n > P.max_rows ? P.max_rows : n);
+  const int start = P.lengths[seq] - count;
+  const int i0 = tile * kLoadRows, i1 = min(count, i0 + kLoadRows);
+  const int per_vec = (P.head_dim + W - 1) / W, per_row = 2 * P.hkv * per_vec;
+  for (int i = threadIdx.x + kThreads * blockIdx.y; i < (i1 - i0) * per_row; i += kThreads * gridDim.y) {
+    const int r = i / per_row, x = i - r * per_row;
+    const int vec = x / per_vec, d = (x - vec * per_vec) * W;
+    const bool value = vec >= P.hkv;
+    const int head = value ? vec - P.hkv : vec;
+    const int pos = start + i0 + r;
+    const int idx = pos >= 0 ? pos / P.block_size : -1, off = pos - idx * P.block_size;
+    const int32_t entry = idx >= 0 && idx < P.table_width ? P.tables[(int64_t)seq * P.table_stride + idx] : -1;
+    float y[W];
+#pragma unroll
+    for (int u = 0; u < W; ++u) y[u] = 0.f;
+    if (entry >= 0 && entry < P.num_blocks) {
+      const int64_t at = value ? (int64_t)entry * P.v_block + (int64_t)off * P.v_token + (int64_t)head * P.v_head + d
+                               : (int64_t)entry * P.k_block + (int64_t)off * P.k_token + (int64_t)head * P.k_head + d;
+      const void* const pool = value ? P.v : P.k;
+      const float* const scales = value ? P.vs : P.ks;
+      const float scale = scales ? scales[(int64_t)entry * P.s_block + (int64_t)off * P.s_token +
+                                          (int64_t)head * P.s_head] : 1.f;
+#pragma unroll
+      for (int u = 0; u < W; ++u) y[u] = pool_value<CT>(pool, at + u) * scale;
+    }
+    const int64_t to = ((begin + i0 + r) * P.hkv + head) * P.head_dim + d;
+    void* const out = value ? P.v_out : P.k_out;
+#pragma unroll
+    for (int u = 0; u < W; ++u) store_from_f32<OT>(out, to + u, y[u]);
+  }
+}
+
+// ---------------------------------------------------------------- dispatch
+
+constexpr int kGroupsWanted = 1024;  // workgroups from which the chip is filled
+
+template <int DT, int MODE>
+int launch_rotary(const Params& P, bool vec, int64_t gx, hipStream_t stream) {
+  const int items = P.hq + (MODE == kApply ? 1 : 2) * P.hkv;
+  const int64_t most = (items + kWavesPerGroup - 1) / kWavesPerGroup, want = (kGroupsWanted + gx - 1) / gx;
+  const dim3 grid((unsigned)gx, (unsigned)(want < most ? want : most));
+  constexpr int W = DT == RLT_F32 ? 4 : 8;
+  const int lanes = P.head_dim / (2 * W);  // that hold a vector
+  if (!vec) rlt_rotary_kernel<DT, 1, 64, MODE><<<grid, kThreads, 0, stream>>>(P);
+  else if (lanes <= 4) rlt_rotary_kernel<DT, W, 4, MODE><<<grid, kThreads, 0, stream>>>(P);
+  else if (lanes <= 8) rlt_rotary_kernel<DT, W, 8, MODE><<<grid, kThreads, 0, stream>>>(P);
+  else if (lanes <= 16) rlt_rotary_kernel<DT, W, 16, MODE><<<grid, kThreads, 0, stream>>>(P);
+  else if constexpr (DT == RLT_F32) rlt_rotary_kernel<DT, W, 32, MODE><<<grid, kThreads, 0, stream>>>(P);
+  return rlt_launch_status();
+}
+
+template <int MODE>
+int launch_rotary_dt(const Params& P, int dtype, bool vec, int64_t gx, hipStream_t stream) {
+  switch (dtype) {
+    case RLT_F32: return launch_rotary<RLT_F32, MODE>(P, vec, gx, stream);
+    case RLT_F16: return launch_rotary<RLT_F16, MODE>(P, vec, gx, stream);
+    case RLT_BF16: return launch_rotary<RLT_BF16, MODE>(P, vec, gx, stream);
+    default: return RLT_ERR_ARGUMENT;
+  }
+}
+
+// 16-byte pieces: every address a multiple of `bytes`, given strides in elements of `elt` bytes
+bool aligned(const void* p, int64_t a, int64_t b, int64_t c, int elt, int bytes) {
+  return (uintptr_t)p % bytes == 0 && a * elt % bytes == 0 && b * elt % bytes == 0 && c * elt % bytes == 0;
+}
+
+// the rotation's part of the arguments
+int set_turns(Params& P, const double* turns, int32_t rotary_dim, float amplitude, int32_t interleaved,
+              int32_t inverse) {
+  if (rotary_dim < 0 || rotary_dim % 2 || rotary_dim > P.head_dim || (rotary_dim && !turns))
+    return RLT_ERR_ARGUMENT;
+  P.turns = turns;
+  P.rotary_dim = rotary_dim;
+  P.amplitude = amplitude;
+  P.interleaved = interleaved ? 1 : 0;
+  P.sign = inverse ? -1.f : 1.f;
+  return RLT_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int rlt_rotary(const void* q, int64_t q_row_stride, int64_t q_head_stride, const void* k,
+               int64_t k_row_stride, int64_t k_head_stride, const int64_t* positions, int64_t rows,
+               const double* turns, int32_t rotary_dim, float amplitude, int32_t interleaved,
+               int32_t inverse, int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim,
+               int32_t dtype, void* q_out, int64_t qo_row_stride, int64_t qo_head_stride,
+               void* k_out, int64_t ko_row_stride, int64_t ko_head_stride, hipStream_t stream) {
+  if (rows < 0 || num_q_heads < 0 || num_kv_heads < 0 || head_dim <= 0 || head_dim > 2 * kMaxPairs)
+    return RLT_ERR_ARGUMENT;
+  if (dtype != RLT_F32 && dtype != RLT_F16 && dtype != RLT_BF16) return RLT_ERR_ARGUMENT;
+  Params P = {};
+  P.q = Side{q, q_row_stride, q_head_stride, q_out, 0, qo_row_stride, qo_head_stride, nullptr};
+  P.k = Side{k, k_row_stride, k_head_stride, k_out, 0, ko_row_stride, ko_head_stride, nullptr};
+  P.hq = num_q_heads;
+  P.hkv = num_kv_heads;
+  P.head_dim = head_dim;
+  P.rows = rows;
+  P.positions = positions;
+  if (const int st = set_turns(P, turns, rotary_dim, amplitude, interleaved, inverse)) return st;
+  if (rows == 0 || num_q_heads + num_kv_heads == 0) return RLT_OK;
+  if (!positions || (num_q_heads && (!q || !q_out)) || (num_kv_heads && (!k || !k_out)))
+    return RLT_ERR_ARGUMENT;
+  const int elt = dtype == RLT_F32 ? 4 : 2, pair = 32 / elt;
+  const bool vec = head_dim % pair == 0 && rotary_dim % pair == 0 &&
+                   aligned(q, q_row_stride, q_head_stride, 0, elt, 16) &&
+                   aligned(k, k_row_stride, k_head_stride, 0, elt, 16) &&
+                   aligned(q_out, qo_row_stride, qo_head_stride, 0, elt, 16) &&
+                   aligned(k_out, ko_row_stride, ko_head_stride, 0, elt, 16);
+  const int64_t gx = (rows + kRows - 1) / kRows;
+  if (gx >= ((int64_t)1 << 31)) return RLT_ERR_UNSUPPORTED;
+  return launch_rotary_dt<kApply>(P, dtype, vec, gx, stream);
+}
+
+int rlt_kv_append(const void* k, int64_t k_row_stride, int64_t k_head_stride, const void* v,
+                  int64_t v_row_stride, int64_t v_head_stride, int32_t dtype, void* key_cache,
+                  void* value_cache, int64_t k_block_stride, int64_t k_token_stride,
+                  int64_t kc_head_stride, int64_t v_block_stride, int64_t v_token_stride,
+                  int64_t vc_head_stride, int32_t num_blocks, int32_t block_size, int32_t kv_dtype,
+                  float* key_scale, float* value_scale, int32_t scale_mode, int64_t s_block_stride,
+                  int64_t s_token_stride, int64_t s_head_stride, const int32_t* block_tables,
+                  int64_t table_stride, int32_t table_width, const int32_t* context_lengths,
+                  const int32_t* cu_seqlens_q, int32_t num_seqs, int32_t max_q_len, int64_t rows,
+                  int32_t num_kv_heads, int32_t head_dim, const int64_t* positions,
+                  const double* turns, int32_t rotary_dim, float amplitude, int32_t interleaved,
+                  const void* q, int64_t q_row_stride, int64_t q_head_stride, int32_t num_q_heads,
+                  void* q_out, int64_t qo_row_stride, int64_t qo_head_stride, hipStream_t stream) {
+  if (rows < 0 || num_seqs < 0 || max_q_len < 0 || num_kv_heads <= 0 || head_dim <= 0 ||
+      head_dim > 2 * kMaxPairs || num_blocks <= 0 || block_size <= 0 || table_width < 0)
+    return RLT_ERR_ARGUMENT;
+  if (2 * num_kv_heads > kMaxKvItems) return RLT_ERR_UNSUPPORTED;
+  if (dtype != RLT_F32 && dtype != RLT_F16 && dtype != RLT_BF16) return RLT_ERR_ARGUMENT;
+  int mode;
+  if (kv_dtype == dtype && scale_mode == 0) mode = kSame;
+  else if (kv_dtype == RLT_FP8_E4M3 && scale_mode == 1) mode = kTensorFp8;
+  else if (kv_dtype == RLT_FP8_E4M3 && scale_mode == 2) mode = kVectorFp8;
+  else if (kv_dtype == RLT_FP8_E4M3 && scale_mode == 3) mode = kBlockFp8;
+  else if (kv_dtype == RLT_INT8 && scale_mode == 3) mode = kBlockInt8;
+  else return RLT_ERR_ARGUMENT;
+  if (scale_mode && (!key_scale || !value_scale)) return RLT_ERR_ARGUMENT;
+  Params P = {};
+  P.hkv = num_kv_heads;
+  P.hq = q ? num_q_heads : 0;
+  P.head_dim = head_dim;
+  P.rows = rows;
+  P.positions = positions;
+  if (const int st = set_turns(P, turns, rotary_dim, amplitude, interleaved, 0)) return st;
+  if (rows == 0 || num_seqs == 0 || max_q_len == 0) return RLT_OK;
+  if (!k || !v || !key_cache || !value_cache || !context_lengths || !cu_seqlens_q ||
+      (table_width && !block_tables) || P.hq < 0 || (P.hq && !q_out))
+    return RLT_ERR_ARGUMENT;
+  P.q = Side{q, q_row_stride, q_head_stride, q_out, 0, qo_row_stride, qo_head_stride, nullptr};
+  P.k = Side{k, k_row_stride, k_head_stride, key_cache, k_block_stride, k_token_stride, kc_head_stride, key_scale};
+  P.v = Side{v, v_row_stride, v_head_stride, value_cache, v_block_stride, v_token_stride, vc_head_stride, value_scale};
+  P.s_block = s_block_stride;
+  P.s_token = s_token_stride;
+  P.s_head = s_head_stride;
+  P.tables = block_tables;
+  P.table_stride = table_stride;
+  P.table_width = table_width;
+  P.num_blocks = num_blocks;
+  P.block_size = block_size;
+  P.lengths = context_lengths;
+  P.cu = cu_seqlens_q;
+  P.num_seqs = num_seqs;
+  P.max_rows = max_q_len;
+  // blocks that a window of max_q_len rows meets, or its groups of kRows rows
+  const int64_t tiles = in_blocks(mode) ? ((int64_t)max_q_len + block_size - 2) / block_size + 1
+                                        : ((int64_t)max_q_len + kRows - 1) / kRows;
+  const int64_t gx = tiles * num_seqs;
+  if (gx >= ((int64_t)1 << 31)) return RLT_ERR_UNSUPPORTED;
+  P.tiles = (int32_t)tiles;
+  const int elt = dtype == RLT_F32 ? 4 : 2, pair = 32 / elt;
+  const int code = mode == kSame ? elt : 1, piece = 16 / elt * code;  // bytes of a piece in the pool
+  const bool vec = head_dim % pair == 0 && rotary_dim % pair == 0 &&
+                   aligned(k, k_row_stride, k_head_stride, 0, elt, 16) &&
+                   aligned(v, v_row_stride, v_head_stride, 0, elt, 16) &&
+                   aligned(key_cache, k_block_stride, k_token_stride, kc_head_stride, code, piece) &&
+                   aligned(value_cache, v_block_stride, v_token_stride, vc_head_stride, code, piece) &&
+                   (!P.hq || (aligned(q, q_row_stride, q_head_stride, 0, elt, 16) &&
+                              aligned(q_out, qo_row_stride, qo_head_stride, 0, elt, 16)));
+  switch (mode) {
+    case kSame: return launch_rotary_dt<kSame>(P, dtype, vec, gx, stream);
+    case kTensorFp8: return launch_rotary_dt<kTensorFp8>(P, dtype, vec, gx, stream);
+    case kVectorFp8: return launch_rotary_dt<kVectorFp8>(P, dtype, vec, gx, stream);
+    case kBlockFp8: return launch_rotary_dt<kBlockFp8>(P, dtype, vec, gx, stream);
+    default: return launch_rotary_dt<kBlockInt8>(P, dtype, vec, gx, stream);
+  }
+}
+
+}  // extern "C"
+
+namespace {
+
+template <int CT, int OT>
+int launch_load(const LoadParams& P, bool vec, dim3 grid, hipStream_t stream) {
+  if (vec) rlt_kv_load_kernel<CT, OT, 8><<<grid, kThreads, 0, stream>>>(P);
+  else rlt_kv_load_kernel<CT, OT, 1><<<grid, kThreads, 0, stream>>>(P);
+  return rlt_launch_status();
+}
+
+template <int CT>
+int launch_load_ot(const LoadParams& P, int out_dtype, bool vec, dim3 grid, hipStream_t stream) {
+  switch (out_dtype) {
+    case RLT_F32: return launch_load<CT, RLT_F32>(P, vec, grid, stream);
+    case RLT_F16: return launch_load<CT, RLT_F16>(P, vec, grid, stream);
+    case RLT_BF16: return launch_load<CT, RLT_BF16>(P, vec, grid, stream);
+    default: return RLT_ERR_ARGUMENT;
+  }
+}
+
+}  // namespace
+
+extern "C" int rlt_kv_load(const void* key_cache, const void* value_cache, int64_t k_block_stride,
+                           int64_t k_token_stride, int64_t k_head_stride, int64_t v_block_stride,
+                           int64_t v_token_stride, int64_t v_head_stride, int32_t num_blocks,
+                           int32_t block_size, int32_t kv_dtype, const float* key_scale,
+                           const float* value_scale, int32_t scale_mode, int64_t s_block_stride,
+                           int64_t s_token_stride, int64_t s_head_stride,
+                           const int32_t* block_tables, int64_t table_stride, int32_t table_width,
+                           const int32_t* context_lengths, const int32_t* cu_seqlens,
+                           int32_t num_seqs, int32_t max_len, int64_t rows, int32_t num_kv_heads,
+                           int32_t head_dim, int32_t out_dtype, void* k_out, void* v_out,
+                           hipStream_t stream) {
+  if (rows < 0 || num_seqs < 0 || max_len < 0 || num_kv_heads <= 0 || head_dim <= 0 ||
+      num_blocks <= 0 || block_size <= 0 || table_width < 0 || scale_mode < 0 || scale_mode > 3)
+    return RLT_ERR_ARGUMENT;
+  const bool codes = kv_dtype == RLT_FP8_E4M3 || kv_dtype == RLT_INT8;
+  if (codes != (scale_mode != 0) || (kv_dtype == RLT_INT8 && scale_mode != 3)) return RLT_ERR_ARGUMENT;
+  if (scale_mode && (!key_scale || !value_scale)) return RLT_ERR_ARGUMENT;
+  if (rows == 0 || num_seqs == 0 || max_len == 0) return RLT_OK;
+  if (!key_cache || !value_cache || !context_lengths || !cu_seqlens || !k_out || !v_out ||
+      (table_width && !block_tables))
+    return RLT_ERR_ARGUMENT;
+  // (a workgroup's items are counted in 32 bits)
+  if ((int64_t)2 * num_kv_heads * head_dim * kLoadRows >= ((int64_t)1 << 31)) return RLT_ERR_UNSUPPORTED;
+  LoadParams P;
+  P.k = key_cache;
+  P.v = value_cache;
+  P.k_block = k_block_stride;
+  P.k_token = k_token_stride;
+  P.k_head = k_head_stride;
+  P.v_block = v_block_stride;
+  P.v_token = v_token_stride;
+  P.v_head = v_head_stride;
+  P.ks = scale_mode ? key_scale : nullptr;
+  P.vs = scale_mode ? value_scale : nullptr;
+  P.s_block = scale_mode >= 2 ? s_block_stride : 0;
+  P.s_token = scale_mode == 2 ? s_token_stride : 0;
+  P.s_head = scale_mode >= 2 ? s_head_stride : 0;
+  P.tables = block_tables;
+  P.table_stride = table_stride;
+  P.table_width = table_width;
+  P.num_blocks = num_blocks;
+  P.block_size = block_size;
+  P.lengths = context_lengths;
+  P.cu = cu_seqlens;
+  P.rows = rows;
+  P.num_seqs = num_seqs;
+  P.max_rows = max_len;
+  P.hkv = num_kv_heads;
+  P.head_dim = head_dim;
+  P.k_out = k_out;
+  P.v_out = v_out;
+  const int64_t tiles = ((int64_t)max_len + kLoadRows - 1) / kLoadRows, gx = tiles * num_seqs;
+  if (gx >= ((int64_t)1 << 31)) return RLT_ERR_UNSUPPORTED;
+  P.tiles = (int32_t)tiles;
+  const bool vec = head_dim % 8 == 0;
+  const int64_t per_group = (int64_t)2 * num_kv_heads * ((head_dim + 7) / 8) * kLoadRows;
+  const int64_t most = (per_group + kThreads - 1) / kThreads, want = (kGroupsWanted + gx - 1) / gx;
+  const dim3 grid((unsigned)gx, (unsigned)(want < most ? want : most));
+  switch (kv_dtype) {
+    case RLT_F32: return launch_load_ot<RLT_F32>(P, out_dtype, vec, grid, stream);
+    case RLT_F16: return launch_load_ot<RLT_F16>(P, out_dtype, vec, grid, stream);
+    case RLT_BF16: return launch_load_ot<RLT_BF16>(P, out_dtype, vec, grid, stream);
+    case RLT_FP8_E4M3: return launch_load_ot<RLT_FP8_E4M3>(P, out_dtype, vec, grid, stream);
+    case RLT_INT8: return launch_load_ot<RLT_INT8>(P, out_dtype, vec, grid, stream);
+    default: return RLT_ERR_ARGUMENT;
+  }
+}

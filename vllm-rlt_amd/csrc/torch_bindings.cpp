@@ -47,6 +47,9 @@ int32_t dtype_code(at::ScalarType t) {
   return -1;
 }
 
+// the code of a KV pool's type: int8 too, where the entry point takes pools with block scales
+int32_t pool_code(at::ScalarType t) { return t == at::kChar ? 4 : dtype_code(t); }
+
 Tensor workspace(size_t bytes, const Tensor& like) {
   return at::empty({(int64_t)std::max<size_t>(bytes, 1)},
                    like.options().dtype(at::kByte));
@@ -919,6 +922,240 @@ Tensor tree_masks(const Tensor& parents, const Tensor& cu_seqlens_q, int64_t row
   return mask;
 }
 
+// ---------------------------------------------------------------- rotary positions, appends
+
+bool row_dtype(at::ScalarType t) { return t == at::kFloat || t == at::kHalf || t == at::kBFloat16; }
+
+// rows [rows, heads, head_dim] of a row type with a unit dim stride
+const Tensor& row_tensor(const Tensor& x, const char* name) {
+  TORCH_CHECK_VALUE(x.dim() == 3 && row_dtype(x.scalar_type()), name,
+                    " must be float32, float16 or bfloat16 [rows, heads, head_dim]");
+  TORCH_CHECK_VALUE(x.size(2) <= 1 || x.stride(2) == 1, name, " must have a unit dim stride");
+  return x;
+}
+
+// `out` takes what is made of `x`: its shape and type, no element of it twice, and either x's own
+// memory in x's order or none of it (an element is read and written by one lane only).
+void check_target(const Tensor& x, const Tensor& out, const char* name) {
+  row_tensor(out, name);
+  TORCH_CHECK_VALUE(out.sizes() == x.sizes() && out.scalar_type() == x.scalar_type(), name,
+                    " must have its input's shape and dtype");
+  if (out.numel() == 0) return;
+  const int64_t elt = out.element_size();
+  TORCH_CHECK_VALUE(!pools::overlap((int64_t)1 << 62, {{out.stride(0) * elt, out.size(0)},
+                                                       {out.stride(1) * elt, out.size(1)},
+                                                       {0, 1}},
+                                    out.size(2) * elt),
+                    name, "'s rows must not share memory");
+  const auto range = [&](const Tensor& t) {
+    const uintptr_t at = (uintptr_t)t.data_ptr();
+    int64_t lo = 0, hi = t.size(2) * elt;
+    for (int d = 0; d < 2; ++d) {
+      const int64_t far = t.stride(d) * (t.size(d) - 1) * elt;
+      (far < 0 ? lo : hi) += far;
+    }
+    return std::make_pair(at + lo, at + hi);
+  };
+  const auto a = range(x), b = range(out);
+  const bool apart = a.second <= b.first || b.second <= a.first;
+  const bool same = x.data_ptr() == out.data_ptr() && x.strides() == out.strides();
+  TORCH_CHECK_VALUE(apart || same, name, " must be its input or apart from it");
+}
+
+// turns float64 [rotary_dim / 2]
+int64_t rotary_dim_of(const OptTensor& turns, int64_t head_dim) {
+  if (!turns.has_value()) return 0;
+  need(*turns, at::kDouble, "turns");
+  TORCH_CHECK_VALUE(turns->dim() == 1 && 2 * turns->size(0) <= head_dim,
+                    "the rotary dims must not exceed head_dim (", head_dim, ")");
+  return 2 * turns->size(0);
+}
+
+// Queries and keys turned by their positions (rlt_rotary).
+void rotary(const Tensor& q, const OptTensor& k, const Tensor& positions, const Tensor& turns,
+            double amplitude, bool interleaved, bool inverse, const Tensor& q_out,
+            const OptTensor& k_out) {
+  row_tensor(q, "q");
+  const int64_t rows = q.size(0), head_dim = q.size(2);
+  TORCH_CHECK_VALUE(head_dim >= 1 && head_dim <= 256, "head_dim must be between 1 and 256");
+  TORCH_CHECK_VALUE(k.has_value() == k_out.has_value(), "k and k_out must be given together");
+  same_device(q, k, positions, turns, q_out, k_out);
+  index_of(positions, rows, "positions");
+  const int64_t rot = rotary_dim_of(turns, head_dim);
+  check_target(q, q_out, "q_out");
+  if (k.has_value()) {
+    row_tensor(*k, "k");
+    TORCH_CHECK_VALUE(k->size(0) == rows && k->size(2) == head_dim &&
+                          k->scalar_type() == q.scalar_type(),
+                      "k must have q's rows, head_dim and dtype");
+    check_target(*k, *k_out, "k_out");
+  }
+  const c10::hip::HIPGuardMasqueradingAsCUDA guard(q.device());
+  const int status = rlt_rotary(
+      ptr(q), q.stride(0), q.stride(1), ptr(k), k.has_value() ? k->stride(0) : 0,
+      k.has_value() ? k->stride(1) : 0, (const int64_t*)ptr(positions), rows,
+      (const double*)ptr(turns), (int32_t)rot, (float)amplitude, interleaved ? 1 : 0,
+      inverse ? 1 : 0, (int32_t)q.size(1), k.has_value() ? (int32_t)k->size(1) : 0,
+      (int32_t)head_dim, dtype_code(q.scalar_type()), ptr(q_out), q_out.stride(0), q_out.stride(1),
+      ptr(k_out), k_out.has_value() ? k_out->stride(0) : 0, k_out.has_value() ? k_out->stride(1) : 0,
+      stream_of(q));
+  check_status(status, "rlt_rotary");
+}
+
+// The pools of an append or a load, their scales and the packed sequences.
+struct CacheArgs {
+  int32_t mode = 0;
+  int64_t s_strides[3] = {0, 0, 0};
+};
+CacheArgs check_cache(const Tensor& key_cache, const Tensor& value_cache, const OptTensor& key_scale,
+                      const OptTensor& value_scale, const Tensor& block_tables,
+                      const Tensor& context_lengths, const Tensor& cu_seqlens) {
+  check_view(key_cache, "key_cache");
+  check_view(value_cache, "value_cache");
+  TORCH_CHECK_VALUE(key_cache.strides() == value_cache.strides() &&
+                        key_cache.sizes() == value_cache.sizes() &&
+                        key_cache.scalar_type() == value_cache.scalar_type(),
+                    "key and value pools must share a layout and dtype");
+  TORCH_CHECK_VALUE(key_cache.size(0) >= 1 && key_cache.size(0) <= INT32_MAX &&
+                        key_cache.size(1) >= 1 && key_cache.size(1) <= INT32_MAX &&
+                        key_cache.size(2) >= 1 && key_cache.size(3) >= 1 && key_cache.size(3) <= 256,
+                    "the pools must hold blocks of tokens with head_dim <= 256");
+  TORCH_CHECK_VALUE(key_scale.has_value() == value_scale.has_value(),
+                    "key_scale and value_scale must be given together");
+  const auto type = key_cache.scalar_type();
+  const bool fp8 = type == at::kFloat8_e4m3fn, int8 = type == at::kChar;
+  TORCH_CHECK_VALUE(fp8 || int8 || row_dtype(type),
+                    "the pools must be float32, float16, bfloat16, float8_e4m3fn or int8");
+  TORCH_CHECK_VALUE((fp8 || int8) == key_scale.has_value(),
+                    "8-bit pools need key_scale / value_scale, other pools take none");
+  CacheArgs c;
+  if (key_scale.has_value()) {
+    const Tensor &ks = *key_scale, &vs = *value_scale;
+    TORCH_CHECK_VALUE(ks.scalar_type() == at::kFloat && vs.scalar_type() == at::kFloat,
+                      "scales must be float32");
+    TORCH_CHECK_VALUE(ks.sizes() == vs.sizes() && ks.strides() == vs.strides(),
+                      "key_scale and value_scale must share a layout");
+    const int64_t nb = key_cache.size(0), bs = key_cache.size(1), h = key_cache.size(2);
+    if (ks.dim() == 2) {
+      TORCH_CHECK_VALUE(ks.size(0) == nb && ks.size(1) == h,
+                        "block scales must be [block, kv_head] of the pool");
+      c.mode = 3;
+      c.s_strides[0] = ks.stride(0);
+      c.s_strides[2] = ks.stride(1);
+    } else {
+      TORCH_CHECK_VALUE(!int8, "an int8 pool needs scales [block, kv_head]");
+      TORCH_CHECK_VALUE(ks.dim() == 0 || (ks.dim() == 3 && ks.size(0) == nb && ks.size(1) == bs &&
+                                          ks.size(2) == h),
+                        "scales must be 0-d, [block, token, kv_head] or [block, kv_head]");
+      c.mode = ks.dim() == 0 ? 1 : 2;
+      for (int i = 0; i < ks.dim(); ++i) c.s_strides[i] = ks.stride(i);
+    }
+  }
+  TORCH_CHECK_VALUE(block_tables.dim() == 2 && block_tables.scalar_type() == at::kInt &&
+                        (block_tables.size(1) <= 1 || block_tables.stride(1) == 1),
+                    "block_tables must be int32 [sequences, width] with unit column stride");
+  TORCH_CHECK_VALUE(context_lengths.dim() == 1 && cu_seqlens.dim() == 1 &&
+                        context_lengths.size(0) == block_tables.size(0) &&
+                        cu_seqlens.size(0) == block_tables.size(0) + 1,
+                    "cu_seqlens must be [sequences + 1] and lengths [sequences]");
+  need(context_lengths, at::kInt, "context_lengths");
+  need(cu_seqlens, at::kInt, "cu_seqlens");
+  return c;
+}
+
+// Windows of rows into the paged cache, turned on the way (rlt_kv_append).
+void append_kv(const Tensor& key_cache, const Tensor& value_cache, const Tensor& k, const Tensor& v,
+               const Tensor& block_tables, const Tensor& context_lengths, const Tensor& cu_seqlens_q,
+               int64_t max_seqlen_q, const OptTensor& key_scale, const OptTensor& value_scale,
+               const OptTensor& positions, const OptTensor& turns, double amplitude, bool interleaved,
+               const OptTensor& q, const OptTensor& q_out) {
+  same_device(key_cache, value_cache, k, v, block_tables, context_lengths, cu_seqlens_q, key_scale,
+              value_scale, positions, turns, q, q_out);
+  const CacheArgs c = check_cache(key_cache, value_cache, key_scale, value_scale, block_tables,
+                                  context_lengths, cu_seqlens_q);
+  row_tensor(k, "k");
+  row_tensor(v, "v");
+  const int64_t rows = k.size(0), heads = key_cache.size(2), head_dim = key_cache.size(3);
+  TORCH_CHECK_VALUE(k.sizes() == v.sizes() && k.scalar_type() == v.scalar_type() &&
+                        k.size(1) == heads && k.size(2) == head_dim,
+                    "k, v must be [rows, kv_heads, head_dim] of the pool and share a dtype");
+  TORCH_CHECK_VALUE(c.mode != 0 || k.scalar_type() == key_cache.scalar_type(),
+                    "rows must have the pool's dtype");
+  TORCH_CHECK_VALUE(max_seqlen_q >= 0 && max_seqlen_q <= INT32_MAX, "max_seqlen_q must be nonnegative");
+  TORCH_CHECK_VALUE(heads <= 256, "at most 256 kv heads");
+  // what is written is written once: two pools, blocks, tokens and heads apart
+  const int64_t elt = key_cache.element_size();
+  TORCH_CHECK_VALUE(!pools::overlap((int64_t)((uintptr_t)ptr(value_cache) - (uintptr_t)ptr(key_cache)),
+                                    {{key_cache.stride(0) * elt, key_cache.size(0)},
+                                     {key_cache.stride(1) * elt, key_cache.size(1)},
+                                     {key_cache.stride(2) * elt, heads}},
+                                    head_dim * elt),
+                    "key and value pools must not overlap, nor their blocks, tokens and heads");
+  if (c.mode >= 2)
+    TORCH_CHECK_VALUE(!pools::overlap((int64_t)((uintptr_t)ptr(value_scale) - (uintptr_t)ptr(key_scale)),
+                                      {{c.s_strides[0] * 4, key_cache.size(0)},
+                                       {c.s_strides[1] * 4, c.mode == 2 ? key_cache.size(1) : 1},
+                                       {c.s_strides[2] * 4, heads}},
+                                      4),
+                      "key and value scales must not overlap");
+  if (positions.has_value()) index_of(*positions, rows, "positions");
+  const int64_t rot = rotary_dim_of(turns, head_dim);
+  TORCH_CHECK_VALUE(q.has_value() == q_out.has_value(), "q and q_out must be given together");
+  if (q.has_value()) {
+    row_tensor(*q, "q");
+    TORCH_CHECK_VALUE(q->size(0) == rows && q->size(2) == head_dim &&
+                          q->scalar_type() == k.scalar_type(),
+                      "q must have k's rows, head_dim and dtype");
+    check_target(*q, *q_out, "q_out");
+  }
+  if (rows == 0 || block_tables.size(0) == 0) return;
+  const c10::hip::HIPGuardMasqueradingAsCUDA guard(key_cache.device());
+  const int status = rlt_kv_append(
+      ptr(k), k.stride(0), k.stride(1), ptr(v), v.stride(0), v.stride(1), dtype_code(k.scalar_type()),
+      ptr(key_cache), ptr(value_cache), key_cache.stride(0), key_cache.stride(1), key_cache.stride(2),
+      value_cache.stride(0), value_cache.stride(1), value_cache.stride(2), (int32_t)key_cache.size(0),
+      (int32_t)key_cache.size(1), pool_code(key_cache.scalar_type()), (float*)ptr(key_scale),
+      (float*)ptr(value_scale), c.mode, c.s_strides[0], c.s_strides[1], c.s_strides[2],
+      (const int32_t*)ptr(block_tables), block_tables.stride(0), (int32_t)block_tables.size(1),
+      (const int32_t*)ptr(context_lengths), (const int32_t*)ptr(cu_seqlens_q),
+      (int32_t)block_tables.size(0), (int32_t)max_seqlen_q, rows, (int32_t)heads, (int32_t)head_dim,
+      (const int64_t*)ptr(positions), (const double*)ptr(turns), (int32_t)rot, (float)amplitude,
+      interleaved ? 1 : 0, ptr(q), q.has_value() ? q->stride(0) : 0, q.has_value() ? q->stride(1) : 0,
+      q.has_value() ? (int32_t)q->size(1) : 0, ptr(q_out), q_out.has_value() ? q_out->stride(0) : 0,
+      q_out.has_value() ? q_out->stride(1) : 0, stream_of(key_cache));
+  check_status(status, "rlt_kv_append");
+}
+
+// Cached positions as numbers (rlt_kv_load).
+std::tuple<Tensor, Tensor> load_kv(const Tensor& key_cache, const Tensor& value_cache,
+                                   const Tensor& block_tables, const Tensor& context_lengths,
+                                   const Tensor& cu_seqlens, int64_t max_seqlen, int64_t rows,
+                                   const OptTensor& key_scale, const OptTensor& value_scale,
+                                   at::ScalarType dtype) {
+  same_device(key_cache, value_cache, block_tables, context_lengths, cu_seqlens, key_scale,
+              value_scale);
+  const CacheArgs c = check_cache(key_cache, value_cache, key_scale, value_scale, block_tables,
+                                  context_lengths, cu_seqlens);
+  TORCH_CHECK_VALUE(row_dtype(dtype), "dtype must be float32, float16 or bfloat16");
+  TORCH_CHECK_VALUE(rows >= 0 && max_seqlen >= 0 && max_seqlen <= INT32_MAX,
+                    "rows and max_seqlen must be nonnegative");
+  const c10::hip::HIPGuardMasqueradingAsCUDA guard(key_cache.device());
+  const auto options = block_tables.options().dtype(dtype);
+  Tensor k = at::empty({rows, key_cache.size(2), key_cache.size(3)}, options), v = at::empty_like(k);
+  if (rows == 0 || block_tables.size(0) == 0) return {k, v};
+  const int status = rlt_kv_load(
+      ptr(key_cache), ptr(value_cache), key_cache.stride(0), key_cache.stride(1), key_cache.stride(2),
+      value_cache.stride(0), value_cache.stride(1), value_cache.stride(2), (int32_t)key_cache.size(0),
+      (int32_t)key_cache.size(1), pool_code(key_cache.scalar_type()), (const float*)ptr(key_scale),
+      (const float*)ptr(value_scale), c.mode, c.s_strides[0], c.s_strides[1], c.s_strides[2],
+      (const int32_t*)ptr(block_tables), block_tables.stride(0), (int32_t)block_tables.size(1),
+      (const int32_t*)ptr(context_lengths), (const int32_t*)ptr(cu_seqlens),
+      (int32_t)block_tables.size(0), (int32_t)max_seqlen, rows, (int32_t)key_cache.size(2),
+      (int32_t)key_cache.size(3), dtype_code(dtype), ptr(k), ptr(v), stream_of(key_cache));
+  check_status(status, "rlt_kv_load");
+  return {k, v};
+}
+
 }  // namespace
 
 TORCH_LIBRARY(rlt_mi355x, m) {
@@ -956,6 +1193,16 @@ TORCH_LIBRARY(rlt_mi355x, m) {
         "-> (Tensor, Tensor, Tensor, Tensor, Tensor)");
   m.def("commit_tree_kv(Tensor(a!) key_pool, Tensor(b!) value_pool, Tensor tables, Tensor starts, "
         "Tensor path, Tensor accepted, int block_size) -> ()");
+  m.def("rotary(Tensor q, Tensor? k, Tensor positions, Tensor turns, float amplitude, "
+        "bool interleaved, bool inverse, Tensor(a!) q_out, Tensor(b!)? k_out) -> ()");
+  m.def("append_kv(Tensor(a!) key_cache, Tensor(b!) value_cache, Tensor k, Tensor v, "
+        "Tensor block_tables, Tensor context_lengths, Tensor cu_seqlens_q, int max_seqlen_q, "
+        "Tensor(c!)? key_scale=None, Tensor(d!)? value_scale=None, Tensor? positions=None, "
+        "Tensor? turns=None, float amplitude=1.0, bool interleaved=False, Tensor? q=None, "
+        "Tensor(e!)? q_out=None) -> ()");
+  m.def("load_kv(Tensor key_cache, Tensor value_cache, Tensor block_tables, "
+        "Tensor context_lengths, Tensor cu_seqlens, int max_seqlen, int rows, "
+        "Tensor? key_scale, Tensor? value_scale, ScalarType dtype) -> (Tensor, Tensor)");
 }
 
 TORCH_LIBRARY_IMPL(rlt_mi355x, CUDA, m) {
@@ -974,4 +1221,7 @@ TORCH_LIBRARY_IMPL(rlt_mi355x, CUDA, m) {
   m.impl("tree_accept", &tree_accept);
   m.impl("token_logprobs", &token_logprobs);
   m.impl("commit_tree_kv", &commit_tree_kv);
+  m.impl("rotary", &rotary);
+  m.impl("append_kv", &append_kv);
+  m.impl("load_kv", &load_kv);
 }

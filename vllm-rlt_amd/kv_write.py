@@ -9,8 +9,10 @@ Same arguments and semantics as
 * vllm_rlt/kernels/routing.py:147-180 ``finalize_kernel`` (``finalize_rows`` here, the
   LAST_EXITED copy into deeper planes),
 plus ``store_kv``, the unmasked index-put writer
-(vllm_rlt/core/kv_cache_manager.py:893-895), and ``commit_tree_kv``, which moves the accepted
-path of a draft tree behind the prefix (the reference's drafts are chains).  Every call
+(vllm_rlt/core/kv_cache_manager.py:893-895), ``commit_tree_kv``, which moves the accepted
+path of a draft tree behind the prefix (the reference's drafts are chains), ``append_kv``, which
+writes windows of rows with the rotary positions applied on the way and holds 8-bit pools over
+scales per tensor, vector or block, and ``load_kv``, which reads a cache back as numbers.  Every call
 enqueues one gfx950 launch on the current stream without host synchronization.  Rows whose block or offset lies
 outside the pool are skipped (the reference's kernels would write out of bounds).
 """
@@ -193,3 +195,79 @@ def commit_tree_kv(key_pool, value_pool, tables, starts, path, accepted, block_s
     _lib.ops().commit_tree_kv(key_pool, value_pool, tables.contiguous(),
                               _index(starts, n, "starts"), path.contiguous(),
                               _index(accepted, n, "accepted"), int(block_size))
+
+
+def _packed(block_tables, context_lengths, cu_seqlens):
+    tables = block_tables if block_tables.dtype == torch.int32 else block_tables.to(torch.int32)
+    tables = tables if tables.ndim != 2 or tables.stride(1) == 1 else tables.contiguous()
+    return (tables, *(x.to(torch.int32).contiguous() for x in (context_lengths, cu_seqlens)))
+
+
+def append_kv(key_cache, value_cache, k, v, block_tables, context_lengths, cu_seqlens_q,
+              max_seqlen_q, key_scale=None, value_scale=None, *, rotary=None, positions=None,
+              q=None, inplace=False):
+    """Append windows of keys and values ``[rows, kv_heads, head_dim]`` to the paged cache, keys
+    (and queries) turned by their positions on the way, in one launch.  Returns the turned
+    ``q``, or None without one.
+
+    Sequence s owns rows ``cu_seqlens_q[s]`` to ``cu_seqlens_q[s + 1] - 1`` (at most
+    ``max_seqlen_q``), which become its last positions: row i goes to position
+    ``context_lengths[s] - rows + i`` of ``block_tables[s]``, as ``prefill`` reads them.
+    ``rotary`` (``Rotary``; None: no rotation) turns k and ``q`` ``[rows, heads, head_dim]`` by
+    that position, or by ``positions`` (``[rows]``) where they differ, as a tree's nodes do;
+    ``inplace`` turns q itself.  Rows before position 0, past the table or whose block lies
+    outside the pool are not written (their q is turned).
+
+    Pools ``[block, token, kv_head, dim]`` of the rows' type, or 8-bit ones with float32 scales:
+
+    * float8_e4m3fn with 0-d scales (read) or with scales ``[block, token, kv_head]`` (written):
+      codes and scales as ``store_fp8``'s of the turned rows in float32;
+    * float8_e4m3fn or int8 with one scale per block and head, ``[block, kv_head]`` (written):
+      ``amax / M`` of the call's rows in the block (M = 448, int8 127; at least the smallest
+      normal float; values that are not finite do not count, infinities clamp, int8 takes NaN
+      as 0).  Where rows go on in a block that already holds tokens, the larger of that and the
+      block's scale; if it grew, the earlier tokens' codes are quantized again over the new
+      scale.  Rows at a block's first token begin it anew.  A block must be written by one
+      sequence of a call only.
+
+    Runs ``torch.ops.rlt_mi355x.append_kv``.
+    """
+    from .rotary import _heads, _positions, _target
+
+    _lib.require_gpu(key_cache, value_cache, k, v, block_tables, context_lengths, cu_seqlens_q,
+                     key_scale, value_scale, positions, q)
+    k, v = _rows(k, "k"), _rows(v, "v")
+    q_out = None
+    if q is not None:
+        q_out = _target(q, True, "q") if inplace else None
+        q = _heads(q, "q")
+        q_out = _target(q, False, "q") if q_out is None else q_out
+    if positions is not None:
+        positions = _positions(positions, k.shape[0])
+    tables, lengths, cu = _packed(block_tables, context_lengths, cu_seqlens_q)
+    _lib.ops().append_kv(key_cache, value_cache, k, v, tables, lengths, cu, int(max_seqlen_q),
+                         key_scale, value_scale, positions,
+                         None if rotary is None else rotary.turns,
+                         1.0 if rotary is None else rotary.amplitude,
+                         False if rotary is None else rotary.interleaved, q, q_out)
+    return q_out
+
+
+def load_kv(key_cache, value_cache, block_tables, context_lengths, cu_seqlens, max_seqlen, rows,
+            key_scale=None, value_scale=None, *, dtype=None):
+    """The keys and values of cached positions as numbers, ``[rows, kv_heads, head_dim]`` each:
+    what ``append_kv`` wrote, code times scale, rounded once to ``dtype`` (the pool's; bfloat16
+    for 8-bit pools).
+
+    Rows ``cu_seqlens[s]`` to ``cu_seqlens[s + 1] - 1`` (at most ``max_seqlen``) are the last
+    positions of sequence s, ``context_lengths[s] - n`` on; ``rows`` is their total.  Positions
+    before 0, past the table or in blocks outside the pool give zeros; rows of no sequence are
+    undefined.  Pools and scales as ``append_kv``'s.  Runs ``torch.ops.rlt_mi355x.load_kv``.
+    """
+    _lib.require_gpu(key_cache, value_cache, block_tables, context_lengths, cu_seqlens, key_scale,
+                     value_scale)
+    if dtype is None:
+        dtype = key_cache.dtype if key_cache.dtype in _ROW_DTYPES else torch.bfloat16
+    tables, lengths, cu = _packed(block_tables, context_lengths, cu_seqlens)
+    return _lib.ops().load_kv(key_cache, value_cache, tables, lengths, cu, int(max_seqlen),
+                              int(rows), key_scale, value_scale, dtype)
