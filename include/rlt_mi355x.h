@@ -72,6 +72,9 @@ int rlt_abi_version(void);
  * Scales (FP8 pools): scale_mode 0 none, 1 per-tensor (key_scale / value_scale
  * point at one float), 2 per-vector pools [block, token, kv_head] with the given
  * strides (vllm_rlt/core/kv_cache_manager.py:267-271, :936-942).
+ * scale_mode 3: one scale per block and kv head, [block, kv_head] (s_token_stride is not
+ * read), for RLT_FP8_E4M3 and RLT_INT8 pools as rlt_kv_append writes them (the only mode of
+ * RLT_INT8; no counterpart in the reference; not in the store and tree entry points).
  * The grid is static (independent of lengths): safe under HIP graph capture.
  */
 size_t rlt_paged_attention_workspace_size(int32_t num_q_rows, int32_t num_q_heads, int32_t head_dim,

@@ -106,6 +106,12 @@ class MI355XPagedAttention:
     q on pools whose block size is a multiple of 16; packed calls then stay on the
     verify kernels at every window length (rows equal per-row rows bit for bit).  ``tree``
     takes it at any block size.
+
+    Pools: q's type; float8_e4m3fn with 0-d scales (per tensor) or scales ``[block, token,
+    kv_head]`` (per vector); float8_e4m3fn or int8 with one scale per block of tokens and kv
+    head, ``[block, kv_head]``, as ``kv_write.append_kv`` writes them (not ``tree``).  With
+    float16 q the value scales of the blocks that a row reads may differ by a factor of 2^20
+    before weights lose bits.
     """
 
     generation = None
@@ -169,7 +175,8 @@ class MI355XPagedAttention:
         scales written into the ``[block, token, kv_head]`` scale views.  Verify windows on
         the MFMA kernels run as one launch pair (the attention waves that read a window
         position store it first); other 16-bit shapes store with ``store_kv`` and attend
-        separately.  Returns the attention output.
+        separately, and so do pools with block scales (``append_kv``; no ``row_lengths``).
+        Returns the attention output.
         """
         _lib.require_gpu(q, k_new, v_new, key_cache, value_cache, block_tables, context_lengths,
                          cu_seqlens_q, key_scale, value_scale, row_lengths)

@@ -86,6 +86,11 @@ __device__ __forceinline__ float load_as_f32<RLT_FP8_E4M3>(const void* base, int
   return fp8x2_to_f32<false>(b).x;
 }
 
+template <>
+__device__ __forceinline__ float load_as_f32<RLT_INT8>(const void* base, int64_t i) {
+  return (float)((const int8_t*)base)[i];
+}
+
 template <int DT>
 __device__ __forceinline__ void store_from_f32(void* base, int64_t i, float v);
 template <>

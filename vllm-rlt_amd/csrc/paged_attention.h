@@ -81,7 +81,7 @@ struct AttnParams {
   const float* k_scale;
   const float* v_scale;
   int64_t s_block_stride, s_token_stride, s_head_stride;
-  int32_t scale_mode;  // 0 none, 1 per-tensor (0-d), 2 per-vector [blk, tok, kvh]
+  int32_t scale_mode;  // 0 none, 1 per-tensor (0-d), 2 per-vector [blk, tok, kvh], 3 per block [blk, kvh]
   int32_t compensate;  // MFMA path: P V also with the bits P loses in its 16-bit cast
   int32_t num_seqs;
   int32_t num_rows;  // total q rows
@@ -128,6 +128,8 @@ constexpr int unit_split() { return KVT == QT ? 2 : 1; }
 template <int QT, int KVT>
 constexpr int unit_chunk() { return KVT == QT ? kChunk : 2 * kChunk; }
 constexpr float kLog2e = 1.4426950408889634f;
+template <int QT>
+constexpr int kBlockLift = QT == RLT_F16 ? 15 : 0;
 
 
 struct SeqView {
@@ -303,10 +305,29 @@ __device__ __forceinline__ uint32_t fp8x2_to_16(uint32_t w) {
     return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.f, kHigh));
   return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.f, kHigh));
 }
-// Four codes -> four values.
+// Four int8 codes -> four packed 16-bit values, exactly (8 bits fit bf16's significand): a
+// byte's float has nothing below its upper half; fp16 takes the byte with its sign bit flipped
+// as the low bits of 1024 + u and 1152 off.
 template <int QT>
-__device__ __forceinline__ uint2 fp8x4_to_16(uint32_t w) {
-  return make_uint2(fp8x2_to_16<QT, false>(w), fp8x2_to_16<QT, true>(w));
+__device__ __forceinline__ uint2 int8x4_to_16(uint32_t w) {
+  if constexpr (QT == RLT_BF16) {
+    const uint32_t f0 = __float_as_uint((float)(int8_t)w), f1 = __float_as_uint((float)(int8_t)(w >> 8));
+    const uint32_t f2 = __float_as_uint((float)(int8_t)(w >> 16)), f3 = __float_as_uint((float)(int8_t)(w >> 24));
+    return make_uint2(__builtin_amdgcn_perm(f1, f0, 0x07060302u), __builtin_amdgcn_perm(f3, f2, 0x07060302u));
+  } else {
+    typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+    const f16x2 off = {(_Float16)1152.f, (_Float16)1152.f};
+    const uint32_t u = w ^ 0x80808080u;
+    const f16x2 a = __builtin_bit_cast(f16x2, __builtin_amdgcn_perm(0x64646464u, u, 0x04010400u)) - off;
+    const f16x2 b = __builtin_bit_cast(f16x2, __builtin_amdgcn_perm(0x64646464u, u, 0x04030402u)) - off;
+    return make_uint2(__builtin_bit_cast(uint32_t, a), __builtin_bit_cast(uint32_t, b));
+  }
+}
+// Four codes -> four values.
+template <int QT, int KVT>
+__device__ __forceinline__ uint2 codes_to_16(uint32_t w) {
+  if constexpr (KVT == RLT_INT8) return int8x4_to_16<QT>(w);
+  else return make_uint2(fp8x2_to_16<QT, false>(w), fp8x2_to_16<QT, true>(w));
 }
 
 // One lane's raw key elements, as loaded from HBM: for contraction step s the
@@ -359,8 +380,8 @@ struct RawSlice {
     if (KVT == QT) {
       r = make_uint4(w[4 * s], w[4 * s + 1], w[4 * s + 2], w[4 * s + 3]);
     } else {
-      const uint2 a = fp8x4_to_16<QT>(w[2 * s]);
-      const uint2 b = fp8x4_to_16<QT>(w[2 * s + 1]);
+      const uint2 a = codes_to_16<QT, KVT>(w[2 * s]);
+      const uint2 b = codes_to_16<QT, KVT>(w[2 * s + 1]);
       r = make_uint4(a.x, a.y, b.x, b.y);
     }
     return r;
@@ -416,6 +437,13 @@ struct ValueQuad {
       a1.x = __builtin_amdgcn_perm(w[1][K], w[0][K], 0x07060302u);
       a0.y = __builtin_amdgcn_perm(w[3][K], w[2][K], 0x05040100u);
       a1.y = __builtin_amdgcn_perm(w[3][K], w[2][K], 0x07060302u);
+    } else if constexpr (KVT == RLT_INT8) {
+      // the bytes of dim 2k of the four positions, and those of dim 2k + 1
+      constexpr int W = kHalfWords ? K : K / 2;
+      constexpr uint32_t sel = kHalfWords || (K & 1) == 0 ? 0x05010400u : 0x07030602u;
+      const uint32_t x = __builtin_amdgcn_perm(w[1][W], w[0][W], sel), y = __builtin_amdgcn_perm(w[3][W], w[2][W], sel);
+      a0 = int8x4_to_16<QT>(__builtin_amdgcn_perm(y, x, 0x05040100u));
+      a1 = int8x4_to_16<QT>(__builtin_amdgcn_perm(y, x, 0x07060302u));
     } else {
       // dims 2k and 2k + 1 of each position widened (exact for e4m3), then as above
       uint32_t f[4];
@@ -594,8 +622,14 @@ __device__ __forceinline__ bool store_window(const AttnParams& P, int seq, int k
 // row-group, kv head, chunk) -- on one wave: the wave streams the kv head over
 // positions [512c + part * 512 / KS, + 512 / KS) for every row of the row-group.
 // tbl_lds: this wave's 512-entry LDS slice for the chunk's block ids.
-// SM: FP8 scale mode (0 none, 1 per-tensor, 2 per-vector).  UB: block_size is a
-// multiple of 16, so the 16 positions of a tile share one block.
+// SM: scale mode (0 none, 1 per-tensor, 2 per-vector, 3 per block).  UB: block_size is a
+// multiple of 16, so the 16 positions of a tile share one block.  With block scales a lane
+// holds the two scales of one tile of the span, loaded once ahead of the tiles: a tile takes
+// its own by a lane read into scalar registers (a load per tile and head less, and no
+// exchange between lanes).  The key scale goes into the scores, the value scale into the
+// weights of the product, over a power of two near the span's largest (and 2^kBlockLift above
+// it for fp16, whose normal numbers end at 2^-14), which the output takes back: exact, so a
+// weight is rounded as without it.
 template <int QT, int KVT, int D, int NT, int SM, bool UB, bool CP>
 __device__ __forceinline__ void attend_span(const AttnParams& P, int seq, int rg, int kvh, int chunk,
                                             int part, int32_t* tbl_lds,
@@ -608,6 +642,7 @@ __device__ __forceinline__ void attend_span(const AttnParams& P, int seq, int rg
   constexpr int KV_ELT = KVT == QT ? 2 : 1;
   constexpr int CH = unit_chunk<QT, KVT>();
   constexpr int kSpan = CH / unit_split<QT, KVT>();
+  static_assert(SM != 3 || (UB && KVT != QT && kSpan <= 64 * kTileTok), "a lane per tile's scales");
   const int lane = threadIdx.x & 63;
   const int l16 = lane & 15;
   const int grp = lane >> 4;
@@ -696,7 +731,18 @@ __device__ __forceinline__ void attend_span(const AttnParams& P, int seq, int rg
     st.v_mul = P.v_scale[0];
   }
 
-  if (P.new_k && t0 < t1) {
+  float k_tile = 0.f, v_tile = 0.f;  // SM 3: the scales of the span's tile `lane`
+  if constexpr (SM == 3) {
+    if (t0 < t1) {
+      const int tile = min(max(lane, t0), t1 - 1);
+      const int64_t so = (int64_t)tbl_lds[w_begin - c_begin + tile * kTileTok] * P.s_block_stride +
+                         (int64_t)kvh * P.s_head_stride;
+      k_tile = P.k_scale[so];
+      v_tile = P.v_scale[so];
+    }
+  }
+
+  if (SM != 3 && P.new_k && t0 < t1) {
     // The window rows' own keys and values, stored through the block table before any
     // tile of this span is read; the wait makes this wave's stores visible to its own
     // loads.
@@ -779,6 +825,18 @@ __device__ __forceinline__ void attend_span(const AttnParams& P, int seq, int rg
     auto scale_of = [&](float x, int b, int r) {
       return __int_as_float(__builtin_amdgcn_ds_bpermute(16 * grp + 64 * b + 4 * r, __float_as_int(x)));
     };
+    if constexpr (SM == 3) {
+      float most = fabsf(v_tile);
+#pragma unroll
+      for (int o = 32; o >= 1; o >>= 1) most = fmaxf(most, __shfl_xor(most, o, RLT_WAVE));
+      // (no scale above 0: the weights are 0 whatever the power)
+      const int e = most > 0.f ? __builtin_amdgcn_frexp_expf(most) : 0;
+      v_tile = __builtin_amdgcn_ldexpf(v_tile, kBlockLift<QT> - e);
+      st.v_mul = __builtin_amdgcn_ldexpf(1.f, e - kBlockLift<QT>);
+    }
+    auto tile_scale = [&](float x, int t) {
+      return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), min(t, tl)));
+    };
     // Wave-uniform fast-path bound: a pair inside [lo of the last row, hi of the
     // first row) is visible to every row of the row-group and fully stored, so
     // it needs no position masks.  (Branches around the masks: two copies of the whole
@@ -832,11 +890,13 @@ __device__ __forceinline__ void attend_span(const AttnParams& P, int seq, int rg
       bool rescale[2] = {false, false};
       float corr[2][NT];
 #pragma unroll
-      for (int b = 0; b < 2; ++b)
+      for (int b = 0; b < 2; ++b) {
+        const float f = SM == 3 ? qk_scale * tile_scale(k_tile, t + b) : qk_scale;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-          for (int r = 0; r < 4; ++r) sc[b][nt][r] *= qk_scale;
+          for (int r = 0; r < 4; ++r) sc[b][nt][r] *= f;
+      }
       if (!full) {
 #pragma unroll
         for (int b = 0; b < 2; ++b)
@@ -875,6 +935,11 @@ __device__ __forceinline__ void attend_span(const AttnParams& P, int seq, int rg
           if (SM == 2) {
 #pragma unroll
             for (int r = 0; r < 4; ++r) pr[b][r] *= vsc[b][r];
+          }
+          if (SM == 3) {
+            const float f = tile_scale(v_tile, t + b);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) pr[b][r] *= f;
           }
           pop[b][nt] = make_uint2(M::pack2(pr[b][0], pr[b][1]), M::pack2(pr[b][2], pr[b][3]));
           if (CP) {

@@ -1,7 +1,7 @@
 // Entry points of the paged attention: the vector path, the merge of a row's chunks, the window
 // store ahead of the prefill tiling, and the dispatch.  The tilings are in paged_attention.h.
 
-#include "paged_attention.h"
+#include "block_attention.h"
 
 namespace {
 
@@ -474,17 +474,20 @@ __global__ __launch_bounds__(kStoreThreads) void rlt_window_store_kernel(AttnPar
 
 // ============================================================ dispatch
 
-// UB: blocks hold whole 16-position tiles and a lane's offset within a tile fits 32 bits.
-// Compensated P V is built for such block sizes only (the reference pools' block size 16
+// Blocks hold whole 16-position tiles and a lane's offset within a tile fits 32 bits.
+bool whole_tiles(const AttnParams& P) {
+  const int64_t most = (int64_t)1 << 26;
+  return P.block_size % kTileTok == 0 && P.k_token_stride >= 0 && P.k_token_stride < most &&
+         P.v_token_stride >= 0 && P.v_token_stride < most;
+}
+
+// UB: whole_tiles.  Compensated P V is built for such block sizes only (the reference pools' block size 16
 // and its multiples).
 template <int QT, int KVT, int D, int SM>
 int launch_mfma_sm(const AttnParams& P, dim3 grid, int nt, hipStream_t stream) {
-  const bool whole = P.block_size % kTileTok == 0;
-  const int64_t most = (int64_t)1 << 26;
-  const bool ub = whole && P.k_token_stride >= 0 && P.k_token_stride < most &&
-                  P.v_token_stride >= 0 && P.v_token_stride < most;
+  const bool ub = whole_tiles(P);
   if (P.compensate) {
-    if (!whole) return RLT_ERR_UNSUPPORTED;
+    if (P.block_size % kTileTok != 0) return RLT_ERR_UNSUPPORTED;
     if (ub) return launch_mfma_ub<QT, KVT, D, SM, true, true>(P, grid, nt, stream);
     return launch_mfma_ub<QT, KVT, D, SM, false, true>(P, grid, nt, stream);
   }
@@ -523,6 +526,7 @@ int launch_vec_q(const AttnParams& P, int kv_dtype, dim3 grid, hipStream_t strea
     case RLT_F16: rlt_attn_vec_kernel<QT, RLT_F16><<<grid, 256, 0, stream>>>(P); break;
     case RLT_BF16: rlt_attn_vec_kernel<QT, RLT_BF16><<<grid, 256, 0, stream>>>(P); break;
     case RLT_FP8_E4M3: rlt_attn_vec_kernel<QT, RLT_FP8_E4M3><<<grid, 256, 0, stream>>>(P); break;
+    case RLT_INT8: rlt_attn_vec_kernel<QT, RLT_INT8><<<grid, 256, 0, stream>>>(P); break;
     default: return RLT_ERR_ARGUMENT;
   }
   return RLT_OK;
@@ -538,10 +542,7 @@ void launch_prefill_sm(const AttnParams& P, dim3 grid, int max_q, hipStream_t st
           <<<(unsigned)(wgs - at < kStoreGrid ? wgs - at : kStoreGrid), kStoreThreads, 0, stream>>>(
               P, (uint32_t)per_seq, (uint32_t)at);
   }
-  // blocks of whole 16-position groups, and lane offsets within a group that fit 32 bits
-  const int64_t most = (int64_t)1 << 26;
-  if (P.block_size % 16 == 0 && P.k_token_stride >= 0 && P.k_token_stride < most &&
-      P.v_token_stride >= 0 && P.v_token_stride < most)
+  if (whole_tiles(P))
     rlt_prefill_kernel<QT, KVT, D, SM, true><<<grid, kPfThreads, 0, stream>>>(P);
   else
     rlt_prefill_kernel<QT, KVT, D, SM, false><<<grid, kPfThreads, 0, stream>>>(P);
@@ -598,7 +599,7 @@ int rlt_abi_version(void) { return RLT_MI355X_ABI_VERSION; }
 
 int rlt_paged_attention_uses_mfma(int32_t q_dtype, int32_t kv_dtype, int32_t head_dim) {
   const bool qok = q_dtype == RLT_BF16 || q_dtype == RLT_F16;
-  const bool kvok = kv_dtype == q_dtype || kv_dtype == RLT_FP8_E4M3;
+  const bool kvok = kv_dtype == q_dtype || kv_dtype == RLT_FP8_E4M3 || kv_dtype == RLT_INT8;
   return qok && kvok && mfma_head_dim(head_dim);
 }
 
@@ -641,10 +642,14 @@ int attention_impl(const void* q, int64_t q_row_stride, int64_t q_head_stride,
   if (num_q_heads <= 0 || num_kv_heads <= 0 || num_q_heads % num_kv_heads) return RLT_ERR_ARGUMENT;
   if (head_dim <= 0 || head_dim > 256 || block_size <= 0 || window < 0) return RLT_ERR_ARGUMENT;
   if (num_seqs < 0 || num_q_rows < 0 || max_q_len < 0 || table_width < 0) return RLT_ERR_ARGUMENT;
-  if (scale_mode < 0 || scale_mode > 2 || (scale_mode && (!key_scale || !value_scale)))
+  if (scale_mode < 0 || scale_mode > 3 || (scale_mode && (!key_scale || !value_scale)))
     return RLT_ERR_ARGUMENT;
   if (kv_dtype == RLT_FP8_E4M3 && scale_mode == 0) return RLT_ERR_ARGUMENT;
-  if (q_dtype == RLT_FP8_E4M3) return RLT_ERR_ARGUMENT;
+  // block scales: 8-bit pools, and all that int8 pools take
+  if (scale_mode == 3 ? kv_dtype != RLT_FP8_E4M3 && kv_dtype != RLT_INT8 : kv_dtype == RLT_INT8)
+    return RLT_ERR_ARGUMENT;
+  if (q_dtype == RLT_FP8_E4M3 || q_dtype == RLT_INT8) return RLT_ERR_ARGUMENT;
+  if (scale_mode == 3 && store) return RLT_ERR_UNSUPPORTED;  // rlt_kv_append, then the attention
   if (flags & ~RLT_ATTN_COMPENSATE) return RLT_ERR_ARGUMENT;
   if (num_blocks <= 0) return RLT_ERR_ARGUMENT;
   if (num_q_rows == 0 || num_seqs == 0) return RLT_OK;
@@ -677,7 +682,7 @@ int attention_impl(const void* q, int64_t q_row_stride, int64_t q_head_stride,
   P.k_scale = key_scale;
   P.v_scale = value_scale;
   P.s_block_stride = s_block_stride;
-  P.s_token_stride = s_token_stride;
+  P.s_token_stride = scale_mode == 3 ? 0 : s_token_stride;
   P.s_head_stride = s_head_stride;
   P.scale_mode = scale_mode;
   P.compensate = (flags & RLT_ATTN_COMPENSATE) ? 1 : 0;
@@ -689,10 +694,11 @@ int attention_impl(const void* q, int64_t q_row_stride, int64_t q_head_stride,
   P.head_dim = head_dim;
   P.block_size = block_size;
   P.window = window;
-  // chunk size: 1024 for fp8 KV on the MFMA path (unit_chunk), 512 otherwise; the
+  // chunk size: 1024 for 8-bit KV on the MFMA path (unit_chunk), 512 otherwise; the
   // workspace query sizes the partials for 512, an upper bound
-  const bool fp8_mfma = kv_dtype == RLT_FP8_E4M3 && rlt_paged_attention_uses_mfma(q_dtype, kv_dtype, head_dim);
-  P.chunk_log2 = fp8_mfma ? 10 : 9;
+  const bool code8 = kv_dtype == RLT_FP8_E4M3 || kv_dtype == RLT_INT8;
+  const bool code8_mfma = code8 && rlt_paged_attention_uses_mfma(q_dtype, kv_dtype, head_dim);
+  P.chunk_log2 = code8_mfma ? 10 : 9;
   P.max_chunks = max_chunks_for(table_width, block_size, 1 << P.chunk_log2);
   P.qk_scale_log2 = kLog2e / sqrtf((float)head_dim);
   P.out = out;
@@ -730,9 +736,9 @@ int attention_impl(const void* q, int64_t q_row_stride, int64_t q_head_stride,
   int st = RLT_OK;
   if (mfma) {
     // 16-byte vector loads of q and of every lane's KV slice.
-    const int64_t kv_elt = kv_dtype == RLT_FP8_E4M3 ? 1 : 2;
-    // (fp8 keys with head_dim % 64 == 0 are read 16 bytes per lane: RawSlice::kWide)
-    const int64_t kv_align = kv_dtype == RLT_FP8_E4M3 && head_dim % 64 != 0 ? 8 : 16;
+    const int64_t kv_elt = code8 ? 1 : 2;
+    // (8-bit keys with head_dim % 64 == 0 are read 16 bytes per lane: RawSlice::kWide)
+    const int64_t kv_align = code8 && head_dim % 64 != 0 ? 8 : 16;
     const bool aligned =
         ((uintptr_t)q % 16 == 0) && (q_row_stride * 2) % 16 == 0 && (q_head_stride * 2) % 16 == 0 &&
         ((uintptr_t)key_cache % 16 == 0) && ((uintptr_t)value_cache % 16 == 0) &&
@@ -754,7 +760,10 @@ int attention_impl(const void* q, int64_t q_row_stride, int64_t q_head_stride,
       const int64_t swgs = (int64_t)num_seqs * num_kv_heads * (((int64_t)max_q_len + 63) / 64);
       if (swgs >= ((int64_t)1 << 31)) return RLT_ERR_UNSUPPORTED;
       const bool fp8 = kv_dtype == RLT_FP8_E4M3;
-      if (q_dtype == RLT_BF16) {
+      if (scale_mode == 3) {
+        if (fp8) rlt_attn::launch_block_prefill_fp8(P, q_dtype, grid, whole_tiles(P), stream);
+        else rlt_attn::launch_block_prefill_int8(P, q_dtype, grid, whole_tiles(P), stream);
+      } else if (q_dtype == RLT_BF16) {
         if (fp8) launch_prefill<RLT_BF16, RLT_FP8_E4M3>(P, head_dim, grid, max_q_len, stream);
         else launch_prefill<RLT_BF16, RLT_BF16>(P, head_dim, grid, max_q_len, stream);
       } else {
@@ -779,18 +788,23 @@ int attention_impl(const void* q, int64_t q_row_stride, int64_t q_head_stride,
     const bool long_store = store && kv_dtype == RLT_FP8_E4M3 && max_q_len >= 32;
     P.shared_lines = num_kv_heads > 1 && !long_store &&
                      ((k_head_stride * kv_elt) % 128 != 0 || (v_head_stride * kv_elt) % 128 != 0 ||
-                      (scale_mode == 2 && s_head_stride * 4 < 128));
+                      (scale_mode >= 2 && s_head_stride * 4 < 128));
     int64_t wgs = (int64_t)num_seqs * P.rowgroups * num_kv_heads * P.max_chunks;
     if (P.persistent) wgs = compute_units();
     if (wgs >= ((int64_t)1 << 31)) return RLT_ERR_UNSUPPORTED;
     dim3 grid((unsigned)wgs);
-    if (q_dtype == RLT_BF16)
+    if (kv_dtype == RLT_INT8)
+      st = rlt_attn::launch_block_int8(P, q_dtype, grid, nt, whole_tiles(P), stream);
+    else if (scale_mode == 3 && whole_tiles(P))
+      st = rlt_attn::launch_block_fp8(P, q_dtype, grid, nt, stream);
+    else if (q_dtype == RLT_BF16)
       st = kv_dtype == RLT_BF16 ? launch_mfma<RLT_BF16, RLT_BF16>(P, grid, nt, stream)
                                 : launch_mfma<RLT_BF16, RLT_FP8_E4M3>(P, grid, nt, stream);
     else
       st = kv_dtype == RLT_F16 ? launch_mfma<RLT_F16, RLT_F16>(P, grid, nt, stream)
                                : launch_mfma<RLT_F16, RLT_FP8_E4M3>(P, grid, nt, stream);
   } else {
+    if (scale_mode == 3) P.scale_mode = 2;  // (token stride 0)
     P.rows_per_rg = kVecRows;
     P.rowgroups = (rows_per_seq + kVecRows - 1) / kVecRows;
     if (P.rowgroups < 1) P.rowgroups = 1;

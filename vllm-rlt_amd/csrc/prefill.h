@@ -159,8 +159,14 @@ __global__ __launch_bounds__(kPfThreads, 2) void rlt_prefill_kernel(AttnParams P
   constexpr int LD = kPfKeys / ROWS_PER_LD / kPfWaves;  // direct loads per wave per tile (K, V each)
   static_assert(LD * ROWS_PER_LD == 16, "a wave's direct loads fill one 16-position group");
   constexpr bool FP8 = KVT != QT;
-  static_assert(!FP8 || KVT == RLT_FP8_E4M3, "16-bit pools match q");
-  static_assert(FP8 == (SM != 0), "scale modes are for fp8 pools");
+  static_assert(!FP8 || KVT == RLT_FP8_E4M3 || KVT == RLT_INT8, "16-bit pools match q");
+  static_assert(FP8 == (SM != 0), "scale modes are for 8-bit pools");
+  // fp16 has few exponents: there the weights times block scales are held over a power of two near
+  // the largest scale that the rows see, kLift above their place, and the running max follows
+  // closer (weights up to 2^kLazy), so that scales down to 2^-20 of the largest keep their bits
+  constexpr bool REFER = SM == 3 && QT == RLT_F16;
+  constexpr float kLazy = REFER ? 1.f : kPfLazy;
+  constexpr int kLift = 15 - (int)kLazy;
   constexpr int FJ = kPfKeys * SLOTS / kPfThreads;  // fp8 LDS slots per thread per tile (K, V each)
   static_assert(FJ * kPfThreads == kPfKeys * SLOTS, "the threads' fp8 slots cover a tile");
   // operand reads in flight ahead of their MFMAs: S^T slices, O^T steps (fp8 tiles leave
@@ -259,7 +265,7 @@ __global__ __launch_bounds__(kPfThreads, 2) void rlt_prefill_kernel(AttnParams P
   int kblk[CUR] = {}, koff[CUR] = {};
   // per-vector scales: wave 0 stages the keys' (with the K tile), wave 1 the values'
   TileCursor scur;
-  const bool scale_wave = SM == 2 && w < 2;
+  const bool scale_wave = SM >= 2 && w < 2;
 
   uint2 kraw[FP8 ? FJ : 1], vraw[FP8 ? FJ : 1];
   float sraw = 0.f;
@@ -335,11 +341,15 @@ __global__ __launch_bounds__(kPfThreads, 2) void rlt_prefill_kernel(AttnParams P
     for (int j = 0; j < NJ; ++j) load_v_piece(b, j, access(blks, j), access(offs, j));
   };
   // the scales of the cursor's tile, read into a register (wave 0 keys, wave 1 values)
+  int v_exp = 0;  // REFER: the weights of the product are taken over 2^(v_exp - kLift)
   auto load_scale = [&](int tile) {
     const float x = (w == 0 ? P.k_scale : P.v_scale)[pool_block(scur.next) * P.s_block_stride +
                                                      (int64_t)scur.off * P.s_token_stride +
                                                      (int64_t)kvh * P.s_head_stride];
     sraw = tile * kPfKeys + lane < hi_last ? x : 0.f;
+    if constexpr (REFER) {
+      if (w == 1) sraw = __builtin_amdgcn_ldexpf(sraw, kLift - v_exp);
+    }
     scur.advance(P, table, dq, dr);
   };
   // fp8: the loaded pieces of K / V of `tile`, widened, into buffer b (two 8-byte halves:
@@ -351,7 +361,7 @@ __global__ __launch_bounds__(kPfThreads, 2) void rlt_prefill_kernel(AttnParams P
       const int r = e / SLOTS, sl = e % SLOTS;
       // (pad slots of 96-dim rows are never read: left unwritten)
       if (PIECES == SLOTS || k_slot<SLOTS>(r, sl) < PIECES) {
-        const uint2 k0 = fp8x4_to_16<QT>(kraw[j].x), k1 = fp8x4_to_16<QT>(kraw[j].y);
+        const uint2 k0 = codes_to_16<QT, KVT>(kraw[j].x), k1 = codes_to_16<QT, KVT>(kraw[j].y);
         uint2* kd = (uint2*)(sh.k[b] + r * L::kRowB + sl * 16);
         kd[0] = k0;
         kd[1] = k1;
@@ -366,8 +376,8 @@ __global__ __launch_bounds__(kPfThreads, 2) void rlt_prefill_kernel(AttnParams P
       if (PIECES == SLOTS || v_slot<SLOTS>(r, sl) < PIECES) {
         uint2 v0 = make_uint2(0, 0), v1 = v0;
         if (tile * kPfKeys + r < hi_last) {
-          v0 = fp8x4_to_16<QT>(vraw[j].x);
-          v1 = fp8x4_to_16<QT>(vraw[j].y);
+          v0 = codes_to_16<QT, KVT>(vraw[j].x);
+          v1 = codes_to_16<QT, KVT>(vraw[j].y);
         }
         uint2* vd = (uint2*)(sh.v[b] + r * L::kRowB + sl * 16);
         vd[0] = v0;
@@ -438,7 +448,7 @@ __global__ __launch_bounds__(kPfThreads, 2) void rlt_prefill_kernel(AttnParams P
   };
   // per-vector key scales and the position mask of the tile's scores, in place
   auto scale_scores = [&](f32x16 (&s)[2], int b) {
-    if constexpr (SM == 2) {
+    if constexpr (SM >= 2) {
 #pragma unroll
       for (int u = 0; u < 2; ++u)
 #pragma unroll
@@ -461,8 +471,8 @@ __global__ __launch_bounds__(kPfThreads, 2) void rlt_prefill_kernel(AttnParams P
         s[u][i] = (pos >= lo && pos < hi) ? s[u][i] : -INFINITY;
       }
   };
-  // The running max moves only when a tile's max exceeds it by more than kPfLazy (weights
-  // stay below 2^kPfLazy), so the accumulators are rarely rescaled; the scale enters as
+  // The running max moves only when a tile's max exceeds it by more than kLazy (weights
+  // stay below 2^kLazy), so the accumulators are rarely rescaled; the scale enters as
   // one fma per score (qk_scale > 0: the max of raw scores scales).
   auto max_quad = [&](float& m, const f32x16 (&s)[2], int g) {
     const int i = 4 * (g & 3);
@@ -471,7 +481,7 @@ __global__ __launch_bounds__(kPfThreads, 2) void rlt_prefill_kernel(AttnParams P
   };
   auto move_max = [&](float m) {
     const float mx = half_max(m) * qk_scale;
-    const bool grow = mx > m_run + kPfLazy;
+    const bool grow = mx > m_run + kLazy;
     if (__builtin_amdgcn_ballot_w64(grow) != 0) {
       const float m_new = grow ? mx : m_run;
       const float use = m_new == -INFINITY ? 0.f : m_new;
@@ -491,7 +501,7 @@ __global__ __launch_bounds__(kPfThreads, 2) void rlt_prefill_kernel(AttnParams P
     for (int i = 0; i < 4; ++i)
       x[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[g >> 2][4 * (g & 3) + i], qk_scale, -m_use));
     l_run += (x[0] + x[1]) + (x[2] + x[3]);
-    if constexpr (SM == 2) {
+    if constexpr (SM >= 2) {
       const f32x4 y = *(const f32x4*)(sh.vs[b] + 8 * g + 4 * h);
 #pragma unroll
       for (int i = 0; i < 4; ++i) x[i] *= y[i];
@@ -533,6 +543,23 @@ __global__ __launch_bounds__(kPfThreads, 2) void rlt_prefill_kernel(AttnParams P
     for (int g = 0; g < 8; ++g)
       if (g >= 8 * i / n && g < 8 * (i + 1) / n) f(g);
   };
+
+  if constexpr (REFER) {
+    // the exponent of the largest value scale that the rows see
+    float most = 0.f;
+    if (kt0 < kt1) {
+      const int last = min((hi_last - 1) / P.block_size, P.table_width - 1);
+      for (int i = lo_first / P.block_size + t; i <= last; i += kPfThreads)
+        most = fmaxf(most, fabsf(P.v_scale[pool_block(table[i]) * P.s_block_stride + (int64_t)kvh * P.s_head_stride]));
+    }
+    for (int off = 32; off >= 1; off >>= 1) most = fmaxf(most, __shfl_xor(most, off, RLT_WAVE));
+    if (lane == 0) sh.vs[0][w] = most;
+    __syncthreads();
+    most = fmaxf(fmaxf(sh.vs[0][0], sh.vs[0][1]), fmaxf(sh.vs[0][2], sh.vs[0][3]));
+    __syncthreads();
+    v_exp = most > 0.f ? __builtin_amdgcn_frexp_expf(most) : 0;
+    v_mul = __builtin_amdgcn_ldexpf(1.f, v_exp - kLift);
+  }
 
   if (kt0 < kt1) {
     // ---- first tiles: K and V of kt0, K of kt0 + 1, the scores of kt0
@@ -588,7 +615,7 @@ __global__ __launch_bounds__(kPfThreads, 2) void rlt_prefill_kernel(AttnParams P
       if constexpr (!FP8) load_v(b ^ 1, vblk, voff);
       if (more) load_k(b);
       if constexpr (kEarlyV) load_v(b ^ 1, vblk, voff);
-      if (SM == 2 && (w == 1 || (w == 0 && more))) load_scale(tile + (w == 0 ? 2 : 1));
+      if (SM >= 2 && (w == 1 || (w == 0 && more))) load_scale(tile + (w == 0 ? 2 : 1));
       uint32_t p[16];
       scores(next_s, b ^ 1, [&](int c) {
         quads(c, NQS, [&](int g) { weigh_quad(cur_s, p, g, b); });
@@ -607,8 +634,8 @@ __global__ __launch_bounds__(kPfThreads, 2) void rlt_prefill_kernel(AttnParams P
       move_max(mx);
       if constexpr (FP8) {
         put_v(tile + 1, b ^ 1);
-        if (SM == 2 && w == 1) sh.vs[b ^ 1][lane] = sraw;
-        if (SM == 2 && w == 0 && more) sh.ks[b][lane] = sraw;
+        if (SM >= 2 && w == 1) sh.vs[b ^ 1][lane] = sraw;
+        if (SM >= 2 && w == 0 && more) sh.ks[b][lane] = sraw;
       } else {
         wait_loads();
         zero_tail(tile + 1, b ^ 1);

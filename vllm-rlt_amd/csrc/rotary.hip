@@ -496,12 +496,6 @@ struct LoadParams {
   void* v_out;
 };
 
-template <int CT>
-__device__ __forceinline__ float pool_value(const void* base, int64_t at) {
-  if constexpr (CT == RLT_INT8) return (float)((const int8_t*)base)[at];
-  else return load_as_f32<CT>(base, at);
-}
-
 // kLoadRows rows of a sequence per workgroup, a thread W elements of a vector at a time.
 constexpr int kLoadRows = 16;
 template <int CT, int OT, int W>
@@ -534,7 +528,7 @@ __global__ __launch_bounds__(kThreads) void rlt_kv_load_kernel(LoadParams P) {
       const float scale = scales ? scales[(int64_t)entry * P.s_block + (int64_t)off * P.s_token +
                                           (int64_t)head * P.s_head] : 1.f;
 #pragma unroll
-      for (int u = 0; u < W; ++u) y[u] = pool_value<CT>(pool, at + u) * scale;
+      for (int u = 0; u < W; ++u) y[u] = load_as_f32<CT>(pool, at + u) * scale;
     }
     const int64_t to = ((begin + i0 + r) * P.hkv + head) * P.head_dim + d;
     void* const out = value ? P.v_out : P.k_out;

@@ -148,6 +148,17 @@ Tensor paged_attention(const Tensor& q, const Tensor& key_cache, const Tensor& v
                       "FP8 scales must be float32");
     if (key_scale->dim() == 0 && value_scale->dim() == 0) {
       mode = 1;
+    } else if (key_scale->dim() == 2) {
+      TORCH_CHECK_VALUE(key_scale->size(0) == num_blocks && key_scale->size(1) == kv_heads &&
+                            value_scale->sizes() == key_scale->sizes() &&
+                            value_scale->strides() == key_scale->strides(),
+                        "block scales must be [block, kv_head] views of the pool sharing strides");
+      TORCH_CHECK_VALUE(key_cache.scalar_type() == at::kFloat8_e4m3fn ||
+                            key_cache.scalar_type() == at::kChar,
+                        "block scales are for float8_e4m3fn and int8 pools");
+      mode = 3;
+      s_strides[0] = key_scale->stride(0);
+      s_strides[2] = key_scale->stride(1);
     } else {
       TORCH_CHECK_VALUE(key_scale->dim() == 3 && key_scale->strides() == value_scale->strides(),
                         "per-vector FP8 scales must be [block, token, kv_head] views sharing "
@@ -158,6 +169,8 @@ Tensor paged_attention(const Tensor& q, const Tensor& key_cache, const Tensor& v
   }
   TORCH_CHECK_VALUE(!(key_cache.scalar_type() == at::kFloat8_e4m3fn && mode == 0),
                     "an FP8 KV pool needs key_scale / value_scale");
+  TORCH_CHECK_VALUE(key_cache.scalar_type() != at::kChar || mode == 3,
+                    "an int8 KV pool needs scales [block, kv_head]");
   TORCH_CHECK_VALUE(block_tables.dim() == 2 && block_tables.scalar_type() == at::kInt &&
                         block_tables.stride(1) == 1,
                     "block_tables must be int32 [sequences, width] with unit column stride");
@@ -196,7 +209,7 @@ Tensor paged_attention(const Tensor& q, const Tensor& key_cache, const Tensor& v
       (const int32_t*)ptr(cu), (int32_t)num_seqs, (int32_t)max_q, (int32_t)rows,
       (const float*)ptr(key_scale), (const float*)ptr(value_scale), mode, s_strides[0],
       s_strides[1], s_strides[2], (int32_t)heads, (int32_t)kv_heads, (int32_t)head_dim,
-      (int32_t)block_size, dtype_code(q.scalar_type()), dtype_code(key_cache.scalar_type()),
+      (int32_t)block_size, dtype_code(q.scalar_type()), pool_code(key_cache.scalar_type()),
       (int32_t)window, compensate ? RLT_ATTN_COMPENSATE : 0, ptr(output), output.stride(0),
       output.stride(1), ptr(ws), ws.numel(), stream_of(q));
   check_status(status, "rlt_paged_attention");
@@ -487,6 +500,12 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor, Tensor> verify_accept(
 
 // ---------------------------------------------------------------- window store + attention
 
+void append_kv(const Tensor& key_cache, const Tensor& value_cache, const Tensor& k, const Tensor& v,
+               const Tensor& block_tables, const Tensor& context_lengths, const Tensor& cu_seqlens_q,
+               int64_t max_seqlen_q, const OptTensor& key_scale, const OptTensor& value_scale,
+               const OptTensor& positions, const OptTensor& turns, double amplitude, bool interleaved,
+               const OptTensor& q, const OptTensor& q_out);
+
 // reference: vllm_rlt/kernels/graph_kv.py:52-67 (the window rows' KV write) followed by
 // vllm_rlt/kernels/triton_attention.py:386-404 (packed window attention).  Row r of
 // k_new / v_new goes to packed q row r's position (context_lengths[s] - q_len + i).
@@ -513,6 +532,28 @@ Tensor paged_attention_store(const Tensor& q, const Tensor& k_new_in, const Tens
   TORCH_CHECK_VALUE(k_new.size(0) == rows && k_new.size(1) == kv_heads && k_new.size(2) == head_dim &&
                         v_new.sizes() == k_new.sizes(),
                     "k_new, v_new must be [q rows, kv_heads, head_dim]");
+  if (key_scale.has_value() && key_scale->dim() == 2) {
+    // block scales: the append, then the attention, whose own checks come first (a type that its
+    // matrix kernels serve is read in 16-byte pieces)
+    TORCH_CHECK_VALUE(!row_lengths.has_value(), "block scales take no row_lengths");
+    TORCH_CHECK_VALUE(k_new.scalar_type() == q.scalar_type(), "k_new, v_new must have q's dtype");
+    TORCH_CHECK_VALUE(head_dim <= 256 && q.size(1) % kv_heads == 0 && q.stride(2) == 1,
+                      "q heads must be a positive multiple of KV heads with a contiguous head_dim <= 256");
+    TORCH_CHECK_VALUE(!compensate || key_cache.size(1) % 16 == 0,
+                      "compensated attention needs a block size that is a multiple of 16");
+    if (rlt_paged_attention_uses_mfma(dtype_code(q.scalar_type()), pool_code(key_cache.scalar_type()),
+                                      (int32_t)head_dim))
+      TORCH_CHECK_VALUE(((uintptr_t)ptr(q) | (uintptr_t)ptr(key_cache) | (uintptr_t)ptr(value_cache)) % 16 == 0 &&
+                            q.stride(0) % 8 == 0 && q.stride(1) % 8 == 0 &&
+                            key_cache.stride(0) % 16 == 0 && key_cache.stride(1) % 16 == 0 &&
+                            key_cache.stride(2) % 16 == 0,
+                        "q and the pools must be 16-byte aligned");
+    append_kv(key_cache, value_cache, k_new, v_new, block_tables, context_lengths, cu_seqlens_q,
+              max_seqlen_q, key_scale, value_scale, std::nullopt, std::nullopt, 1.0, false,
+              std::nullopt, std::nullopt);
+    return paged_attention(q, key_cache, value_cache, block_tables, context_lengths, key_scale,
+                           value_scale, cu_seqlens_q, max_seqlen_q, 0, std::nullopt, compensate);
+  }
   const bool fp8 = key_cache.scalar_type() == at::kFloat8_e4m3fn;
   const bool half = q.scalar_type() == at::kBFloat16 || q.scalar_type() == at::kHalf;
   // everything is checked before anything is stored: the attention's own checks must
