@@ -129,7 +129,15 @@ def test_refusals(pkg, dev):
                 lambda: pkg.apply_rotary(q, None, pos, pkg.Rotary(64, device="cpu"))):
         with pytest.raises(ValueError):
             bad()
-    flat = torch.zeros(9 * 64, device=dev)
-    a, b = flat[:512].view(4, 2, 64), flat[64:].view(4, 2, 64)
-    with pytest.raises(ValueError, match="apart"):
-        torch.ops.rlt_mi355x.rotary(a, None, pos, plan.turns, 1.0, False, False, b, None)
+    with pytest.raises(ValueError, match="share"):
+        pkg.apply_rotary(q, q, pos, plan, inplace=True)
+    fused = torch.zeros(4, 12, 64, device=dev)
+    for a, b in ((fused[:, :8], fused[:, 7:9]), (fused[:, 2:10], fused[:, 1:3]), (fused[:, :3], fused[..., :2, :]),
+                 (fused[:2], fused[1:3]), (fused[::2], fused[:2])):
+        with pytest.raises(ValueError, match="share"):
+            pkg.apply_rotary(a, b, pos[:len(a)], plan, inplace=True)
+    for a, b in ((fused[:, :8], fused[:, 8:10]), (fused[:, 2:10], fused[:, :2]), (fused[:, 4:], fused[:, :4]),
+                 (fused[:2], fused[2:])):
+        pkg.apply_rotary(a, b, pos[:len(a)], plan, inplace=True)
+    with pytest.raises(ValueError, match="stride"):
+        pkg.apply_rotary(torch.zeros(4, 64, 2, device=dev).transpose(1, 2), None, pos, plan, inplace=True)

@@ -76,7 +76,8 @@ def test_fake_shapes(pkg):
                                             torch.float16)
         assert k.shape == v.shape == (11, 4, 64) and k.dtype == torch.float16
         x = torch.empty(11, 4, 64)
-        assert torch.ops.rlt_mi355x.append_kv(pool, pool, x, x, tables, lengths, cu, 9, scale, scale) is None
+        q = torch.ops.rlt_mi355x.append_kv(pool, pool, x, x, tables, lengths, cu, 9, scale, scale, q=x)
+        assert q.shape == x.shape
 
 
 def test_c_entries_refuse(pkg):

@@ -82,6 +82,7 @@ struct AttnParams {
   const float* v_scale;
   int64_t s_block_stride, s_token_stride, s_head_stride;
   int32_t scale_mode;  // 0 none, 1 per-tensor (0-d), 2 per-vector [blk, tok, kvh], 3 per block [blk, kvh]
+  int32_t direct;      // block scales: rows of one chunk or none are written without the merge
   int32_t compensate;  // MFMA path: P V also with the bits P loses in its 16-bit cast
   int32_t num_seqs;
   int32_t num_rows;  // total q rows
@@ -128,8 +129,6 @@ constexpr int unit_split() { return KVT == QT ? 2 : 1; }
 template <int QT, int KVT>
 constexpr int unit_chunk() { return KVT == QT ? kChunk : 2 * kChunk; }
 constexpr float kLog2e = 1.4426950408889634f;
-template <int QT>
-constexpr int kBlockLift = QT == RLT_F16 ? 15 : 0;
 
 
 struct SeqView {
@@ -437,6 +436,18 @@ struct ValueQuad {
       a1.x = __builtin_amdgcn_perm(w[1][K], w[0][K], 0x07060302u);
       a0.y = __builtin_amdgcn_perm(w[3][K], w[2][K], 0x05040100u);
       a1.y = __builtin_amdgcn_perm(w[3][K], w[2][K], 0x07060302u);
+    } else if constexpr (KVT == RLT_INT8 && QT == RLT_BF16) {
+      constexpr int W = kHalfWords ? K : K / 2, S = kHalfWords || (K & 1) == 0 ? 0 : 16;
+      uint32_t f[4], g[4];  // dims 2k and 2k + 1 of the positions, whose floats end in their upper halves
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        f[i] = __float_as_uint((float)(int8_t)(w[i][W] >> S));
+        g[i] = __float_as_uint((float)(int8_t)(w[i][W] >> (S + 8)));
+      }
+      a0.x = __builtin_amdgcn_perm(f[1], f[0], 0x07060302u);
+      a1.x = __builtin_amdgcn_perm(g[1], g[0], 0x07060302u);
+      a0.y = __builtin_amdgcn_perm(f[3], f[2], 0x07060302u);
+      a1.y = __builtin_amdgcn_perm(g[3], g[2], 0x07060302u);
     } else if constexpr (KVT == RLT_INT8) {
       // the bytes of dim 2k of the four positions, and those of dim 2k + 1
       constexpr int W = kHalfWords ? K : K / 2;
@@ -622,14 +633,8 @@ __device__ __forceinline__ bool store_window(const AttnParams& P, int seq, int k
 // row-group, kv head, chunk) -- on one wave: the wave streams the kv head over
 // positions [512c + part * 512 / KS, + 512 / KS) for every row of the row-group.
 // tbl_lds: this wave's 512-entry LDS slice for the chunk's block ids.
-// SM: scale mode (0 none, 1 per-tensor, 2 per-vector, 3 per block).  UB: block_size is a
-// multiple of 16, so the 16 positions of a tile share one block.  With block scales a lane
-// holds the two scales of one tile of the span, loaded once ahead of the tiles: a tile takes
-// its own by a lane read into scalar registers (a load per tile and head less, and no
-// exchange between lanes).  The key scale goes into the scores, the value scale into the
-// weights of the product, over a power of two near the span's largest (and 2^kBlockLift above
-// it for fp16, whose normal numbers end at 2^-14), which the output takes back: exact, so a
-// weight is rounded as without it.
+// SM: FP8 scale mode (0 none, 1 per-tensor, 2 per-vector).  UB: block_size is a
+// multiple of 16, so the 16 positions of a tile share one block.
 template <int QT, int KVT, int D, int NT, int SM, bool UB, bool CP>
 __device__ __forceinline__ void attend_span(const AttnParams& P, int seq, int rg, int kvh, int chunk,
                                             int part, int32_t* tbl_lds,
@@ -642,7 +647,6 @@ __device__ __forceinline__ void attend_span(const AttnParams& P, int seq, int rg
   constexpr int KV_ELT = KVT == QT ? 2 : 1;
   constexpr int CH = unit_chunk<QT, KVT>();
   constexpr int kSpan = CH / unit_split<QT, KVT>();
-  static_assert(SM != 3 || (UB && KVT != QT && kSpan <= 64 * kTileTok), "a lane per tile's scales");
   const int lane = threadIdx.x & 63;
   const int l16 = lane & 15;
   const int grp = lane >> 4;
@@ -731,18 +735,7 @@ __device__ __forceinline__ void attend_span(const AttnParams& P, int seq, int rg
     st.v_mul = P.v_scale[0];
   }
 
-  float k_tile = 0.f, v_tile = 0.f;  // SM 3: the scales of the span's tile `lane`
-  if constexpr (SM == 3) {
-    if (t0 < t1) {
-      const int tile = min(max(lane, t0), t1 - 1);
-      const int64_t so = (int64_t)tbl_lds[w_begin - c_begin + tile * kTileTok] * P.s_block_stride +
-                         (int64_t)kvh * P.s_head_stride;
-      k_tile = P.k_scale[so];
-      v_tile = P.v_scale[so];
-    }
-  }
-
-  if (SM != 3 && P.new_k && t0 < t1) {
+  if (P.new_k && t0 < t1) {
     // The window rows' own keys and values, stored through the block table before any
     // tile of this span is read; the wait makes this wave's stores visible to its own
     // loads.
@@ -825,18 +818,6 @@ __device__ __forceinline__ void attend_span(const AttnParams& P, int seq, int rg
     auto scale_of = [&](float x, int b, int r) {
       return __int_as_float(__builtin_amdgcn_ds_bpermute(16 * grp + 64 * b + 4 * r, __float_as_int(x)));
     };
-    if constexpr (SM == 3) {
-      float most = fabsf(v_tile);
-#pragma unroll
-      for (int o = 32; o >= 1; o >>= 1) most = fmaxf(most, __shfl_xor(most, o, RLT_WAVE));
-      // (no scale above 0: the weights are 0 whatever the power)
-      const int e = most > 0.f ? __builtin_amdgcn_frexp_expf(most) : 0;
-      v_tile = __builtin_amdgcn_ldexpf(v_tile, kBlockLift<QT> - e);
-      st.v_mul = __builtin_amdgcn_ldexpf(1.f, e - kBlockLift<QT>);
-    }
-    auto tile_scale = [&](float x, int t) {
-      return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), min(t, tl)));
-    };
     // Wave-uniform fast-path bound: a pair inside [lo of the last row, hi of the
     // first row) is visible to every row of the row-group and fully stored, so
     // it needs no position masks.  (Branches around the masks: two copies of the whole
@@ -890,13 +871,11 @@ __device__ __forceinline__ void attend_span(const AttnParams& P, int seq, int rg
       bool rescale[2] = {false, false};
       float corr[2][NT];
 #pragma unroll
-      for (int b = 0; b < 2; ++b) {
-        const float f = SM == 3 ? qk_scale * tile_scale(k_tile, t + b) : qk_scale;
+      for (int b = 0; b < 2; ++b)
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-          for (int r = 0; r < 4; ++r) sc[b][nt][r] *= f;
-      }
+          for (int r = 0; r < 4; ++r) sc[b][nt][r] *= qk_scale;
       if (!full) {
 #pragma unroll
         for (int b = 0; b < 2; ++b)
@@ -935,11 +914,6 @@ __device__ __forceinline__ void attend_span(const AttnParams& P, int seq, int rg
           if (SM == 2) {
 #pragma unroll
             for (int r = 0; r < 4; ++r) pr[b][r] *= vsc[b][r];
-          }
-          if (SM == 3) {
-            const float f = tile_scale(v_tile, t + b);
-#pragma unroll
-            for (int r = 0; r < 4; ++r) pr[b][r] *= f;
           }
           pop[b][nt] = make_uint2(M::pack2(pr[b][0], pr[b][1]), M::pack2(pr[b][2], pr[b][3]));
           if (CP) {

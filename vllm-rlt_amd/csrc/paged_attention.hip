@@ -250,6 +250,7 @@ __global__ __launch_bounds__(256) void rlt_merge_kernel(AttnParams P) {
   row_range(P, sv, qi, lo, hi);
   const int c0 = lo >> P.chunk_log2, c1 = (hi + (1 << P.chunk_log2) - 1) >> P.chunk_log2;
   const int nc = c1 - c0;
+  if (P.direct && nc <= 1) return;  // (written by the attention kernel)
   const int64_t base = ((int64_t)row * P.hq + head) * P.max_chunks + c0;
   const int64_t out_off = (int64_t)row * P.out_row_stride + (int64_t)head * P.out_head_stride;
   const int D = P.head_dim;
@@ -686,6 +687,7 @@ int attention_impl(const void* q, int64_t q_row_stride, int64_t q_head_stride,
   P.s_head_stride = s_head_stride;
   P.scale_mode = scale_mode;
   P.compensate = (flags & RLT_ATTN_COMPENSATE) ? 1 : 0;
+  P.direct = 0;
   P.num_seqs = num_seqs;
   P.num_rows = num_q_rows;
   P.hq = num_q_heads;
@@ -698,7 +700,7 @@ int attention_impl(const void* q, int64_t q_row_stride, int64_t q_head_stride,
   // workspace query sizes the partials for 512, an upper bound
   const bool code8 = kv_dtype == RLT_FP8_E4M3 || kv_dtype == RLT_INT8;
   const bool code8_mfma = code8 && rlt_paged_attention_uses_mfma(q_dtype, kv_dtype, head_dim);
-  P.chunk_log2 = code8_mfma ? 10 : 9;
+  P.chunk_log2 = !code8_mfma ? 9 : scale_mode == 3 && whole_tiles(P) ? rlt_attn::block_chunk_log2() : 10;
   P.max_chunks = max_chunks_for(table_width, block_size, 1 << P.chunk_log2);
   P.qk_scale_log2 = kLog2e / sqrtf((float)head_dim);
   P.out = out;
@@ -779,7 +781,9 @@ int attention_impl(const void* q, int64_t q_row_stride, int64_t q_head_stride,
     // Persistent workgroups, one per CU, unless the pair index does not fit in LDS.
     P.head_groups = num_kv_heads;
     const int64_t pairs = (int64_t)num_seqs * P.rowgroups;
-    P.persistent = pairs <= kMaxPairs;
+    const bool blocks = scale_mode == 3 && whole_tiles(P);
+    P.direct = blocks;
+    P.persistent = pairs <= (blocks ? rlt_attn::kMaxBlockPairs : kMaxPairs);
     // (not with an fp8 store of 32 rows or more: quantizing them is a good part of its unit's time,
     // and neighbouring heads of the chunk that holds the window put such units on the same
     // workgroups.  8 windows of up to 24 / 32 / 48 / 63 rows behind 3000, 55 heads of 96, apart
@@ -788,9 +792,10 @@ int attention_impl(const void* q, int64_t q_row_stride, int64_t q_head_stride,
     const bool long_store = store && kv_dtype == RLT_FP8_E4M3 && max_q_len >= 32;
     P.shared_lines = num_kv_heads > 1 && !long_store &&
                      ((k_head_stride * kv_elt) % 128 != 0 || (v_head_stride * kv_elt) % 128 != 0 ||
-                      (scale_mode >= 2 && s_head_stride * 4 < 128));
+                      (scale_mode == 2 && s_head_stride * 4 < 128));
     int64_t wgs = (int64_t)num_seqs * P.rowgroups * num_kv_heads * P.max_chunks;
-    if (P.persistent) wgs = compute_units();
+    if (P.persistent)
+      wgs = (int64_t)compute_units() * (blocks ? rlt_attn::block_groups_per_cu(head_dim, nt) : 1);
     if (wgs >= ((int64_t)1 << 31)) return RLT_ERR_UNSUPPORTED;
     dim3 grid((unsigned)wgs);
     if (kv_dtype == RLT_INT8)
@@ -822,6 +827,7 @@ int attention_impl(const void* q, int64_t q_row_stride, int64_t q_head_stride,
     }
   }
   if (st != RLT_OK) return st;
+  if (P.direct && P.max_chunks <= 1) return rlt_launch_status();
   P.max_q = cu_seqlens_q ? max_q_len : 1;
   const int64_t merge_rows = cu_seqlens_q ? (int64_t)num_seqs * max_q_len : num_q_rows;
   if (merge_rows >= ((int64_t)1 << 31)) return RLT_ERR_UNSUPPORTED;

@@ -29,6 +29,8 @@
 
 #include <math.h>
 
+#include <type_traits>
+
 namespace {
 
 constexpr int kThreads = 256;
@@ -98,25 +100,48 @@ __device__ __forceinline__ float2 turn(double t) {
 
 // ---------------------------------------------------------------- pieces of W elements
 
+// as loaded: 16 bytes, or one element
 template <int DT, int W>
-__device__ __forceinline__ void load_piece(const void* base, int64_t at, float (&x)[W]) {
-  if constexpr (W == 1) {
-    x[0] = load_as_f32<DT>(base, at);
-  } else if constexpr (DT == RLT_F32) {
-    static_assert(W == 4, "16-byte pieces");
-    const float4 v = *(const float4*)((const float*)base + at);
-    x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w;
-  } else {
-    static_assert(W == 8, "16-byte pieces");
-    const uint4 v = *(const uint4*)((const uint16_t*)base + at);
-    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+struct Piece {
+  static_assert(W == 1 || W == (DT == RLT_F32 ? 4 : 8), "16-byte pieces");
+  typedef typename std::conditional<W == 1, float, uint4>::type T;
+  T raw;
+
+  __device__ __forceinline__ void load(const void* base, int64_t at) {
+    if constexpr (W == 1) raw = load_as_f32<DT>(base, at);
+    else if constexpr (DT == RLT_F32) raw = *(const uint4*)((const float*)base + at);
+    else raw = *(const uint4*)((const uint16_t*)base + at);
+  }
+  __device__ __forceinline__ void clear() {
+    if constexpr (W == 1) raw = 0.f;
+    else raw = make_uint4(0, 0, 0, 0);
+  }
+  __device__ __forceinline__ void floats(float (&x)[W]) const {
+    if constexpr (W == 1) {
+      x[0] = raw;
+    } else {
+      const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      x[2 * i] = DT == RLT_BF16 ? bf16_bits_to_f32((uint16_t)w[i]) : f16_bits_to_f32((uint16_t)w[i]);
-      x[2 * i + 1] = DT == RLT_BF16 ? bf16_bits_to_f32((uint16_t)(w[i] >> 16))
-                                    : f16_bits_to_f32((uint16_t)(w[i] >> 16));
+      for (int i = 0; i < 4; ++i) {
+        if constexpr (DT == RLT_F32) {
+          x[i] = __uint_as_float(w[i]);
+        } else if constexpr (DT == RLT_BF16) {
+          x[2 * i] = bf16_bits_to_f32((uint16_t)w[i]);
+          x[2 * i + 1] = bf16_bits_to_f32((uint16_t)(w[i] >> 16));
+        } else {
+          x[2 * i] = f16_bits_to_f32((uint16_t)w[i]);
+          x[2 * i + 1] = f16_bits_to_f32((uint16_t)(w[i] >> 16));
+        }
+      }
     }
   }
+};
+
+template <int DT, int W>
+__device__ __forceinline__ void load_piece(const void* base, int64_t at, float (&x)[W]) {
+  Piece<DT, W> p;
+  p.load(base, at);
+  p.floats(x);
 }
 
 template <int DT>
@@ -149,16 +174,45 @@ __device__ __forceinline__ void store_piece(void* base, int64_t at, const float 
 template <int MODE>
 constexpr float top_of() { return MODE == kBlockInt8 ? 127.f : rlt_fp8::kMax; }
 
-// The code of x / scale (IEEE division, round to nearest even): e4m3 keeps NaN and clamps the
-// rest to +-448; int8 has no NaN and takes it as 0.
+// A scale and its reciprocal.
+struct Divisor {
+  float by, inverse;
+};
+__device__ __forceinline__ Divisor divisor(float scale) { return Divisor{scale, 1.f / scale}; }
+
+// x / scale, correctly rounded: the reciprocal is, the first quotient is off by an ulp at most and
+// the remainder exact (as long as it is no subnormal number), so that one more step rounds as
+// the division does, in 3 instructions for its 10.
+__device__ __forceinline__ float quotient(float x, const Divisor& d) {
+  const float q = x * d.inverse;
+  return copysignf(fmaf(fmaf(-q, d.by, x), d.inverse, q), x);  // (the step turns -0 into 0)
+}
+
+// Codes of a block-scaled pool, round to nearest even: e4m3 keeps NaN and clamps the rest to
+// +-448; int8 has no NaN and takes it as 0.  (Infinities would make the remainder NaN.)
 template <int MODE>
-__device__ __forceinline__ uint32_t code_of(float x, float scale) {
+__device__ __forceinline__ float clamped(float x, const Divisor& d) {
+  constexpr float M = MODE == kBlockInt8 ? 127.f : rlt_fp8::kMax;
+  const float y = fabsf(x) < INFINITY ? quotient(x, d) : x;
+  const float c = fminf(fmaxf(y, -M), M);
+  return y != y ? (MODE == kBlockInt8 ? 0.f : y) : c;
+}
+// four codes
+template <int MODE>
+__device__ __forceinline__ uint32_t codes4(const float (&x)[4], const Divisor& d) {
   if constexpr (MODE == kBlockInt8) {
-    const float y = x / scale;
-    const float c = fminf(fmaxf(y, -127.f), 127.f);
-    return (uint32_t)(int)(y != y ? 0.f : rintf(c)) & 0xffu;
+    uint32_t b[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) b[i] = (uint32_t)(int)rintf(clamped<MODE>(x[i], d)) & 0xffu;
+    return b[0] | b[1] << 8 | b[2] << 16 | b[3] << 24;
+  } else if constexpr (MODE == kBlockFp8) {
+    int w = __builtin_amdgcn_cvt_pk_fp8_f32(clamped<MODE>(x[0], d), clamped<MODE>(x[1], d), 0, false);
+    return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(clamped<MODE>(x[2], d), clamped<MODE>(x[3], d), w, true);
   } else {
-    return rlt_fp8::encode(x, scale);
+    uint32_t w = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w |= rlt_fp8::encode(x[i], d.by) << (8 * i);
+    return w;
   }
 }
 template <int MODE>
@@ -168,17 +222,17 @@ __device__ __forceinline__ float value_of(uint32_t code) {
 }
 
 template <int MODE, int W>
-__device__ __forceinline__ void store_codes(void* pool, int64_t at, const float (&x)[W], float scale) {
+__device__ __forceinline__ void store_codes(void* pool, int64_t at, const float (&x)[W], const Divisor& d) {
   uint8_t* const p = (uint8_t*)pool + at;
   if constexpr (W == 1) {
-    *p = (uint8_t)code_of<MODE>(x[0], scale);
+    const float y[4] = {x[0], 0.f, 0.f, 0.f};
+    *p = (uint8_t)codes4<MODE>(y, d);
   } else {
     uint32_t w[W / 4];
 #pragma unroll
     for (int i = 0; i < W / 4; ++i) {
-      w[i] = 0;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) w[i] |= code_of<MODE>(x[4 * i + j], scale) << (8 * j);
+      const float y[4] = {x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]};
+      w[i] = codes4<MODE>(y, d);
     }
     if constexpr (W == 8) *(uint2*)p = make_uint2(w[0], w[1]);
     else *(uint32_t*)p = w[0];
@@ -200,6 +254,11 @@ struct Held {
   float x[NSTEP][NS][2][W];
 };
 
+template <int DT, int W, int NS, int NSTEP>
+struct Raw {
+  Piece<DT, W> x[NSTEP][NS][2];
+};
+
 template <int DT, int W, int LP, int MODE>
 __global__ __launch_bounds__(kThreads) void rlt_rotary_kernel(Params P) {
   constexpr int NS = W == 1 ? 2 : 1;
@@ -211,6 +270,8 @@ __global__ __launch_bounds__(kThreads) void rlt_rotary_kernel(Params P) {
   const int t = threadIdx.x, lane = t & 63;
   const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
   const int pairs = P.rotary_dim / 2;
+  // (before the chain of loads that finds the rows)
+  const double turns0 = pairs ? P.turns[t % pairs] : 0.0;
 
   // ---- the tile's rows [i0, i1) of its sequence
   int64_t begin = 0;    // packed row of the sequence's first
@@ -247,7 +308,7 @@ __global__ __launch_bounds__(kThreads) void rlt_rotary_kernel(Params P) {
     const int32_t e = idx >= 0 && idx < P.table_width ? P.tables[(int64_t)seq * P.table_stride + idx] : -1;
     return e >= 0 && e < P.num_blocks ? e : -1;
   };
-  const int entry = BLOCKS ? __builtin_amdgcn_readfirstlane(block_at(page)) : 0;
+  const int entry = BLOCKS ? block_at(page) : 0;
   const int o0 = BLOCKS ? start + i0 - page * P.block_size : 0;  // offset of row i0 in its block
 
   auto sines = [&](int c0, int c1) {
@@ -255,7 +316,7 @@ __global__ __launch_bounds__(kThreads) void rlt_rotary_kernel(Params P) {
       const int r = e / pairs, p = e - r * pairs;
       const int64_t row = begin + c0 + r;
       const int64_t pos = P.positions ? P.positions[row] : (int64_t)start + c0 + r;
-      const float2 cs = turn((double)pos * P.turns[p]);
+      const float2 cs = turn((double)pos * (e == t || kThreads % pairs == 0 ? turns0 : P.turns[p]));
       table[r * pairs + p] = make_float2(cs.x * P.amplitude, cs.y * P.amplitude * P.sign);
     }
   };
@@ -280,8 +341,8 @@ __global__ __launch_bounds__(kThreads) void rlt_rotary_kernel(Params P) {
     }
   }
 
-  // rows [c0, c1) of one head, turned if `turns`
-  auto fetch = [&](Held<W, NS, NSTEP>& held, const Side& s, int head, bool turns, int c0, int c1) {
+  // rows [c0, c1) of one head, as loaded
+  auto fetch = [&](Raw<DT, W, NS, NSTEP>& raw, const Side& s, int head, int c0, int c1) {
 #pragma unroll
     for (int st = 0; st < NSTEP; ++st) {
       if (st * RPW >= c1 - c0) continue;  // uniform
@@ -289,14 +350,24 @@ __global__ __launch_bounds__(kThreads) void rlt_rotary_kernel(Params P) {
       const int64_t at = (begin + c0 + r) * s.src_row + (int64_t)head * s.src_head;
 #pragma unroll
       for (int n = 0; n < NS; ++n) {
-        float(&a)[W] = held.x[st][n][0];
-        float(&b)[W] = held.x[st][n][1];
-#pragma unroll
-        for (int e = 0; e < W; ++e) a[e] = b[e] = 0.f;
+        raw.x[st][n][0].clear();
+        raw.x[st][n][1].clear();
         if (r < c1 - c0) {
-          if (at_a[n] >= 0) load_piece<DT, W>(s.src, at + at_a[n], a);
-          if (at_b[n] >= 0) load_piece<DT, W>(s.src, at + at_b[n], b);
+          if (at_a[n] >= 0) raw.x[st][n][0].load(s.src, at + at_a[n]);
+          if (at_b[n] >= 0) raw.x[st][n][1].load(s.src, at + at_b[n]);
         }
+      }
+    }
+  };
+  // as float32, turned if `turns`
+  auto expand = [&](Held<W, NS, NSTEP>& held, const Raw<DT, W, NS, NSTEP>& raw, bool turns, int c0, int c1) {
+#pragma unroll
+    for (int st = 0; st < NSTEP; ++st) {
+      if (st * RPW >= c1 - c0) continue;
+#pragma unroll
+      for (int n = 0; n < NS; ++n) {
+        raw.x[st][n][0].floats(held.x[st][n][0]);
+        raw.x[st][n][1].floats(held.x[st][n][1]);
       }
     }
     if (!turns) return;
@@ -355,7 +426,13 @@ __global__ __launch_bounds__(kThreads) void rlt_rotary_kernel(Params P) {
   const int kv_items = MODE == kApply ? P.hkv : 2 * P.hkv;
   const int items = kv_items + P.hq;
   const int first_item = wave + kWavesPerGroup * blockIdx.y, step = kWavesPerGroup * gridDim.y;
+  auto side = [&](int item) -> const Side& { return item >= kv_items ? P.q : item < P.hkv ? P.k : P.v; };
+  auto head_of = [&](int item) { return item >= kv_items ? item - kv_items : item < P.hkv ? item : item - P.hkv; };
+  auto scale_at = [&](int item) {
+    return side(item).scale + (int64_t)entry * P.s_block + (int64_t)head_of(item) * P.s_head;
+  };
   const bool several = BLOCKS && i1 - i0 > kRows;
+  Raw<DT, W, NS, NSTEP> raw;
   if constexpr (BLOCKS) {
     if (several) {
       // a block of more rows than are held: its maxima first
@@ -366,9 +443,9 @@ __global__ __launch_bounds__(kThreads) void rlt_rotary_kernel(Params P) {
         sines(c0, c1);
         __syncthreads();
         for (int item = first_item; item < kv_items; item += step) {
-          const bool key = item < P.hkv;
           Held<W, NS, NSTEP> held;
-          fetch(held, key ? P.k : P.v, key ? item : item - P.hkv, key, c0, c1);
+          fetch(raw, side(item), head_of(item), c0, c1);
+          expand(held, raw, item < P.hkv, c0, c1);
           const float m = top(held, c1 - c0);
           if (lane == 0) tops[item] = fmaxf(tops[item], m);
         }
@@ -377,16 +454,26 @@ __global__ __launch_bounds__(kThreads) void rlt_rotary_kernel(Params P) {
   }
   for (int c0 = i0; c0 < i1; c0 += kRows) {
     const int c1 = min(c0 + kRows, i1);
+    // an item's rows and its block's scale are loaded while the one before it is worked on, the
+    // first one's while the sines are made
+    float old_next = 0.f;
+    auto ahead = [&](int item) {
+      if (item >= items) return;
+      fetch(raw, side(item), head_of(item), c0, c1);
+      if (BLOCKS && item < kv_items && entry >= 0) old_next = *scale_at(item);
+    };
+    ahead(first_item);
     if (several) __syncthreads();
     sines(c0, c1);
     __syncthreads();
     for (int item = first_item; item < items; item += step) {
       const bool is_q = item >= kv_items;
-      const bool key = item < P.hkv;
-      const int head = is_q ? item - kv_items : key ? item : item - P.hkv;
-      const Side& s = is_q ? P.q : key ? P.k : P.v;
+      const int head = head_of(item);
+      const Side& s = side(item);
       Held<W, NS, NSTEP> held;
-      fetch(held, s, head, is_q || key, c0, c1);
+      expand(held, raw, is_q || item < P.hkv, c0, c1);
+      const float old = old_next;
+      ahead(item + step);
 
       if (MODE == kApply || is_q) {
 #pragma unroll
@@ -404,11 +491,10 @@ __global__ __launch_bounds__(kThreads) void rlt_rotary_kernel(Params P) {
       }
       if constexpr (BLOCKS) {
         if (entry < 0) continue;
-        float* const scale_at = s.scale + (int64_t)entry * P.s_block + (int64_t)head * P.s_head;
-        const float old = *scale_at;
         const float m = several ? tops[item] : top(held, c1 - c0);
         const float fresh = fmaxf(m * (1.f / top_of<MODE>()), rlt_fp8::kTiny);
         const float scale = o0 > 0 && old > fresh ? old : fresh;
+        const Divisor by = divisor(scale);
         const int64_t base = (int64_t)entry * s.dst_block + (int64_t)head * s.dst_head;
         if (c0 == i0 && o0 > 0 && scale > old) {
           // the block's earlier codes, over the new scale
@@ -419,10 +505,10 @@ __global__ __launch_bounds__(kThreads) void rlt_rotary_kernel(Params P) {
             float x[W];
 #pragma unroll
             for (int u = 0; u < W; ++u) x[u] = value_of<MODE>(((const uint8_t*)s.dst)[at + u]) * old;
-            store_codes<MODE, W>(s.dst, at, x, scale);
+            store_codes<MODE, W>(s.dst, at, x, by);
           }
         }
-        if (lane == 0 && c1 == i1) *scale_at = scale;  // (the last chunk: all read the old one)
+        if (lane == 0 && c1 == i1) *scale_at(item) = scale;  // (the last chunk: all read the old one)
 #pragma unroll
         for (int st = 0; st < NSTEP; ++st) {
           const int r = st * RPW + group;
@@ -430,8 +516,8 @@ __global__ __launch_bounds__(kThreads) void rlt_rotary_kernel(Params P) {
           const int64_t at = base + (int64_t)(o0 + (c0 - i0) + r) * s.dst_row;
 #pragma unroll
           for (int n = 0; n < NS; ++n) {
-            if (at_a[n] >= 0) store_codes<MODE, W>(s.dst, at + at_a[n], held.x[st][n][0], scale);
-            if (at_b[n] >= 0) store_codes<MODE, W>(s.dst, at + at_b[n], held.x[st][n][1], scale);
+            if (at_a[n] >= 0) store_codes<MODE, W>(s.dst, at + at_a[n], held.x[st][n][0], by);
+            if (at_b[n] >= 0) store_codes<MODE, W>(s.dst, at + at_b[n], held.x[st][n][1], by);
           }
         }
       } else if constexpr (MODE != kApply) {
@@ -467,7 +553,7 @@ __global__ __launch_bounds__(kThreads) void rlt_rotary_kernel(Params P) {
               const int el = half ? at_b[n] : at_a[n];
               if (el < 0) continue;
               if constexpr (MODE == kSame) store_piece<DT, W>(s.dst, at + el, held.x[st][n][half]);
-              else store_codes<MODE, W>(s.dst, at + el, held.x[st][n][half], scale);
+              else store_codes<MODE, W>(s.dst, at + el, held.x[st][n][half], Divisor{scale, 0.f});
             }
           }
         }
@@ -491,49 +577,111 @@ struct LoadParams {
   const int32_t* lengths;
   const int32_t* cu;
   int64_t rows;
-  int32_t num_seqs, max_rows, tiles, hkv, head_dim;
+  int32_t num_seqs, max_rows, tiles, tile_rows, hkv, head_dim;
   void* k_out;
   void* v_out;
 };
 
-// kLoadRows rows of a sequence per workgroup, a thread W elements of a vector at a time.
+// W consecutive elements of a pool as float32, in one load where W is more than 1.
+template <int CT, int W>
+__device__ __forceinline__ void load_elements(const void* pool, int64_t at, float (&x)[W]) {
+  if constexpr (W == 1) {
+    x[0] = load_as_f32<CT>(pool, at);
+  } else if constexpr (CT == RLT_FP8_E4M3 || CT == RLT_INT8) {
+    static_assert(W == 16, "16-byte pieces");
+    const uint4 v = *(const uint4*)((const uint8_t*)pool + at);
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (CT == RLT_INT8) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) x[4 * i + j] = (float)(int8_t)(w[i] >> (8 * j));
+      } else {
+        const float2 lo = fp8x2_to_f32<false>(w[i]), hi = fp8x2_to_f32<true>(w[i]);
+        x[4 * i] = lo.x; x[4 * i + 1] = lo.y; x[4 * i + 2] = hi.x; x[4 * i + 3] = hi.y;
+      }
+    }
+  } else {
+    load_piece<CT, W>(pool, at, x);
+  }
+}
+
+// W consecutive floats to an output, 16 bytes a store.
+template <int OT, int W>
+__device__ __forceinline__ void store_elements(void* out, int64_t at, const float (&x)[W]) {
+  if constexpr (W == 1) {
+    store_from_f32<OT>(out, at, x[0]);
+  } else {
+    constexpr int P = OT == RLT_F32 ? 4 : 8;
+    static_assert(W % P == 0 || W < P, "whole stores");
+    if constexpr (W < P) {
+      // (float32 pools read as 16 bits: 8 bytes)
+      *(uint2*)((uint16_t*)out + at) = make_uint2(pack2<OT>(x[0], x[1]), pack2<OT>(x[2], x[3]));
+    } else {
+#pragma unroll
+      for (int i = 0; i < W / P; ++i) {
+        float y[P];
+#pragma unroll
+        for (int j = 0; j < P; ++j) y[j] = x[P * i + j];
+        store_piece<OT, P>(out, at + P * i, y);
+      }
+    }
+  }
+}
+
+// A workgroup takes `tile_rows` rows of a sequence, whose blocks it looks up once; a thread a
+// column of W elements over the rows, so that its loads are in flight together.  HBM bounds it.
 constexpr int kLoadRows = 16;
 template <int CT, int OT, int W>
 __global__ __launch_bounds__(kThreads) void rlt_kv_load_kernel(LoadParams P) {
+  __shared__ int entries[kLoadRows], offsets[kLoadRows];
   const int seq = (int)(blockIdx.x / (uint32_t)P.tiles);
   const int tile = (int)(blockIdx.x - (uint32_t)seq * P.tiles);
   const int64_t b = P.cu[seq], e = P.cu[seq + 1];
   const int64_t begin = b < 0 ? 0 : b > P.rows ? P.rows : b;
   const int64_t n = (e > P.rows ? P.rows : e) - begin;
   const int count = (int)(n < 0 ? 0 : n > P.max_rows ? P.max_rows : n);
-  const int start = P.lengths[seq] - count;
-  const int i0 = tile * kLoadRows, i1 = min(count, i0 + kLoadRows);
-  const int per_vec = (P.head_dim + W - 1) / W, per_row = 2 * P.hkv * per_vec;
-  for (int i = threadIdx.x + kThreads * blockIdx.y; i < (i1 - i0) * per_row; i += kThreads * gridDim.y) {
-    const int r = i / per_row, x = i - r * per_row;
-    const int vec = x / per_vec, d = (x - vec * per_vec) * W;
+  const int i0 = tile * P.tile_rows, rows = min(count - i0, P.tile_rows);
+  if (rows <= 0) return;  // uniform over the workgroup
+  const int t = threadIdx.x;
+  if (t < rows) {
+    const int pos = P.lengths[seq] - count + i0 + t;
+    const int idx = pos >= 0 ? pos / P.block_size : -1;
+    const int32_t x = idx >= 0 && idx < P.table_width ? P.tables[(int64_t)seq * P.table_stride + idx] : -1;
+    entries[t] = x >= 0 && x < P.num_blocks ? x : -1;
+    offsets[t] = pos - idx * P.block_size;
+  }
+  __syncthreads();
+  // columns of a row (k, then v); where they are fewer than the threads these take several rows
+  const int per_vec = (P.head_dim + W - 1) / W, columns = 2 * P.hkv * per_vec;
+  const int together = columns < kThreads ? kThreads / columns : 1;
+  const int first = columns < kThreads ? t / columns : 0;
+  if (first >= together) return;
+  for (int c = t - first * columns; c < columns; c += kThreads) {
+    const int vec = c / per_vec, d = (c - vec * per_vec) * W;
     const bool value = vec >= P.hkv;
     const int head = value ? vec - P.hkv : vec;
-    const int pos = start + i0 + r;
-    const int idx = pos >= 0 ? pos / P.block_size : -1, off = pos - idx * P.block_size;
-    const int32_t entry = idx >= 0 && idx < P.table_width ? P.tables[(int64_t)seq * P.table_stride + idx] : -1;
-    float y[W];
-#pragma unroll
-    for (int u = 0; u < W; ++u) y[u] = 0.f;
-    if (entry >= 0 && entry < P.num_blocks) {
-      const int64_t at = value ? (int64_t)entry * P.v_block + (int64_t)off * P.v_token + (int64_t)head * P.v_head + d
-                               : (int64_t)entry * P.k_block + (int64_t)off * P.k_token + (int64_t)head * P.k_head + d;
-      const void* const pool = value ? P.v : P.k;
-      const float* const scales = value ? P.vs : P.ks;
-      const float scale = scales ? scales[(int64_t)entry * P.s_block + (int64_t)off * P.s_token +
-                                          (int64_t)head * P.s_head] : 1.f;
-#pragma unroll
-      for (int u = 0; u < W; ++u) y[u] = load_as_f32<CT>(pool, at + u) * scale;
-    }
-    const int64_t to = ((begin + i0 + r) * P.hkv + head) * P.head_dim + d;
+    const void* const pool = value ? P.v : P.k;
+    const float* const scales = value ? P.vs : P.ks;
+    const int64_t block = value ? P.v_block : P.k_block, token = value ? P.v_token : P.k_token;
+    const int64_t from = (int64_t)head * (value ? P.v_head : P.k_head) + d;
     void* const out = value ? P.v_out : P.k_out;
+    const int64_t to = ((begin + i0) * P.hkv + head) * P.head_dim + d, row = (int64_t)P.hkv * P.head_dim;
+#pragma unroll 4
+    for (int r = first; r < rows; r += together) {
+      const int entry = entries[r], off = offsets[r];
+      float x[W];
 #pragma unroll
-    for (int u = 0; u < W; ++u) store_from_f32<OT>(out, to + u, y[u]);
+      for (int u = 0; u < W; ++u) x[u] = 0.f;
+      if (entry >= 0) {
+        const float scale = scales ? scales[(int64_t)entry * P.s_block + (int64_t)off * P.s_token +
+                                            (int64_t)head * P.s_head] : 1.f;
+        load_elements<CT, W>(pool, (int64_t)entry * block + (int64_t)off * token + from, x);
+#pragma unroll
+        for (int u = 0; u < W; ++u) x[u] *= scale;
+      }
+      store_elements<OT, W>(out, to + r * row, x);
+    }
   }
 }
 
@@ -702,7 +850,8 @@ namespace {
 
 template <int CT, int OT>
 int launch_load(const LoadParams& P, bool vec, dim3 grid, hipStream_t stream) {
-  if (vec) rlt_kv_load_kernel<CT, OT, 8><<<grid, kThreads, 0, stream>>>(P);
+  constexpr int W = CT == RLT_F32 ? 4 : CT == RLT_FP8_E4M3 || CT == RLT_INT8 ? 16 : 8;
+  if (vec) rlt_kv_load_kernel<CT, OT, W><<<grid, kThreads, 0, stream>>>(P);
   else rlt_kv_load_kernel<CT, OT, 1><<<grid, kThreads, 0, stream>>>(P);
   return rlt_launch_status();
 }
@@ -740,8 +889,6 @@ extern "C" int rlt_kv_load(const void* key_cache, const void* value_cache, int64
   if (!key_cache || !value_cache || !context_lengths || !cu_seqlens || !k_out || !v_out ||
       (table_width && !block_tables))
     return RLT_ERR_ARGUMENT;
-  // (a workgroup's items are counted in 32 bits)
-  if ((int64_t)2 * num_kv_heads * head_dim * kLoadRows >= ((int64_t)1 << 31)) return RLT_ERR_UNSUPPORTED;
   LoadParams P;
   P.k = key_cache;
   P.v = value_cache;
@@ -770,13 +917,19 @@ extern "C" int rlt_kv_load(const void* key_cache, const void* value_cache, int64
   P.head_dim = head_dim;
   P.k_out = k_out;
   P.v_out = v_out;
-  const int64_t tiles = ((int64_t)max_len + kLoadRows - 1) / kLoadRows, gx = tiles * num_seqs;
+  // (few rows: shorter tiles, whose threads wait for fewer loads in turn)
+  P.tile_rows = kLoadRows;
+  auto groups = [&]() { return ((int64_t)max_len + P.tile_rows - 1) / P.tile_rows * num_seqs; };
+  while (P.tile_rows > 4 && groups() < kGroupsWanted) P.tile_rows /= 2;
+  const int64_t gx = groups();
   if (gx >= ((int64_t)1 << 31)) return RLT_ERR_UNSUPPORTED;
-  P.tiles = (int32_t)tiles;
-  const bool vec = head_dim % 8 == 0;
-  const int64_t per_group = (int64_t)2 * num_kv_heads * ((head_dim + 7) / 8) * kLoadRows;
-  const int64_t most = (per_group + kThreads - 1) / kThreads, want = (kGroupsWanted + gx - 1) / gx;
-  const dim3 grid((unsigned)gx, (unsigned)(want < most ? want : most));
+  P.tiles = (int32_t)(gx / num_seqs);
+  const int elt = kv_dtype == RLT_F32 ? 4 : codes ? 1 : 2;
+  const bool vec = head_dim % (16 / elt) == 0 &&
+                   aligned(key_cache, k_block_stride, k_token_stride, k_head_stride, elt, 16) &&
+                   aligned(value_cache, v_block_stride, v_token_stride, v_head_stride, elt, 16) &&
+                   ((uintptr_t)k_out | (uintptr_t)v_out) % 16 == 0;
+  const dim3 grid((unsigned)gx);
   switch (kv_dtype) {
     case RLT_F32: return launch_load_ot<RLT_F32>(P, out_dtype, vec, grid, stream);
     case RLT_F16: return launch_load_ot<RLT_F16>(P, out_dtype, vec, grid, stream);

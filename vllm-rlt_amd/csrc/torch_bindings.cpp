@@ -500,11 +500,11 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor, Tensor> verify_accept(
 
 // ---------------------------------------------------------------- window store + attention
 
-void append_kv(const Tensor& key_cache, const Tensor& value_cache, const Tensor& k, const Tensor& v,
-               const Tensor& block_tables, const Tensor& context_lengths, const Tensor& cu_seqlens_q,
-               int64_t max_seqlen_q, const OptTensor& key_scale, const OptTensor& value_scale,
-               const OptTensor& positions, const OptTensor& turns, double amplitude, bool interleaved,
-               const OptTensor& q, const OptTensor& q_out);
+Tensor append_kv(const Tensor& key_cache, const Tensor& value_cache, const Tensor& k, const Tensor& v,
+                 const Tensor& block_tables, const Tensor& context_lengths, const Tensor& cu_seqlens_q,
+                 int64_t max_seqlen_q, const OptTensor& key_scale, const OptTensor& value_scale,
+                 const OptTensor& positions, const OptTensor& turns, double amplitude,
+                 bool interleaved, const OptTensor& q);
 
 // reference: vllm_rlt/kernels/graph_kv.py:52-67 (the window rows' KV write) followed by
 // vllm_rlt/kernels/triton_attention.py:386-404 (packed window attention).  Row r of
@@ -550,7 +550,7 @@ Tensor paged_attention_store(const Tensor& q, const Tensor& k_new_in, const Tens
                         "q and the pools must be 16-byte aligned");
     append_kv(key_cache, value_cache, k_new, v_new, block_tables, context_lengths, cu_seqlens_q,
               max_seqlen_q, key_scale, value_scale, std::nullopt, std::nullopt, 1.0, false,
-              std::nullopt, std::nullopt);
+              std::nullopt);
     return paged_attention(q, key_cache, value_cache, block_tables, context_lengths, key_scale,
                            value_scale, cu_seqlens_q, max_seqlen_q, 0, std::nullopt, compensate);
   }
@@ -975,32 +975,38 @@ const Tensor& row_tensor(const Tensor& x, const char* name) {
   return x;
 }
 
-// `out` takes what is made of `x`: its shape and type, no element of it twice, and either x's own
-// memory in x's order or none of it (an element is read and written by one lane only).
-void check_target(const Tensor& x, const Tensor& out, const char* name) {
-  row_tensor(out, name);
-  TORCH_CHECK_VALUE(out.sizes() == x.sizes() && out.scalar_type() == x.scalar_type(), name,
-                    " must have its input's shape and dtype");
-  if (out.numel() == 0) return;
-  const int64_t elt = out.element_size();
-  TORCH_CHECK_VALUE(!pools::overlap((int64_t)1 << 62, {{out.stride(0) * elt, out.size(0)},
-                                                       {out.stride(1) * elt, out.size(1)},
+// an element is read and written by one lane only
+void check_in_place(const Tensor& x, const char* name) {
+  const int64_t elt = x.element_size();
+  TORCH_CHECK_VALUE(x.numel() == 0 || !pools::overlap((int64_t)1 << 62,
+                                                      {{x.stride(0) * elt, x.size(0)},
+                                                       {x.stride(1) * elt, x.size(1)},
                                                        {0, 1}},
-                                    out.size(2) * elt),
-                    name, "'s rows must not share memory");
-  const auto range = [&](const Tensor& t) {
-    const uintptr_t at = (uintptr_t)t.data_ptr();
-    int64_t lo = 0, hi = t.size(2) * elt;
-    for (int d = 0; d < 2; ++d) {
-      const int64_t far = t.stride(d) * (t.size(d) - 1) * elt;
-      (far < 0 ? lo : hi) += far;
-    }
-    return std::make_pair(at + lo, at + hi);
+                                                      x.size(2) * elt),
+                    name, " cannot be turned in place: its rows share memory");
+}
+
+// Whether rows of q and k [rows, heads, dim] share elements: exact where they have the same
+// strides (heads of one fused tensor), by their address ranges otherwise.
+bool share_rows(const Tensor& q, const Tensor& k) {
+  if (q.numel() == 0 || k.numel() == 0) return false;
+  const int64_t rows = q.size(0), dim = q.size(2);
+  const auto span = [&](const Tensor& x) {
+    return (rows - 1) * std::abs(x.stride(0)) + (x.size(1) - 1) * std::abs(x.stride(1)) + dim;
   };
-  const auto a = range(x), b = range(out);
-  const bool apart = a.second <= b.first || b.second <= a.first;
-  const bool same = x.data_ptr() == out.data_ptr() && x.strides() == out.strides();
-  TORCH_CHECK_VALUE(apart || same, name, " must be its input or apart from it");
+  const int64_t delta = (int64_t)((intptr_t)k.data_ptr() - (intptr_t)q.data_ptr()) / q.element_size();
+  if (delta >= span(q) || -delta >= span(k)) return false;
+  const int64_t row = q.stride(0), head = q.stride(1);
+  if (k.stride(0) != row || k.stride(1) != head || head < dim || (rows > 1 && row < 1)) return true;
+  // k's row j + r lies r rows behind q's row j, and then n heads
+  const int64_t near = rows > 1 ? delta / row : 0;
+  for (int64_t r = near - 1; r <= near + 1; ++r) {
+    if (std::abs(r) >= rows) continue;
+    const int64_t left = delta - (rows > 1 ? r * row : 0);
+    for (int64_t n = left / head - 1; n <= left / head + 1; ++n)
+      if (n > -k.size(1) && n < q.size(1) && std::abs(left - n * head) < dim) return true;
+  }
+  return false;
 }
 
 // turns float64 [rotary_dim / 2]
@@ -1013,34 +1019,57 @@ int64_t rotary_dim_of(const OptTensor& turns, int64_t head_dim) {
 }
 
 // Queries and keys turned by their positions (rlt_rotary).
-void rotary(const Tensor& q, const OptTensor& k, const Tensor& positions, const Tensor& turns,
-            double amplitude, bool interleaved, bool inverse, const Tensor& q_out,
-            const OptTensor& k_out) {
-  row_tensor(q, "q");
+void turn_rows(const Tensor& q, const OptTensor& k, const Tensor& positions, const Tensor& turns,
+               double amplitude, bool interleaved, bool inverse, const Tensor& q_out,
+               const OptTensor& k_out) {
   const int64_t rows = q.size(0), head_dim = q.size(2);
-  TORCH_CHECK_VALUE(head_dim >= 1 && head_dim <= 256, "head_dim must be between 1 and 256");
-  TORCH_CHECK_VALUE(k.has_value() == k_out.has_value(), "k and k_out must be given together");
-  same_device(q, k, positions, turns, q_out, k_out);
-  index_of(positions, rows, "positions");
-  const int64_t rot = rotary_dim_of(turns, head_dim);
-  check_target(q, q_out, "q_out");
-  if (k.has_value()) {
-    row_tensor(*k, "k");
-    TORCH_CHECK_VALUE(k->size(0) == rows && k->size(2) == head_dim &&
-                          k->scalar_type() == q.scalar_type(),
-                      "k must have q's rows, head_dim and dtype");
-    check_target(*k, *k_out, "k_out");
-  }
   const c10::hip::HIPGuardMasqueradingAsCUDA guard(q.device());
   const int status = rlt_rotary(
       ptr(q), q.stride(0), q.stride(1), ptr(k), k.has_value() ? k->stride(0) : 0,
       k.has_value() ? k->stride(1) : 0, (const int64_t*)ptr(positions), rows,
-      (const double*)ptr(turns), (int32_t)rot, (float)amplitude, interleaved ? 1 : 0,
+      (const double*)ptr(turns), 2 * (int32_t)turns.size(0), (float)amplitude, interleaved ? 1 : 0,
       inverse ? 1 : 0, (int32_t)q.size(1), k.has_value() ? (int32_t)k->size(1) : 0,
       (int32_t)head_dim, dtype_code(q.scalar_type()), ptr(q_out), q_out.stride(0), q_out.stride(1),
       ptr(k_out), k_out.has_value() ? k_out->stride(0) : 0, k_out.has_value() ? k_out->stride(1) : 0,
       stream_of(q));
   check_status(status, "rlt_rotary");
+}
+
+void check_turn(const Tensor& q, const OptTensor& k, const Tensor& positions, const Tensor& turns) {
+  row_tensor(q, "q");
+  const int64_t rows = q.size(0), head_dim = q.size(2);
+  TORCH_CHECK_VALUE(head_dim >= 1 && head_dim <= 256, "head_dim must be between 1 and 256");
+  same_device(q, k, positions, turns);
+  index_of(positions, rows, "positions");
+  rotary_dim_of(turns, head_dim);
+  if (k.has_value()) {
+    row_tensor(*k, "k");
+    TORCH_CHECK_VALUE(k->size(0) == rows && k->size(2) == head_dim &&
+                          k->scalar_type() == q.scalar_type(),
+                      "k must have q's rows, head_dim and dtype");
+  }
+}
+
+// (q', k'); without k the second is an empty tensor
+std::tuple<Tensor, Tensor> rotary(const Tensor& q, const OptTensor& k, const Tensor& positions,
+                                  const Tensor& turns, double amplitude, bool interleaved, bool inverse) {
+  check_turn(q, k, positions, turns);
+  Tensor q_out = at::empty(q.sizes(), q.options());
+  Tensor k_out = k.has_value() ? at::empty(k->sizes(), q.options()) : at::empty({0}, q.options());
+  turn_rows(q, k, positions, turns, amplitude, interleaved, inverse, q_out,
+            k.has_value() ? OptTensor(k_out) : std::nullopt);
+  return {q_out, k_out};
+}
+
+void rotary_(const Tensor& q, const OptTensor& k, const Tensor& positions, const Tensor& turns,
+             double amplitude, bool interleaved, bool inverse) {
+  check_turn(q, k, positions, turns);
+  check_in_place(q, "q");
+  if (k.has_value()) {
+    check_in_place(*k, "k");
+    TORCH_CHECK_VALUE(!share_rows(q, *k), "q and k cannot be turned in place: they share memory");
+  }
+  turn_rows(q, k, positions, turns, amplitude, interleaved, inverse, q, k);
 }
 
 // The pools of an append or a load, their scales and the packed sequences.
@@ -1105,13 +1134,14 @@ CacheArgs check_cache(const Tensor& key_cache, const Tensor& value_cache, const 
 }
 
 // Windows of rows into the paged cache, turned on the way (rlt_kv_append).
-void append_kv(const Tensor& key_cache, const Tensor& value_cache, const Tensor& k, const Tensor& v,
-               const Tensor& block_tables, const Tensor& context_lengths, const Tensor& cu_seqlens_q,
-               int64_t max_seqlen_q, const OptTensor& key_scale, const OptTensor& value_scale,
-               const OptTensor& positions, const OptTensor& turns, double amplitude, bool interleaved,
-               const OptTensor& q, const OptTensor& q_out) {
+// Returns the turned q (an empty tensor without one).
+Tensor append_kv(const Tensor& key_cache, const Tensor& value_cache, const Tensor& k, const Tensor& v,
+                 const Tensor& block_tables, const Tensor& context_lengths, const Tensor& cu_seqlens_q,
+                 int64_t max_seqlen_q, const OptTensor& key_scale, const OptTensor& value_scale,
+                 const OptTensor& positions, const OptTensor& turns, double amplitude,
+                 bool interleaved, const OptTensor& q) {
   same_device(key_cache, value_cache, k, v, block_tables, context_lengths, cu_seqlens_q, key_scale,
-              value_scale, positions, turns, q, q_out);
+              value_scale, positions, turns, q);
   const CacheArgs c = check_cache(key_cache, value_cache, key_scale, value_scale, block_tables,
                                   context_lengths, cu_seqlens_q);
   row_tensor(k, "k");
@@ -1141,15 +1171,14 @@ void append_kv(const Tensor& key_cache, const Tensor& value_cache, const Tensor&
                       "key and value scales must not overlap");
   if (positions.has_value()) index_of(*positions, rows, "positions");
   const int64_t rot = rotary_dim_of(turns, head_dim);
-  TORCH_CHECK_VALUE(q.has_value() == q_out.has_value(), "q and q_out must be given together");
   if (q.has_value()) {
     row_tensor(*q, "q");
     TORCH_CHECK_VALUE(q->size(0) == rows && q->size(2) == head_dim &&
                           q->scalar_type() == k.scalar_type(),
                       "q must have k's rows, head_dim and dtype");
-    check_target(*q, *q_out, "q_out");
   }
-  if (rows == 0 || block_tables.size(0) == 0) return;
+  Tensor q_out = q.has_value() ? at::empty(q->sizes(), q->options()) : at::empty({0}, k.options());
+  if (rows == 0 || block_tables.size(0) == 0) return q_out;
   const c10::hip::HIPGuardMasqueradingAsCUDA guard(key_cache.device());
   const int status = rlt_kv_append(
       ptr(k), k.stride(0), k.stride(1), ptr(v), v.stride(0), v.stride(1), dtype_code(k.scalar_type()),
@@ -1162,9 +1191,10 @@ void append_kv(const Tensor& key_cache, const Tensor& value_cache, const Tensor&
       (int32_t)block_tables.size(0), (int32_t)max_seqlen_q, rows, (int32_t)heads, (int32_t)head_dim,
       (const int64_t*)ptr(positions), (const double*)ptr(turns), (int32_t)rot, (float)amplitude,
       interleaved ? 1 : 0, ptr(q), q.has_value() ? q->stride(0) : 0, q.has_value() ? q->stride(1) : 0,
-      q.has_value() ? (int32_t)q->size(1) : 0, ptr(q_out), q_out.has_value() ? q_out->stride(0) : 0,
-      q_out.has_value() ? q_out->stride(1) : 0, stream_of(key_cache));
+      q.has_value() ? (int32_t)q->size(1) : 0, ptr(q_out), q.has_value() ? q_out.stride(0) : 0,
+      q.has_value() ? q_out.stride(1) : 0, stream_of(key_cache));
   check_status(status, "rlt_kv_append");
+  return q_out;
 }
 
 // Cached positions as numbers (rlt_kv_load).
@@ -1235,12 +1265,13 @@ TORCH_LIBRARY(rlt_mi355x, m) {
   m.def("commit_tree_kv(Tensor(a!) key_pool, Tensor(b!) value_pool, Tensor tables, Tensor starts, "
         "Tensor path, Tensor accepted, int block_size) -> ()");
   m.def("rotary(Tensor q, Tensor? k, Tensor positions, Tensor turns, float amplitude, "
-        "bool interleaved, bool inverse, Tensor(a!) q_out, Tensor(b!)? k_out) -> ()");
+        "bool interleaved, bool inverse) -> (Tensor, Tensor)");
+  m.def("rotary_(Tensor(a!) q, Tensor(b!)? k, Tensor positions, Tensor turns, float amplitude, "
+        "bool interleaved, bool inverse) -> ()");
   m.def("append_kv(Tensor(a!) key_cache, Tensor(b!) value_cache, Tensor k, Tensor v, "
         "Tensor block_tables, Tensor context_lengths, Tensor cu_seqlens_q, int max_seqlen_q, "
         "Tensor(c!)? key_scale=None, Tensor(d!)? value_scale=None, Tensor? positions=None, "
-        "Tensor? turns=None, float amplitude=1.0, bool interleaved=False, Tensor? q=None, "
-        "Tensor(e!)? q_out=None) -> ()");
+        "Tensor? turns=None, float amplitude=1.0, bool interleaved=False, Tensor? q=None) -> Tensor");
   m.def("load_kv(Tensor key_cache, Tensor value_cache, Tensor block_tables, "
         "Tensor context_lengths, Tensor cu_seqlens, int max_seqlen, int rows, "
         "Tensor? key_scale, Tensor? value_scale, ScalarType dtype) -> (Tensor, Tensor)");
@@ -1263,6 +1294,7 @@ TORCH_LIBRARY_IMPL(rlt_mi355x, CUDA, m) {
   m.impl("token_logprobs", &token_logprobs);
   m.impl("commit_tree_kv", &commit_tree_kv);
   m.impl("rotary", &rotary);
+  m.impl("rotary_", &rotary_);
   m.impl("append_kv", &append_kv);
   m.impl("load_kv", &load_kv);
 }

@@ -200,12 +200,13 @@ def commit_tree_kv(key_pool, value_pool, tables, starts, path, accepted, block_s
 def _packed(block_tables, context_lengths, cu_seqlens):
     tables = block_tables if block_tables.dtype == torch.int32 else block_tables.to(torch.int32)
     tables = tables if tables.ndim != 2 or tables.stride(1) == 1 else tables.contiguous()
-    return (tables, *(x.to(torch.int32).contiguous() for x in (context_lengths, cu_seqlens)))
+    return (tables, *(x if x.dtype == torch.int32 and x.is_contiguous() else
+                      x.to(torch.int32).contiguous() for x in (context_lengths, cu_seqlens)))
 
 
 def append_kv(key_cache, value_cache, k, v, block_tables, context_lengths, cu_seqlens_q,
               max_seqlen_q, key_scale=None, value_scale=None, *, rotary=None, positions=None,
-              q=None, inplace=False):
+              q=None):
     """Append windows of keys and values ``[rows, kv_heads, head_dim]`` to the paged cache, keys
     (and queries) turned by their positions on the way, in one launch.  Returns the turned
     ``q``, or None without one.
@@ -214,8 +215,7 @@ def append_kv(key_cache, value_cache, k, v, block_tables, context_lengths, cu_se
     ``max_seqlen_q``), which become its last positions: row i goes to position
     ``context_lengths[s] - rows + i`` of ``block_tables[s]``, as ``prefill`` reads them.
     ``rotary`` (``Rotary``; None: no rotation) turns k and ``q`` ``[rows, heads, head_dim]`` by
-    that position, or by ``positions`` (``[rows]``) where they differ, as a tree's nodes do;
-    ``inplace`` turns q itself.  Rows before position 0, past the table or whose block lies
+    that position, or by ``positions`` (``[rows]``) where they differ, as a tree's nodes do.  Rows before position 0, past the table or whose block lies
     outside the pool are not written (their q is turned).
 
     Pools ``[block, token, kv_head, dim]`` of the rows' type, or 8-bit ones with float32 scales:
@@ -232,25 +232,20 @@ def append_kv(key_cache, value_cache, k, v, block_tables, context_lengths, cu_se
 
     Runs ``torch.ops.rlt_mi355x.append_kv``.
     """
-    from .rotary import _heads, _positions, _target
+    from .rotary import _heads, _positions
 
     _lib.require_gpu(key_cache, value_cache, k, v, block_tables, context_lengths, cu_seqlens_q,
                      key_scale, value_scale, positions, q)
     k, v = _rows(k, "k"), _rows(v, "v")
-    q_out = None
-    if q is not None:
-        q_out = _target(q, True, "q") if inplace else None
-        q = _heads(q, "q")
-        q_out = _target(q, False, "q") if q_out is None else q_out
+    q = None if q is None else _heads(q, "q")
     if positions is not None:
         positions = _positions(positions, k.shape[0])
     tables, lengths, cu = _packed(block_tables, context_lengths, cu_seqlens_q)
-    _lib.ops().append_kv(key_cache, value_cache, k, v, tables, lengths, cu, int(max_seqlen_q),
-                         key_scale, value_scale, positions,
-                         None if rotary is None else rotary.turns,
-                         1.0 if rotary is None else rotary.amplitude,
-                         False if rotary is None else rotary.interleaved, q, q_out)
-    return q_out
+    turn = (None, 1.0, False) if rotary is None else (rotary.turns, rotary.amplitude,
+                                                      rotary.interleaved)
+    q_out = _lib.ops().append_kv(key_cache, value_cache, k, v, tables, lengths, cu,
+                                 int(max_seqlen_q), key_scale, value_scale, positions, *turn, q)
+    return None if q is None else q_out
 
 
 def load_kv(key_cache, value_cache, block_tables, context_lengths, cu_seqlens, max_seqlen, rows,

@@ -7,7 +7,7 @@ kernels: the per-step entry points -- ``paged_attention``, ``paged_attention_sto
 ``store_kv``, ``spec_probs``, ``categorical``, ``spec_accept``, ``greedy_accept``,
 ``verify_distributions``, ``verify_accept``, and those of the draft-tree round
 (``tree_attention``, ``tree_masks``, ``tree_accept``, ``greedy_tree_accept``,
-``commit_tree_kv``, ``token_logprobs``), ``rotary``, ``append_kv`` and ``load_kv`` -- are C++ operators
+``commit_tree_kv``, ``token_logprobs``), ``rotary``, ``rotary_``, ``append_kv`` and ``load_kv`` -- are C++ operators
 (``csrc/torch_bindings.cpp`` -> ``_C.so``: schema, argument checks, workspace and
 launch, one dispatcher call per step); the rest are Python ``torch.library``
 custom ops over the same library.  Every operator has an implementation for ROCm
@@ -47,15 +47,20 @@ def _(q, key_cache, value_cache, block_tables, context_lengths, cu_seqlens_q, ma
 
 
 @torch.library.register_fake("rlt_mi355x::rotary")
-def _(q, k, positions, turns, amplitude, interleaved, inverse, q_out, k_out):
+def _(q, k, positions, turns, amplitude, interleaved, inverse):
+    return q.new_empty(q.shape), q.new_empty((0,) if k is None else k.shape)
+
+
+@torch.library.register_fake("rlt_mi355x::rotary_")
+def _(q, k, positions, turns, amplitude, interleaved, inverse):
     return None
 
 
 @torch.library.register_fake("rlt_mi355x::append_kv")
 def _(key_cache, value_cache, k, v, block_tables, context_lengths, cu_seqlens_q, max_seqlen_q,
       key_scale=None, value_scale=None, positions=None, turns=None, amplitude=1.0,
-      interleaved=False, q=None, q_out=None):
-    return None
+      interleaved=False, q=None):
+    return k.new_empty((0,) if q is None else q.shape)
 
 
 @torch.library.register_fake("rlt_mi355x::load_kv")
@@ -228,4 +233,4 @@ OPS = ("paged_attention", "paged_attention_store", "tree_attention", "tree_masks
        "greedy_tree_accept", "tree_accept", "token_logprobs", "commit_tree_kv", "spec_probs",
        "categorical", "spec_accept", "greedy_accept", "propose_drafts", "verify_distributions", "verify_accept", "merge_random_round",
        "rejection_rows", "store_kv",
-       "store_fp8", "finalize_rows", "rotary", "append_kv", "load_kv")
+       "store_fp8", "finalize_rows", "rotary", "rotary_", "append_kv", "load_kv")

@@ -102,15 +102,6 @@ def _positions(positions, rows):
     return p if p.is_contiguous() else p.contiguous()
 
 
-def _target(x, inplace, name):
-    """Where a turned tensor goes: a fresh one, or the tensor itself."""
-    if not inplace:
-        return torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    if x.stride(-1) != 1 or any(n > 1 and s == 0 for n, s in zip(x.shape, x.stride())):
-        raise ValueError(f"{name} cannot be turned in place: its rows share memory or are strided")
-    return x
-
-
 def apply_rotary(q, k, positions, rotary, *, inverse=False, inplace=False):
     """Queries ``[rows, heads, head_dim]`` and keys ``[rows, kv_heads, head_dim]`` (or None)
     turned by ``positions`` (``[rows]``), in one launch: ``(q', k')``.
@@ -119,15 +110,14 @@ def apply_rotary(q, k, positions, rotary, *, inverse=False, inplace=False):
     turn and the rest is copied.  ``inverse`` turns back (the transpose of the rotation times
     the amplitude, so that it takes a gradient of the outputs to one of the inputs);
     ``inplace`` writes q and k themselves.  Angles are reduced in float64, sums are float32,
-    rounded once.  Runs ``torch.ops.rlt_mi355x.rotary``.
+    rounded once.  Runs ``torch.ops.rlt_mi355x.rotary`` (``rotary_`` in place).
     """
     _lib.require_gpu(q, k, positions, rotary.turns)
+    rest = (_positions(positions, q.shape[0]), rotary.turns, rotary.amplitude, rotary.interleaved,
+            bool(inverse))
     if inplace:
-        q_out, k_out = _target(q, True, "q"), None if k is None else _target(k, True, "k")
-    q = _heads(q, "q")
-    k = None if k is None else _heads(k, "k")
-    if not inplace:
-        q_out, k_out = _target(q, False, "q"), None if k is None else _target(k, False, "k")
-    _lib.ops().rotary(q, k, _positions(positions, q.shape[0]), rotary.turns, rotary.amplitude,
-                      rotary.interleaved, bool(inverse), q_out, k_out)
-    return q_out, k_out
+        _lib.ops().rotary_(q, k, *rest)
+        return q, k
+    if k is None:
+        return _lib.ops().rotary(_heads(q, "q"), None, *rest)[0], None
+    return _lib.ops().rotary(_heads(q, "q"), _heads(k, "k"), *rest)
