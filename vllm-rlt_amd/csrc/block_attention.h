@@ -16,9 +16,11 @@
 // 32 positions as one contraction.  A lane holds the place and the two scales of one tile of
 // its span, looked up once, which a tile takes by lane reads into scalar registers: no table, no
 // division and no scale load inside the stream.  The key scale enters with the exponent's one
-// fma; the value scale multiplies the weights of the product, over a power of two near the span's
-// largest, which the output takes back (exact; fp16 weights lie 2^kBlockLift above their place,
-// since its normal numbers end at 2^-14).  The running maximum moves only when it is passed by
+// fma.  The product with the values is fp16's whatever q's type: codes are exact in it, and it rounds
+// a weight to 11 bits (outputs 1.05 times as far from float64 as one of float32 weights, rounded to
+// bf16; with bf16 weights 1.42 times).  Its weights take the value scale over a power of two near
+// the span's largest, which the output takes back, and lie 2^kBlockLift above their place, since
+// fp16's normal numbers end at 2^-14.  The running maximum moves only when it is passed by
 // 2^kBlockLazy, and sums stay with the lanes until the end.
 #pragma once
 
@@ -48,8 +50,7 @@ constexpr int kBlockParts = 4;                           // waves of a unit
 constexpr int kBlockChunk = 1024;
 constexpr int kBlockSpan = kBlockChunk / kBlockParts;    // positions of a wave
 constexpr float kBlockLazy = 4.f;                        // log2 headroom before the running maximum moves
-template <int QT>
-constexpr int kBlockLift = QT == RLT_F16 ? 15 - (int)kBlockLazy : 0;
+constexpr int kBlockLift = 15 - (int)kBlockLazy;
 // registers: 168 hold one row tile of up to 128 dims, 256 the others
 template <int D, int NT>
 constexpr int block_waves_per_simd() { return D <= 128 && NT == 1 ? 3 : 2; }
@@ -131,8 +132,9 @@ template <int QT, int KVT, int D, int NT, bool CP>
 __device__ __forceinline__ void block_part(const AttnParams& P, const SeqView& sv, int seq, int rg_begin, int rg_rows,
                                            int kvh, int w_begin, int part, BlockShared<NT, D>& sh) {
   using M = Mfma<QT>;
+  using W = Mfma<RLT_F16>;  // weights and values
   using KeySlice = BlockKeys<QT, KVT, D>;
-  using VQ = BlockValues<QT, KVT, D>;
+  using VQ = BlockValues<RLT_F16, KVT, D>;
   constexpr int NQS = D / 32;  // 32-wide contraction slices
   constexpr int ND = D / 16;   // 16-wide output column tiles (= dims per lane)
   const int lane = threadIdx.x & 63, l16 = lane & 15, grp = lane >> 4;
@@ -227,7 +229,7 @@ __device__ __forceinline__ void block_part(const AttnParams& P, const SeqView& s
   float most = fabsf(v_tile);
 #pragma unroll
   for (int o = 32; o >= 1; o >>= 1) most = fmaxf(most, __shfl_xor(most, o, RLT_WAVE));
-  const int v_exp = (most > 0.f ? __builtin_amdgcn_frexp_expf(most) : 0) - kBlockLift<QT>;
+  const int v_exp = (most > 0.f ? __builtin_amdgcn_frexp_expf(most) : 0) - kBlockLift;
   v_tile = __builtin_amdgcn_ldexpf(v_tile, -v_exp);
 
   // pairs inside [full_lo, full_hi) are visible to every row
@@ -303,10 +305,10 @@ __device__ __forceinline__ void block_part(const AttnParams& P, const SeqView& s
         x[0][r] *= g0;
         x[1][r] *= g1;
       }
-      p[nt] = make_uint4(M::pack2(x[0][0], x[0][1]), M::pack2(x[0][2], x[0][3]),
-                         M::pack2(x[1][0], x[1][1]), M::pack2(x[1][2], x[1][3]));
+      p[nt] = make_uint4(W::pack2(x[0][0], x[0][1]), W::pack2(x[0][2], x[0][3]),
+                         W::pack2(x[1][0], x[1][1]), W::pack2(x[1][2], x[1][3]));
       if (CP) {
-        auto rest = [&](uint32_t w, float a, float b) { return M::pack2(a - M::lo_f32(w), b - M::hi_f32(w)); };
+        auto rest = [&](uint32_t w, float a, float b) { return W::pack2(a - W::lo_f32(w), b - W::hi_f32(w)); };
         dropped[nt] = make_uint4(rest(p[nt].x, x[0][0], x[0][1]), rest(p[nt].y, x[0][2], x[0][3]),
                                  rest(p[nt].z, x[1][0], x[1][1]), rest(p[nt].w, x[1][2], x[1][3]));
       }
@@ -334,11 +336,11 @@ __device__ __forceinline__ void block_part(const AttnParams& P, const SeqView& s
       const uint4 v0 = make_uint4(a0.x, a0.y, b0.x, b0.y), v1 = make_uint4(a1.x, a1.y, b1.x, b1.y);
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
-        oacc[nt][2 * K] = M::qk(v0, p[nt], oacc[nt][2 * K]);
-        oacc[nt][2 * K + 1] = M::qk(v1, p[nt], oacc[nt][2 * K + 1]);
+        oacc[nt][2 * K] = W::qk(v0, p[nt], oacc[nt][2 * K]);
+        oacc[nt][2 * K + 1] = W::qk(v1, p[nt], oacc[nt][2 * K + 1]);
         if (CP) {
-          oacc[nt][2 * K] = M::qk(v0, dropped[nt], oacc[nt][2 * K]);
-          oacc[nt][2 * K + 1] = M::qk(v1, dropped[nt], oacc[nt][2 * K + 1]);
+          oacc[nt][2 * K] = W::qk(v0, dropped[nt], oacc[nt][2 * K]);
+          oacc[nt][2 * K + 1] = W::qk(v1, dropped[nt], oacc[nt][2 * K + 1]);
         }
       }
     });

@@ -161,10 +161,13 @@ __global__ __launch_bounds__(kPfThreads, 2) void rlt_prefill_kernel(AttnParams P
   constexpr bool FP8 = KVT != QT;
   static_assert(!FP8 || KVT == RLT_FP8_E4M3 || KVT == RLT_INT8, "16-bit pools match q");
   static_assert(FP8 == (SM != 0), "scale modes are for 8-bit pools");
-  // fp16 has few exponents: there the weights times block scales are held over a power of two near
-  // the largest scale that the rows see, kLift above their place, and the running max follows
-  // closer (weights up to 2^kLazy), so that scales down to 2^-20 of the largest keep their bits
-  constexpr bool REFER = SM == 3 && QT == RLT_F16;
+  // Block scales: the product with the values is fp16's whatever q's type, since codes are exact in
+  // it and it rounds a weight to 11 bits.  fp16 has few exponents: weights times scales are held
+  // over a power of two near the largest scale that the rows see, kLift above their place, and the
+  // running max follows closer (weights up to 2^kLazy), so that scales down to 2^-20 of the
+  // largest keep their bits
+  constexpr bool REFER = SM == 3;
+  constexpr int VT = SM == 3 ? RLT_F16 : QT;  // of the weights and values in the product
   constexpr float kLazy = REFER ? 1.f : kPfLazy;
   constexpr int kLift = 15 - (int)kLazy;
   constexpr int FJ = kPfKeys * SLOTS / kPfThreads;  // fp8 LDS slots per thread per tile (K, V each)
@@ -376,8 +379,8 @@ __global__ __launch_bounds__(kPfThreads, 2) void rlt_prefill_kernel(AttnParams P
       if (PIECES == SLOTS || v_slot<SLOTS>(r, sl) < PIECES) {
         uint2 v0 = make_uint2(0, 0), v1 = v0;
         if (tile * kPfKeys + r < hi_last) {
-          v0 = codes_to_16<QT, KVT>(vraw[j].x);
-          v1 = codes_to_16<QT, KVT>(vraw[j].y);
+          v0 = codes_to_16<VT, KVT>(vraw[j].x);
+          v1 = codes_to_16<VT, KVT>(vraw[j].y);
         }
         uint2* vd = (uint2*)(sh.v[b] + r * L::kRowB + sl * 16);
         vd[0] = v0;
@@ -506,8 +509,8 @@ __global__ __launch_bounds__(kPfThreads, 2) void rlt_prefill_kernel(AttnParams P
 #pragma unroll
       for (int i = 0; i < 4; ++i) x[i] *= y[i];
     }
-    p[2 * g] = M::pack2(x[0], x[1]);
-    p[2 * g + 1] = M::pack2(x[2], x[3]);
+    p[2 * g] = Mfma<VT>::pack2(x[0], x[1]);
+    p[2 * g + 1] = Mfma<VT>::pack2(x[2], x[3]);
     // (made here: the compiler would sink them to their use, behind the mask's branch)
     asm volatile("" : "+v"(p[2 * g]), "+v"(p[2 * g + 1]), "+v"(l_run));
   };
@@ -532,7 +535,7 @@ __global__ __launch_bounds__(kPfThreads, 2) void rlt_prefill_kernel(AttnParams P
       __builtin_amdgcn_sched_barrier(0);
       if (n + kAheadV < 4 * ND) read_v(a[(n + kAheadV) % (kAheadV + 1)], n + kAheadV, b);
       const u32x4 pc = {p[4 * c], p[4 * c + 1], p[4 * c + 2], p[4 * c + 3]};
-      oacc[dt] = mfma32<QT>(a[n % (kAheadV + 1)], pc, oacc[dt]);
+      oacc[dt] = mfma32<VT>(a[n % (kAheadV + 1)], pc, oacc[dt]);
       beside(n);
     }
     __builtin_amdgcn_sched_barrier(0);
