@@ -168,6 +168,11 @@ __global__ __launch_bounds__(kPfThreads, 2) void rlt_prefill_kernel(AttnParams P
   // largest keep their bits
   constexpr bool REFER = SM == 3;
   constexpr int VT = SM == 3 ? RLT_F16 : QT;  // of the weights and values in the product
+  // A tile's four 16-position groups then have one scale each: the key scale goes into the maxima
+  // and the exponent's fma, the value scale (at least 2^-60 of the largest, below which it adds
+  // nothing) into the exponent as its log2, which each group's sum takes back: 76 multiplies of a
+  // tile's 32 weights a lane become 16, and 16 LDS reads 3.  8 x 2048 in int8 234 -> XX us.
+  constexpr bool GROUPS = SM == 3 && UB;
   constexpr float kLazy = REFER ? 1.f : kPfLazy;
   constexpr int kLift = 15 - (int)kLazy;
   constexpr int FJ = kPfKeys * SLOTS / kPfThreads;  // fp8 LDS slots per thread per tile (K, V each)
@@ -344,14 +349,28 @@ __global__ __launch_bounds__(kPfThreads, 2) void rlt_prefill_kernel(AttnParams P
     for (int j = 0; j < NJ; ++j) load_v_piece(b, j, access(blks, j), access(offs, j));
   };
   // the scales of the cursor's tile, read into a register (wave 0 keys, wave 1 values)
+  float qk_scale = P.qk_scale_log2;
   int v_exp = 0;  // REFER: the weights of the product are taken over 2^(v_exp - kLift)
   auto load_scale = [&](int tile) {
     const float x = (w == 0 ? P.k_scale : P.v_scale)[pool_block(scur.next) * P.s_block_stride +
                                                      (int64_t)scur.off * P.s_token_stride +
                                                      (int64_t)kvh * P.s_head_stride];
-    sraw = tile * kPfKeys + lane < hi_last ? x : 0.f;
-    if constexpr (REFER) {
-      if (w == 1) sraw = __builtin_amdgcn_ldexpf(sraw, kLift - v_exp);
+    if constexpr (GROUPS) {
+      // lanes j and 4 + j: group j's (a group that no row sees has keys and weights of any scale)
+      const int at = tile * kPfKeys + 16 * (lane & 3);
+      const bool seen = at < hi_last && at + 16 > lo_first;
+      if (w == 0) {
+        sraw = seen ? (x < 1.17549435e-38f ? 1.17549435e-38f : x) * qk_scale : 1.f;
+      } else {
+        const float r = seen ? __builtin_amdgcn_ldexpf(x, -v_exp) : 1.f;
+        const float e = __builtin_amdgcn_logf(r < 8.67361738e-19f ? 8.67361738e-19f : r) + (float)kLift;
+        sraw = lane & 4 ? __builtin_amdgcn_exp2f(-e) : e;
+      }
+    } else {
+      sraw = tile * kPfKeys + lane < hi_last ? x : 0.f;
+      if constexpr (REFER) {
+        if (w == 1) sraw = __builtin_amdgcn_ldexpf(sraw, kLift - v_exp);
+      }
     }
     scur.advance(P, table, dq, dr);
   };
@@ -378,7 +397,8 @@ __global__ __launch_bounds__(kPfThreads, 2) void rlt_prefill_kernel(AttnParams P
       const int r = e / SLOTS, sl = e % SLOTS;
       if (PIECES == SLOTS || v_slot<SLOTS>(r, sl) < PIECES) {
         uint2 v0 = make_uint2(0, 0), v1 = v0;
-        if (tile * kPfKeys + r < hi_last) {
+        // (block scales: those before a sliding window's first position may be any, too)
+        if (tile * kPfKeys + r < hi_last && (SM != 3 || tile * kPfKeys + r >= lo_first)) {
           v0 = codes_to_16<VT, KVT>(vraw[j].x);
           v1 = codes_to_16<VT, KVT>(vraw[j].y);
         }
@@ -416,7 +436,6 @@ __global__ __launch_bounds__(kPfThreads, 2) void rlt_prefill_kernel(AttnParams P
                      (lane & 1) * 8;
   const int v_x = SLOTS >= 16 ? i4 : i4 >> 1;
 
-  float qk_scale = P.qk_scale_log2;
   float v_mul = 1.f;
   if (SM == 1) {
     qk_scale *= P.k_scale[0];
@@ -451,7 +470,7 @@ __global__ __launch_bounds__(kPfThreads, 2) void rlt_prefill_kernel(AttnParams P
   };
   // per-vector key scales and the position mask of the tile's scores, in place
   auto scale_scores = [&](f32x16 (&s)[2], int b) {
-    if constexpr (SM >= 2) {
+    if constexpr (SM >= 2 && !GROUPS) {
 #pragma unroll
       for (int u = 0; u < 2; ++u)
 #pragma unroll
@@ -482,8 +501,15 @@ __global__ __launch_bounds__(kPfThreads, 2) void rlt_prefill_kernel(AttnParams P
     m = fmaxf(fmaxf(m, s[g >> 2][i]), s[g >> 2][i + 1]);
     m = fmaxf(fmaxf(m, s[g >> 2][i + 2]), s[g >> 2][i + 3]);
   };
-  auto move_max = [&](float m) {
-    const float mx = half_max(m) * qk_scale;
+  // the largest score: of the groups' maxima, raw, in the tile of buffer b
+  constexpr int NM = GROUPS ? 4 : 1;
+  auto move_max = [&](const float (&ms)[NM], int b) {
+    float m = ms[0];
+    if constexpr (GROUPS) {
+      const f32x4 f = *(const f32x4*)sh.ks[b];
+      m = fmaxf(fmaxf(ms[0] * f[0], ms[1] * f[1]), fmaxf(ms[2] * f[2], ms[3] * f[3]));
+    }
+    const float mx = GROUPS ? half_max(m) : half_max(m) * qk_scale;
     const bool grow = mx > m_run + kLazy;
     if (__builtin_amdgcn_ballot_w64(grow) != 0) {
       const float m_new = grow ? mx : m_run;
@@ -498,13 +524,30 @@ __global__ __launch_bounds__(kPfThreads, 2) void rlt_prefill_kernel(AttnParams P
   };
   // ---- weights of four of the tile's scores (positions 8 g + 4 h + [0, 4)): words 2 g and
   // 2 g + 1 of the P^T operands (chunk g / 2)
+  // GROUPS: the scales of the tile whose weights are made
+  // (in scalar registers: the vector ones are all taken)
+  float gk[4], ge[4], gi[4];
+  auto take_scales = [&](int b) {
+    if constexpr (GROUPS) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        gk[j] = __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(sh.ks[b][j])));
+        ge[j] = __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(sh.vs[b][j])));
+        gi[j] = __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(sh.vs[b][4 + j])));
+      }
+    }
+  };
   auto weigh_quad = [&](const f32x16 (&s)[2], uint32_t (&p)[16], int g, int b) {
     float x[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      x[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[g >> 2][4 * (g & 3) + i], qk_scale, -m_use));
-    l_run += (x[0] + x[1]) + (x[2] + x[3]);
-    if constexpr (SM >= 2) {
+    for (int i = 0; i < 4; ++i) {
+      const float y = s[g >> 2][4 * (g & 3) + i];
+      x[i] = GROUPS ? __builtin_amdgcn_exp2f(__builtin_fmaf(y, gk[g >> 1], ge[g >> 1] - m_use))
+                    : __builtin_amdgcn_exp2f(__builtin_fmaf(y, qk_scale, -m_use));
+    }
+    if constexpr (GROUPS) l_run += ((x[0] + x[1]) + (x[2] + x[3])) * gi[g >> 1];
+    else l_run += (x[0] + x[1]) + (x[2] + x[3]);
+    if constexpr (SM >= 2 && !GROUPS) {
       const f32x4 y = *(const f32x4*)(sh.vs[b] + 8 * g + 4 * h);
 #pragma unroll
       for (int i = 0; i < 4; ++i) x[i] *= y[i];
@@ -568,7 +611,7 @@ __global__ __launch_bounds__(kPfThreads, 2) void rlt_prefill_kernel(AttnParams P
     // ---- first tiles: K and V of kt0, K of kt0 + 1, the scores of kt0
 #pragma unroll
     for (int c = 0; c < CUR; ++c) cur[c].start(P, table, kt0 * kPfKeys + cursor_row(c));
-    if (scale_wave) scur.start(P, table, kt0 * kPfKeys + lane);
+    if (scale_wave) scur.start(P, table, kt0 * kPfKeys + (GROUPS ? 16 * (lane & 3) : lane));
     next_blocks();
     load_k(0);
     load_v(0, kblk, koff);
@@ -600,9 +643,11 @@ __global__ __launch_bounds__(kPfThreads, 2) void rlt_prefill_kernel(AttnParams P
     scores(sa, 0, [](int) {});
     scale_scores(sa, 0);
     mask(sa, kt0);
-    float mx = -INFINITY;
-    quads(0, 1, [&](int g) { max_quad(mx, sa, g); });
-    move_max(mx);
+    float mx[NM];
+#pragma unroll
+    for (int i = 0; i < NM; ++i) mx[i] = -INFINITY;
+    quads(0, 1, [&](int g) { max_quad(mx[GROUPS ? g >> 1 : 0], sa, g); });
+    move_max(mx, 0);
     __syncthreads();  // K buffer 0 is free
 
     // one tile: `cur_s` are its scores, b its buffers; the next tile's scores go to `next_s`
@@ -620,6 +665,7 @@ __global__ __launch_bounds__(kPfThreads, 2) void rlt_prefill_kernel(AttnParams P
       if constexpr (kEarlyV) load_v(b ^ 1, vblk, voff);
       if (SM >= 2 && (w == 1 || (w == 0 && more))) load_scale(tile + (w == 0 ? 2 : 1));
       uint32_t p[16];
+      take_scales(b);
       scores(next_s, b ^ 1, [&](int c) {
         quads(c, NQS, [&](int g) { weigh_quad(cur_s, p, g, b); });
       });
@@ -630,11 +676,13 @@ __global__ __launch_bounds__(kPfThreads, 2) void rlt_prefill_kernel(AttnParams P
       }
       scale_scores(next_s, b ^ 1);
       mask(next_s, tile + 1);
-      float mx = -INFINITY;
+      float mx[NM];
+#pragma unroll
+      for (int i = 0; i < NM; ++i) mx[i] = -INFINITY;
       accumulate(p, b, [&](int n) {
-        quads(n, 4 * ND, [&](int g) { max_quad(mx, next_s, g); });
+        quads(n, 4 * ND, [&](int g) { max_quad(mx[GROUPS ? g >> 1 : 0], next_s, g); });
       });
-      move_max(mx);
+      move_max(mx, b ^ 1);
       if constexpr (FP8) {
         put_v(tile + 1, b ^ 1);
         if (SM >= 2 && w == 1) sh.vs[b ^ 1][lane] = sraw;
@@ -647,6 +695,7 @@ __global__ __launch_bounds__(kPfThreads, 2) void rlt_prefill_kernel(AttnParams P
     };
     auto last = [&](int b, f32x16 (&cur_s)[2]) {
       uint32_t p[16];
+      take_scales(b);
       quads(0, 1, [&](int g) { weigh_quad(cur_s, p, g, b); });
       accumulate(p, b, [](int) {});
     };
