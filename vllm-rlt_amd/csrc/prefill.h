@@ -171,7 +171,7 @@ __global__ __launch_bounds__(kPfThreads, 2) void rlt_prefill_kernel(AttnParams P
   // A tile's four 16-position groups then have one scale each: the key scale goes into the maxima
   // and the exponent's fma, the value scale (at least 2^-60 of the largest, below which it adds
   // nothing) into the exponent as its log2, which each group's sum takes back: 76 multiplies of a
-  // tile's 32 weights a lane become 16, and 16 LDS reads 3.  8 x 2048 in int8 234 -> XX us.
+  // tile's 32 weights a lane become 16, and 16 LDS reads 3.  8 x 2048 in int8 234 -> 212 us.
   constexpr bool GROUPS = SM == 3 && UB;
   constexpr float kLazy = REFER ? 1.f : kPfLazy;
   constexpr int kLift = 15 - (int)kLazy;
@@ -185,7 +185,11 @@ __global__ __launch_bounds__(kPfThreads, 2) void rlt_prefill_kernel(AttnParams P
   // latency shows on cold keys: 8 windows of up to 130 rows behind 3000, 16 heads of 64 dims,
   // 80.7 -> 62.3 us; with per-vector scales it took 88.6 -> 93.1)
   constexpr bool kEarlyV = SM == 1 && D <= 64;
-  constexpr int NC = FP8 ? FJ : 1;  // 16-position groups a wave loads from per tile
+  // block scales: a wave's rows are one 16-position group, as those of direct loads, so that it
+  // follows one block and not four (their addresses were 360 scalar instructions a tile: 8 x 2048
+  // in int8 212 -> 195 us)
+  constexpr bool OWN = !FP8 || GROUPS;
+  constexpr int NC = OWN ? 1 : FJ;  // 16-position groups a wave loads from per tile
   __shared__ L sh;
   const int t = threadIdx.x, lane = t & 63, l32 = lane & 31, h = lane >> 5;
   const int w = __builtin_amdgcn_readfirstlane(t >> 6);
@@ -263,7 +267,7 @@ __global__ __launch_bounds__(kPfThreads, 2) void rlt_prefill_kernel(AttnParams P
   // per access took 44.3 us where this takes 30.0, 4 prompts of 300-500 rows at block size 8)
   auto cursor_row = [&](int c) {
     const int i = UB ? ROWS_PER_LD * c : lane & 15;
-    const int r = FP8 ? i / ROWS_PER_LD * (kPfThreads / SLOTS) + w * ROWS_PER_LD + i % ROWS_PER_LD
+    const int r = !OWN ? i / ROWS_PER_LD * (kPfThreads / SLOTS) + w * ROWS_PER_LD + i % ROWS_PER_LD
                       : 16 * w + i;
     return UB ? r & ~15 : r;
   };
@@ -281,8 +285,8 @@ __global__ __launch_bounds__(kPfThreads, 2) void rlt_prefill_kernel(AttnParams P
   // bytes from a 16-position group's first row to what this lane reads of it.  The swizzle's
   // piece of an fp8 item is the same for every j; a direct load's rows are ROWS_PER_LD
   // apart (the scalar base moves), which changes the piece of K only
-  const int lane_r = FP8 ? (t / SLOTS) & 15 : ld_row;
-  const int lane_sl = FP8 ? t % SLOTS : ld_slot;
+  const int lane_r = !OWN ? (t / SLOTS) & 15 : ld_row;
+  const int lane_sl = !OWN ? t % SLOTS : ld_slot;
   constexpr int ELT = FP8 ? 1 : 2;  // bytes of a pool element
   const uint32_t k_tok = (uint32_t)P.k_token_stride * ELT, v_tok = (uint32_t)P.v_token_stride * ELT;
   const int v_piece = v_slot<SLOTS>(lane_r, lane_sl);
@@ -293,8 +297,8 @@ __global__ __launch_bounds__(kPfThreads, 2) void rlt_prefill_kernel(AttnParams P
   auto load_k_piece = [&](int b, int j, int64_t blk, int off) {
     const uint8_t* base = (const uint8_t*)P.k +
                           (blk * P.k_block_stride + k_head + (int64_t)off * P.k_token_stride) * ELT;
-    const int pc = k_slot<SLOTS>(lane_r + (FP8 ? 0 : ROWS_PER_LD * j), lane_sl);
-    if (UB && !FP8) base += (int64_t)(ROWS_PER_LD * j) * k_tok;
+    const int pc = k_slot<SLOTS>(lane_r + (OWN ? ROWS_PER_LD * j : 0), lane_sl);
+    if (UB && OWN) base += (int64_t)(ROWS_PER_LD * j) * k_tok;
     const uint32_t lane_off = lane_r * k_tok + pc * 8 * ELT;
     // padded rows: lanes whose slot holds a piece past the row load nothing
     if (PIECES == SLOTS || pc < PIECES) {
@@ -310,9 +314,9 @@ __global__ __launch_bounds__(kPfThreads, 2) void rlt_prefill_kernel(AttnParams P
   auto load_v_piece = [&](int b, int j, int64_t blk, int off) {
     const uint8_t* base = (const uint8_t*)P.v +
                           (blk * P.v_block_stride + v_head + (int64_t)off * P.v_token_stride) * ELT;
-    static_assert(FP8 || ROWS_PER_LD % 4 == 0, "one V piece per lane");
+    static_assert(!OWN || ROWS_PER_LD % 4 == 0, "one V piece per lane");
     const int pc = v_piece;
-    if (UB && !FP8) base += (int64_t)(ROWS_PER_LD * j) * v_tok;
+    if (UB && OWN) base += (int64_t)(ROWS_PER_LD * j) * v_tok;
     if (PIECES == SLOTS || pc < PIECES) {
       if constexpr (FP8) {
         vraw[j] = UB ? *(const uint2*)(base + v_off) : *(const uint2*)(base + pc * 8);
@@ -336,7 +340,7 @@ __global__ __launch_bounds__(kPfThreads, 2) void rlt_prefill_kernel(AttnParams P
   };
   // block and offset of this lane's j-th access among the wave's
   auto access = [&](const int (&x)[CUR], int j) {
-    if (UB) return x[FP8 ? j : 0];
+    if (UB) return x[OWN ? 0 : j];
     return __builtin_amdgcn_ds_bpermute(4 * (ROWS_PER_LD * j + lane / SLOTS), x[0]);
   };
   auto load_k = [&](int b) {
@@ -380,7 +384,7 @@ __global__ __launch_bounds__(kPfThreads, 2) void rlt_prefill_kernel(AttnParams P
 #pragma unroll
     for (int j = 0; j < FJ; ++j) {
       const int e = j * kPfThreads + t;
-      const int r = e / SLOTS, sl = e % SLOTS;
+      const int r = OWN ? 16 * w + ROWS_PER_LD * j + ld_row : e / SLOTS, sl = OWN ? ld_slot : e % SLOTS;
       // (pad slots of 96-dim rows are never read: left unwritten)
       if (PIECES == SLOTS || k_slot<SLOTS>(r, sl) < PIECES) {
         const uint2 k0 = codes_to_16<QT, KVT>(kraw[j].x), k1 = codes_to_16<QT, KVT>(kraw[j].y);
@@ -394,7 +398,7 @@ __global__ __launch_bounds__(kPfThreads, 2) void rlt_prefill_kernel(AttnParams P
 #pragma unroll
     for (int j = 0; j < FJ; ++j) {
       const int e = j * kPfThreads + t;
-      const int r = e / SLOTS, sl = e % SLOTS;
+      const int r = OWN ? 16 * w + ROWS_PER_LD * j + ld_row : e / SLOTS, sl = OWN ? ld_slot : e % SLOTS;
       if (PIECES == SLOTS || v_slot<SLOTS>(r, sl) < PIECES) {
         uint2 v0 = make_uint2(0, 0), v1 = v0;
         // (block scales: those before a sliding window's first position may be any, too)
