@@ -293,6 +293,43 @@ def test_a_layer_step_by_step(pkg, dev, codes, rows):
         assert torch.equal(a.contiguous().view(torch.uint8), b.contiguous().view(torch.uint8))
 
 
+@pytest.mark.parametrize("codes", CODES)
+def test_queries_that_are_not_numbers(kernel, dev, codes):
+    """A NaN query gives NaN, in its own row alone; a sequence's blocks before a sliding window may hold any
+    scales (where blocks hold whole tiles, and in prompts)."""
+    _say("block nan")
+    for rows in (4, 70):
+        for bs in (16, 8):
+            c = Case(codes, torch.bfloat16, [(1500, rows), (90, rows)], 4, 2, 64, bs, seed=14)
+            want = c.packed(kernel, dev)
+            c.q[1, 2], c.q[rows + 2, 1, 5] = float("nan"), float("nan")
+            got = c.packed(kernel, dev)
+            bad = torch.zeros(got.shape[:2], dtype=torch.bool)
+            bad[1, 2] = bad[rows + 2, 1] = True
+            assert got[bad].isnan().all() and torch.equal(got[~bad], want[~bad])
+            c = Case(codes, torch.bfloat16, [(1500, rows)], 4, 2, 64, bs, seed=15)
+            want = c.packed(kernel, dev, window=40)
+            hidden = c.tables[0][:(1500 - rows + 1 - 40) // bs].long()
+            c.ks[hidden] = c.vs[hidden] = float("nan")
+            if bs == 16 or rows == 70:
+                assert torch.equal(c.packed(kernel, dev, window=40), want)
+
+
+def test_a_batch_with_padding(kernel, dev):
+    """Sequences without rows or without keys between others, and rows behind the last sequence: these are left."""
+    _say("block padding")
+    for codes in CODES:
+        c = Case(codes, torch.bfloat16, [(700, 3), (0, 2), (1100, 0), (33, 1), (0, 0)], 4, 2, 64, 16, seed=16)
+        q, k, v, tables, lengths, cu, ks, vs = c.args(dev)
+        got = c.packed(kernel, dev)
+        for s in (0, 3):
+            a, b = int(c.cu[s]), int(c.cu[s + 1])
+            one = kernel.prefill(q[a:b], k[:, 1], v[:, 1], tables[s:s + 1], lengths[s:s + 1],
+                                 torch.tensor([0, b - a], dtype=torch.int32, device=dev), b - a, ks[:, 1], vs[:, 1])
+            assert torch.equal(one.cpu(), got[a:b])
+        assert not got[3:5].any()
+
+
 def test_more_pairs_than_a_workgroup_lists(kernel, dev):
     """Batches past the persistent kernel's index run one workgroup per unit: the same bits."""
     _say("block many")

@@ -261,6 +261,11 @@ def dtype_code(dtype):
         raise ValueError(f"unsupported dtype {dtype}") from None
 
 
+def pool_code(dtype):
+    """A KV pool's type, int8 among them where its scales are the blocks'."""
+    return RLT_INT8 if dtype == torch.int8 else dtype_code(dtype)
+
+
 def check(status, what):
     if status != 0:
         raise RuntimeError(f"{what}: {_STATUS.get(status, f'status {status}')}")

@@ -109,9 +109,9 @@ class MI355XPagedAttention:
 
     Pools: q's type; float8_e4m3fn with 0-d scales (per tensor) or scales ``[block, token,
     kv_head]`` (per vector); float8_e4m3fn or int8 with one scale per block of tokens and kv
-    head, ``[block, kv_head]``, as ``kv_write.append_kv`` writes them (not ``tree``).  With
-    float16 q the value scales of the blocks that a row reads may differ by a factor of 2^20
-    before weights lose bits.
+    head, ``[block, kv_head]``, as ``kv_write.append_kv`` writes them: positive (not ``tree``).
+    Value scales of the blocks that a row reads may differ by a factor of 2^20 before weights
+    of the smaller ones lose bits.
     """
 
     generation = None
@@ -216,14 +216,14 @@ class MI355XPagedAttention:
     def uses_mfma(self, q_dtype, kv_dtype, head_dim):
         lib = _lib.library()
         return bool(lib.rlt_paged_attention_uses_mfma(_lib.dtype_code(q_dtype),
-                                                      _lib.dtype_code(kv_dtype), head_dim))
+                                                      _lib.pool_code(kv_dtype), head_dim))
 
     def uses_prefill_tiling(self, q_dtype, kv_dtype, head_dim, max_seqlen_q):
         """True when ``prefill`` calls with this longest window take the long-prompt
         tiling (equal to the per-row form within tolerance, not bit for bit)."""
         lib = _lib.library()
         return bool(lib.rlt_paged_attention_uses_prefill(
-            _lib.dtype_code(q_dtype), _lib.dtype_code(kv_dtype), head_dim, max_seqlen_q))
+            _lib.dtype_code(q_dtype), _lib.pool_code(kv_dtype), head_dim, max_seqlen_q))
 
 
 _BACKEND_NAMES = ("auto", "mi355x")

@@ -3,9 +3,16 @@
 //
 //   out = sum_t w_t s_v[b(t)] c_v(t) / sum_t w_t,  w_t = exp(q . c_k(t) s_k[b(t)] / sqrt(D) - m)
 //
+// What bounds it: HBM reads.  64 rows at 16k-32k positions of 8 heads in int8, 3.18 GB: 611 us with
+// the merge, 5.2 TB/s (1 GB: 218 us), whatever the kv heads, block size, loads in flight (one or
+// two pairs of tiles) and waves (8 or 12 a CU); non-temporal loads are slower (629).  Windows of 5
+// over GQA 4, 157 MB, 46 us: one or two units a workgroup, each a chain of lengths -> table ->
+// tiles -> combine; one row at 700 positions 11.4 us.
+//
 // Work.  A unit is (sequence, row-group, kv head, chunk): 1024 absolute key positions, a quarter
 // of them to each of a workgroup's four waves, whose softmax states (maximum, sum,
-// unnormalized output) are combined through LDS in part order.  A row whose keys lie in one chunk
+// unnormalized output) are combined through LDS in part order.  (Chunks of 512 leave twice the
+// partials: 611 -> 656 us; a wave alone on a chunk, 36 us for the one row.)  A row whose keys lie in one chunk
 // is normalized there; others leave a partial per chunk for rlt_merge_kernel.  Persistent
 // workgroups, as many as share the CUs' registers, take the units of all sequences in turn, as
 // rlt_attn_mfma_kernel does; a row's arithmetic depends on its own keys and absolute positions
@@ -223,9 +230,10 @@ __device__ __forceinline__ void block_part(const AttnParams& P, const SeqView& s
     for (int dt = 0; dt < ND; ++dt) oacc[nt][dt] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
 
-  // scales: positive (a key scale of 0 counts as the smallest normal number: a masked score
-  // times it stays -inf)
-  k_tile = P.qk_scale_log2 * (k_tile < 1.17549435e-38f ? 1.17549435e-38f : k_tile);
+  // (scales are positive; one of 0 counts as the smallest normal number: a masked score times it
+  // stays -inf)
+  k_tile *= P.qk_scale_log2;
+  k_tile = k_tile < 1.17549435e-38f ? 1.17549435e-38f : k_tile;
   float most = fabsf(v_tile);
 #pragma unroll
   for (int o = 32; o >= 1; o >>= 1) most = fmaxf(most, __shfl_xor(most, o, RLT_WAVE));
@@ -465,10 +473,11 @@ void rlt_block_attention_kernel(AttnParams P) {
       for (int i = 0; i < kBlockParts; ++i) m = fmaxf(m, sh.ml[i][row][0]);
 #pragma unroll
       for (int i = 0; i < kBlockParts; ++i) {
-        const float mi = sh.ml[i][row][0];
-        if (mi == -INFINITY) continue;  // (a part without a key)
-        const float s = __builtin_amdgcn_exp2f(mi - m);
-        l += sh.ml[i][row][1] * s;
+        const float mi = sh.ml[i][row][0], li = sh.ml[i][row][1];
+        if (mi == -INFINITY && li == 0.f) continue;  // (a part without a key)
+        // (scores that are all NaN leave no maximum, and a NaN for a sum)
+        const float s = mi == -INFINITY ? li : __builtin_amdgcn_exp2f(mi - m);
+        l += li * s;
         o += *(const f32x4*)(sh.o[i] + row * BlockShared<NT, D>::kStride + d) * s;
       }
       if (chunks <= 1) {
@@ -488,8 +497,18 @@ void rlt_block_attention_kernel(AttnParams P) {
   }
 }
 
+// Where a workgroup for every (row-group, kv head, chunk) of the tables fits on the CUs at once,
+// each takes its own, without the list of units (two barriers and the lengths of all sequences:
+// one row at 700 positions 12.0 -> 11.4 us, 8 windows of 5 at 2-4k 23.2 -> 22.2); more of them
+// than that would leave the order in which they read to the dispatcher (64 rows at 512-4096,
+// 16 heads: 142 us, and 183 so).
 template <int QT, int KVT, int D, bool CP>
-int launch_block_cp(const AttnParams& P, dim3 grid, int nt, hipStream_t stream) {
+int launch_block_cp(AttnParams P, dim3 grid, int nt, hipStream_t stream) {
+  const int64_t all = (int64_t)P.num_seqs * P.rowgroups * P.hkv * P.max_chunks;
+  if (P.persistent && all <= (int64_t)grid.x) {
+    P.persistent = 0;
+    grid = dim3((unsigned)all);
+  }
   if (nt == 1) rlt_block_attention_kernel<QT, KVT, D, 1, CP><<<grid, 64 * kBlockParts, 0, stream>>>(P);
   else if (D <= 128)
     rlt_block_attention_kernel<QT, KVT, D, (D <= 128 ? 2 : 1), CP><<<grid, 64 * kBlockParts, 0, stream>>>(P);

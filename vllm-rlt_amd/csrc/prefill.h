@@ -364,7 +364,8 @@ __global__ __launch_bounds__(kPfThreads, 2) void rlt_prefill_kernel(AttnParams P
       const int at = tile * kPfKeys + 16 * (lane & 3);
       const bool seen = at < hi_last && at + 16 > lo_first;
       if (w == 0) {
-        sraw = seen ? (x < 1.17549435e-38f ? 1.17549435e-38f : x) * qk_scale : 1.f;
+        const float f = x * qk_scale;  // (at least a normal number: a masked score times it stays -inf)
+        sraw = !seen ? 1.f : f < 1.17549435e-38f ? 1.17549435e-38f : f;
       } else {
         const float r = seen ? __builtin_amdgcn_ldexpf(x, -v_exp) : 1.f;
         const float e = __builtin_amdgcn_logf(r < 8.67361738e-19f ? 8.67361738e-19f : r) + (float)kLift;
@@ -373,6 +374,7 @@ __global__ __launch_bounds__(kPfThreads, 2) void rlt_prefill_kernel(AttnParams P
     } else {
       sraw = tile * kPfKeys + lane < hi_last ? x : 0.f;
       if constexpr (REFER) {
+        if (tile * kPfKeys + lane < lo_first) sraw = 0.f;
         if (w == 1) sraw = __builtin_amdgcn_ldexpf(sraw, kLift - v_exp);
       }
     }

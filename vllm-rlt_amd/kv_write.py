@@ -20,6 +20,7 @@ outside the pool are skipped (the reference's kernels would write out of bounds)
 import torch
 
 from . import _lib
+from .rotary import _heads, _positions
 
 FP8_E4M3_MAX = 448.0
 _ROW_DTYPES = (torch.float32, torch.float16, torch.bfloat16)
@@ -197,11 +198,15 @@ def commit_tree_kv(key_pool, value_pool, tables, starts, path, accepted, block_s
                               _index(accepted, n, "accepted"), int(block_size))
 
 
+def _int32(x):
+    return x if x.dtype == torch.int32 and x.is_contiguous() else x.to(torch.int32).contiguous()
+
+
 def _packed(block_tables, context_lengths, cu_seqlens):
-    tables = block_tables if block_tables.dtype == torch.int32 else block_tables.to(torch.int32)
-    tables = tables if tables.ndim != 2 or tables.stride(1) == 1 else tables.contiguous()
-    return (tables, *(x if x.dtype == torch.int32 and x.is_contiguous() else
-                      x.to(torch.int32).contiguous() for x in (context_lengths, cu_seqlens)))
+    # (a table's rows may lie apart)
+    as_is = block_tables.dtype == torch.int32 and block_tables.ndim == 2 and block_tables.stride(1) == 1
+    return (block_tables if as_is else _int32(block_tables), _int32(context_lengths),
+            _int32(cu_seqlens))
 
 
 def append_kv(key_cache, value_cache, k, v, block_tables, context_lengths, cu_seqlens_q,
@@ -228,24 +233,23 @@ def append_kv(key_cache, value_cache, k, v, block_tables, context_lengths, cu_se
       as 0).  Where rows go on in a block that already holds tokens, the larger of that and the
       block's scale; if it grew, the earlier tokens' codes are quantized again over the new
       scale.  Rows at a block's first token begin it anew.  A block must be written by one
-      sequence of a call only.
+      sequence of a call only.  (``finalize_rows`` and ``commit_tree_kv`` move codes as they are:
+      not between blocks of such a cache, whose scales differ.)
 
+    Rows of no sequence, and those past ``max_seqlen_q`` of one, are left; their q' is undefined.
     Runs ``torch.ops.rlt_mi355x.append_kv``.
     """
-    from .rotary import _heads, _positions
-
     _lib.require_gpu(key_cache, value_cache, k, v, block_tables, context_lengths, cu_seqlens_q,
                      key_scale, value_scale, positions, q)
-    k, v = _rows(k, "k"), _rows(v, "v")
-    q = None if q is None else _heads(q, "q")
     if positions is not None:
-        positions = _positions(positions, k.shape[0])
+        positions = _positions(positions)
     tables, lengths, cu = _packed(block_tables, context_lengths, cu_seqlens_q)
     turn = (None, 1.0, False) if rotary is None else (rotary.turns, rotary.amplitude,
                                                       rotary.interleaved)
-    q_out = _lib.ops().append_kv(key_cache, value_cache, k, v, tables, lengths, cu,
-                                 int(max_seqlen_q), key_scale, value_scale, positions, *turn, q)
-    return None if q is None else q_out
+    turned = _lib.ops().append_kv(key_cache, value_cache, _heads(k), _heads(v), tables, lengths, cu,
+                                  int(max_seqlen_q), key_scale, value_scale, positions, *turn,
+                                  None if q is None else _heads(q))
+    return None if q is None else turned
 
 
 def load_kv(key_cache, value_cache, block_tables, context_lengths, cu_seqlens, max_seqlen, rows,

@@ -13,7 +13,6 @@ import torch
 from . import _lib
 
 SCALINGS = (None, "none", "linear", "ntk", "yarn", "bands")
-_ROW_DTYPES = (torch.float32, torch.float16, torch.bfloat16)
 
 
 class Rotary:
@@ -89,15 +88,12 @@ class Rotary:
                                   device=device)
 
 
-def _heads(x, name):
-    if x.ndim != 3 or x.dtype not in _ROW_DTYPES:
-        raise ValueError(f"{name} must be float32, float16 or bfloat16 [rows, heads, head_dim]")
-    return x if x.stride(-1) == 1 or x.shape[-1] <= 1 else x.contiguous()
+# (shapes, dtypes and devices are the operators' checks; what they read as it is, is made so here)
+def _heads(x):
+    return x if x.ndim != 3 or x.stride(2) == 1 else x.contiguous()
 
 
-def _positions(positions, rows):
-    if positions.shape != (rows,):
-        raise ValueError(f"positions must have shape [{rows}]")
+def _positions(positions):
     p = positions if positions.dtype == torch.int64 else positions.long()
     return p if p.is_contiguous() else p.contiguous()
 
@@ -113,11 +109,10 @@ def apply_rotary(q, k, positions, rotary, *, inverse=False, inplace=False):
     rounded once.  Runs ``torch.ops.rlt_mi355x.rotary`` (``rotary_`` in place).
     """
     _lib.require_gpu(q, k, positions, rotary.turns)
-    rest = (_positions(positions, q.shape[0]), rotary.turns, rotary.amplitude, rotary.interleaved,
-            bool(inverse))
+    rest = (_positions(positions), rotary.turns, rotary.amplitude, rotary.interleaved, bool(inverse))
     if inplace:
         _lib.ops().rotary_(q, k, *rest)
         return q, k
     if k is None:
-        return _lib.ops().rotary(_heads(q, "q"), None, *rest)[0], None
-    return _lib.ops().rotary(_heads(q, "q"), _heads(k, "k"), *rest)
+        return _lib.ops().rotary(_heads(q), None, *rest)[0], None
+    return _lib.ops().rotary(_heads(q), _heads(k), *rest)
