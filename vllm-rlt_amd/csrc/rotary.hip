@@ -20,8 +20,10 @@
 // a time), makes their sines and cosines once in LDS, and its four waves take the heads of q, k
 // and v in turn.  A lane holds both halves of its pairs (2 x 16 bytes), a group of LP lanes one
 // head vector, so that maxima are lane exchanges and a block's rows stay in registers between
-// its maximum and its codes.  What bounds it: each row is read and written once (HBM), and at a
-// few rows the chain lengths -> table -> rows -> scale -> codes of one launch.
+// its maximum and its codes.  What bounds it: each row is read and written once, at the rate of
+// a large copy (16384 rows of 20 heads of 128 in bf16, 168 MB: 34.8 us, 4.8 TB/s; 8 prompts of
+// 2048 into an int8 cache 45 us), and at a few rows the chain lengths -> table -> rows -> scale
+// -> codes of one launch (1 row: 3.4 us, 6.5 into block scales).
 
 #include "common.h"
 #include "fp8_codec.h"
@@ -635,7 +637,8 @@ __device__ __forceinline__ void store_elements(void* out, int64_t at, const floa
 }
 
 // A workgroup takes `tile_rows` rows of a sequence, whose blocks it looks up once; a thread a
-// column of W elements over the rows, so that its loads are in flight together.  HBM bounds it.
+// column of W elements over the rows, so that its loads are in flight together.  HBM bounds it
+// (16 sequences of up to 8192 positions of 8 heads in int8: 122 us, 4.5 TB/s).
 constexpr int kLoadRows = 8;
 template <int CT, int OT, int W>
 __global__ __launch_bounds__(kThreads) void rlt_kv_load_kernel(LoadParams P) {

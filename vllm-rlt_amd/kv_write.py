@@ -220,8 +220,9 @@ def append_kv(key_cache, value_cache, k, v, block_tables, context_lengths, cu_se
     ``max_seqlen_q``), which become its last positions: row i goes to position
     ``context_lengths[s] - rows + i`` of ``block_tables[s]``, as ``prefill`` reads them.
     ``rotary`` (``Rotary``; None: no rotation) turns k and ``q`` ``[rows, heads, head_dim]`` by
-    that position, or by ``positions`` (``[rows]``) where they differ, as a tree's nodes do.  Rows before position 0, past the table or whose block lies
-    outside the pool are not written (their q is turned).
+    that position, or by ``positions`` (``[rows]``) where they differ, as a tree's nodes do.  Rows
+    before position 0, past the table or whose block lies outside the pool are not written (their
+    q is turned).
 
     Pools ``[block, token, kv_head, dim]`` of the rows' type, or 8-bit ones with float32 scales:
 
