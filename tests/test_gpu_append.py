@@ -1,5 +1,7 @@
 """Appends into the paged cache and its reading back, against ``oracle/rotary.py``."""
 
+import math
+
 import pytest
 import torch
 
@@ -230,6 +232,27 @@ def test_tiny_and_huge_values(pkg, dev):
         _equal(r.run(pkg, dev), r.expect())
 
 
+@pytest.mark.parametrize("exponent", (-140, -126, -91, -90, -60, 60, 119, 120, 121, 126))
+def test_given_scales_at_both_ends(pkg, dev, exponent):
+    """Codes over one scale that is given are ``store_fp8``'s: values about, far above and far
+    below it, zeros of both signs, infinities and NaN."""
+    _say("given", exponent)
+    for sign in (1.0, -1.0):
+        r = Round("tensor", torch.float32, 16, 2, 64, [0, 2], [5, 5], seed=14)
+        r.ks = r.vs = torch.tensor(sign * 1.37 * 2.0 ** exponent)
+        for x in (r.new_k, r.new_v):
+            x *= float(r.ks) * 90
+            x[0, 0, :9] = torch.tensor([0.0, -0.0, 3e38, -3e38, 1e-44, -1e-44, math.inf, -math.inf, math.nan])
+        got = r.run(pkg, dev)
+        k, v = (_layer(x).to(dev) for x in (r.k, r.v))
+        scales = torch.zeros(k.shape[:3], device=dev)
+        blocks = r.tables[torch.repeat_interleave(torch.arange(2), torch.tensor(r.counts)), r.places // 16]
+        pkg.store_fp8(r.new_k.to(dev), r.new_v.to(dev), k, v, scales, scales.clone(), blocks.long().to(dev),
+                      (r.places % 16).to(dev), 448.0, fixed_scale=float(r.ks))
+        for a, b in zip(got[:2], (k, v)):
+            assert torch.equal(_bits(_layer(a)), _bits(b).cpu())
+
+
 def test_repeated_single_tokens(pkg, dev):
     """A sequence grown token by token, over several blocks, in place on the device."""
     _say("token by token")
@@ -329,6 +352,24 @@ def test_captured_appends_replay(pkg, dev):
         assert torch.equal(q, want)
         for a, b in zip((k, v, ks, vs), eager):
             assert torch.equal(_bits(a), _bits(b))
+
+
+@pytest.mark.parametrize("kind", POOLS)
+def test_a_longest_window_known_by_its_bound_only(pkg, dev, kind):
+    """``max_seqlen_q`` far above the rows: the same pools, and the same numbers read back."""
+    _say("bound", kind)
+    r = Round(kind, torch.bfloat16, 16, 2, 64, [0, 37, 5], [3, 40, 0], 31)
+    want, most = r.run(pkg, dev), max(r.counts)
+    for bound in (4096, 2 ** 31 - 1):
+        r.counts = [*r.counts[:2], bound]  # (run takes the largest)
+        got = r.run(pkg, dev)
+        r.counts[2] = 0
+        for a, b in zip(want, got):
+            assert (a is None) == (b is None) and (a is None or torch.equal(_bits(a), _bits(b)))
+        k, v, ks, vs = (None if x is None else x.to(dev) for x in got[:4])
+        rest = (r.tables.to(dev), torch.tensor(r.lengths, dtype=torch.int32, device=dev), r.cu.to(dev))
+        loads = [pkg.load_kv(_layer(k), _layer(v), *rest, n, 43, _layer(ks), _layer(vs)) for n in (most, bound)]
+        assert all(torch.equal(a, b) for a, b in zip(*loads))
 
 
 def test_another_stream(pkg, dev):

@@ -330,6 +330,16 @@ def test_a_batch_with_padding(kernel, dev):
         assert not got[3:5].any()
 
 
+def test_tables_without_columns(kernel, dev):
+    """No sequence has a block: rows of zeros, whatever the lengths."""
+    _say("block no columns")
+    for codes in CODES:
+        for rows in (1, 5, 80):
+            c = Case(codes, torch.bfloat16, [(90, rows), (90, rows)], 4, 2, 64, 16, seed=17)
+            c.tables = c.tables[:, :0].contiguous()
+            assert not c.packed(kernel, dev).any()
+
+
 def test_more_pairs_than_a_workgroup_lists(kernel, dev):
     """Batches past the persistent kernel's index run one workgroup per unit: the same bits."""
     _say("block many")

@@ -178,38 +178,49 @@ __device__ __forceinline__ void store_piece(void* base, int64_t at, const float 
 template <int MODE>
 constexpr float top_of() { return MODE == kBlockInt8 ? 127.f : rlt_fp8::kMax; }
 
-// A scale and its reciprocal.
+// A scale and its reciprocal; 0 where quotient() is not for it: a scale that is no positive number,
+// or at the ends of float32, where the reciprocal or the remainder would be subnormal.
 struct Divisor {
   float by, inverse;
 };
-__device__ __forceinline__ Divisor divisor(float scale) { return Divisor{scale, 1.f / scale}; }
+__device__ __forceinline__ Divisor divisor(float scale) {
+  return Divisor{scale, scale >= 0x1p-90f && scale <= 0x1p120f ? 1.f / scale : 0.f};
+}
 
 // x / scale, correctly rounded: the reciprocal is, the first quotient is off by an ulp at most and
-// the remainder exact (as long as it is no subnormal number), so that one more step rounds as
-// the division does, in 3 instructions for its 10.
+// the remainder exact (where the code is not 0: multiples of 2^-33 2^-113), so that one more step
+// rounds as the division does, in 3 instructions for its 10.
 __device__ __forceinline__ float quotient(float x, const Divisor& d) {
   const float q = x * d.inverse;
   return copysignf(fmaf(fmaf(-q, d.by, x), d.inverse, q), x);  // (the step turns -0 into 0)
 }
 
-// Codes of a block-scaled pool, round to nearest even: e4m3 keeps NaN and clamps the rest to
-// +-448; int8 has no NaN and takes it as 0.  (Infinities would make the remainder NaN.)
+// x / scale within +-M, NaN kept.  (Infinities would make the remainder NaN, and so would the
+// quotient of a scale that is given, far below x / M.)
 template <int MODE>
 __device__ __forceinline__ float clamped(float x, const Divisor& d) {
   constexpr float M = MODE == kBlockInt8 ? 127.f : rlt_fp8::kMax;
-  const float y = fabsf(x) < INFINITY ? quotient(x, d) : x;
+  const float far = MODE == kTensorFp8 ? x * d.inverse : x;
+  const float y = fabsf(far) < (MODE == kTensorFp8 ? 2.f * M : INFINITY) ? quotient(x, d) : far;
   const float c = fminf(fmaxf(y, -M), M);
-  return y != y ? (MODE == kBlockInt8 ? 0.f : y) : c;
+  return y != y ? y : c;
 }
-// four codes
+
+// Four codes, round to nearest even: e4m3 keeps NaN, int8 takes it as 0.
 template <int MODE>
 __device__ __forceinline__ uint32_t codes4(const float (&x)[4], const Divisor& d) {
+  bool plain = d.inverse != 0.f;
+  // (a NaN's sign stays, as store_fp8's; a vector that holds one has a scale of NaN)
+  if constexpr (MODE == kTensorFp8) plain &= x[0] == x[0] && x[1] == x[1] && x[2] == x[2] && x[3] == x[3];
   if constexpr (MODE == kBlockInt8) {
-    uint32_t b[4];
+    uint32_t w = 0;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) b[i] = (uint32_t)(int)rintf(clamped<MODE>(x[i], d)) & 0xffu;
-    return b[0] | b[1] << 8 | b[2] << 16 | b[3] << 24;
-  } else if constexpr (MODE == kBlockFp8) {
+    for (int i = 0; i < 4; ++i) {
+      const float y = plain ? clamped<MODE>(x[i], d) : fminf(fmaxf(x[i] / d.by, -127.f), 127.f);
+      w |= ((uint32_t)(int)rintf(x[i] != x[i] ? 0.f : y) & 0xffu) << (8 * i);
+    }
+    return w;
+  } else if (plain) {
     int w = __builtin_amdgcn_cvt_pk_fp8_f32(clamped<MODE>(x[0], d), clamped<MODE>(x[1], d), 0, false);
     return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(clamped<MODE>(x[2], d), clamped<MODE>(x[3], d), w, true);
   } else {
@@ -550,6 +561,7 @@ __global__ __launch_bounds__(kThreads, 4) void rlt_rotary_kernel(Params P) {
             scale = rlt_fp8::dynamic_scale(m);
           }
           if (e < 0) continue;
+          const Divisor by = divisor(scale);
           const int64_t at = (int64_t)e * s.dst_block + (int64_t)off * s.dst_row + (int64_t)head * s.dst_head;
           if (MODE == kVectorFp8 && in_group == 0)
             s.scale[(int64_t)e * P.s_block + (int64_t)off * P.s_token + (int64_t)head * P.s_head] = scale;
@@ -560,7 +572,7 @@ __global__ __launch_bounds__(kThreads, 4) void rlt_rotary_kernel(Params P) {
               const int el = half ? at_b[n] : at_a[n];
               if (el < 0) continue;
               if constexpr (MODE == kSame) store_piece<DT, W>(s.dst, at + el, held.x[st][n][half]);
-              else store_codes<MODE, W>(s.dst, at + el, held.x[st][n][half], Divisor{scale, 0.f});
+              else store_codes<MODE, W>(s.dst, at + el, held.x[st][n][half], by);
             }
           }
         }
@@ -831,12 +843,13 @@ int rlt_kv_append(const void* k, int64_t k_row_stride, int64_t k_head_stride, co
   P.lengths = context_lengths;
   P.cu = cu_seqlens_q;
   P.num_seqs = num_seqs;
-  P.max_rows = max_q_len;
+  if (max_q_len > rows) max_q_len = (int32_t)rows;  // (a longest window known by its bound only)
   // blocks that a window of max_q_len rows meets, or its groups of rows
   const int64_t tiles = in_blocks(mode) ? ((int64_t)max_q_len + block_size - 2) / block_size + 1
                                         : ((int64_t)max_q_len + rows_of(mode) - 1) / rows_of(mode);
   const int64_t gx = tiles * num_seqs;
   if (gx >= ((int64_t)1 << 31)) return RLT_ERR_UNSUPPORTED;
+  P.max_rows = max_q_len;
   P.tiles = (int32_t)tiles;
   const int elt = dtype == RLT_F32 ? 4 : 2, pair = 32 / elt;
   const int code = mode == kSame ? elt : 1, piece = 16 / elt * code;  // bytes of a piece in the pool
@@ -901,6 +914,7 @@ extern "C" int rlt_kv_load(const void* key_cache, const void* value_cache, int64
   if (!key_cache || !value_cache || !context_lengths || !cu_seqlens || !k_out || !v_out ||
       (table_width && !block_tables))
     return RLT_ERR_ARGUMENT;
+  if (max_len > rows) max_len = (int32_t)rows;
   LoadParams P;
   P.k = key_cache;
   P.v = value_cache;
