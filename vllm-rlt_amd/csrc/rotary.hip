@@ -179,12 +179,17 @@ template <int MODE>
 constexpr float top_of() { return MODE == kBlockInt8 ? 127.f : rlt_fp8::kMax; }
 
 // A scale and its reciprocal; 0 where quotient() is not for it: a scale that is no positive number,
-// or at the ends of float32, where the reciprocal or the remainder would be subnormal.
+// or at the ends of float32, where the reciprocal or the remainder would be subnormal.  (Scales
+// of blocks are positive, 2^122 at most; below 2^-90 they take the step all the same, whose
+// quotient may then be off by an ulp: a second form of the codes costs blocks of 64 int8
+// tokens 39.3 -> 41.6 us.)
 struct Divisor {
   float by, inverse;
 };
+template <int MODE>
 __device__ __forceinline__ Divisor divisor(float scale) {
-  return Divisor{scale, scale >= 0x1p-90f && scale <= 0x1p120f ? 1.f / scale : 0.f};
+  const bool fits = in_blocks(MODE) || (scale >= 0x1p-90f && scale <= 0x1p120f);
+  return Divisor{scale, fits ? 1.f / scale : 0.f};
 }
 
 // x / scale, correctly rounded: the reciprocal is, the first quotient is off by an ulp at most and
@@ -195,35 +200,38 @@ __device__ __forceinline__ float quotient(float x, const Divisor& d) {
   return copysignf(fmaf(fmaf(-q, d.by, x), d.inverse, q), x);  // (the step turns -0 into 0)
 }
 
-// x / scale within +-M, NaN kept.  (Infinities would make the remainder NaN, and so would the
+// x / scale within +-M; e4m3 keeps NaN, int8 takes it as 0.  (Infinities would make the remainder NaN, and so would the
 // quotient of a scale that is given, far below x / M.)
 template <int MODE>
 __device__ __forceinline__ float clamped(float x, const Divisor& d) {
   constexpr float M = MODE == kBlockInt8 ? 127.f : rlt_fp8::kMax;
-  const float far = MODE == kTensorFp8 ? x * d.inverse : x;
-  const float y = fabsf(far) < (MODE == kTensorFp8 ? 2.f * M : INFINITY) ? quotient(x, d) : far;
+  float y;
+  if constexpr (MODE == kTensorFp8) {
+    const float q = x * d.inverse;
+    y = fabsf(q) < 2.f * M ? quotient(x, d) : q;
+  } else {
+    y = fabsf(x) < INFINITY ? quotient(x, d) : x;
+  }
   const float c = fminf(fmaxf(y, -M), M);
-  return y != y ? y : c;
+  return y != y ? (MODE == kBlockInt8 ? 0.f : y) : c;
 }
 
-// Four codes, round to nearest even: e4m3 keeps NaN, int8 takes it as 0.
+// four codes, round to nearest even
 template <int MODE>
 __device__ __forceinline__ uint32_t codes4(const float (&x)[4], const Divisor& d) {
-  bool plain = d.inverse != 0.f;
-  // (a NaN's sign stays, as store_fp8's; a vector that holds one has a scale of NaN)
-  if constexpr (MODE == kTensorFp8) plain &= x[0] == x[0] && x[1] == x[1] && x[2] == x[2] && x[3] == x[3];
   if constexpr (MODE == kBlockInt8) {
-    uint32_t w = 0;
+    uint32_t b[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float y = plain ? clamped<MODE>(x[i], d) : fminf(fmaxf(x[i] / d.by, -127.f), 127.f);
-      w |= ((uint32_t)(int)rintf(x[i] != x[i] ? 0.f : y) & 0xffu) << (8 * i);
-    }
-    return w;
-  } else if (plain) {
-    int w = __builtin_amdgcn_cvt_pk_fp8_f32(clamped<MODE>(x[0], d), clamped<MODE>(x[1], d), 0, false);
-    return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(clamped<MODE>(x[2], d), clamped<MODE>(x[3], d), w, true);
+    for (int i = 0; i < 4; ++i) b[i] = (uint32_t)(int)rintf(clamped<MODE>(x[i], d)) & 0xffu;
+    return b[0] | b[1] << 8 | b[2] << 16 | b[3] << 24;
   } else {
+    bool plain = in_blocks(MODE) || d.inverse != 0.f;
+    // (a NaN's sign stays, as store_fp8's; a vector that holds one has a scale of NaN)
+    if constexpr (MODE == kTensorFp8) plain &= x[0] == x[0] && x[1] == x[1] && x[2] == x[2] && x[3] == x[3];
+    if (plain) {
+      int w = __builtin_amdgcn_cvt_pk_fp8_f32(clamped<MODE>(x[0], d), clamped<MODE>(x[1], d), 0, false);
+      return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(clamped<MODE>(x[2], d), clamped<MODE>(x[3], d), w, true);
+    }
     uint32_t w = 0;
 #pragma unroll
     for (int i = 0; i < 4; ++i) w |= rlt_fp8::encode(x[i], d.by) << (8 * i);
@@ -512,7 +520,7 @@ __global__ __launch_bounds__(kThreads, 4) void rlt_rotary_kernel(Params P) {
         const float m = several ? tops[item] : top(held, c1 - c0);
         const float fresh = fmaxf(m * (1.f / top_of<MODE>()), rlt_fp8::kTiny);
         const float scale = o0 > 0 && old > fresh ? old : fresh;
-        const Divisor by = divisor(scale);
+        const Divisor by = divisor<MODE>(scale);
         const int64_t base = (int64_t)entry * s.dst_block + (int64_t)head * s.dst_head;
         if (c0 == i0 && o0 > 0 && scale > old) {
           // the block's earlier codes, over the new scale
@@ -561,7 +569,7 @@ __global__ __launch_bounds__(kThreads, 4) void rlt_rotary_kernel(Params P) {
             scale = rlt_fp8::dynamic_scale(m);
           }
           if (e < 0) continue;
-          const Divisor by = divisor(scale);
+          const Divisor by = divisor<MODE>(scale);
           const int64_t at = (int64_t)e * s.dst_block + (int64_t)off * s.dst_row + (int64_t)head * s.dst_head;
           if (MODE == kVectorFp8 && in_group == 0)
             s.scale[(int64_t)e * P.s_block + (int64_t)off * P.s_token + (int64_t)head * P.s_head] = scale;
