@@ -47,6 +47,9 @@ def test_scaled_frequencies(pkg):
     ((64,), {"scaling": "yarn", "factor": 2.0}), ((2,), {"scaling": "ntk", "factor": 2.0}),
     ((64,), {"scaling": "bands", "factor": 2.0, "original_length": 10, "fast": 1.0}),
     ((64,), {"divisors": [1.0]}), ((4,), {"divisors": [1.0, 0.0]}),
+    ((4,), {"divisors": [1.0, math.inf]}), ((64,), {"amplitude": math.nan}),
+    ((64,), {"scaling": "yarn", "factor": 2.0, "original_length": math.inf}),
+    ((64,), {"scaling": "bands", "factor": 2.0, "original_length": 10, "fast": math.inf}),
 ])
 def test_plans_refuse(pkg, args, kwargs):
     with pytest.raises(ValueError):

@@ -58,10 +58,10 @@ class Rotary:
         if scaling == "linear":
             f = [x / factor for x in f]
         elif scaling in ("yarn", "bands"):
-            if original_length is None or original_length <= 0:
+            if original_length is None or not 0 < original_length < math.inf:
                 raise ValueError(f"{scaling} scaling needs original_length")
             fast = (32.0 if scaling == "yarn" else 4.0) if fast is None else fast
-            if not fast > slow > 0:
+            if not math.inf > fast > slow > 0:
                 raise ValueError("fast must be above slow, both positive")
             if scaling == "yarn":
                 if base == 1.0:
@@ -78,9 +78,11 @@ class Rotary:
                 divided = [1.0 - min(max((n - slow) / (fast - slow), 0.0), 1.0) for n in turns]
             f = [x * (1.0 - d) + x / factor * d for x, d in zip(f, divided)]
         if divisors is not None:
-            if len(divisors) != half or not all(d > 0 for d in divisors):
+            if len(divisors) != half or not all(0 < d < math.inf for d in divisors):
                 raise ValueError("divisors must be rotary_dim / 2 positive numbers")
             f = [x / float(d) for x, d in zip(f, divisors)]
+        if amplitude is not None and not math.isfinite(amplitude):
+            raise ValueError("amplitude must be a number")
         self.rotary_dim = rotary_dim
         self.interleaved = bool(interleaved)
         self.amplitude = 1.0 if amplitude is None else float(amplitude)
