@@ -17,6 +17,11 @@
 // direct loads of K(i+2) and V(i+1) are in flight, into the buffers whose tiles were
 // last read in iteration i - 1.  The order inside a phase is fixed by scheduling barriers
 // (left to itself the compiler moves the exponentials behind the products).
+// Scales have the buffers of their tiles, and iteration i = tile of buffer b ends with one
+// barrier, ahead of which wave 0 stores the key scales of tile i + 2 into ks[b] and wave 1 the
+// value scales of tile i + 1 into vs[b ^ 1]: between two barriers ks is read at b ^ 1 only (the
+// scores and the maximum of tile i + 1) and vs at b only (the weights of tile i).  Key scales
+// that the weights need too (block scales) go on in registers from the maximum.
 //
 // What bounds it: a 128-row tile needs ~1030 cycles of a SIMD's matrix core, ~600 of its
 // vector unit and ~1020 of the CU's LDS reads (32 KB a wave: every wave reads the whole K
@@ -508,11 +513,16 @@ __global__ __launch_bounds__(kPfThreads, 2) void rlt_prefill_kernel(AttnParams P
     m = fmaxf(fmaxf(m, s[g >> 2][i + 2]), s[g >> 2][i + 3]);
   };
   // the largest score: of the groups' maxima, raw, in the tile of buffer b
+  // GROUPS: the scales of the tile whose weights are made next, the keys' from its maximum on
+  // (in scalar registers: the vector ones are all taken)
+  float gk[4], ge[4], gi[4];
   constexpr int NM = GROUPS ? 4 : 1;
   auto move_max = [&](const float (&ms)[NM], int b) {
     float m = ms[0];
     if constexpr (GROUPS) {
       const f32x4 f = *(const f32x4*)sh.ks[b];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) gk[j] = __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(f[j])));
       m = fmaxf(fmaxf(ms[0] * f[0], ms[1] * f[1]), fmaxf(ms[2] * f[2], ms[3] * f[3]));
     }
     const float mx = GROUPS ? half_max(m) : half_max(m) * qk_scale;
@@ -530,14 +540,11 @@ __global__ __launch_bounds__(kPfThreads, 2) void rlt_prefill_kernel(AttnParams P
   };
   // ---- weights of four of the tile's scores (positions 8 g + 4 h + [0, 4)): words 2 g and
   // 2 g + 1 of the P^T operands (chunk g / 2)
-  // GROUPS: the scales of the tile whose weights are made
-  // (in scalar registers: the vector ones are all taken)
-  float gk[4], ge[4], gi[4];
+  // (the key scales of its buffer may be the next tile's by now)
   auto take_scales = [&](int b) {
     if constexpr (GROUPS) {
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        gk[j] = __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(sh.ks[b][j])));
         ge[j] = __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(sh.vs[b][j])));
         gi[j] = __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(sh.vs[b][4 + j])));
       }
