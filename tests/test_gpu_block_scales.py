@@ -28,3 +28,62 @@ def test_prompts_whose_key_scales_differ_by_tile(kernel, dev, codes, dtype, dim,
         _near(got, *c.expect(window), c.q)
         for _ in range(8):
             assert torch.equal(c.packed(kernel, dev, window), got)
+
+
+def _single(kernel, dev, c, window=0, lengths=None):
+    """The rows of a packed case one by one; by their own lengths where those are given."""
+    q, k, v, tables, _, _, ks, vs = c.args(dev)
+    seq = torch.cat([torch.full((n,), s) for s, (_, n) in enumerate(c.seqs)]).to(dev)
+    if lengths is None:
+        lengths = torch.cat([torch.arange(n - r + 1, n + 1) for n, r in c.seqs])
+    rest = (tables[seq], lengths.int().to(dev))
+    if window:
+        return kernel.windowed(q, k[:, 1], v[:, 1], *rest, window, ks[:, 1], vs[:, 1]).cpu()
+    return kernel(q, k[:, 1], v[:, 1], *rest, ks[:, 1], vs[:, 1]).cpu()
+
+
+ACROSS = [(706, 5), (690, 4), (1025, 5), (33, 20), (20, 20), (1030, 16), (1281, 3), (17, 2)]
+
+
+@pytest.mark.parametrize("codes", CODES)
+@pytest.mark.parametrize("dtype,hq,hkv,dim,bs", [(torch.bfloat16, 8, 4, 128, 16), (torch.float16, 4, 1, 64, 16),
+                                                 (torch.bfloat16, 2, 2, 256, 32), (torch.bfloat16, 8, 4, 96, 16)])
+@pytest.mark.parametrize("log2", (12, 24, 40, 90))
+def test_rows_beside_a_block_of_larger_values(pkg, kernel, dev, codes, dtype, hq, hkv, dim, bs, log2):
+    """The scale of a block that only the rows beside it see does not reach a row: packed rows have the bits
+    of single ones, and are as near float64 as without it."""
+    if dtype == torch.float16 and log2 > 12:
+        return  # (such outputs are past its largest number)
+    _say("larger beside", codes, dtype, dim, log2)
+    c = Case(codes, dtype, ACROSS, hq, hkv, dim, bs, seed=22)
+    last = torch.tensor([int(c.tables[s][-(-n // bs) - 1]) for s, (n, _) in enumerate(c.seqs)])
+    c.vs[last] *= 2.0 ** log2
+    c.q *= 2  # (weights over a wider range)
+    got = c.packed(kernel, dev)
+    assert torch.equal(got, _single(kernel, dev, c))
+    assert torch.equal(c.packed(pkg.MI355XPagedAttention(compensate=True), dev),
+                       _single(pkg.MI355XPagedAttention(compensate=True), dev, c))
+    want, most = c.expect()
+    reads = torch.cat([torch.arange(n - r, n) // bs == (n - 1) // bs for n, r in c.seqs])
+    _near(got[~reads], want[~reads], most[~reads], c.q)
+    if log2 <= 12:
+        _near(got, want, most, c.q)
+    # a sliding window that the first rows' larger block leaves
+    first = torch.tensor([int(c.tables[s][(n - r - 32) // bs]) for s, (n, r) in enumerate(c.seqs) if n - r > 48])
+    c.vs[first] *= 2.0 ** min(log2, 24)
+    assert torch.equal(c.packed(kernel, dev, window=33), _single(kernel, dev, c, window=33))
+
+
+@pytest.mark.parametrize("codes", CODES)
+def test_row_lengths_far_apart_beside_larger_values(kernel, dev, codes):
+    """Explicit row lengths in any order, every block with values a thousand times those of the one before."""
+    _say("lengths apart", codes)
+    c = Case(codes, torch.bfloat16, [(900, 30), (130, 14)], 4, 2, 128, 16, seed=23)
+    for s, (n, _) in enumerate(c.seqs):
+        for i in range(-(-n // 16)):
+            c.vs[int(c.tables[s][i])] *= 2.0 ** (10 * (i % 9))
+    g = torch.Generator().manual_seed(24)
+    rl = torch.cat([torch.randint(0, n + 1, (r,), generator=g) for n, r in c.seqs]).int()
+    q, k, v, tables, lengths, cu, ks, vs = c.args(dev)
+    got = kernel.prefill(q, k[:, 1], v[:, 1], tables, lengths, cu, 30, ks[:, 1], vs[:, 1], row_lengths=rl.to(dev))
+    assert torch.equal(got.cpu(), _single(kernel, dev, c, lengths=rl))

@@ -27,8 +27,9 @@
 // fma.  The product with the values is fp16's whatever q's type: codes are exact in it, and it rounds
 // a weight to 11 bits (outputs 1.05 times as far from float64 as one of float32 weights, rounded to
 // bf16; with bf16 weights 1.42 times).  Its weights take the value scale over a power of two near
-// the span's largest, which the output takes back, and lie 2^kBlockLift above their place, since
-// fp16's normal numbers end at 2^-14.  The running maximum moves only when it is passed by
+// the largest that their row sees in the span (the row's own, as the maximum, or rows would
+// round by what those beside them see: 0.4 us of the one row's 12), which the output takes back, and
+// lie 2^kBlockLift above their place, since fp16's normal numbers end at 2^-14.  The running maximum moves only when it is passed by
 // 2^kBlockLazy, and sums stay with the lanes until the end.
 #pragma once
 
@@ -235,11 +236,40 @@ __device__ __forceinline__ void block_part(const AttnParams& P, const SeqView& s
   // stays -inf)
   k_tile *= P.qk_scale_log2;
   k_tile = k_tile < 1.17549435e-38f ? 1.17549435e-38f : k_tile;
-  float most = fabsf(v_tile);
+  // the power of two that a row's weights are taken over: of the largest value scale among the tiles
+  // that it sees itself, whatever the rows beside it see
+  int v_exp[NT];
+  {
+    float most[NT];
+    if (lo_last < w_begin + (v0 + 1) * kTileTok && hi_first > w_begin + tl * kTileTok) {
+      // (every row sees some of the first and the last tile, and so all, which lanes 0 to 15 hold)
+      float all = fabsf(v_tile);
+      auto turned = [&](auto ctrl) {
+        return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(all), decltype(ctrl)::value, 0xf, 0xf, false));
+      };
+      all = fmaxf(all, turned(std::integral_constant<int, 0x128>{}));  // lanes 8 on, of 16
+      all = fmaxf(all, turned(std::integral_constant<int, 0x124>{}));
+      all = fmaxf(all, turned(std::integral_constant<int, 0x122>{}));
+      all = fmaxf(all, turned(std::integral_constant<int, 0x121>{}));
+      all = __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(all)));
 #pragma unroll
-  for (int o = 32; o >= 1; o >>= 1) most = fmaxf(most, __shfl_xor(most, o, RLT_WAVE));
-  const int v_exp = (most > 0.f ? __builtin_amdgcn_frexp_expf(most) : 0) - kBlockLift;
-  v_tile = __builtin_amdgcn_ldexpf(v_tile, -v_exp);
+      for (int nt = 0; nt < NT; ++nt) most[nt] = all;
+    } else {
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) most[nt] = 0.f;
+#pragma unroll 1
+      for (int t = v0; t < t1; ++t) {
+        const float x = fabsf(tile_scale(v_tile, t));
+        const int tb = w_begin + t * kTileTok;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+          most[nt] = tb < row_hi[nt] && tb + kTileTok > row_lo[nt] ? fmaxf(most[nt], x) : most[nt];
+      }
+    }
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+      v_exp[nt] = (most[nt] > 0.f ? __builtin_amdgcn_frexp_expf(most[nt]) : 0) - kBlockLift;
+  }
 
   // pairs inside [full_lo, full_hi) are visible to every row
   const int span_end = w_begin + kBlockSpan;
@@ -276,8 +306,19 @@ __device__ __forceinline__ void block_part(const AttnParams& P, const SeqView& s
         }
     }
     const float f0 = tile_scale(k_tile, t), f1 = tile_scale(k_tile, t + 1);
-    const float g0 = tile_scale(v_tile, t), g1 = tile_scale(v_tile, t + 1);
-    float mx[NT];
+    const float s0 = tile_scale(v_tile, t), s1 = tile_scale(v_tile, t + 1);
+    float g0[NT], g1[NT], mx[NT];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      g0[nt] = __builtin_amdgcn_ldexpf(s0, -v_exp[nt]);
+      g1[nt] = __builtin_amdgcn_ldexpf(s1, -v_exp[nt]);
+      if (!full) {
+        // (the scale of a tile that the row does not see is any multiple of its largest)
+        const int lo = row_lo[nt] - tb, hi = row_hi[nt] - tb;
+        g0[nt] = hi > 0 && lo < kTileTok ? g0[nt] : 0.f;
+        g1[nt] = hi > kTileTok && lo < 2 * kTileTok ? g1[nt] : 0.f;
+      }
+    }
     bool grow = false;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
@@ -311,8 +352,8 @@ __device__ __forceinline__ void block_part(const AttnParams& P, const SeqView& s
       l_run[nt] += ((x[0][0] + x[0][1]) + (x[0][2] + x[0][3])) + ((x[1][0] + x[1][1]) + (x[1][2] + x[1][3]));
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        x[0][r] *= g0;
-        x[1][r] *= g1;
+        x[0][r] *= g0[nt];
+        x[1][r] *= g1[nt];
       }
       p[nt] = make_uint4(W::pack2(x[0][0], x[0][1]), W::pack2(x[0][2], x[0][3]),
                          W::pack2(x[1][0], x[1][1]), W::pack2(x[1][2], x[1][3]));
@@ -359,9 +400,9 @@ __device__ __forceinline__ void block_part(const AttnParams& P, const SeqView& s
 #pragma unroll 1
   for (int t = t0; t < t1; t += 2) pair(t);
 
-  const float back = __builtin_amdgcn_ldexpf(1.f, v_exp);
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
+    const float back = __builtin_amdgcn_ldexpf(1.f, v_exp[nt]);
     const float l = group_sum(l_run[nt]);
     const int row = nt * 16 + l16;
     if (grp == 0) {
