@@ -87,3 +87,30 @@ def test_row_lengths_far_apart_beside_larger_values(kernel, dev, codes):
     q, k, v, tables, lengths, cu, ks, vs = c.args(dev)
     got = kernel.prefill(q, k[:, 1], v[:, 1], tables, lengths, cu, 30, ks[:, 1], vs[:, 1], row_lengths=rl.to(dev))
     assert torch.equal(got.cpu(), _single(kernel, dev, c, lengths=rl))
+
+
+@pytest.mark.parametrize("codes", CODES)
+@pytest.mark.parametrize("dtype,hq,hkv,dim,bs", [(torch.bfloat16, 8, 2, 128, 16), (torch.bfloat16, 4, 4, 64, 64),
+                                                 (torch.bfloat16, 2, 1, 96, 8), (torch.float16, 4, 4, 128, 32)])
+@pytest.mark.parametrize("log2", (12, 30, 75))
+def test_prompts_beside_a_block_of_larger_values(kernel, dev, codes, dtype, hq, hkv, dim, bs, log2):
+    """Rows of a prompt whose last block's values are far larger: those that do not see it are as near float64
+    as without it; so are rows that a sliding window took past one."""
+    if dtype == torch.float16 and log2 > 12:
+        return  # (such outputs are past its largest number)
+    _say("prompts, larger beside", codes, dtype, dim, bs, log2)
+    c = Case(codes, dtype, [(400, 400), (333, 100), (129, 129), (70, 65)], hq, hkv, dim, bs, seed=25)
+    last = torch.tensor([int(c.tables[s][-(-n // bs) - 1]) for s, (n, _) in enumerate(c.seqs)])
+    c.vs[last] *= 2.0 ** log2
+    got = c.packed(kernel, dev)
+    want, most = c.expect()
+    reads = torch.cat([torch.arange(n - r, n) // bs == (n - 1) // bs for n, r in c.seqs])
+    _near(got[~reads], want[~reads], most[~reads], c.q)
+    if log2 <= 12:
+        _near(got, want, most, c.q)
+    c.vs[last] *= 2.0 ** -log2
+    c.vs[int(c.tables[0][300 // bs])] *= 2.0 ** log2
+    got, (want, most) = c.packed(kernel, dev, 50), c.expect(50)
+    at = torch.cat([torch.arange(n - r, n) for n, r in c.seqs])
+    reads = (at < 400) & (torch.arange(len(at)) < 400) & (at // bs >= 300 // bs) & ((at - 49) // bs <= 300 // bs)
+    _near(got[~reads], want[~reads], most[~reads], c.q)

@@ -168,18 +168,20 @@ __global__ __launch_bounds__(kPfThreads, 2) void rlt_prefill_kernel(AttnParams P
   static_assert(FP8 == (SM != 0), "scale modes are for 8-bit pools");
   // Block scales: the product with the values is fp16's whatever q's type, since codes are exact in
   // it and it rounds a weight to 11 bits.  fp16 has few exponents: weights times scales are held
-  // over a power of two near the largest scale that the rows see, kLift above their place, and the
+  // over a power of two near the largest scale that their row sees, kLift above their place, and the
   // running max follows closer (weights up to 2^kLazy), so that scales down to 2^-20 of the
-  // largest keep their bits
+  // row's largest keep their bits.  (Staged scales are over the rows' largest, from which a row's
+  // weights and sum take what its own is below that, up to 2^kBelow)
   constexpr bool REFER = SM == 3;
   constexpr int VT = SM == 3 ? RLT_F16 : QT;  // of the weights and values in the product
   // A tile's four 16-position groups then have one scale each: the key scale goes into the maxima
-  // and the exponent's fma, the value scale (at least 2^-60 of the largest, below which it adds
-  // nothing) into the exponent as its log2, which each group's sum takes back: 76 multiplies of a
+  // and the exponent's fma, the value scale (at least 2^-100 of the rows' largest: 2^-20 of that of
+  // a row 2^kBelow below it) into the exponent as its log2, which each group's sum takes back: 76 multiplies of a
   // tile's 32 weights a lane become 16, and 16 LDS reads 3.  8 x 2048 in int8 234 -> 212 us.
   constexpr bool GROUPS = SM == 3 && UB;
   constexpr float kLazy = REFER ? 1.f : kPfLazy;
   constexpr int kLift = 15 - (int)kLazy;
+  constexpr int kBelow = 80;  // (a row's sum is up to 2^kBelow times its weights')
   constexpr int FJ = kPfKeys * SLOTS / kPfThreads;  // fp8 LDS slots per thread per tile (K, V each)
   static_assert(FJ * kPfThreads == kPfKeys * SLOTS, "the threads' fp8 slots cover a tile");
   // operand reads in flight ahead of their MFMAs: S^T slices, O^T steps (fp8 tiles leave
@@ -359,7 +361,8 @@ __global__ __launch_bounds__(kPfThreads, 2) void rlt_prefill_kernel(AttnParams P
   };
   // the scales of the cursor's tile, read into a register (wave 0 keys, wave 1 values)
   float qk_scale = P.qk_scale_log2;
-  int v_exp = 0;  // REFER: the weights of the product are taken over 2^(v_exp - kLift)
+  int v_exp = 0;      // REFER: staged value scales are over 2^(v_exp - kLift),
+  float below = 0.f;  // and this lane's row's weights over 2^(v_exp - kLift - below)
   auto load_scale = [&](int tile) {
     const float x = (w == 0 ? P.k_scale : P.v_scale)[pool_block(scur.next) * P.s_block_stride +
                                                      (int64_t)scur.off * P.s_token_stride +
@@ -373,7 +376,7 @@ __global__ __launch_bounds__(kPfThreads, 2) void rlt_prefill_kernel(AttnParams P
         sraw = !seen ? 1.f : f < 1.17549435e-38f ? 1.17549435e-38f : f;
       } else {
         const float r = seen ? __builtin_amdgcn_ldexpf(x, -v_exp) : 1.f;
-        const float e = __builtin_amdgcn_logf(r < 8.67361738e-19f ? 8.67361738e-19f : r) + (float)kLift;
+        const float e = __builtin_amdgcn_logf(r < 0x1p-100f ? 0x1p-100f : r) + (float)kLift;
         sraw = lane & 4 ? __builtin_amdgcn_exp2f(-e) : e;
       }
     } else {
@@ -535,7 +538,7 @@ __global__ __launch_bounds__(kPfThreads, 2) void rlt_prefill_kernel(AttnParams P
 #pragma unroll
       for (int dt = 0; dt < ND; ++dt) oacc[dt] *= corr;
       m_run = m_new;
-      m_use = use;
+      m_use = REFER ? use - below : use;
     }
   };
   // ---- weights of four of the tile's scores (positions 8 g + 4 h + [0, 4)): words 2 g and
@@ -604,19 +607,41 @@ __global__ __launch_bounds__(kPfThreads, 2) void rlt_prefill_kernel(AttnParams P
   };
 
   if constexpr (REFER) {
-    // the exponent of the largest value scale that the rows see
-    float most = 0.f;
+    // The exponents of the largest value scales, of all rows and of this lane's: of the blocks
+    // [b0, b1] that some rows see all see [c0, c1], and the few others go through LDS (windows of
+    // consecutive rows: 258 at most).
+    const auto scale_of = [&](int i) {
+      return fabsf(P.v_scale[pool_block(table[i]) * P.s_block_stride + (int64_t)kvh * P.s_head_stride]);
+    };
+    float most = 0.f, own = 0.f;
+    float* const some = (float*)sh.k[0];
+    int b0 = 0, c0 = 0, c1 = -1, b1 = -1;
     if (kt0 < kt1) {
-      const int last = min((hi_last - 1) / P.block_size, P.table_width - 1);
-      for (int i = lo_first / P.block_size + t; i <= last; i += kPfThreads)
-        most = fmaxf(most, fabsf(P.v_scale[pool_block(table[i]) * P.s_block_stride + (int64_t)kvh * P.s_head_stride]));
+      b0 = c0 = lo_first / P.block_size;
+      b1 = min((hi_last - 1) / P.block_size, P.table_width - 1);
+      c1 = c0 - 1;
+      if (lo_last < hi_first) {
+        c0 = lo_last / P.block_size;
+        c1 = min((hi_first - 1) / P.block_size, b1);
+      }
     }
-    for (int off = 32; off >= 1; off >>= 1) most = fmaxf(most, __shfl_xor(most, off, RLT_WAVE));
-    if (lane == 0) sh.vs[0][w] = most;
+    const int lower = c0 - b0, others = lower + b1 - c1;
+    const auto other = [&](int j) { return j < lower ? b0 + j : c1 + 1 + (j - lower); };
+    for (int i = c0 + t; i <= c1; i += kPfThreads) own = fmaxf(own, scale_of(i));
+    for (int j = t; j < others; j += kPfThreads) some[j] = scale_of(other(j));
+    for (int off = 32; off >= 1; off >>= 1) own = fmaxf(own, __shfl_xor(own, off, RLT_WAVE));
+    if (lane == 0) sh.vs[0][w] = own;
     __syncthreads();
-    most = fmaxf(fmaxf(sh.vs[0][0], sh.vs[0][1]), fmaxf(sh.vs[0][2], sh.vs[0][3]));
+    most = own = fmaxf(fmaxf(sh.vs[0][0], sh.vs[0][1]), fmaxf(sh.vs[0][2], sh.vs[0][3]));
+    for (int j = 0; j < others; ++j) {
+      const float x = some[j];
+      const int at = other(j) * P.block_size;
+      most = fmaxf(most, x);
+      own = at < row_hi && at + P.block_size > row_lo ? fmaxf(own, x) : own;
+    }
     __syncthreads();
     v_exp = most > 0.f ? __builtin_amdgcn_frexp_expf(most) : 0;
+    below = own > 0.f ? (float)min(v_exp - __builtin_amdgcn_frexp_expf(own), kBelow) : 0.f;
     v_mul = __builtin_amdgcn_ldexpf(1.f, v_exp - kLift);
   }
 
