@@ -114,3 +114,25 @@ def test_prompts_beside_a_block_of_larger_values(kernel, dev, codes, dtype, hq, 
     at = torch.cat([torch.arange(n - r, n) for n, r in c.seqs])
     reads = (at < 400) & (torch.arange(len(at)) < 400) & (at // bs >= 300 // bs) & ((at - 49) // bs <= 300 // bs)
     _near(got[~reads], want[~reads], most[~reads], c.q)
+
+
+@pytest.mark.parametrize("codes", CODES)
+@pytest.mark.parametrize("hq,hkv,dim,bs", [(4, 2, 128, 8), (8, 1, 64, 24), (2, 2, 256, 3), (6, 2, 96, 40)])
+@pytest.mark.parametrize("factor", (1e-2, 1e-3, 300.0))
+def test_small_and_large_values_in_blocks_of_any_size(kernel, dev, codes, hq, hkv, dim, bs, factor):
+    """fp16 weights keep their bits where blocks hold no whole 16-position tiles, whatever the size of the
+    values and beside a block of larger ones; packed rows have the bits of single ones."""
+    _say("any block", codes, dim, bs, factor)
+    c = Case(codes, torch.float16, ACROSS, hq, hkv, dim, bs, seed=26, spread=0.05)
+    c.vs *= factor
+    got = c.packed(kernel, dev)
+    _near(got, *c.expect(), c.q)
+    assert torch.equal(got, _single(kernel, dev, c))
+    last = torch.tensor([int(c.tables[s][-(-n // bs) - 1]) for s, (n, _) in enumerate(c.seqs)])
+    c.vs[last] *= 64 if factor > 1 else 2.0 ** 16
+    got, (want, most) = c.packed(kernel, dev), c.expect()
+    assert torch.equal(got, _single(kernel, dev, c))
+    reads = torch.cat([torch.arange(n - r, n) // bs == (n - 1) // bs for n, r in c.seqs])
+    _near(got[~reads], want[~reads], most[~reads], c.q)
+    got = c.packed(kernel, dev, window=21)
+    assert torch.equal(got, _single(kernel, dev, c, window=21))

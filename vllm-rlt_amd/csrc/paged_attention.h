@@ -633,8 +633,10 @@ __device__ __forceinline__ bool store_window(const AttnParams& P, int seq, int k
 // row-group, kv head, chunk) -- on one wave: the wave streams the kv head over
 // positions [512c + part * 512 / KS, + 512 / KS) for every row of the row-group.
 // tbl_lds: this wave's 512-entry LDS slice for the chunk's block ids.
-// SM: FP8 scale mode (0 none, 1 per-tensor, 2 per-vector).  UB: block_size is a
-// multiple of 16, so the 16 positions of a tile share one block.
+// SM: scale mode of 8-bit pools (0 none, 1 per-tensor, 2 per-vector, 3 per block and kv head where
+// a weight's fp16 does not hold scales of any size: as 2, but weights are over a power of two near
+// the largest value scale that the row sees in the span; bf16 weights over block scales take 2).
+// UB: block_size is a multiple of 16, so the 16 positions of a tile share one block.
 template <int QT, int KVT, int D, int NT, int SM, bool UB, bool CP>
 __device__ __forceinline__ void attend_span(const AttnParams& P, int seq, int rg, int kvh, int chunk,
                                             int part, int32_t* tbl_lds,
@@ -735,7 +737,7 @@ __device__ __forceinline__ void attend_span(const AttnParams& P, int seq, int rg
     st.v_mul = P.v_scale[0];
   }
 
-  if (P.new_k && t0 < t1) {
+  if (SM != 3 && P.new_k && t0 < t1) {
     // The window rows' own keys and values, stored through the block table before any
     // tile of this span is read; the wait makes this wave's stores visible to its own
     // loads.
@@ -756,6 +758,17 @@ __device__ __forceinline__ void attend_span(const AttnParams& P, int seq, int rg
     const int64_t k_head = (int64_t)kvh * P.k_head_stride + grp * Raw::kGroupElems;
     const int64_t v_head = (int64_t)kvh * P.v_head_stride + l16 * ND;
     const int32_t* tbl = tbl_lds - c_begin;  // tbl[pos] for pos in the chunk
+    // SM 3: a row's weights and their sum are over 2^v_exp, so that weights times scales lie 2^15 above
+    // their place at most (2^-64 and smaller scales leave nothing that an fp16 output holds).  The
+    // span's value scales are read ahead of its first tiles.
+    float v_exp[NT], span_scale[SM == 3 ? kSpan / 64 : 1];
+    if constexpr (SM == 3) {
+#pragma unroll
+      for (int i = 0; i < kSpan / 64; ++i) {
+        const int at = w_begin + 64 * i + lane;
+        span_scale[i] = P.v_scale[tbl[at] * P.s_block_stride + (int64_t)kvh * P.s_head_stride];
+      }
+    }
     // positions from hi_last on are masked, their values taken as zeros (they may hold any
     // bits, NaN included)
     auto inside = [&](int pos) { return pos < hi_last; };
@@ -807,7 +820,7 @@ __device__ __forceinline__ void attend_span(const AttnParams& P, int seq, int rg
     // load instructions than the keys and values: 8 windows of 5 at 2-4k, 8 kv heads, 67.8
     // -> 52.9 us).
     auto issue_scales = [&](int t) {
-      if (SM == 2) {
+      if (SM >= 2) {
         const int tb = (grp & 1) ? tile_base(t + 1) : tile_base(t);
         const int64_t so = (int64_t)tbl[UB ? tb : tb + l16] * P.s_block_stride +
                            (int64_t)((tb + l16) % P.block_size) * P.s_token_stride +
@@ -854,7 +867,7 @@ __device__ __forceinline__ void attend_span(const AttnParams& P, int seq, int rg
       // ---- online softmax (log2 domain) and the P^T operands: contraction slot 4 grp + j
       // of tile b holds its position 4 grp + j
       float vsc[2][4];
-      if (SM == 2) {
+      if (SM >= 2) {
         const float mine = inside(tb + (grp & 1) * kTileTok + l16) ? sraw : 0.f;
 #pragma unroll
         for (int b = 0; b < 2; ++b)
@@ -904,14 +917,15 @@ __device__ __forceinline__ void attend_span(const AttnParams& P, int seq, int rg
           rescale[b] |= corr[b][nt] != 1.f;
           m_run[nt] = m_new;
 #pragma unroll
-          for (int r = 0; r < 4; ++r) pr[b][r] = __builtin_amdgcn_exp2f(sc[b][nt][r] - m_use);
+          for (int r = 0; r < 4; ++r)
+            pr[b][r] = __builtin_amdgcn_exp2f(sc[b][nt][r] - (SM == 3 ? m_use + v_exp[nt] : m_use));
         }
 #pragma unroll
         for (int b = 0; b < 2; ++b) rs[b] = group_sum(((pr[b][0] + pr[b][1]) + pr[b][2]) + pr[b][3]);
 #pragma unroll
         for (int b = 0; b < 2; ++b) {
           l_run[nt] = l_run[nt] * corr[b][nt] + rs[b];
-          if (SM == 2) {
+          if (SM >= 2) {
 #pragma unroll
             for (int r = 0; r < 4; ++r) pr[b][r] *= vsc[b][r];
           }
@@ -976,8 +990,52 @@ __device__ __forceinline__ void attend_span(const AttnParams& P, int seq, int rg
     issue_scales(t0);
 #pragma unroll
     for (int b = 0; b < 2; ++b) issue_v(t0 + b, b);
+    if constexpr (SM == 3) {
+      float all = 0.f;  // of the positions that every row sees
+#pragma unroll
+      for (int i = 0; i < kSpan / 64; ++i) {
+        const int at = w_begin + 64 * i + lane;
+        all = at >= lo_last && at < hi_first ? fmaxf(all, fabsf(span_scale[i])) : all;
+      }
+#pragma unroll
+      for (int o = 32; o >= 1; o >>= 1) all = fmaxf(all, __shfl_xor(all, o, RLT_WAVE));
+      float most[NT];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) most[nt] = all;
+      // and of the others, 64 read at a time
+      auto some = [&](int from, int to) {
+        from = max(from, w_begin);
+        to = min(to, w_begin + kSpan);
+#pragma unroll 1
+        for (int p0 = from; p0 < to; p0 += 64) {
+          const int64_t blk = tbl[min(p0 + lane, to - 1)];
+          const float x = fabsf(P.v_scale[blk * P.s_block_stride + (int64_t)kvh * P.s_head_stride]);
+#pragma unroll 1
+          for (int p = p0; p < min(p0 + 64, to); ++p) {
+            const float y = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), p - p0));
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+              most[nt] = p >= row_lo[nt] && p < row_hi[nt] ? fmaxf(most[nt], y) : most[nt];
+          }
+        }
+      };
+      some(lo_first, lo_last < hi_first ? lo_last : hi_last);
+      if (lo_last < hi_first) some(hi_first, hi_last);
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+        v_exp[nt] = (float)((most[nt] > 0.f ? max(__builtin_amdgcn_frexp_expf(most[nt]), -64) : 0) - 15);
+    }
 #pragma unroll 1
     for (int t = t0; t < t1; t += 2) compute(t);
+    if constexpr (SM == 3) {
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        const float back = __builtin_amdgcn_ldexpf(1.f, (int)v_exp[nt]);
+        l_run[nt] *= back;
+#pragma unroll
+        for (int dt = 0; dt < ND; ++dt) oacc[nt][dt] *= back;
+      }
+    }
   }
 
 }
