@@ -313,11 +313,13 @@ __global__ __launch_bounds__(kThreads, 4) void rlt_rotary_kernel(Params P) {
     const int tile = (int)(blockIdx.x - (uint32_t)seq * P.tiles);
     const int64_t b = P.cu[seq], e = P.cu[seq + 1];
     begin = b < 0 ? 0 : b > P.rows ? P.rows : b;
-    const int64_t n = (e > P.rows ? P.rows : e) - begin;
-    count = (int)(n < 0 ? 0 : n > P.max_rows ? P.max_rows : n);
-    start = P.lengths[seq] - count;
+    // (all n rows end at the sequence's last position; the first max_rows of them are worked on)
+    const int64_t n = max((e > P.rows ? P.rows : e) - begin, (int64_t)0);
+    count = (int)min(n, (int64_t)P.max_rows);
+    start = (int)(P.lengths[seq] - n);
     if constexpr (BLOCKS) {
-      const int first = start >= 0 ? start / P.block_size : -((-start + P.block_size - 1) / P.block_size);
+      const int first = start >= 0 ? start / P.block_size
+                                   : -(int)(((int64_t)P.block_size - 1 - start) / P.block_size);
       page = first + tile;
       const int64_t from = (int64_t)page * P.block_size - start;
       i0 = (int)(from < 0 ? 0 : from);
@@ -667,13 +669,13 @@ __global__ __launch_bounds__(kThreads) void rlt_kv_load_kernel(LoadParams P) {
   const int tile = (int)(blockIdx.x - (uint32_t)seq * P.tiles);
   const int64_t b = P.cu[seq], e = P.cu[seq + 1];
   const int64_t begin = b < 0 ? 0 : b > P.rows ? P.rows : b;
-  const int64_t n = (e > P.rows ? P.rows : e) - begin;
-  const int count = (int)(n < 0 ? 0 : n > P.max_rows ? P.max_rows : n);
+  const int64_t n = max((e > P.rows ? P.rows : e) - begin, (int64_t)0);
+  const int count = (int)min(n, (int64_t)P.max_rows), start = (int)(P.lengths[seq] - n);
   const int i0 = tile * P.tile_rows, rows = min(count - i0, P.tile_rows);
   if (rows <= 0) return;  // uniform over the workgroup
   const int t = threadIdx.x;
   if (t < rows) {
-    const int pos = P.lengths[seq] - count + i0 + t;
+    const int pos = start + i0 + t;
     const int idx = pos >= 0 ? pos / P.block_size : -1;
     const int32_t x = idx >= 0 && idx < P.table_width ? P.tables[(int64_t)seq * P.table_stride + idx] : -1;
     entries[t] = x >= 0 && x < P.num_blocks ? x : -1;
