@@ -1,4 +1,5 @@
-"""Appends and loads at the bounds of their arguments: windows longer than ``max_seqlen_q``."""
+"""Appends, loads and rotations at the bounds of their arguments: windows longer than ``max_seqlen_q``, and
+calls whose padded windows or rows are more than one launch holds (2^32 threads)."""
 
 import pytest
 import torch
@@ -39,3 +40,49 @@ def test_windows_longer_than_their_bound(pkg, dev, kind):
     for x, (pool, scale) in zip((a, b), want):
         whole = orot.load(_layer(pool), _layer(scale), r.tables, r.lengths, counts)
         assert torch.equal(x.cpu()[kept], whole.float()[kept])
+
+
+@pytest.mark.parametrize("kind", ("same", "int8"))
+def test_padded_windows_past_one_launch(pkg, dev, kind):
+    """One long window beside a thousand single tokens: 2^24 tiles of 256 threads, nearly all without rows."""
+    _say("past one launch", kind)
+    # (tiles of 8 rows; blocks of 8 tokens)
+    n, long = 1040, (1 << 17) + 8
+    bs, rows = 8, n - 1 + long
+    g = torch.Generator(device=dev).manual_seed(42)
+    counts = torch.ones(n, dtype=torch.int32, device=dev)
+    counts[n - 2] = long  # (a place past the first launch's)
+    cu = torch.cat([counts.new_zeros(1), counts.cumsum(0).int()])
+    width = long // bs
+    blocks = width + n
+    tables = torch.full((n, width), -1, dtype=torch.int32, device=dev)
+    tables[:, 0] = torch.arange(n, device=dev, dtype=torch.int32) + width
+    tables[n - 2] = torch.arange(width, device=dev, dtype=torch.int32)
+    dtype = torch.bfloat16 if kind == "same" else torch.int8
+    k, v = (torch.zeros(blocks, bs, 1, 16, dtype=dtype, device=dev) for _ in range(2))
+    ks, vs = (None, None) if kind == "same" else (torch.zeros(blocks, 1, device=dev) for _ in range(2))
+    new_k, new_v = (torch.randn(rows, 1, 16, generator=g, device=dev).to(torch.bfloat16) for _ in range(2))
+    pkg.append_kv(k, v, new_k, new_v, tables, counts, cu, long, ks, vs)
+    a, b = pkg.load_kv(k, v, tables, counts, cu, long, rows, ks, vs, dtype=torch.float32)
+    for x, rows_in, scale in ((a, new_k, ks), (b, new_v, vs)):
+        if kind == "same":
+            assert torch.equal(x, rows_in.float())
+        else:
+            # half a step of the row's block, at most 127 of them, and two roundings of float32
+            at = torch.cat([torch.full((1,), width + s, device=dev) if s != n - 2 else
+                            torch.arange(long, device=dev) // bs for s in range(n)])
+            near = scale[at][:, None] * (0.5 + 2.0 ** -15)
+            assert ((x - rows_in.float()).abs() <= near).all()
+
+
+def test_rotations_past_one_launch(pkg, dev):
+    """2^27 rows and some: those at both ends and across the launches' borders as a call of them alone."""
+    _say("rotations past one launch")
+    plan = pkg.Rotary(2, device=dev)
+    rows = (1 << 27) + 77
+    q = torch.empty(rows, 1, 2, dtype=torch.bfloat16, device=dev).uniform_(-1, 1)
+    pos = torch.arange(rows, device=dev)
+    got = pkg.apply_rotary(q, None, pos, plan)[0]
+    for at in (0, (1 << 26) - 100, (1 << 27) - 100, rows - 200):
+        part = slice(at, at + 200)
+        assert torch.equal(got[part], pkg.apply_rotary(q[part], None, pos[part], plan)[0])

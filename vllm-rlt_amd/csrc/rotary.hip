@@ -39,6 +39,9 @@ constexpr int kThreads = 256;
 constexpr int kWavesPerGroup = kThreads / 64;
 constexpr int kMaxPairs = 128;   // head_dim <= 256
 constexpr int kMaxKvItems = 512; // k and v heads, whose maxima over long blocks are kept in LDS
+// Workgroups of one launch: a grid holds fewer than 2^32 threads, and a call may ask for more (its
+// windows are padded to the longest); those behind go into further launches.
+constexpr int64_t kGridGroups = (int64_t)1 << 23;
 
 // What the rows are written to.
 enum Mode {
@@ -78,6 +81,7 @@ struct Params {
   const int32_t* lengths;
   const int32_t* cu;
   int32_t num_seqs, max_rows, tiles;
+  uint32_t first_group;  // of the launch
 };
 
 // ---------------------------------------------------------------- sines
@@ -300,17 +304,18 @@ __global__ __launch_bounds__(kThreads, 4) void rlt_rotary_kernel(Params P) {
   const double turns0 = pairs ? P.turns[t % pairs] : 0.0;
 
   // ---- the tile's rows [i0, i1) of its sequence
+  const uint32_t tile_index = P.first_group + blockIdx.x;
   int64_t begin = 0;    // packed row of the sequence's first
   int count, start = 0; // its rows, and the position of the first
   int seq = 0, i0, i1, page = 0;
   if constexpr (MODE == kApply) {
-    begin = (int64_t)blockIdx.x * kRows;
+    begin = (int64_t)tile_index * kRows;
     count = (int)min((int64_t)kRows, P.rows - begin);
     i0 = 0;
     i1 = count;
   } else {
-    seq = (int)(blockIdx.x / (uint32_t)P.tiles);
-    const int tile = (int)(blockIdx.x - (uint32_t)seq * P.tiles);
+    seq = (int)(tile_index / (uint32_t)P.tiles);
+    const int tile = (int)(tile_index - (uint32_t)seq * P.tiles);
     const int64_t b = P.cu[seq], e = P.cu[seq + 1];
     begin = b < 0 ? 0 : b > P.rows ? P.rows : b;
     // (all n rows end at the sequence's last position; the first max_rows of them are worked on)
@@ -607,6 +612,7 @@ struct LoadParams {
   const int32_t* cu;
   int64_t rows;
   int32_t num_seqs, max_rows, tiles, tile_rows, hkv, head_dim;
+  uint32_t first_group;  // of the launch
   void* k_out;
   void* v_out;
 };
@@ -665,8 +671,9 @@ constexpr int kLoadRows = 8;
 template <int CT, int OT, int W>
 __global__ __launch_bounds__(kThreads) void rlt_kv_load_kernel(LoadParams P) {
   __shared__ int entries[kLoadRows], offsets[kLoadRows];
-  const int seq = (int)(blockIdx.x / (uint32_t)P.tiles);
-  const int tile = (int)(blockIdx.x - (uint32_t)seq * P.tiles);
+  const uint32_t tile_index = P.first_group + blockIdx.x;
+  const int seq = (int)(tile_index / (uint32_t)P.tiles);
+  const int tile = (int)(tile_index - (uint32_t)seq * P.tiles);
   const int64_t b = P.cu[seq], e = P.cu[seq + 1];
   const int64_t begin = b < 0 ? 0 : b > P.rows ? P.rows : b;
   const int64_t n = max((e > P.rows ? P.rows : e) - begin, (int64_t)0);
@@ -723,18 +730,21 @@ constexpr int kGroupsWanted = 1024;  // workgroups from which the chip is filled
 // for each sequence (6 ragged windows of up to 700 rows, of whose 528 tiles 330 have some, into
 // fp8 with a scale per vector: 21.6 -> 19.4 us)
 template <int DT, int MODE>
-int launch_rotary(const Params& P, bool vec, int64_t gx, hipStream_t stream) {
+int launch_rotary(Params P, bool vec, int64_t gx, hipStream_t stream) {
   const int items = P.hq + (MODE == kApply ? 1 : 2) * P.hkv;
   const int64_t some = P.rows / rows_of(MODE) + (MODE == kApply ? 1 : P.num_seqs), filled = some < gx ? some : gx;
   const int64_t most = (items + kWavesPerGroup - 1) / kWavesPerGroup, want = (kGroupsWanted + filled - 1) / filled;
-  const dim3 grid((unsigned)gx, (unsigned)(want < most ? want : most));
   constexpr int W = DT == RLT_F32 ? 4 : 8;
   const int lanes = P.head_dim / (2 * W);  // that hold a vector
-  if (!vec) rlt_rotary_kernel<DT, 1, 64, MODE><<<grid, kThreads, 0, stream>>>(P);
-  else if (lanes <= 4) rlt_rotary_kernel<DT, W, 4, MODE><<<grid, kThreads, 0, stream>>>(P);
-  else if (lanes <= 8) rlt_rotary_kernel<DT, W, 8, MODE><<<grid, kThreads, 0, stream>>>(P);
-  else if (lanes <= 16) rlt_rotary_kernel<DT, W, 16, MODE><<<grid, kThreads, 0, stream>>>(P);
-  else if constexpr (DT == RLT_F32) rlt_rotary_kernel<DT, W, 32, MODE><<<grid, kThreads, 0, stream>>>(P);
+  for (int64_t at = 0; at < gx; at += kGridGroups) {
+    const dim3 grid((unsigned)(gx - at < kGridGroups ? gx - at : kGridGroups), (unsigned)(want < most ? want : most));
+    P.first_group = (uint32_t)at;
+    if (!vec) rlt_rotary_kernel<DT, 1, 64, MODE><<<grid, kThreads, 0, stream>>>(P);
+    else if (lanes <= 4) rlt_rotary_kernel<DT, W, 4, MODE><<<grid, kThreads, 0, stream>>>(P);
+    else if (lanes <= 8) rlt_rotary_kernel<DT, W, 8, MODE><<<grid, kThreads, 0, stream>>>(P);
+    else if (lanes <= 16) rlt_rotary_kernel<DT, W, 16, MODE><<<grid, kThreads, 0, stream>>>(P);
+    else if constexpr (DT == RLT_F32) rlt_rotary_kernel<DT, W, 32, MODE><<<grid, kThreads, 0, stream>>>(P);
+  }
   return rlt_launch_status();
 }
 
@@ -884,19 +894,23 @@ int rlt_kv_append(const void* k, int64_t k_row_stride, int64_t k_head_stride, co
 namespace {
 
 template <int CT, int OT>
-int launch_load(const LoadParams& P, bool vec, dim3 grid, hipStream_t stream) {
+int launch_load(LoadParams P, bool vec, int64_t gx, hipStream_t stream) {
   constexpr int W = CT == RLT_F32 ? 4 : CT == RLT_FP8_E4M3 || CT == RLT_INT8 ? 16 : 8;
-  if (vec) rlt_kv_load_kernel<CT, OT, W><<<grid, kThreads, 0, stream>>>(P);
-  else rlt_kv_load_kernel<CT, OT, 1><<<grid, kThreads, 0, stream>>>(P);
+  for (int64_t at = 0; at < gx; at += kGridGroups) {
+    const unsigned grid = (unsigned)(gx - at < kGridGroups ? gx - at : kGridGroups);
+    P.first_group = (uint32_t)at;
+    if (vec) rlt_kv_load_kernel<CT, OT, W><<<grid, kThreads, 0, stream>>>(P);
+    else rlt_kv_load_kernel<CT, OT, 1><<<grid, kThreads, 0, stream>>>(P);
+  }
   return rlt_launch_status();
 }
 
 template <int CT>
-int launch_load_ot(const LoadParams& P, int out_dtype, bool vec, dim3 grid, hipStream_t stream) {
+int launch_load_ot(const LoadParams& P, int out_dtype, bool vec, int64_t gx, hipStream_t stream) {
   switch (out_dtype) {
-    case RLT_F32: return launch_load<CT, RLT_F32>(P, vec, grid, stream);
-    case RLT_F16: return launch_load<CT, RLT_F16>(P, vec, grid, stream);
-    case RLT_BF16: return launch_load<CT, RLT_BF16>(P, vec, grid, stream);
+    case RLT_F32: return launch_load<CT, RLT_F32>(P, vec, gx, stream);
+    case RLT_F16: return launch_load<CT, RLT_F16>(P, vec, gx, stream);
+    case RLT_BF16: return launch_load<CT, RLT_BF16>(P, vec, gx, stream);
     default: return RLT_ERR_ARGUMENT;
   }
 }
@@ -925,7 +939,7 @@ extern "C" int rlt_kv_load(const void* key_cache, const void* value_cache, int64
       (table_width && !block_tables))
     return RLT_ERR_ARGUMENT;
   if (max_len > rows) max_len = (int32_t)rows;
-  LoadParams P;
+  LoadParams P = {};
   P.k = key_cache;
   P.v = value_cache;
   P.k_block = k_block_stride;
@@ -965,13 +979,12 @@ extern "C" int rlt_kv_load(const void* key_cache, const void* value_cache, int64
                    aligned(key_cache, k_block_stride, k_token_stride, k_head_stride, elt, 16) &&
                    aligned(value_cache, v_block_stride, v_token_stride, v_head_stride, elt, 16) &&
                    ((uintptr_t)k_out | (uintptr_t)v_out) % 16 == 0;
-  const dim3 grid((unsigned)gx);
   switch (kv_dtype) {
-    case RLT_F32: return launch_load_ot<RLT_F32>(P, out_dtype, vec, grid, stream);
-    case RLT_F16: return launch_load_ot<RLT_F16>(P, out_dtype, vec, grid, stream);
-    case RLT_BF16: return launch_load_ot<RLT_BF16>(P, out_dtype, vec, grid, stream);
-    case RLT_FP8_E4M3: return launch_load_ot<RLT_FP8_E4M3>(P, out_dtype, vec, grid, stream);
-    case RLT_INT8: return launch_load_ot<RLT_INT8>(P, out_dtype, vec, grid, stream);
+    case RLT_F32: return launch_load_ot<RLT_F32>(P, out_dtype, vec, gx, stream);
+    case RLT_F16: return launch_load_ot<RLT_F16>(P, out_dtype, vec, gx, stream);
+    case RLT_BF16: return launch_load_ot<RLT_BF16>(P, out_dtype, vec, gx, stream);
+    case RLT_FP8_E4M3: return launch_load_ot<RLT_FP8_E4M3>(P, out_dtype, vec, gx, stream);
+    case RLT_INT8: return launch_load_ot<RLT_INT8>(P, out_dtype, vec, gx, stream);
     default: return RLT_ERR_ARGUMENT;
   }
 }
