@@ -86,3 +86,34 @@ def test_rotations_past_one_launch(pkg, dev):
     for at in (0, (1 << 26) - 100, (1 << 27) - 100, rows - 200):
         part = slice(at, at + 200)
         assert torch.equal(got[part], pkg.apply_rotary(q[part], None, pos[part], plan)[0])
+
+
+@pytest.mark.parametrize("kind", ("fp8", "int8"))
+@pytest.mark.parametrize("exponent", (-126, -120, -112, -100, -91, -90, -80, 0, 100))
+def test_codes_of_values_at_the_middle_of_two(pkg, dev, kind, exponent):
+    """Rows at and next to the border of two codes, over scales of any size: the division's codes, bit for bit,
+    those of earlier rows among them where a block's scale grows."""
+    _say("middle", kind, exponent)
+    g = torch.Generator().manual_seed(200 + exponent)
+    top = 127 if kind == "int8" else 448
+    r = Round(kind, torch.float32, 16, 4, 64, [0, 5, 16, 3], [6, 9, 40, 1], seed=43)
+    for name in ("new_k", "new_v"):
+        # (scales of every mantissa: a row's largest value gives its block's, the same for all of its rows)
+        most = (1 + torch.rand(1, 4, 1, generator=g)) * 2.0 ** exponent * top
+        scale = most * torch.tensor(1.0 / top, dtype=torch.float32)
+        shape = (len(r.places), 4, 64)
+        if kind == "int8":
+            middle = torch.randint(-126, 126, shape, generator=g) + 0.5
+        else:
+            step = 2.0 ** torch.randint(-9, 5, shape, generator=g)
+            middle = (torch.randint(8, 15, shape, generator=g) + 0.5) * step
+        x = (middle.double() * scale.double()).float()
+        near = torch.randint(-1, 2, shape, generator=g, dtype=torch.int32)
+        x = (x.view(torch.int32) + near).view(torch.float32)
+        x[..., 0] = most[..., 0]
+        setattr(r, name, x)
+    for name in ("ks", "vs"):  # earlier tokens over a scale that grows, or does not
+        held = getattr(r, name)
+        held.fill_(2.0 ** max(exponent - 1, -126))
+        held *= (1 + torch.rand(held.shape, generator=g)) * (0.7 if exponent > -126 else 1)
+    _equal(r.run(pkg, dev), r.expect())

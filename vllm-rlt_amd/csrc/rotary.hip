@@ -184,15 +184,15 @@ constexpr float top_of() { return MODE == kBlockInt8 ? 127.f : rlt_fp8::kMax; }
 
 // A scale and its reciprocal; 0 where quotient() is not for it: a scale that is no positive number,
 // or at the ends of float32, where the reciprocal or the remainder would be subnormal.  (Scales
-// of blocks are positive, 2^122 at most; below 2^-90 they take the step all the same, whose
-// quotient may then be off by an ulp: a second form of the codes costs blocks of 64 int8
-// tokens 39.3 -> 41.6 us.)
+// of blocks are positive, 2^122 at most; below kSmallScale they and their rows are taken kRaise
+// times, which moves no bit of a quotient.)
+constexpr float kSmallScale = 0x1p-90f, kRaise = 0x1p64f;
 struct Divisor {
   float by, inverse;
 };
 template <int MODE>
 __device__ __forceinline__ Divisor divisor(float scale) {
-  const bool fits = in_blocks(MODE) || (scale >= 0x1p-90f && scale <= 0x1p120f);
+  const bool fits = in_blocks(MODE) || (scale >= kSmallScale && scale <= 0x1p120f);
   return Divisor{scale, fits ? 1.f / scale : 0.f};
 }
 
@@ -527,7 +527,9 @@ __global__ __launch_bounds__(kThreads, 4) void rlt_rotary_kernel(Params P) {
         const float m = several ? tops[item] : top(held, c1 - c0);
         const float fresh = fmaxf(m * (1.f / top_of<MODE>()), rlt_fp8::kTiny);
         const float scale = o0 > 0 && old > fresh ? old : fresh;
-        const Divisor by = divisor<MODE>(scale);
+        const float raise =
+            __builtin_amdgcn_readfirstlane(__float_as_int(scale)) < __float_as_int(kSmallScale) ? kRaise : 1.f;
+        const Divisor by = divisor<MODE>(scale * raise);
         const int64_t base = (int64_t)entry * s.dst_block + (int64_t)head * s.dst_head;
         if (c0 == i0 && o0 > 0 && scale > old) {
           // the block's earlier codes, over the new scale
@@ -537,7 +539,7 @@ __global__ __launch_bounds__(kThreads, 4) void rlt_rotary_kernel(Params P) {
             const int64_t at = base + (int64_t)r * s.dst_row + (e - r * per_row) * W;
             float x[W];
 #pragma unroll
-            for (int u = 0; u < W; ++u) x[u] = value_of<MODE>(((const uint8_t*)s.dst)[at + u]) * old;
+            for (int u = 0; u < W; ++u) x[u] = value_of<MODE>(((const uint8_t*)s.dst)[at + u]) * old * raise;
             store_codes<MODE, W>(s.dst, at, x, by);
           }
         }
@@ -549,8 +551,15 @@ __global__ __launch_bounds__(kThreads, 4) void rlt_rotary_kernel(Params P) {
           const int64_t at = base + (int64_t)(o0 + (c0 - i0) + r) * s.dst_row;
 #pragma unroll
           for (int n = 0; n < NS; ++n) {
-            if (at_a[n] >= 0) store_codes<MODE, W>(s.dst, at + at_a[n], held.x[st][n][0], by);
-            if (at_b[n] >= 0) store_codes<MODE, W>(s.dst, at + at_b[n], held.x[st][n][1], by);
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+              const int el = half ? at_b[n] : at_a[n];
+              if (el < 0) continue;
+              float x[W];
+#pragma unroll
+              for (int u = 0; u < W; ++u) x[u] = held.x[st][n][half][u] * raise;
+              store_codes<MODE, W>(s.dst, at + el, x, by);
+            }
           }
         }
       } else if constexpr (MODE != kApply) {
