@@ -43,4 +43,22 @@ inline bool overlap(int64_t delta, const Axis (&layout)[3], int64_t row) {
   return meets(delta, axes, n, row);
 }
 
+// Rows [i, a head of `heads`] and [j, a head of `others`] of `dim` elements, i and j below `rows`, in
+// tensors of the same row and head strides (not negative) that begin `delta` elements apart, share one.
+inline bool rows_meet(int64_t delta, int64_t row, int64_t head, int64_t rows, int64_t heads, int64_t others,
+                      int64_t dim) {
+  if (rows < 2) row = 0;
+  for (int64_t n = 1 - others; n < heads; ++n) {
+    const int64_t left = delta - n * head;
+    // (row differences next to the one that leaves nothing, or the last of them)
+    int64_t q = row ? left / row : 0;
+    q = q < -rows ? -rows : q > rows ? rows : q;
+    for (int64_t r = q - 1; r <= q + 1; ++r) {
+      const int64_t away = left - r * row;
+      if (r > -rows && r < rows && away < dim && -away < dim) return true;
+    }
+  }
+  return false;
+}
+
 }  // namespace pools

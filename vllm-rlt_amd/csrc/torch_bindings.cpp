@@ -996,17 +996,10 @@ bool share_rows(const Tensor& q, const Tensor& k) {
   };
   const int64_t delta = (int64_t)((intptr_t)k.data_ptr() - (intptr_t)q.data_ptr()) / q.element_size();
   if (delta >= span(q) || -delta >= span(k)) return false;
-  const int64_t row = q.stride(0), head = q.stride(1);
-  if (k.stride(0) != row || k.stride(1) != head || head < dim || (rows > 1 && row < 1)) return true;
-  // k's row j + r lies r rows behind q's row j, and then n heads
-  const int64_t near = rows > 1 ? delta / row : 0;
-  for (int64_t r = near - 1; r <= near + 1; ++r) {
-    if (std::abs(r) >= rows) continue;
-    const int64_t left = delta - (rows > 1 ? r * row : 0);
-    for (int64_t n = left / head - 1; n <= left / head + 1; ++n)
-      if (n > -k.size(1) && n < q.size(1) && std::abs(left - n * head) < dim) return true;
-  }
-  return false;
+  // (the stride of an axis of one is any)
+  const bool heads = q.size(1) > 1 && k.size(1) > 1;
+  if ((rows > 1 && k.stride(0) != q.stride(0)) || (heads && k.stride(1) != q.stride(1))) return true;
+  return pools::rows_meet(delta, q.stride(0), (q.size(1) > 1 ? q : k).stride(1), rows, q.size(1), k.size(1), dim);
 }
 
 // turns float64 [rotary_dim / 2]
