@@ -136,3 +136,51 @@ def test_small_and_large_values_in_blocks_of_any_size(kernel, dev, codes, hq, hk
     _near(got[~reads], want[~reads], most[~reads], c.q)
     got = c.packed(kernel, dev, window=21)
     assert torch.equal(got, _single(kernel, dev, c, window=21))
+
+
+def _bytes(x):
+    return x.contiguous().view(torch.uint8)
+
+
+def test_stores_are_refused_before_the_append(kernel, dev):
+    """A call that the attention would refuse leaves the cache and its scales as they were."""
+    _say("refused stores")
+    c = Case(torch.int8, torch.bfloat16, [(10, 3)], 4, 2, 64, 16, seed=27)
+    q, k, v, tables, lengths, cu, ks, vs = c.args(dev)
+    k, v, ks, vs = k[:, 1], v[:, 1], ks[:, 1], vs[:, 1]
+    new = torch.ones(3, 2, 64, dtype=torch.bfloat16, device=dev) * 50
+    apart = torch.zeros(1, 2, dtype=torch.int32, device=dev)[:, ::2]  # (one column, two apart)
+    before = [x.clone() for x in (k, v, ks, vs)]
+    for bad in (dict(block_tables=apart), dict(q=q[:, :0]), dict(q=q[:, :3]), dict(max_seqlen_q=0),
+                dict(max_seqlen_q=1 << 31)):
+        args = dict(q=q, block_tables=tables, max_seqlen_q=3)
+        args.update(bad)
+        with pytest.raises(ValueError):
+            kernel.prefill_store(args["q"], new, new, k, v, args["block_tables"], lengths, cu,
+                                 args["max_seqlen_q"], ks, vs)
+        torch.cuda.synchronize()
+        for a, b in zip((k, v, ks, vs), before):
+            assert torch.equal(_bytes(a), _bytes(b))
+
+
+@pytest.mark.parametrize("codes", CODES)
+@pytest.mark.parametrize("rows", (3, 70))
+def test_stores_by_a_bound(kernel, dev, codes, rows):
+    """``max_seqlen_q`` far above the windows: the same outputs and scales."""
+    _say("store bound", codes, rows)
+    c = Case(codes, torch.bfloat16, [(rows + 9, rows)], 4, 2, 96, 16, seed=28)
+    q, k, v, tables, lengths, cu, ks, vs = c.args(dev)
+    g = torch.Generator().manual_seed(29)
+    new_k, new_v = (torch.randn(rows, 2, 96, generator=g).to(torch.bfloat16).to(dev) for _ in range(2))
+
+    def pool(x, apart):
+        out = torch.zeros(x.shape[0], 16, 2, apart, dtype=torch.uint8, device=dev)[..., :96]
+        return out.copy_(x[:, 1].view(torch.uint8)).view(codes)
+
+    outs = []
+    for apart, bound in ((96, rows), (96, 4096), (96, 2 ** 31 - 1)):
+        held = pool(k, apart), pool(v, apart), ks[:, 1].clone(), vs[:, 1].clone()
+        out = kernel.prefill_store(q, new_k, new_v, *held[:2], tables, lengths, cu, bound, *held[2:])
+        outs.append((out, *map(_bytes, held)))
+    for other in outs[1:]:
+        assert all(torch.equal(a, b) for a, b in zip(outs[0], other))

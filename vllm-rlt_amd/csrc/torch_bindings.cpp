@@ -537,8 +537,13 @@ Tensor paged_attention_store(const Tensor& q, const Tensor& k_new_in, const Tens
     // matrix kernels serve is read in 16-byte pieces)
     TORCH_CHECK_VALUE(!row_lengths.has_value(), "block scales take no row_lengths");
     TORCH_CHECK_VALUE(k_new.scalar_type() == q.scalar_type(), "k_new, v_new must have q's dtype");
-    TORCH_CHECK_VALUE(head_dim <= 256 && q.size(1) % kv_heads == 0 && q.stride(2) == 1,
+    TORCH_CHECK_VALUE(head_dim <= 256 && kv_heads > 0 && q.size(1) > 0 && q.size(1) % kv_heads == 0 &&
+                          q.stride(2) == 1,
                       "q heads must be a positive multiple of KV heads with a contiguous head_dim <= 256");
+    TORCH_CHECK_VALUE(block_tables.dim() == 2 && block_tables.stride(1) == 1,
+                      "block_tables must be int32 [sequences, width] with unit column stride");
+    TORCH_CHECK_VALUE(max_seqlen_q >= 0 && max_seqlen_q <= INT32_MAX && (max_seqlen_q > 0 || rows == 0),
+                      "max_seqlen_q must be the longest window");
     TORCH_CHECK_VALUE(!compensate || key_cache.size(1) % 16 == 0,
                       "compensated attention needs a block size that is a multiple of 16");
     if (rlt_paged_attention_uses_mfma(dtype_code(q.scalar_type()), pool_code(key_cache.scalar_type()),
@@ -548,6 +553,8 @@ Tensor paged_attention_store(const Tensor& q, const Tensor& k_new_in, const Tens
                             key_cache.stride(0) % 16 == 0 && key_cache.stride(1) % 16 == 0 &&
                             key_cache.stride(2) % 16 == 0,
                         "q and the pools must be 16-byte aligned");
+    // (a longest window known by its bound only)
+    max_seqlen_q = std::min(max_seqlen_q, rows);
     append_kv(key_cache, value_cache, k_new, v_new, block_tables, context_lengths, cu_seqlens_q,
               max_seqlen_q, key_scale, value_scale, std::nullopt, std::nullopt, 1.0, false,
               std::nullopt);
