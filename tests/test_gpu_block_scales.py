@@ -165,8 +165,8 @@ def test_stores_are_refused_before_the_append(kernel, dev):
 
 @pytest.mark.parametrize("codes", CODES)
 @pytest.mark.parametrize("rows", (3, 70))
-def test_stores_by_a_bound(kernel, dev, codes, rows):
-    """``max_seqlen_q`` far above the windows: the same outputs and scales."""
+def test_stores_by_a_bound_and_over_strides_of_8_bytes(kernel, dev, codes, rows):
+    """``max_seqlen_q`` far above the windows, and 96-dim heads 104 bytes apart: the same outputs and scales."""
     _say("store bound", codes, rows)
     c = Case(codes, torch.bfloat16, [(rows + 9, rows)], 4, 2, 96, 16, seed=28)
     q, k, v, tables, lengths, cu, ks, vs = c.args(dev)
@@ -178,7 +178,7 @@ def test_stores_by_a_bound(kernel, dev, codes, rows):
         return out.copy_(x[:, 1].view(torch.uint8)).view(codes)
 
     outs = []
-    for apart, bound in ((96, rows), (96, 4096), (96, 2 ** 31 - 1)):
+    for apart, bound in ((96, rows), (104, rows), (96, 2 ** 31 - 1), (104, 2 ** 31 - 1)):
         held = pool(k, apart), pool(v, apart), ks[:, 1].clone(), vs[:, 1].clone()
         out = kernel.prefill_store(q, new_k, new_v, *held[:2], tables, lengths, cu, bound, *held[2:])
         outs.append((out, *map(_bytes, held)))

@@ -547,12 +547,14 @@ Tensor paged_attention_store(const Tensor& q, const Tensor& k_new_in, const Tens
     TORCH_CHECK_VALUE(!compensate || key_cache.size(1) % 16 == 0,
                       "compensated attention needs a block size that is a multiple of 16");
     if (rlt_paged_attention_uses_mfma(dtype_code(q.scalar_type()), pool_code(key_cache.scalar_type()),
-                                      (int32_t)head_dim))
+                                      (int32_t)head_dim)) {
+      const int64_t align = head_dim % 64 ? 8 : 16;
       TORCH_CHECK_VALUE(((uintptr_t)ptr(q) | (uintptr_t)ptr(key_cache) | (uintptr_t)ptr(value_cache)) % 16 == 0 &&
                             q.stride(0) % 8 == 0 && q.stride(1) % 8 == 0 &&
-                            key_cache.stride(0) % 16 == 0 && key_cache.stride(1) % 16 == 0 &&
-                            key_cache.stride(2) % 16 == 0,
-                        "q and the pools must be 16-byte aligned");
+                            key_cache.stride(0) % align == 0 && key_cache.stride(1) % align == 0 &&
+                            key_cache.stride(2) % align == 0,
+                        "q and the pools must be 16-byte aligned, the pools' strides ", align, "-byte");
+    }
     // (a longest window known by its bound only)
     max_seqlen_q = std::min(max_seqlen_q, rows);
     append_kv(key_cache, value_cache, k_new, v_new, block_tables, context_lengths, cu_seqlens_q,
