@@ -628,9 +628,9 @@ int rlt_rotary(const void* q, int64_t q_row_stride, int64_t q_head_stride, const
 
 /*
  * Windows of rows into the paged cache, keys and queries turned on the way (as rlt_rotary;
- * rotary_dim 0: not at all).  Sequence s owns rows cu_seqlens_q[s] .. cu_seqlens_q[s + 1] - 1, at
- * most max_q_len; row i of its n goes to position context_lengths[s] - n + i of its table
- * and turns by it, or by positions[row] (int64, optional).  Rows before position 0, past the
+ * rotary_dim 0: not at all).  Sequence s owns rows cu_seqlens_q[s] .. cu_seqlens_q[s + 1] - 1; row i
+ * of its n goes to position context_lengths[s] - n + i of its table and turns by it, or by
+ * positions[row] (int64, optional).  Rows from the max_q_len-th of a sequence on are left.  Rows before position 0, past the
  * table or whose entry lies outside the pool are not written.  k, v [rows, num_kv_heads,
  * head_dim] and q (optional) of `dtype`; q_out as in rlt_rotary.  Pools:
  *   - kv_dtype == dtype, scale_mode 0: turned rows rounded once;
@@ -640,8 +640,8 @@ int rlt_rotary(const void* q, int64_t q_row_stride, int64_t q_head_stride, const
  *     FLT_MIN) of the call's rows in the block (M = 448, int8 127; values that are not finite
  *     do not count); where they go on behind earlier tokens of the block, the larger of that
  *     and the block's scale, and if it grew the earlier codes' values are quantized again over
- *     it.  Codes: x / scale (IEEE), clamped to +-M, to the nearest even; e4m3 keeps NaN, int8
- *     takes it as 0.  A block is written by one sequence of a call only.
+ *     it, off by half a step of it each time.  Codes: x / scale (IEEE), clamped to +-M, to the
+ *     nearest even; e4m3 keeps NaN, int8 takes it as 0.  A block is written by one sequence of a call only.
  * The pools must not overlap, nor blocks, tokens and heads of one.  num_kv_heads <= 256,
  * head_dim <= 256.  No workspace.  Replaces, behind the rotation, the writers
  * vllm_rlt/kernels/graph_kv.py:52-67 and vllm_rlt/kernels/triton_attention.py:506-623 for

@@ -111,7 +111,8 @@ class MI355XPagedAttention:
     kv_head]`` (per vector); float8_e4m3fn or int8 with one scale per block of tokens and kv
     head, ``[block, kv_head]``, as ``kv_write.append_kv`` writes them: positive (not ``tree``).
     Value scales of the blocks that a row reads may differ by a factor of 2^20 before weights
-    of the smaller ones lose bits.
+    of the smaller ones lose bits; those of blocks that it does not read have no effect (in
+    prompts: up to 2^80 times its own).
     """
 
     generation = None

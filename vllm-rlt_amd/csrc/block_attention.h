@@ -7,8 +7,8 @@
 // the merge, 5.2 TB/s (1 GB: 218 us), whatever the kv heads, block size, loads in flight (one or
 // two pairs of tiles) and waves (8 or 12 a CU); a unit's first loads issued before the one
 // ahead of it is combined gain nothing (616), non-temporal loads are slower (629).  Windows of 5
-// over GQA 4, 157 MB, 46 us: one or two units a workgroup, each a chain of lengths -> table ->
-// tiles -> combine; one row at 700 positions 11.4 us.
+// over GQA 4, 157 MB, 47 us: one or two units a workgroup, each a chain of lengths -> table ->
+// tiles -> combine; one row at 700 positions 11.9 us.
 //
 // Work.  A unit is (sequence, row-group, kv head, chunk): 1024 absolute key positions, a quarter
 // of them to each of a workgroup's four waves, whose softmax states (maximum, sum,

@@ -14,7 +14,9 @@
 // scale per block of tokens and kv head, amax / M of the call's rows in the block (M = 448 for
 // e4m3, 127 for int8).  A block that the sequence's earlier tokens had begun keeps the larger of
 // its scale and that, and where it grew its earlier codes are held over the new one: the values
-// they stand for are quantized again, off by half a step of the new scale at most.
+// they stand for are quantized again, each time off by half a step of that scale at most.  (N(0, 1)
+// tokens one by one into blocks of 16: 2.4 growths in the mean, rms error 1.25 times that of quantizing
+// the block once in int8, where values are off by up to 2.9 steps, and 1.34 times in e4m3.)
 //
 // Work: a workgroup takes 8 rows of a sequence (with block scales: one block of it, 16 rows at
 // a time), makes their sines and cosines once in LDS, and its four waves take the heads of q, k
@@ -23,7 +25,7 @@
 // its maximum and its codes.  What bounds it: each row is read and written once, at the rate of
 // a large copy (16384 rows of 20 heads of 128 in bf16, 168 MB: 34.8 us, 4.8 TB/s; 8 prompts of
 // 2048 into an int8 cache 45 us), and at a few rows the chain lengths -> table -> rows -> scale
-// -> codes of one launch (1 row: 3.4 us, 6.5 into block scales).
+// -> codes of one launch (1 row: 3.4 us in a replayed graph, 6.3 into block scales).
 
 #include "common.h"
 #include "fp8_codec.h"

@@ -233,7 +233,9 @@ def append_kv(key_cache, value_cache, k, v, block_tables, context_lengths, cu_se
       normal float; values that are not finite do not count, infinities clamp, int8 takes NaN
       as 0).  Where rows go on in a block that already holds tokens, the larger of that and the
       block's scale; if it grew, the earlier tokens' codes are quantized again over the new
-      scale.  Rows at a block's first token begin it anew.  A block must be written by one
+      scale, off by half a step of it each time.  A scale does not fall until rows at its
+      block's first token begin the block anew: drafts that raised it and were rejected leave
+      the block's other codes coarser.  A block must be written by one
       sequence of a call only.  (``finalize_rows`` and ``commit_tree_kv`` move codes as they are:
       not between blocks of such a cache, whose scales differ.)
 
