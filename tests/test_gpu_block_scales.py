@@ -184,3 +184,33 @@ def test_stores_by_a_bound_and_over_strides_of_8_bytes(kernel, dev, codes, rows)
         outs.append((out, *map(_bytes, held)))
     for other in outs[1:]:
         assert all(torch.equal(a, b) for a, b in zip(outs[0], other))
+
+
+def test_calls_of_more_units_than_a_launch(kernel, dev):
+    """2^24 units of 256 threads, nearly all without keys: single rows over tables padded to 65536 positions, and
+    prompts whose longest window is known by its bound; as the same rows in a small call."""
+    _say("past one launch")
+    n, heads, width = 4112, 64, 4096  # 4112 x 64 x 64 chunks
+    g = torch.Generator(device=dev).manual_seed(30)
+    k, v = (torch.randint(-127, 128, (64, 16, heads, 64), generator=g, device=dev, dtype=torch.int8) for _ in range(2))
+    ks, vs = (torch.rand(64, heads, generator=g, device=dev) * 0.02 + 0.001 for _ in range(2))
+    few = torch.randint(0, 64, (n, 4), generator=g, device=dev, dtype=torch.int32)
+    tables = torch.full((n, width), -1, dtype=torch.int32, device=dev)
+    tables[:, :4] = few
+    lengths = torch.randint(1, 65, (n,), generator=g, device=dev, dtype=torch.int32)
+    q = torch.randn(n, heads, 64, generator=g, device=dev).to(torch.bfloat16)
+    got = kernel(q, k, v, tables, lengths, ks, vs)
+    for part in (slice(0, 40), slice(n // 2 - 20, n // 2 + 20), slice(n - 40, n)):
+        assert torch.equal(got[part], kernel(q[part], k, v, few[part].contiguous(), lengths[part], ks, vs))
+    del tables
+    # 64 rows of every eighth sequence, none of the others: 1040 x 64 heads x 256 groups of 128 rows
+    seqs, bound = 1040, 32768
+    counts = torch.zeros(seqs, dtype=torch.int32, device=dev)
+    counts[::8] = 64
+    counts[-1] = 64
+    cu = torch.cat([counts.new_zeros(1), counts.cumsum(0).int()])
+    rows = int(cu[-1])
+    q = torch.randn(rows, heads, 64, generator=g, device=dev).to(torch.bfloat16)
+    args = (few[:seqs].contiguous(), counts, cu)
+    got = kernel.prefill(q, k, v, *args, bound, ks, vs)
+    assert torch.equal(got, kernel.prefill(q, k, v, *args, 64, ks, vs))

@@ -50,6 +50,9 @@ void launch_block_prefill_int8(const AttnParams& P, int q_dtype, dim3 grid, bool
 
 // (sequence, row-group) pairs that the persistent form lists
 constexpr int kMaxBlockPairs = 1024;
+// Workgroups of one launch: a grid holds fewer than 2^32 threads, and a call may ask for more (its
+// tables and windows are padded to the longest); those behind go into further launches.
+constexpr unsigned kBlockGrid = 1u << 23;
 
 }  // namespace rlt_attn
 
@@ -476,7 +479,7 @@ void rlt_block_attention_kernel(AttnParams P) {
       c0 = sh.c0[seq * P.rowgroups + rg];
     } else {
       // (more pairs than are listed: a workgroup each)
-      const WorkItem wi = work_item(P, blockIdx.x);
+      const WorkItem wi = work_item(P, P.first_group + blockIdx.x);
       seq = wi.seq;
       rg = wi.rg;
       kvh = wi.hg;
@@ -551,10 +554,12 @@ int launch_block_cp(AttnParams P, dim3 grid, int nt, hipStream_t stream) {
     P.persistent = 0;
     grid = dim3((unsigned)all);
   }
-  if (nt == 1) rlt_block_attention_kernel<QT, KVT, D, 1, CP><<<grid, 64 * kBlockParts, 0, stream>>>(P);
-  else if (D <= 128)
-    rlt_block_attention_kernel<QT, KVT, D, (D <= 128 ? 2 : 1), CP><<<grid, 64 * kBlockParts, 0, stream>>>(P);
-  else return RLT_ERR_UNSUPPORTED;
+  if (nt != 1 && D > 128) return RLT_ERR_UNSUPPORTED;
+  for (unsigned left = grid.x; left; left -= grid.x, P.first_group += grid.x) {
+    grid.x = left < rlt_attn::kBlockGrid ? left : rlt_attn::kBlockGrid;
+    if (nt == 1) rlt_block_attention_kernel<QT, KVT, D, 1, CP><<<grid, 64 * kBlockParts, 0, stream>>>(P);
+    else rlt_block_attention_kernel<QT, KVT, D, (D <= 128 ? 2 : 1), CP><<<grid, 64 * kBlockParts, 0, stream>>>(P);
+  }
   return RLT_OK;
 }
 
@@ -587,9 +592,12 @@ int launch_block(const AttnParams& P, int q_dtype, dim3 grid, int nt, bool whole
 }
 
 template <int QT, int KVT, int D>
-void launch_block_prefill_d(const AttnParams& P, dim3 grid, bool whole, hipStream_t stream) {
-  if (whole) rlt_prefill_kernel<QT, KVT, D, 3, true><<<grid, kPfThreads, 0, stream>>>(P);
-  else rlt_prefill_kernel<QT, KVT, D, 3, false><<<grid, kPfThreads, 0, stream>>>(P);
+void launch_block_prefill_d(AttnParams P, dim3 grid, bool whole, hipStream_t stream) {
+  for (unsigned left = grid.x; left; left -= grid.x, P.first_group += grid.x) {
+    grid.x = left < rlt_attn::kBlockGrid ? left : rlt_attn::kBlockGrid;
+    if (whole) rlt_prefill_kernel<QT, KVT, D, 3, true><<<grid, kPfThreads, 0, stream>>>(P);
+    else rlt_prefill_kernel<QT, KVT, D, 3, false><<<grid, kPfThreads, 0, stream>>>(P);
+  }
 }
 
 template <int QT, int KVT>

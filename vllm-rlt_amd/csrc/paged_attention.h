@@ -83,6 +83,7 @@ struct AttnParams {
   int64_t s_block_stride, s_token_stride, s_head_stride;
   int32_t scale_mode;  // 0 none, 1 per-tensor (0-d), 2 per-vector [blk, tok, kvh], 3 per block [blk, kvh]
   int32_t direct;      // block scales: rows of one chunk or none are written without the merge
+  uint32_t first_group;  // block scales, prompts: the launch's first workgroup
   int32_t compensate;  // MFMA path: P V also with the bits P loses in its 16-bit cast
   int32_t num_seqs;
   int32_t num_rows;  // total q rows

@@ -688,6 +688,7 @@ int attention_impl(const void* q, int64_t q_row_stride, int64_t q_head_stride,
   P.scale_mode = scale_mode;
   P.compensate = (flags & RLT_ATTN_COMPENSATE) ? 1 : 0;
   P.direct = 0;
+  P.first_group = 0;
   P.num_seqs = num_seqs;
   P.num_rows = num_q_rows;
   P.hq = num_q_heads;

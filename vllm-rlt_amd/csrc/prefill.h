@@ -203,7 +203,7 @@ __global__ __launch_bounds__(kPfThreads, 2) void rlt_prefill_kernel(AttnParams P
 
   // heaviest row-groups (latest positions) first across the whole batch: the
   // row-group index is outermost, then the sequence, then the kv head
-  const int64_t id = blockIdx.x;
+  const int64_t id = P.first_group + blockIdx.x;
   const int kvh = (int)(id % P.hkv);
   const int64_t sr = id / P.hkv;
   const int seq = (int)(sr % P.num_seqs);
