@@ -630,9 +630,9 @@ int rlt_rotary(const void* q, int64_t q_row_stride, int64_t q_head_stride, const
  * Windows of rows into the paged cache, keys and queries turned on the way (as rlt_rotary;
  * rotary_dim 0: not at all).  Sequence s owns rows cu_seqlens_q[s] .. cu_seqlens_q[s + 1] - 1; row i
  * of its n goes to position context_lengths[s] - n + i of its table and turns by it, or by
- * positions[row] (int64, optional).  Rows from the max_q_len-th of a sequence on are left.  Rows before position 0, past the
- * table or whose entry lies outside the pool are not written.  k, v [rows, num_kv_heads,
- * head_dim] and q (optional) of `dtype`; q_out as in rlt_rotary.  Pools:
+ * positions[row] (int64, optional).  Rows from the max_q_len-th of a sequence on are left; rows
+ * before position 0, past the table or whose entry lies outside the pool are not written.  k, v
+ * [rows, num_kv_heads, head_dim] and q (optional) of `dtype`; q_out as in rlt_rotary.  Pools:
  *   - kv_dtype == dtype, scale_mode 0: turned rows rounded once;
  *   - RLT_FP8_E4M3, scale_mode 1 (one float each, read) or 2 ([block, token, kv_head],
  *     written): codes and scales of the float32 rows as rlt_kv_store_fp8's;

@@ -214,3 +214,22 @@ def test_calls_of_more_units_than_a_launch(kernel, dev):
     args = (few[:seqs].contiguous(), counts, cu)
     got = kernel.prefill(q, k, v, *args, bound, ks, vs)
     assert torch.equal(got, kernel.prefill(q, k, v, *args, 64, ks, vs))
+
+
+@pytest.mark.parametrize("codes", CODES)
+@pytest.mark.parametrize("hq,hkv,dim,bs", [(4, 2, 128, 8), (8, 1, 64, 24), (2, 2, 256, 3), (6, 2, 96, 40),
+                                           (4, 2, 128, 16), (6, 2, 96, 32)])
+def test_weights_are_rounded_to_fp16_whatever_the_queries(kernel, dev, codes, hq, hkv, dim, bs):
+    """bfloat16 windows in blocks of any size.  A weight times its scale is float32 until it is rounded to fp16
+    (2^-11, half a step), float32 scores put a weight off by 2^-18 and sums by 2^-16 over these lengths, and the
+    output is rounded once (2^-8)."""
+    _say("fp16 weights", codes, dim, bs)
+    short = [(n, min(n, 5)) for n in range(1, 40)]
+    c = Case(codes, torch.bfloat16, ACROSS + short, hq, hkv, dim, bs, seed=31)
+    scales = c.vs.clone()
+    for factor in (1.0, 2.0 ** -85, 2.0 ** 75):
+        c.vs = scales * factor
+        got, (want, most) = c.packed(kernel, dev), c.expect()
+        near = most * (2.0 ** -11 + 2.0 ** -15) + want.abs() * 2.0 ** -8
+        assert ((got.double() - want).abs() <= near * 1.01).all()
+        assert torch.equal(got, _single(kernel, dev, c))

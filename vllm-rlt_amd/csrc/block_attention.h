@@ -41,8 +41,7 @@ namespace rlt_attn {
 int block_chunk_log2();
 int block_groups_per_cu(int head_dim, int nt);
 // The verify kernels (`whole`: blocks hold whole 16-position tiles and a lane's offset within
-// one fits 32 bits; other blocks take their scales position by position, of e4m3 pools with fp16 q
-// only: with bf16 they take the per-vector form) and the prefill tiling.
+// one fits 32 bits; other blocks take their scales position by position) and the prefill tiling.
 int launch_block_fp8(const AttnParams& P, int q_dtype, dim3 grid, int nt, bool whole, hipStream_t stream);
 int launch_block_int8(const AttnParams& P, int q_dtype, dim3 grid, int nt, bool whole, hipStream_t stream);
 void launch_block_prefill_fp8(const AttnParams& P, int q_dtype, dim3 grid, bool whole, hipStream_t stream);
@@ -569,8 +568,7 @@ int launch_block_d(const AttnParams& P, dim3 grid, int nt, bool whole, hipStream
     if (P.compensate) return launch_block_cp<QT, KVT, D, true>(P, grid, nt, stream);
     return launch_block_cp<QT, KVT, D, false>(P, grid, nt, stream);
   }
-  if constexpr (KVT == RLT_INT8 || QT == RLT_F16)
-    if (!P.compensate) return launch_mfma_ub<QT, KVT, D, QT == RLT_F16 ? 3 : 2, false, false>(P, grid, nt, stream);
+  if (!P.compensate) return launch_mfma_ub<QT, KVT, D, 3, false, false>(P, grid, nt, stream);
   return RLT_ERR_UNSUPPORTED;
 }
 

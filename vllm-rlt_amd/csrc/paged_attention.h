@@ -634,17 +634,19 @@ __device__ __forceinline__ bool store_window(const AttnParams& P, int seq, int k
 // row-group, kv head, chunk) -- on one wave: the wave streams the kv head over
 // positions [512c + part * 512 / KS, + 512 / KS) for every row of the row-group.
 // tbl_lds: this wave's 512-entry LDS slice for the chunk's block ids.
-// SM: scale mode of 8-bit pools (0 none, 1 per-tensor, 2 per-vector, 3 per block and kv head where
-// a weight's fp16 does not hold scales of any size: as 2, but weights are over a power of two near
-// the largest value scale that the row sees in the span; bf16 weights over block scales take 2).
+// SM: scale mode of 8-bit pools (0 none, 1 per-tensor, 2 per-vector, 3 per block and kv head: as 2,
+// but the product with the values is fp16's whatever q's type, its weights over a power of two
+// near the largest value scale that the row sees in the span, as in block_attention.h).
 // UB: block_size is a multiple of 16, so the 16 positions of a tile share one block.
 template <int QT, int KVT, int D, int NT, int SM, bool UB, bool CP>
 __device__ __forceinline__ void attend_span(const AttnParams& P, int seq, int rg, int kvh, int chunk,
                                             int part, int32_t* tbl_lds,
                                             UnitState<NT, D / 16>& st) {
+  constexpr int VT = SM == 3 ? RLT_F16 : QT;  // of weights and values
   using M = Mfma<QT>;
+  using W = Mfma<VT>;
   using Raw = RawSlice<QT, KVT, D>;
-  using VQ = ValueQuad<QT, KVT, D>;
+  using VQ = ValueQuad<VT, KVT, D>;
   constexpr int NQS = D / 32;  // 32-wide contraction slices
   constexpr int ND = D / 16;   // 16-wide output column tiles (= dims per lane)
   constexpr int KV_ELT = KVT == QT ? 2 : 1;
@@ -760,8 +762,8 @@ __device__ __forceinline__ void attend_span(const AttnParams& P, int seq, int rg
     const int64_t v_head = (int64_t)kvh * P.v_head_stride + l16 * ND;
     const int32_t* tbl = tbl_lds - c_begin;  // tbl[pos] for pos in the chunk
     // SM 3: a row's weights and their sum are over 2^v_exp, so that weights times scales lie 2^15 above
-    // their place at most (2^-64 and smaller scales leave nothing that an fp16 output holds).  The
-    // span's value scales are read ahead of its first tiles.
+    // their place at most (scales below 2^-100 count as that: 1024 weights over 2^-115 still add up).
+    // The span's value scales are read ahead of its first tiles.
     float v_exp[NT], span_scale[SM == 3 ? kSpan / 64 : 1];
     if constexpr (SM == 3) {
 #pragma unroll
@@ -930,12 +932,12 @@ __device__ __forceinline__ void attend_span(const AttnParams& P, int seq, int rg
 #pragma unroll
             for (int r = 0; r < 4; ++r) pr[b][r] *= vsc[b][r];
           }
-          pop[b][nt] = make_uint2(M::pack2(pr[b][0], pr[b][1]), M::pack2(pr[b][2], pr[b][3]));
+          pop[b][nt] = make_uint2(W::pack2(pr[b][0], pr[b][1]), W::pack2(pr[b][2], pr[b][3]));
           if (CP) {
             // what the cast dropped, as a second 16-bit operand (the reference's
             // compensated dot, vllm_rlt/kernels/triton_attention.py:368-371)
             auto dropped = [&](uint32_t w, int r) {
-              return M::pack2(pr[b][r] - M::lo_f32(w), pr[b][r + 1] - M::hi_f32(w));
+              return W::pack2(pr[b][r] - W::lo_f32(w), pr[b][r + 1] - W::hi_f32(w));
             };
             plo[b][nt] = make_uint2(dropped(pop[b][nt].x, 0), dropped(pop[b][nt].y, 2));
           }
@@ -969,11 +971,11 @@ __device__ __forceinline__ void attend_span(const AttnParams& P, int seq, int rg
           vq[B].template op2<K>(a0, a1);
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
-            oacc[nt][2 * K] = M::pv(a0, pop[B][nt], oacc[nt][2 * K]);
-            oacc[nt][2 * K + 1] = M::pv(a1, pop[B][nt], oacc[nt][2 * K + 1]);
+            oacc[nt][2 * K] = W::pv(a0, pop[B][nt], oacc[nt][2 * K]);
+            oacc[nt][2 * K + 1] = W::pv(a1, pop[B][nt], oacc[nt][2 * K + 1]);
             if (CP) {
-              oacc[nt][2 * K] = M::pv(a0, plo[B][nt], oacc[nt][2 * K]);
-              oacc[nt][2 * K + 1] = M::pv(a1, plo[B][nt], oacc[nt][2 * K + 1]);
+              oacc[nt][2 * K] = W::pv(a0, plo[B][nt], oacc[nt][2 * K]);
+              oacc[nt][2 * K + 1] = W::pv(a1, plo[B][nt], oacc[nt][2 * K + 1]);
             }
           }
         });
@@ -1024,7 +1026,7 @@ __device__ __forceinline__ void attend_span(const AttnParams& P, int seq, int rg
       if (lo_last < hi_first) some(hi_first, hi_last);
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
-        v_exp[nt] = (float)((most[nt] > 0.f ? max(__builtin_amdgcn_frexp_expf(most[nt]), -64) : 0) - 15);
+        v_exp[nt] = (float)((most[nt] > 0.f ? max(__builtin_amdgcn_frexp_expf(most[nt]), -100) : 0) - 15);
     }
 #pragma unroll 1
     for (int t = t0; t < t1; t += 2) compute(t);

@@ -801,7 +801,7 @@ int attention_impl(const void* q, int64_t q_row_stride, int64_t q_head_stride,
     dim3 grid((unsigned)wgs);
     if (kv_dtype == RLT_INT8)
       st = rlt_attn::launch_block_int8(P, q_dtype, grid, nt, whole_tiles(P), stream);
-    else if (scale_mode == 3 && (whole_tiles(P) || (q_dtype == RLT_F16 && !P.compensate)))
+    else if (scale_mode == 3 && (whole_tiles(P) || !P.compensate))
       st = rlt_attn::launch_block_fp8(P, q_dtype, grid, nt, whole_tiles(P), stream);
     else if (q_dtype == RLT_BF16)
       st = kv_dtype == RLT_BF16 ? launch_mfma<RLT_BF16, RLT_BF16>(P, grid, nt, stream)
