@@ -77,10 +77,9 @@ struct BlockShared {
   int32_t wave_total[kBlockParts];
 };
 
-// Keys and values as paged_attention.h's slices, but for 96 dims, whose 96-byte vectors take fewer
-// loads in other pieces: a lane group's 24 consecutive key codes in two (three 8-byte ones), a
-// lane's six value codes in one of 8 bytes, the last lane's two bytes ahead so that it ends with
-// the vector (three of 2 bytes).  16 windows of 16 rows, 2048 positions, 55 heads: 133 -> 96 us.
+// Keys as paged_attention.h's slices, but for 96 dims, whose 96-byte vectors take fewer loads in other
+// pieces: a lane group's 24 consecutive key codes in two (three 8-byte ones).  With the values'
+// (BlockValues), 16 windows of 16 rows, 2048 positions, 55 heads: 133 -> 96 us.
 template <int QT, int KVT, int D>
 struct BlockKeys : RawSlice<QT, KVT, D> {};
 template <int QT, int KVT>
@@ -92,38 +91,6 @@ struct BlockKeys<QT, KVT, 96> {
   __device__ __forceinline__ uint4 op(int s) const {
     const uint2 a = codes_to_16<QT, KVT>(w[2 * s]), b = codes_to_16<QT, KVT>(w[2 * s + 1]);
     return make_uint4(a.x, a.y, b.x, b.y);
-  }
-};
-
-template <int QT, int KVT, int D>
-struct BlockValues : ValueQuad<QT, KVT, D> {
-  // bytes from a vector's first to what a lane loads
-  __device__ static int lane_bytes(int l16) { return D / 16 * l16; }
-  __device__ __forceinline__ void arrange(int) {}
-};
-template <int QT, int KVT>
-struct BlockValues<QT, KVT, 96> {
-  uint32_t w[4][2];
-  __device__ static int lane_bytes(int l16) { return l16 == 15 ? 88 : 6 * l16; }
-  __device__ __forceinline__ void load(int i, const uint8_t* p) {
-    __builtin_memcpy(w[i], __builtin_assume_aligned(p, 2), 8);
-  }
-  __device__ __forceinline__ void zero(int i) { w[i][0] = w[i][1] = 0; }
-  // (once loaded) the lane's six codes to the front
-  __device__ __forceinline__ void arrange(int l16) {
-    const int skip = l16 == 15 ? 2 : 0;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      w[i][0] = __builtin_amdgcn_alignbyte(w[i][1], w[i][0], skip);
-      w[i][1] >>= 8 * skip;
-    }
-  }
-  template <int K>
-  __device__ __forceinline__ void op2(uint2& a0, uint2& a1) const {
-    ValueQuad<QT, KVT, 64> quad;  // (words of four codes, as its)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) quad.w[i][0] = w[i][K / 2];
-    quad.template op2<K % 2>(a0, a1);
   }
 };
 

@@ -470,6 +470,40 @@ struct ValueQuad {
   }
 };
 
+// Values of pools with block scales: as above, but for 96 dims, where a lane's six codes come in one
+// load of 8 bytes (three of 2), the last lane's two bytes ahead so that it ends with the vector.
+template <int QT, int KVT, int D>
+struct BlockValues : ValueQuad<QT, KVT, D> {
+  // bytes from a vector's first to what a lane loads
+  __device__ static int lane_bytes(int l16) { return D / 16 * l16; }
+  __device__ __forceinline__ void arrange(int) {}
+};
+template <int QT, int KVT>
+struct BlockValues<QT, KVT, 96> {
+  uint32_t w[4][2];
+  __device__ static int lane_bytes(int l16) { return l16 == 15 ? 88 : 6 * l16; }
+  __device__ __forceinline__ void load(int i, const uint8_t* p) {
+    __builtin_memcpy(w[i], __builtin_assume_aligned(p, 2), 8);
+  }
+  __device__ __forceinline__ void zero(int i) { w[i][0] = w[i][1] = 0; }
+  // (once loaded) the lane's six codes to the front
+  __device__ __forceinline__ void arrange(int l16) {
+    const int skip = l16 == 15 ? 2 : 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      w[i][0] = __builtin_amdgcn_alignbyte(w[i][1], w[i][0], skip);
+      w[i][1] >>= 8 * skip;
+    }
+  }
+  template <int K>
+  __device__ __forceinline__ void op2(uint2& a0, uint2& a1) const {
+    ValueQuad<QT, KVT, 64> quad;  // (words of four codes, as its)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) quad.w[i][0] = w[i][K / 2];
+    quad.template op2<K % 2>(a0, a1);
+  }
+};
+
 template <int ND, int NT, class F, int K = 0>
 __device__ __forceinline__ void for_pairs(F&& f) {
   if constexpr (K < ND / 2) {
@@ -646,7 +680,7 @@ __device__ __forceinline__ void attend_span(const AttnParams& P, int seq, int rg
   using M = Mfma<QT>;
   using W = Mfma<VT>;
   using Raw = RawSlice<QT, KVT, D>;
-  using VQ = ValueQuad<VT, KVT, D>;
+  using VQ = typename std::conditional<SM == 3, BlockValues<VT, KVT, D>, ValueQuad<VT, KVT, D>>::type;
   constexpr int NQS = D / 32;  // 32-wide contraction slices
   constexpr int ND = D / 16;   // 16-wide output column tiles (= dims per lane)
   constexpr int KV_ELT = KVT == QT ? 2 : 1;
@@ -759,17 +793,30 @@ __device__ __forceinline__ void attend_span(const AttnParams& P, int seq, int rg
     VQ vq[2];
     float sraw = 0.f;
     const int64_t k_head = (int64_t)kvh * P.k_head_stride + grp * Raw::kGroupElems;
-    const int64_t v_head = (int64_t)kvh * P.v_head_stride + l16 * ND;
+    int v_first = l16 * ND;  // element that this lane's value loads begin at
+    if constexpr (SM == 3) v_first = VQ::lane_bytes(l16);
+    const int64_t v_head = (int64_t)kvh * P.v_head_stride + v_first;
     const int32_t* tbl = tbl_lds - c_begin;  // tbl[pos] for pos in the chunk
     // SM 3: a row's weights and their sum are over 2^v_exp, so that weights times scales lie 2^15 above
     // their place at most (scales below 2^-100 count as that: 1024 weights over 2^-115 still add up).
-    // The span's value scales are read ahead of its first tiles.
-    float v_exp[NT], span_scale[SM == 3 ? kSpan / 64 : 1];
+    // The value scales of the blocks that every row sees are read ahead of the first tiles, a lane a
+    // block.
+    constexpr int kScales = 4;
+    float v_exp[NT], shared_scale[SM == 3 ? kScales : 1];
+    const auto value_scale = [&](int pos) {
+      return fabsf(P.v_scale[tbl[pos] * P.s_block_stride + (int64_t)kvh * P.s_head_stride]);
+    };
+    const int shared_lo = max(lo_last, w_begin), shared_hi = min(hi_first, w_begin + kSpan);
+    int blk0 = 0, blocks = 0;
     if constexpr (SM == 3) {
+      if (shared_lo < shared_hi) {
+        blk0 = shared_lo / P.block_size;
+        blocks = (shared_hi - 1) / P.block_size - blk0 + 1;
+      }
 #pragma unroll
-      for (int i = 0; i < kSpan / 64; ++i) {
-        const int at = w_begin + 64 * i + lane;
-        span_scale[i] = P.v_scale[tbl[at] * P.s_block_stride + (int64_t)kvh * P.s_head_stride];
+      for (int i = 0; i < kScales; ++i) {
+        const int j = 64 * i + lane;
+        shared_scale[i] = j < blocks ? value_scale(max((blk0 + j) * P.block_size, w_begin)) : 0.f;
       }
     }
     // positions from hi_last on are masked, their values taken as zeros (they may hold any
@@ -782,7 +829,7 @@ __device__ __forceinline__ void attend_span(const AttnParams& P, int seq, int rg
     // With whole tiles per block the block is wave-uniform: a scalar base and a 32-bit lane
     // offset (fewer address registers; launch_mfma_sm bounds the strides).
     const uint32_t k_lane = (uint32_t)(l16 * (uint32_t)P.k_token_stride + grp * Raw::kGroupElems) * KV_ELT;
-    const uint32_t v_lane = (uint32_t)(4 * grp * (uint32_t)P.v_token_stride + l16 * ND) * KV_ELT;
+    const uint32_t v_lane = (uint32_t)(4 * grp * (uint32_t)P.v_token_stride + v_first) * KV_ELT;
     auto issue_k = [&](int t, int b) {
       const int tb = tile_base(t);
       if (UB) {
@@ -945,6 +992,10 @@ __device__ __forceinline__ void attend_span(const AttnParams& P, int seq, int rg
       }
       issue_scales(t + 2);
       __builtin_amdgcn_sched_barrier(0);
+      if constexpr (SM == 3) {
+#pragma unroll
+        for (int b = 0; b < 2; ++b) vq[b].arrange(l16);
+      }
       // positions outside the span may hold any bits (NaN included): zero them
       if (!full) {
 #pragma unroll
@@ -988,31 +1039,34 @@ __device__ __forceinline__ void attend_span(const AttnParams& P, int seq, int rg
       issue_v(t + 2, 0);
       issue_v(t + 3, 1);
     };
+    // (SM 3: in the order of the loop's own, whose waits count what follows a load: 45 rows at 805 to
+    // 6440 positions, 8 heads of 64 in int8, blocks of 8, 91.8 -> 87.1 us)
 #pragma unroll
     for (int b = 0; b < 2; ++b) issue_k(t0 + b, b);
+    if (SM == 3) __builtin_amdgcn_sched_barrier(0);
     issue_scales(t0);
+    if (SM == 3) __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int b = 0; b < 2; ++b) issue_v(t0 + b, b);
+    if (SM == 3) __builtin_amdgcn_sched_barrier(0);
     if constexpr (SM == 3) {
-      float all = 0.f;  // of the positions that every row sees
+      float all = 0.f;  // of the blocks that every row sees
 #pragma unroll
-      for (int i = 0; i < kSpan / 64; ++i) {
-        const int at = w_begin + 64 * i + lane;
-        all = at >= lo_last && at < hi_first ? fmaxf(all, fabsf(span_scale[i])) : all;
-      }
+      for (int i = 0; i < kScales; ++i) all = fmaxf(all, shared_scale[i]);
+      for (int j = 64 * kScales + lane; j < blocks; j += 64)
+        all = fmaxf(all, value_scale(max((blk0 + j) * P.block_size, w_begin)));
 #pragma unroll
       for (int o = 32; o >= 1; o >>= 1) all = fmaxf(all, __shfl_xor(all, o, RLT_WAVE));
       float most[NT];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) most[nt] = all;
-      // and of the others, 64 read at a time
+      // and of the positions that some do not see, 64 read at a time
       auto some = [&](int from, int to) {
         from = max(from, w_begin);
         to = min(to, w_begin + kSpan);
 #pragma unroll 1
         for (int p0 = from; p0 < to; p0 += 64) {
-          const int64_t blk = tbl[min(p0 + lane, to - 1)];
-          const float x = fabsf(P.v_scale[blk * P.s_block_stride + (int64_t)kvh * P.s_head_stride]);
+          const float x = value_scale(min(p0 + lane, to - 1));
 #pragma unroll 1
           for (int p = p0; p < min(p0 + 64, to); ++p) {
             const float y = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), p - p0));
